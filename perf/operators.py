@@ -32,22 +32,22 @@ ESIZE = {"bf16": 2, "f16": 2, "f32": 4}
 def listed():
     return [
         # One decode step's new tokens of 256 sequences (Llama-3-8B heads): latency counts.
-        {"name": "append-decode", "op": "append", "dtype": "bf16", "tokens": 256, "hkv": 8,
-         "d": 128, "strided": True, "pad": 7},
+        {"name": "append-decode", "op": "append", "dtype": "bf16", "tokens": 256, "run": 1,
+         "hkv": 8, "d": 128, "strided": True, "pad": 7},
         # A prefill round of 64 sequences x 512 tokens: HBM-bound.
-        {"name": "append-prefill", "op": "append", "dtype": "bf16", "tokens": 32768, "hkv": 8,
-         "d": 128, "strided": True, "pad": 0},
+        {"name": "append-prefill", "op": "append", "dtype": "bf16", "tokens": 32768, "run": 512,
+         "hkv": 8, "d": 128, "strided": True, "pad": 0},
         # Decode step of 256 sequences: rotary positions scaled for long contexts, then the write.
-        {"name": "rotary-decode", "op": "rotary", "dtype": "bf16", "tokens": 256, "hq": 32,
-         "hkv": 8, "d": 128, "rd": 128, "interleaved": False, "scaling": "wavelength",
+        {"name": "rotary-decode", "op": "rotary", "dtype": "bf16", "tokens": 256, "run": 1,
+         "hq": 32, "hkv": 8, "d": 128, "rd": 128, "interleaved": False, "scaling": "wavelength",
          "quant": True, "maxpos": 131072},
         # A long prompt's chunk round into the 8-bit cache, odd token count.
-        {"name": "rotary-prefill", "op": "rotary", "dtype": "bf16", "tokens": 16381, "hq": 32,
-         "hkv": 8, "d": 128, "rd": 128, "interleaved": False, "scaling": "wavelength",
+        {"name": "rotary-prefill", "op": "rotary", "dtype": "bf16", "tokens": 16381, "run": 512,
+         "hq": 32, "hkv": 8, "d": 128, "rd": 128, "interleaved": False, "scaling": "wavelength",
          "quant": True, "maxpos": 131072},
         # Interleaved pairs on half of each head, stretched positions, cache in the model's type.
-        {"name": "rotary-partial", "op": "rotary", "dtype": "f16", "tokens": 4099, "hq": 64,
-         "hkv": 8, "d": 128, "rd": 64, "interleaved": True, "scaling": "factor",
+        {"name": "rotary-partial", "op": "rotary", "dtype": "f16", "tokens": 4099, "run": 100,
+         "hq": 64, "hkv": 8, "d": 128, "rd": 64, "interleaved": True, "scaling": "factor",
          "quant": False, "maxpos": 32768},
         # One sequence's context read back (handing a cached prefix to another process).
         {"name": "read-one", "op": "read", "dtype": "bf16", "seqs": 1, "median": 1500,
@@ -84,12 +84,14 @@ def draw(rng):
     hkv = rng.choice([1, 2, 4, 8])
     if op == "append":
         return {"op": op, "dtype": rng.choice(["bf16", "f16", "f32"]),
-                "tokens": _log_int(rng, 1, 16384), "hkv": hkv, "d": d,
+                "tokens": _log_int(rng, 1, 16384), "run": rng.choice([1, 100, 512]),
+                "hkv": hkv, "d": d,
                 "strided": rng.random() < 0.5, "pad": rng.choice([0, 3, 7])}  # fmt: skip
     g = rng.choice([1, 2, 4, 5, 7, 8, 16])
     if op == "rotary":
         return {"op": op, "dtype": rng.choice(["bf16", "f16", "f32"]),
-                "tokens": _log_int(rng, 1, 8192), "hq": hkv * min(g, 8), "hkv": hkv, "d": d,
+                "tokens": _log_int(rng, 1, 8192), "run": rng.choice([1, 100, 512]),
+                "hq": hkv * min(g, 8), "hkv": hkv, "d": d,
                 "rd": rng.choice([d, d // 2]), "interleaved": rng.random() < 0.5,
                 "scaling": rng.choice(["none", "wavelength", "factor"]),
                 "quant": rng.random() < 0.7, "maxpos": _log_int(rng, 64, 131072)}  # fmt: skip
@@ -219,9 +221,15 @@ def prepare(case, seed):
     dt, d, hkv = DTYPES[case["dtype"]], case["d"], case["hkv"]
     s = {"case": case}
     if case["op"] in ("append", "rotary"):
-        t = case["tokens"]
-        blocks = -(-t // BLOCK) + 4
-        slots = r.permutation(blocks * BLOCK)[:t].astype(np.int64)
+        # Sequences of `run` new tokens each, every sequence in blocks of its own anywhere in
+        # the pool: run 1 is a decode step (any place in its last block), more a prefill chunk.
+        t, run = case["tokens"], case["run"]
+        seqs, width = -(-t // run), -(-run // BLOCK)
+        blocks = seqs * width + 4
+        home = r.permutation(blocks)[: seqs * width].reshape(seqs, width)
+        seq, at = np.divmod(np.arange(t), run)
+        off = r.integers(0, BLOCK, t) if run == 1 else at % BLOCK
+        slots = (home[seq, at // BLOCK] * BLOCK + off).astype(np.int64)
         if case.get("pad"):
             slots[:: case["pad"]] = -1
         s["slots"] = torch.from_numpy(slots).cuda()
@@ -241,7 +249,8 @@ def prepare(case, seed):
     elif case["op"] == "rotary":
         hq = case["hq"]
         s["qkv"] = _rows(g, t, hq + 2 * hkv, d, dt).view(t, -1)
-        s["pos"] = torch.from_numpy(r.integers(0, case["maxpos"], t).astype(np.int64)).cuda()
+        first = r.integers(0, max(1, case["maxpos"] - run + 1), seqs)
+        s["pos"] = torch.from_numpy((first[seq] + at).astype(np.int64)).cuda()
         s["inv_freq"], s["mscale"] = _inv_freq(case)
         s["q_out"] = torch.zeros(t, hq, d, dtype=dt, device="cuda")
     elif case["op"] == "read":
