@@ -349,6 +349,112 @@ int ts_rope_and_cache(const void* qkv, int64_t qkv_token_stride, void* q_out, vo
                       int64_t num_blocks, int32_t dtype, int32_t* error_flag, void* stream);
 
 /*
+ * The 8-bit KV cache.
+ *
+ * K and V rows are stored as e4m3 codes with one float32 scale per (token, KV head):
+ *   key_pool, value_pool:     [num_blocks][num_kv_heads][block_size][head_dim] one byte each
+ *   key_scales, value_scales: [num_blocks][num_kv_heads][block_size] float32
+ *   scale = max(amax|x| / 448, 2^-126), code = e4m3(x / scale) (nearest even), value = code * scale
+ * A row with an infinity or a NaN gets scale NaN and NaN codes, and reads back as NaN; NaN codes
+ * occur in no other row. Scales are not negative. All pools contiguous. A (token, head) takes
+ * head_dim + 4 bytes instead of 2 head_dim, so attention reads, and a pool holds, about half.
+ * Blocks are copied and swapped like those of a 16-bit pool, with one more call for the scales
+ * (planes of num_kv_heads * block_size * 4 bytes per block).
+ */
+
+/*
+ * ts_reshape_and_cache into the 8-bit cache: key and value rows of `dtype` are quantised as they
+ * are written. Other arguments, padding, tags and the error flag as ts_reshape_and_cache; the
+ * slots of one call are distinct.
+ *
+ * Replaces: the same slot mapping and write (src/tokenserve/backends/base.py:40-45,
+ * src/tokenserve/backends/simulated.py:156-160); the reference has no quantised cache.
+ */
+int ts_reshape_and_cache_fp8(const void* key, const void* value, int64_t key_token_stride,
+                             int64_t value_token_stride, void* key_pool, void* value_pool,
+                             float* key_scales, float* value_scales, const int64_t* slot_mapping,
+                             int64_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t block_size, int64_t num_blocks, int32_t dtype,
+                             const int32_t* token_tags, int32_t* tag_pool, int32_t* error_flag,
+                             void* stream);
+
+/*
+ * Rotary positions of q and k in every layout models use, fused with the cache write. qkv, q_out,
+ * slots, positions and the error flag as ts_rope_and_cache; here
+ *   - the first rotary_dim (even, <= head_dim) dims of each head turn, the rest pass through;
+ *   - pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0;
+ *   - inv_freq: fp32 [rotary_dim / 2], any frequencies (scaled for long contexts or not);
+ *     attention_scaling multiplies cos and sin;
+ *   - the angle positions[t] * inv_freq[i] is reduced in 64 bits, so far positions are exact, and
+ *     the rotation is done in fp32 and rounded once (ts_rope_and_cache instead repeats the
+ *     roundings of the transformers module);
+ *   - with key_scales and value_scales the pools are an 8-bit cache and k and v are quantised
+ *     from fp32; with both NULL they hold `dtype`.
+ *
+ * Replaces: apply_rotary_pos_emb (models/llama/modeling_llama.py:146-168) and the rotary modules'
+ * scaled frequencies, run per layer by src/tokenserve/backends/hf.py:71.
+ */
+int ts_rotary_and_cache(const void* qkv, int64_t qkv_token_stride, void* q_out, void* key_pool,
+                        void* value_pool, float* key_scales, float* value_scales,
+                        const int64_t* slot_mapping, const int64_t* positions,
+                        const float* inv_freq, int64_t num_tokens, int32_t num_q_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+                        int32_t interleaved, float attention_scaling, int32_t block_size,
+                        int64_t num_blocks, int32_t dtype, int32_t* error_flag, void* stream);
+
+/*
+ * Reads an 8-bit cache back: row token_start_loc[s] + p of key_out and value_out
+ * ([num_tokens][num_kv_heads][head_dim] of `dtype`, contiguous) becomes position p of sequence s.
+ *
+ * Replaces: the read half of SimulatedBackend._write_and_verify
+ * (src/tokenserve/backends/simulated.py:161-169) for quantised rows.
+ *
+ * block_tables:    int32 [num_seqs][max_blocks_per_seq].
+ * token_start_loc: int32 [num_seqs + 1], ascending; sequence s owns rows token_start_loc[s] ..
+ *                  token_start_loc[s + 1] - 1. Rows of no sequence are left as they were.
+ * A position past the table, or in a block outside the pool, gives zeros and sets *error_flag.
+ */
+int ts_read_cache_fp8(void* key_out, void* value_out, const void* key_pool, const void* value_pool,
+                      const float* key_scales, const float* value_scales,
+                      const int32_t* block_tables, int32_t max_blocks_per_seq,
+                      const int32_t* token_start_loc, int32_t num_seqs, int64_t num_tokens,
+                      int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                      int64_t num_blocks, int32_t dtype, int32_t* error_flag, void* stream);
+
+/*
+ * ts_paged_decode over an 8-bit cache: out and query of `dtype`, the workspace (and its size, from
+ * ts_paged_decode_workspace_size) and the plan as there; reuse_plan = 1 is
+ * ts_paged_decode_planned. Shapes as ts_paged_decode: bf16/fp16 queries with block size 16,
+ * head_dim 64 or 128 and at most 16 query heads per KV head on tensor cores, else head_dim 32, 64,
+ * 128 or 256 on CUDA cores (no workspace).
+ *
+ * Replaces: the same eager attention as ts_paged_decode (src/tokenserve/backends/hf.py:71).
+ */
+int ts_paged_decode_fp8(void* out, const void* query, int64_t query_token_stride,
+                        const void* key_pool, const void* value_pool, const float* key_scales,
+                        const float* value_scales, const int32_t* block_tables,
+                        int32_t max_blocks_per_seq, const int32_t* context_lens, int32_t batch,
+                        int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                        int32_t block_size, int64_t num_blocks, float scale, int32_t dtype,
+                        void* workspace, size_t workspace_bytes, int32_t reuse_plan, void* stream);
+
+/*
+ * ts_paged_prefill over an 8-bit cache (the chunk's rows already written). Arguments as there.
+ * A query row whose position is negative (context shorter than the chunk) sees nothing and gets
+ * zeros; rows of no sequence are left as they were.
+ *
+ * Replaces: the same eager attention as ts_paged_prefill (src/tokenserve/backends/hf.py:62-71).
+ */
+int ts_paged_prefill_fp8(void* out, const void* query, int64_t query_token_stride,
+                         const void* key_pool, const void* value_pool, const float* key_scales,
+                         const float* value_scales, const int32_t* block_tables,
+                         int32_t max_blocks_per_seq, const int32_t* query_start_loc,
+                         const int32_t* context_lens, int32_t num_seqs, int32_t num_query_tokens,
+                         int32_t max_query_len, int32_t num_q_heads, int32_t num_kv_heads,
+                         int32_t head_dim, int32_t block_size, int64_t num_blocks, float scale,
+                         int32_t dtype, void* stream);
+
+/*
  * ts_silu_mul: out[r][c] = dtype(dtype(silu(gate_up[r][c])) * gate_up[r][intermediate + c])
  * (LlamaMLP act_fn(gate) * up, :184); gate_up: [num_rows][2 * intermediate].
  */

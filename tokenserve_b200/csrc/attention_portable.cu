@@ -8,16 +8,19 @@
 //
 // One CTA per (query row, query head); its four warps stride over the context tokens with an
 // online softmax each and merge their (m, l, o) states through shared memory at the end.
-#include "common.cuh"
+//
+// FP8: the pools hold e4m3 codes with a float32 scale per (token, KV head) row (fp8.cuh).
+#include "fp8.cuh"
 
 namespace {
 
 constexpr int kWarps = 4;
 
-template <typename T, int NDL>  // NDL = head_dim / 32 dims per lane
+template <typename T, int NDL, bool FP8>  // NDL = head_dim / 32 dims per lane
 __global__ void __launch_bounds__(kWarps * 32) paged_attention_portable_kernel(
     T* __restrict__ out, const T* __restrict__ query, int64_t q_stride,
-    const T* __restrict__ key_pool, const T* __restrict__ value_pool,
+    const void* __restrict__ key_pool, const void* __restrict__ value_pool,
+    const float* __restrict__ key_scales, const float* __restrict__ value_scales,
     const int32_t* __restrict__ block_tables, int max_blocks, const int32_t* __restrict__ qsl,
     const int32_t* __restrict__ context_lens, int num_seqs, int num_q_heads, int num_kv_heads,
     int block_size, int64_t num_blocks, float scale) {
@@ -33,6 +36,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attention_portable_kernel(
     seq = row;
     n_attend = context_lens[row];
   } else {
+    // Rows of no sequence are left as they were.
+    if (FP8 && (row < __ldg(qsl) || row >= __ldg(qsl + num_seqs))) return;
     int lo = 0, hi = num_seqs - 1;
     while (lo < hi) {  // largest s with qsl[s] <= row
       const int mid = (lo + hi + 1) / 2;
@@ -58,14 +63,23 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attention_portable_kernel(
   for (int j = warp; j < n_attend; j += kWarps) {
     const int64_t phys = __ldg(table + j / block_size);
     if (phys < 0 || phys >= num_blocks) continue;  // never reads outside the pool
-    const int64_t r = ((phys * num_kv_heads + kvh) * block_size + j % block_size) * D;
+    const int64_t prow = (phys * num_kv_heads + kvh) * block_size + j % block_size;
+    const int64_t r = prow * D;
     float dot = 0.f;
     float v[NDL];
+    const float vs = FP8 ? __ldg(value_scales + prow) : 1.f;
 #pragma unroll
     for (int k = 0; k < NDL; ++k) {
-      dot += q[k] * ts::to_float(key_pool[r + lane + 32 * k]);
-      v[k] = ts::to_float(value_pool[r + lane + 32 * k]);
+      const int64_t e = r + lane + 32 * k;
+      if (FP8) {
+        dot += q[k] * ts::fp8_float(static_cast<const uint8_t*>(key_pool)[e]);
+        v[k] = ts::fp8_float(static_cast<const uint8_t*>(value_pool)[e]) * vs;
+      } else {
+        dot += q[k] * ts::to_float(static_cast<const T*>(key_pool)[e]);
+        v[k] = ts::to_float(static_cast<const T*>(value_pool)[e]);
+      }
     }
+    if (FP8) dot *= __ldg(key_scales + prow);
 #pragma unroll
     for (int w = 16; w > 0; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
     const float s = dot * scale;
@@ -110,15 +124,20 @@ template <typename T>
 int launch_portable(void* out, const void* query, int64_t q_stride, const void* kp,
                     const void* vp, const int32_t* bt, int max_blocks, const int32_t* qsl,
                     const int32_t* cl, int num_seqs, int num_rows, int hq, int hkv, int hd,
-                    int bs, int64_t nb, float scale, cudaStream_t s) {
+                    int bs, int64_t nb, float scale, cudaStream_t s, const float* ks,
+                    const float* vs) {
   dim3 grid(num_rows, hq);
   auto o = static_cast<T*>(out);
   auto q = static_cast<const T*>(query);
-  auto k = static_cast<const T*>(kp);
-  auto v = static_cast<const T*>(vp);
 #define TS_P(NDL)                                                                              \
-  paged_attention_portable_kernel<T, NDL><<<grid, kWarps * 32, 0, s>>>(                        \
-      o, q, q_stride, k, v, bt, max_blocks, qsl, cl, num_seqs, hq, hkv, bs, nb, scale)
+  if (ks != nullptr)                                                                           \
+    paged_attention_portable_kernel<T, NDL, true><<<grid, kWarps * 32, 0, s>>>(                \
+        o, q, q_stride, kp, vp, ks, vs, bt, max_blocks, qsl, cl, num_seqs, hq, hkv, bs, nb,    \
+        scale);                                                                                \
+  else                                                                                         \
+    paged_attention_portable_kernel<T, NDL, false><<<grid, kWarps * 32, 0, s>>>(               \
+        o, q, q_stride, kp, vp, ks, vs, bt, max_blocks, qsl, cl, num_seqs, hq, hkv, bs, nb,    \
+        scale)
   switch (hd) {
     case 32: TS_P(1); break;
     case 64: TS_P(2); break;
@@ -135,25 +154,26 @@ int launch_portable(void* out, const void* query, int64_t q_stride, const void* 
 
 namespace ts {
 
-// Launches the CUDA-core kernel; `qsl == nullptr` means one query row per sequence (decode).
+// Launches the CUDA-core kernel; `qsl == nullptr` means one query row per sequence (decode), `ks`
+// and `vs` are an 8-bit cache's scales (else nullptr).
 int paged_attention_portable(void* out, const void* query, int64_t q_stride, const void* kp,
                              const void* vp, const int32_t* bt, int max_blocks,
                              const int32_t* qsl, const int32_t* cl, int num_seqs, int num_rows,
                              int hq, int hkv, int hd, int bs, int64_t nb, float scale, int dtype,
-                             cudaStream_t s) {
+                             cudaStream_t s, const float* ks, const float* vs) {
   if (num_rows == 0) return ok();
   if (num_rows > 2147483647 || hq > 65535)
     return set_error(TS_ERR_UNSUPPORTED, "paged attention: grid too large");
   switch (dtype) {
     case TS_FLOAT32:
       return launch_portable<float>(out, query, q_stride, kp, vp, bt, max_blocks, qsl, cl,
-                                    num_seqs, num_rows, hq, hkv, hd, bs, nb, scale, s);
+                                    num_seqs, num_rows, hq, hkv, hd, bs, nb, scale, s, ks, vs);
     case TS_FLOAT16:
       return launch_portable<__half>(out, query, q_stride, kp, vp, bt, max_blocks, qsl, cl,
-                                     num_seqs, num_rows, hq, hkv, hd, bs, nb, scale, s);
+                                     num_seqs, num_rows, hq, hkv, hd, bs, nb, scale, s, ks, vs);
     case TS_BFLOAT16:
       return launch_portable<__nv_bfloat16>(out, query, q_stride, kp, vp, bt, max_blocks, qsl,
-                                            cl, num_seqs, num_rows, hq, hkv, hd, bs, nb, scale, s);
+                                            cl, num_seqs, num_rows, hq, hkv, hd, bs, nb, scale, s, ks, vs);
     default:
       return set_error(TS_ERR_INVALID_ARGUMENT, "paged attention: bad dtype %d", dtype);
   }

@@ -1,0 +1,45 @@
+// The 8-bit KV cache's row format: D e4m3 codes and one float32 scale per (token, KV head) row.
+//
+//   scale = max(amax|x| / 448, 2^-126),  code = e4m3(x / scale),  value = code * scale
+//
+// 448 is e4m3's largest value, so a row uses the whole range whatever its magnitude; the floor
+// keeps scale and 1 / scale normal (an all-zero row has codes 0). A row that holds an infinity or
+// a NaN gets scale NaN and NaN codes: it reads back as NaN everywhere instead of as wrong numbers.
+// Codes are rounded to nearest even, at most half a step (2^-4 of the value) away.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace ts {
+
+constexpr float kE4m3Max = 448.f;
+
+// Bits of |x|: as unsigned integers they order like the magnitudes, with NaN above infinity.
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Scale of a row whose largest |x| has these bits.
+__device__ __forceinline__ float fp8_row_scale(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return fmaxf(__fdiv_rn(__uint_as_float(amax_bits), kE4m3Max), 0x1p-126f);
+}
+
+// Four codes of x * inv (element 0 in the low byte), saturating; NaN stays NaN.
+__device__ __forceinline__ uint32_t fp8_pack4(float x0, float x1, float x2, float x3, float inv) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x0 * inv, x1 * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x2 * inv, x3 * inv), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+// Two codes (low half of `w`) as f16x2; exact, e4m3's values are f16 numbers.
+__device__ __forceinline__ __half2 fp8_half2(uint32_t w) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
+  return __half2(r);
+}
+
+__device__ __forceinline__ float fp8_float(uint8_t c) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+}
+
+}  // namespace ts

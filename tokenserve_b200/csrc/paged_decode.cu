@@ -25,6 +25,18 @@
 //   * Online softmax in fp32 (exp2 domain) per block; partitions of one (b, h) are merged by the
 //     last warp to finish one (log-sum-exp merge in fixed partition order), tracked with an
 //     arrival counter.
+//
+// The 8-bit cache (fp8.cuh: e4m3 codes, one float32 scale per token and KV head) runs the same
+// plan, ring and merge, FP8 = true below. Its block is 2 x (16 D + 64) bytes, about half.
+//   * Codes become f16 operands with integer operations alone: sign | exponent and mantissa << 7
+//     is the f16 number code * 2^-8 (subnormals too), so the products are exact. A byte pair
+//     order falls out of the masks (even bytes, odd bytes); K's is undone in the order of q's
+//     words, V's (read by ldmatrix.trans as pairs of dims) is a permutation of O's rows.
+//   * q is scaled per head by a power of two into f16's range (bf16 q stays exact).
+//   * K's scale multiplies the score. V's is added to the exponent of the weight: with t = s +
+//     log2(vs), the running maximum is that of t, w = 2^(t - m) <= 1 goes to the PV product as
+//     f16 (11 bits: 2^-12 of itself, once) and the sum gets 2^(s - m) in 32 bits.
+//   * Slots past the context may hold any codes: they become finite f16 numbers with w = 0.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -32,7 +44,7 @@
 #include <cstring>
 #include <mutex>
 
-#include "common.cuh"
+#include "fp8.cuh"
 
 namespace {
 
@@ -87,6 +99,9 @@ constexpr int kMaxGridWarps = 8192;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct DecodeArgs {
+  // Scales of an 8-bit cache, [num_blocks][num_kv_heads][16] each (else nullptr).
+  const float* k_scales;
+  const float* v_scales;
   // Output rows: sequence b, query head j (of this call's num_q_heads) goes to
   // dst + b * out_row_stride + (out_head0 + j) * head_dim for dst = out, or, with n_out > 0,
   // for every dst in outs[0..n_out) (the ranks' full buffers of a KV-head-sharded model).
@@ -457,18 +472,40 @@ __device__ __forceinline__ uint32_t movmatrix_pack(float lo, float hi) {
   return ts::movmatrix_trans(Mma::pack(lo, hi));
 }
 
-template <int D>
+template <int D, bool FP8 = false>
 struct Geometry {
-  static constexpr int kHalves = D / 64;              // 64-column TMA boxes per row
-  static constexpr int kTileBytes = kBlock * D * 2;   // one block's K (or V) for one head
+  static constexpr int kHalves = D / 64;              // 64-column TMA boxes per row (16-bit pool)
+  static constexpr int kTileBytes = kBlock * D * (FP8 ? 1 : 2);  // one block's K (or V), one head
   static constexpr int kStageBytes = 2 * kTileBytes;  // K tile then V tile
-  static constexpr int kStages = D == 128 ? TS_DECODE_STAGES_D128 : 6;
-  static constexpr bool kOneBox = TS_DECODE_ONE_BOX && D == 128;
+  static constexpr int kStages = FP8 ? (D == 128 ? 6 : 10) : (D == 128 ? TS_DECODE_STAGES_D128 : 6);
+  static constexpr bool kOneBox = TS_DECODE_ONE_BOX && D == 128 && !FP8;
   static constexpr int kRingBytes = kStages * kStageBytes;
-  // ring, then one mbarrier (8 B) and one item descriptor (32 B) per stage, + alignment slack
+  static constexpr int kScaleBytes = FP8 ? 2 * kBlock * 4 : 0;  // a block's K then V scales
+  // ring, then one mbarrier (8 B) and one item descriptor (32 B) per stage and the stages'
+  // scales, + alignment slack
   static constexpr int kBarBytes = (kWarps * kStages * 8 + 15) / 16 * 16;
-  static constexpr int kSmemBytes = kWarps * kRingBytes + kBarBytes + kWarps * kStages * 32 + 1024;
+  static constexpr int kMetaBytes = kWarps * kStages * 32;
+  static constexpr int kSmemBytes = kWarps * kRingBytes + kBarBytes + kMetaBytes +
+                                    kWarps * kStages * kScaleBytes + 1024;
 };
+
+// Byte offset of 16-byte chunk `cg` (dims 16cg..16cg+15) of token `t` inside an 8-bit tile: one
+// box of 16 rows of D bytes, 128-byte swizzled (D = 128) or 64-byte swizzled (D = 64: the chunk's
+// two bits are XORed with bits 7-8 of the offset).
+template <int D>
+__device__ __forceinline__ uint32_t tile_off_fp8(int t, int cg) {
+  if constexpr (D == 128) return t * 128 + ((cg ^ (t & 7)) << 4);
+  return t * 64 + ((cg ^ ((t >> 1) & 3)) << 4);
+}
+
+// Codes become f16 numbers times 2^-8 (see the head of the file); K's and V's both.
+constexpr float kCodeScale = 256.f;
+
+// Four codes -> (byte 0, byte 2) and (byte 1, byte 3) as f16x2.
+__device__ __forceinline__ void fp8_expand(uint32_t x, uint32_t& even, uint32_t& odd) {
+  even = ((x << 8) & 0x80008000u) | ((x << 7) & 0x3f803f80u);
+  odd = (x & 0x80008000u) | ((x >> 1) & 0x3f803f80u);
+}
 
 // Byte offset of 16-byte chunk `cg` (dims 8cg..8cg+7) of token `t` inside a K or V tile in
 // shared memory, as the 128-byte-swizzled TMA boxes lay it out: either two 64-dim boxes of
@@ -487,12 +524,13 @@ struct ItemInfo {
   int b, h, blk0, nparts, ctx, nblk, part_global, slot0;
 };
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool FP8 = false>
 __global__ void __launch_bounds__(kWarps * 32, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const DecodeArgs a) {
-  using G = Geometry<D>;
+  using G = Geometry<D, FP8>;
   using Mma = ts::MmaOp<T>;
+  constexpr float kOutScale = FP8 ? kCodeScale : 1.f;  // what O's accumulators are divided by
   constexpr int S = G::kStages;
   constexpr int KSTEPS = D / 16;
   constexpr int MTILES = D / 16;
@@ -535,6 +573,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   // slot of the partition}.
   int4* meta =
       reinterpret_cast<int4*>(smem + kWarps * G::kRingBytes + G::kBarBytes) + warp * S * 2;
+  // 8-bit cache: per stage, the block's 16 K scales then its 16 V scales.
+  float* scales = reinterpret_cast<float*>(smem + kWarps * G::kRingBytes + G::kBarBytes +
+                                           G::kMetaBytes) + warp * S * 2 * kBlock;
 
   if (lane == 0) {
     for (int s = 0; s < S; ++s) ts::mbar_init(&bars[s], 1);
@@ -648,10 +689,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       meta[2 * s + 1] = make_int4(p_it.slot0, p_it.nparts | (p_it.h << 16), p_it.ctx,
                                   p_it.part_global);  // nparts < 2^16, h < 2^15
       if (valid) {
-        ts::mbar_arrive_expect_tx(&bars[s], G::kStageBytes);
+        ts::mbar_arrive_expect_tx(&bars[s], G::kStageBytes + G::kScaleBytes);
         const int row = (phys * a.num_kv_heads + p_it.h) * kBlock;
         uint8_t* st = ring + s * G::kStageBytes;
-        if constexpr (G::kOneBox) {
+        if constexpr (FP8) {
+          ts::tma_load_2d(st, &kmap, &bars[s], 0, row);
+          ts::tma_load_2d(st + G::kTileBytes, &vmap, &bars[s], 0, row);
+          ts::bulk_load(scales + s * 2 * kBlock, a.k_scales + row, &bars[s], kBlock * 4);
+          ts::bulk_load(scales + s * 2 * kBlock + kBlock, a.v_scales + row, &bars[s], kBlock * 4);
+        } else if constexpr (G::kOneBox) {
           ts::tma_load_2d(st, &kmap, &bars[s], 0, 2 * row);
           ts::tma_load_2d(st + G::kTileBytes, &vmap, &bars[s], 0, 2 * row);
         } else {
@@ -679,6 +725,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   uint32_t qf[NT][KSTEPS][2];
   float oacc[NT][MTILES][4];
   float m_run[NT][2], l_run[NT][2];
+  float qs[NT][2];  // 8-bit cache: score factor of heads 2t, 2t + 1 (softmax scale, q's scale)
 
   auto start_item = [&](const int4& m0, const int4& m1) {
     cur_item = m0.x;
@@ -696,8 +743,33 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       const bool hv = head < a.group;
       const uint32_t* qrow =
           reinterpret_cast<const uint32_t*>(qb + int64_t(it.h * a.group + head) * D);
+      if constexpr (FP8) {
+        // Words (4t, 4t + 2) and (4t + 1, 4t + 3) of each 16 dims, the order fp8_expand gives K.
+        // The quad holds the head's row: q is multiplied by 2^(14 - exponent of its amax).
+        float2 qv[KSTEPS][2];
+        uint32_t m = 0;
 #pragma unroll
-      for (int ks = 0; ks < KSTEPS; ++ks) {
+        for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            qv[ks][w] = Mma::unpack(hv ? __ldg(qrow + ks * 8 + 2 * t + w) : 0u);
+            m = max(m, max(ts::abs_bits(qv[ks][w].x), ts::abs_bits(qv[ks][w].y)));
+          }
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int e = max(int(m >> 23), 27);  // biased exponent; tiny rows keep a finite factor
+        const float up = __uint_as_float(uint32_t(127 + 14 + 127 - e) << 23);
+        const float down = ldexpf(a.scale_log2 * kCodeScale, e - 127 - 14);
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+          qf[nt][ks][0] = ts::MmaOp<__half>::pack(qv[ks][0].x * up, qv[ks][1].x * up);
+          qf[nt][ks][1] = ts::MmaOp<__half>::pack(qv[ks][0].y * up, qv[ks][1].y * up);
+        }
+        qs[nt][0] = __shfl_sync(0xffffffffu, down, (2 * t) << 2);
+        qs[nt][1] = __shfl_sync(0xffffffffu, down, (2 * t + 1) << 2);
+      }
+#pragma unroll
+      for (int ks = 0; !FP8 && ks < KSTEPS; ++ks) {
         qf[nt][ks][0] = hv ? __ldg(qrow + (ks * 16 + 2 * t) / 2) : 0u;
         qf[nt][ks][1] = hv ? __ldg(qrow + (ks * 16 + 8 + 2 * t) / 2) : 0u;
       }
@@ -739,6 +811,32 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         l_run[nt][j] = l;
       }
+    if (FP8 && it.nparts == 1) {
+      // O's rows are permuted (row g is dim 2g of the tile, row g + 8 dim 2g + 1), so after the
+      // transposes lane (g, t) has dims (4t, 4t + 2) and (4t + 1, 4t + 3) of head g: 8 bytes.
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float i0 = l_run[nt][0] > 0.f ? kOutScale / l_run[nt][0] : l_run[nt][0];
+        const float i1 = l_run[nt][1] > 0.f ? kOutScale / l_run[nt][1] : l_run[nt][1];
+        const int head = nt * 8 + g;
+        bool vec;
+        T* orow = dst_row(0, it.b, it.h * a.group + head, vec);
+#pragma unroll
+        for (int mt = 0; mt < MTILES; ++mt) {
+          const uint32_t ev = movmatrix_pack<Mma>(oacc[nt][mt][0] * i0, oacc[nt][mt][1] * i1);
+          const uint32_t od = movmatrix_pack<Mma>(oacc[nt][mt][2] * i0, oacc[nt][mt][3] * i1);
+          const uint2 w = make_uint2(__byte_perm(ev, od, 0x5410), __byte_perm(ev, od, 0x7632));
+          uint32_t* dst = reinterpret_cast<uint32_t*>(orow) + mt * 8 + 2 * t;
+          if (head < a.group && vec) {
+            *reinterpret_cast<uint2*>(dst) = w;
+          } else if (head < a.group) {
+            dst[0] = w.x;
+            dst[1] = w.y;
+          }
+        }
+      }
+      return;
+    }
     if (it.nparts == 1) {
       // After the transpose lane (g, t) holds, for head nt * 8 + g, the words of dims
       // 16 mt + 2t (lo) and 16 mt + 8 + 2t (hi): a quad covers 16-byte chunk c = 2 mt (+1 for
@@ -794,9 +892,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int mt = 0; mt < MTILES; ++mt) {
-        *reinterpret_cast<float2*>(po + (mt * 16 + g) * NT8 + nt * 8 + 2 * t) =
+        const int d0 = FP8 ? mt * 16 + 2 * g : mt * 16 + g;  // dims of accumulator rows g, g + 8
+        const int d1 = FP8 ? d0 + 1 : d0 + 8;
+        *reinterpret_cast<float2*>(po + d0 * NT8 + nt * 8 + 2 * t) =
             make_float2(oacc[nt][mt][0], oacc[nt][mt][1]);
-        *reinterpret_cast<float2*>(po + (mt * 16 + 8 + g) * NT8 + nt * 8 + 2 * t) =
+        *reinterpret_cast<float2*>(po + d1 * NT8 + nt * 8 + 2 * t) =
             make_float2(oacc[nt][mt][2], oacc[nt][mt][3]);
       }
     if (g == 0) {
@@ -872,7 +972,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
 #pragma unroll
       for (int i = 0; i < PER; ++i) acc[i] += w * __ldcg(src + lane + 32 * i);
     }
-    const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+    const float inv = lsum > 0.f ? kOutScale / lsum : FP8 ? lsum : 0.f;
     // Lane (hd, kq = lane / NT8) holds dims kq + LPH * i of head hd. Gather each 16-byte chunk
     // (8 consecutive dims) of a head into lane kq = chunk % LPH and store it as one vector.
     constexpr int LPH = 32 / NT8;     // lanes per head
@@ -908,6 +1008,88 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     if (lane == 0) a.arrive[it.b * a.num_kv_heads + it.h] = 0;
   };
 
+  // One block of an 8-bit cache: scores, online softmax and PV product.
+  auto block_fp8 = [&](uint32_t kb, uint32_t vb, const float* sc, int nvalid) {
+    using MmaH = ts::MmaOp<__half>;
+    const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
+    float sacc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sacc[nt][j] = 0.f;
+#pragma unroll
+    for (int kp = 0; kp < KSTEPS / 2; ++kp) {
+      uint32_t r[4];  // tokens g and g + 8 of 16 dims, then of the next 16
+      ts::ldmatrix_x4(r, kb + tile_off_fp8<D>(row, kp * 2 + (lane >> 4)));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t af[4];
+        fp8_expand(r[2 * u], af[0], af[2]);
+        fp8_expand(r[2 * u + 1], af[1], af[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          MmaH::run(sacc[nt], af, qf[nt][2 * kp + u][0], qf[nt][2 * kp + u][1]);
+      }
+    }
+    const bool in0 = g < nvalid, in1 = g + 8 < nvalid;
+    const float k0 = sc[g], k1 = sc[g + 8];
+    // In the maximum a scale of 0 counts as 2^-126, so it stays finite; its row weighs nothing.
+    const float v0 = in0 ? sc[kBlock + g] : 1.f, v1 = in1 ? sc[kBlock + g + 8] : 1.f;
+    const float lv0 = __log2f(v0 == 0.f ? 0x1p-126f : v0);
+    const float lv1 = __log2f(v1 == 0.f ? 0x1p-126f : v1);
+    uint32_t pb[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float s00 = in0 ? sacc[nt][0] * (k0 * qs[nt][0]) : -INFINITY;
+      const float s01 = in0 ? sacc[nt][1] * (k0 * qs[nt][1]) : -INFINITY;
+      const float s10 = in1 ? sacc[nt][2] * (k1 * qs[nt][0]) : -INFINITY;
+      const float s11 = in1 ? sacc[nt][3] * (k1 * qs[nt][1]) : -INFINITY;
+      const float t00 = s00 + lv0, t01 = s01 + lv0, t10 = s10 + lv1, t11 = s11 + lv1;
+      float bm0 = fmaxf(t00, t10), bm1 = fmaxf(t01, t11);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, o));
+        bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, o));
+      }
+      const float mn0 = fmaxf(m_run[nt][0], bm0), mn1 = fmaxf(m_run[nt][1], bm1);
+      const bool moved = mn0 != m_run[nt][0] || mn1 != m_run[nt][1];
+      if (__any_sync(0xffffffffu, moved)) {
+        const float c0 = exp2f(m_run[nt][0] - mn0), c1 = exp2f(m_run[nt][1] - mn1);
+        l_run[nt][0] *= c0;
+        l_run[nt][1] *= c1;
+#pragma unroll
+        for (int mt = 0; mt < MTILES; ++mt) {
+          oacc[nt][mt][0] *= c0;
+          oacc[nt][mt][1] *= c1;
+          oacc[nt][mt][2] *= c0;
+          oacc[nt][mt][3] *= c1;
+        }
+        m_run[nt][0] = mn0;
+        m_run[nt][1] = mn1;
+      }
+      l_run[nt][0] += exp2f(s00 - mn0) + exp2f(s10 - mn0);
+      l_run[nt][1] += exp2f(s01 - mn1) + exp2f(s11 - mn1);
+      const uint32_t w0 = MmaH::pack(exp2f(t00 - mn0), exp2f(t01 - mn1));
+      const uint32_t w1 = MmaH::pack(exp2f(t10 - mn0), exp2f(t11 - mn1));
+      pb[nt][0] = ts::movmatrix_trans(v0 == 0.f ? 0u : w0);
+      pb[nt][1] = ts::movmatrix_trans(v1 == 0.f ? 0u : w1);
+    }
+#pragma unroll
+    for (int mp = 0; mp < MTILES / 2; ++mp) {
+      uint32_t r[4];  // dims 2g, 2g + 1 of tokens 2t, 2t + 1 (+ 8), then of the next 16 dims
+      ts::ldmatrix_x4_trans(r, vb + tile_off_fp8<D>(row, mp * 2 + (lane >> 4)));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t af[4];
+        fp8_expand(r[2 * u], af[0], af[1]);
+        fp8_expand(r[2 * u + 1], af[2], af[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          MmaH::run(oacc[nt][2 * mp + u], af, pb[nt][0], pb[nt][1]);
+      }
+    }
+  };
+
   uint32_t k = 0;
   bool failed = false;
 #pragma unroll 1
@@ -929,6 +1111,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       const uint32_t vb = kb + G::kTileBytes;
       const int tok0 = (it.blk0 + md.y) * kBlock;
       const int nvalid = it.ctx - tok0;
+      if constexpr (FP8) {
+        block_fp8(kb, vb, scales + s * 2 * kBlock, nvalid);
+      } else {
 
       // S^T[token][head] = K Q^T
       float sacc[NT][4];
@@ -997,6 +1182,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
             Mma::run(oacc[nt][mt], af, pb[nt][2], pb[nt][3]);
           }
         }
+      }
       }
     }
     __syncwarp();
@@ -1112,11 +1298,26 @@ bool make_pool_map(CUtensorMap* map, const void* pool, int64_t rows, int hd, int
   return r == CUDA_SUCCESS;
 }
 
-template <typename T, int D, int NT>
+// The 8-bit pool [rows][hd]: one box of 16 rows, swizzled by its row length.
+bool make_pool_map_fp8(CUtensorMap* map, const void* pool, int64_t rows, int hd) {
+  auto encode = get_encode();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {cuuint64_t(hd), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(hd)};
+  const cuuint32_t box[2] = {cuuint32_t(hd), cuuint32_t(kBlock)};
+  const cuuint32_t estr[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pool), dims, strides, box,
+                estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, int NT, bool FP8 = false>
 int launch_fast(DecodeArgs a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s,
                 bool plan = true) {
-  using G = Geometry<D>;
-  auto kern = paged_decode_kernel<T, D, NT>;
+  using G = Geometry<D, FP8>;
+  auto kern = paged_decode_kernel<T, D, NT, FP8>;
   // Once per device: later calls may be captured into a CUDA graph.
   static bool attr_done[64] = {};
   int dev = 0;
@@ -1176,7 +1377,8 @@ int paged_attention_portable(void* out, const void* query, int64_t q_stride, con
                              const void* vp, const int32_t* bt, int max_blocks,
                              const int32_t* qsl, const int32_t* cl, int num_seqs, int num_rows,
                              int hq, int hkv, int hd, int bs, int64_t nb, float scale, int dtype,
-                             cudaStream_t s);
+                             cudaStream_t s, const float* k_scales = nullptr,
+                             const float* v_scales = nullptr);
 }
 
 extern "C" size_t ts_paged_decode_workspace_size(int32_t batch, int32_t num_q_heads,
@@ -1198,7 +1400,9 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
                       int32_t max_blocks_per_seq, const int32_t* context_lens, int32_t batch,
                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                       int32_t block_size, int64_t num_blocks, float scale, int32_t dtype,
-                      void* workspace, size_t workspace_bytes, void* stream, bool plan) {
+                      void* workspace, size_t workspace_bytes, void* stream, bool plan,
+                      const float* k_scales = nullptr, const float* v_scales = nullptr) {
+  const bool fp8 = k_scales != nullptr;
   if (ts::dtype_size(dtype) == 0)
     return ts::set_error(TS_ERR_INVALID_ARGUMENT, "paged_decode: bad dtype %d", dtype);
   if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
@@ -1214,12 +1418,15 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
   if (!out || !query || !key_pool || !value_pool || !block_tables || !context_lens)
     return ts::set_error(TS_ERR_INVALID_ARGUMENT, "paged_decode: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // An 8-bit block's scales are copied 64 bytes at a time from 16-byte aligned addresses.
   if (!fast_path(num_q_heads, num_kv_heads, head_dim, block_size, dtype, num_blocks, key_pool,
-                 value_pool, query, query_token_stride, out))
+                 value_pool, query, query_token_stride, out) ||
+      (reinterpret_cast<uint64_t>(k_scales) | reinterpret_cast<uint64_t>(v_scales)) % 16)
     return ts::paged_attention_portable(out, query, query_token_stride, key_pool, value_pool,
                                         block_tables, max_blocks_per_seq, nullptr, context_lens,
                                         batch, batch, num_q_heads, num_kv_heads, head_dim,
-                                        block_size, num_blocks, scale, dtype, s);
+                                        block_size, num_blocks, scale, dtype, s, k_scales,
+                                        v_scales);
   if (batch > 8192)
     return ts::set_error(TS_ERR_UNSUPPORTED, "paged_decode: batch %d above 8192", batch);
   if (int64_t(batch) * max_blocks_per_seq >= (int64_t(1) << 31) ||
@@ -1236,11 +1443,15 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
     return ts::set_error(TS_ERR_MISALIGNED, "paged_decode: workspace not 256-byte aligned");
   CUtensorMap km, vm;
   const int64_t rows = num_blocks * num_kv_heads * kBlock;
-  if (!make_pool_map(&km, key_pool, rows, head_dim, dtype) ||
-      !make_pool_map(&vm, value_pool, rows, head_dim, dtype))
+  if (!(fp8 ? make_pool_map_fp8(&km, key_pool, rows, head_dim) &&
+                  make_pool_map_fp8(&vm, value_pool, rows, head_dim)
+            : make_pool_map(&km, key_pool, rows, head_dim, dtype) &&
+                  make_pool_map(&vm, value_pool, rows, head_dim, dtype)))
     return ts::set_error(TS_ERR_INVALID_ARGUMENT, "paged_decode: cannot encode TMA map of pool");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DecodeArgs a;
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
   a.out = out;
   a.outs = nullptr;
   a.n_out = 0;
@@ -1271,6 +1482,12 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
   a.part_o = reinterpret_cast<float*>(ws + w.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
 #define TS_FAST(T)                                                             \
+  if (fp8 && head_dim == 128)                                                  \
+    return nt == 1 ? launch_fast<T, 128, 1, true>(a, km, vm, s, plan)          \
+                   : launch_fast<T, 128, 2, true>(a, km, vm, s, plan);         \
+  if (fp8)                                                                     \
+    return nt == 1 ? launch_fast<T, 64, 1, true>(a, km, vm, s, plan)           \
+                   : launch_fast<T, 64, 2, true>(a, km, vm, s, plan);          \
   if (head_dim == 128)                                                         \
     return nt == 1 ? launch_fast<T, 128, 1>(a, km, vm, s, plan)                \
                    : launch_fast<T, 128, 2>(a, km, vm, s, plan);               \
@@ -1310,6 +1527,24 @@ extern "C" int ts_paged_decode_planned(void* out, const void* query, int64_t que
                            max_blocks_per_seq, context_lens, batch, num_q_heads, num_kv_heads,
                            head_dim, block_size, num_blocks, scale, dtype, workspace,
                            workspace_bytes, stream, false);
+}
+
+extern "C" int ts_paged_decode_fp8(void* out, const void* query, int64_t query_token_stride,
+                                   const void* key_pool, const void* value_pool,
+                                   const float* key_scales, const float* value_scales,
+                                   const int32_t* block_tables, int32_t max_blocks_per_seq,
+                                   const int32_t* context_lens, int32_t batch, int32_t num_q_heads,
+                                   int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                   int64_t num_blocks, float scale, int32_t dtype, void* workspace,
+                                   size_t workspace_bytes, int32_t reuse_plan, void* stream) {
+  if (batch != 0 && (!key_scales || !value_scales))
+    return ts::set_error(TS_ERR_INVALID_ARGUMENT, "paged_decode_fp8: null scales");
+  if ((reinterpret_cast<uint64_t>(key_scales) | reinterpret_cast<uint64_t>(value_scales)) % 4)
+    return ts::set_error(TS_ERR_MISALIGNED, "paged_decode_fp8: scales not element-aligned");
+  return paged_decode_call(out, query, query_token_stride, key_pool, value_pool, block_tables,
+                           max_blocks_per_seq, context_lens, batch, num_q_heads, num_kv_heads,
+                           head_dim, block_size, num_blocks, scale, dtype, workspace,
+                           workspace_bytes, stream, reuse_plan == 0, key_scales, value_scales);
 }
 
 // --------------------------------------------------------------------------- no-alloc variant
@@ -1411,6 +1646,7 @@ extern "C" int ts_paged_decode_no_alloc(void* out, const void* query, int64_t qu
   // every call; the partial-result slots are always written before they are read.
   uint8_t* ws = static_cast<uint8_t*>(scratch);
   DecodeArgs a;
+  a.k_scales = a.v_scales = nullptr;
   a.out = out;
   a.outs = nullptr;
   a.n_out = 0;
@@ -1534,6 +1770,7 @@ int paged_decode_exchange(bool pull, void* const* dst_outs, int32_t world, int32
     return ts::set_error(TS_ERR_INVALID_ARGUMENT, "paged_decode_peer: cannot encode TMA map of pool");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DecodeArgs a;
+  a.k_scales = a.v_scales = nullptr;
   a.out = nullptr;
   // push: this rank's rows go into every rank's buffer; pull: into its own buffer only, and
   // the other ranks fetch them (ts_gather_peers).

@@ -36,7 +36,8 @@ int paged_attention_portable(void* out, const void* query, int64_t q_stride, con
                              const void* vp, const int32_t* bt, int max_blocks,
                              const int32_t* qsl, const int32_t* cl, int num_seqs, int num_rows,
                              int hq, int hkv, int hd, int bs, int64_t nb, float scale, int dtype,
-                             cudaStream_t s);
+                             cudaStream_t s, const float* k_scales = nullptr,
+                             const float* v_scales = nullptr);
 }
 
 namespace {

@@ -79,6 +79,30 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _p, _p],
     ),
     "ts_silu_mul": (ctypes.c_int, [_p, _p, _i64, _i32, _i32, _p]),
+    "ts_reshape_and_cache_fp8": (
+        ctypes.c_int,
+        [_p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i64, _i32, _p, _p, _p,
+         _p],
+    ),
+    "ts_rotary_and_cache": (
+        ctypes.c_int,
+        [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32,
+         _i64, _i32, _p, _p],
+    ),
+    "ts_read_cache_fp8": (
+        ctypes.c_int,
+        [_p, _p, _p, _p, _p, _p, _p, _i32, _p, _i32, _i64, _i32, _i32, _i32, _i64, _i32, _p, _p],
+    ),
+    "ts_paged_decode_fp8": (
+        ctypes.c_int,
+        [_p, _p, _i64, _p, _p, _p, _p, _p, _i32, _p, _i32, _i32, _i32, _i32, _i32, _i64, _f32,
+         _i32, _p, _sz, _i32, _p],
+    ),
+    "ts_paged_prefill_fp8": (
+        ctypes.c_int,
+        [_p, _p, _i64, _p, _p, _p, _p, _p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32,
+         _i32, _i64, _f32, _i32, _p],
+    ),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -358,3 +382,263 @@ def silu_mul(out: torch.Tensor, gate_up: torch.Tensor) -> None:
     code = load_library().ts_silu_mul(_ptr(out), _ptr(gate_up), rows, two_i // 2,
                                       _dtype(gate_up), _stream())  # fmt: skip
     _check(code, "silu_mul")
+
+
+# ------------------------------------------------------------------------------ 8-bit KV cache
+#
+# Pools [num_blocks, kv_heads, block_size, head_dim] of torch.float8_e4m3fn with float32 scales
+# [num_blocks, kv_heads, block_size]; a row stands for code * scale (include/tokenserve_b200.h).
+# The operators below run on their tensors' device, on its current stream.
+
+
+def _cuda(what: str, *tensors: torch.Tensor | None) -> torch.device:
+    """The one CUDA device all the (present) tensors live on."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or (dev is not None and t.device != dev):
+            raise KernelError(f"{what}: tensors must be on one CUDA device")
+        dev = t.device
+    return dev
+
+
+def _launch(what: str, device: torch.device, fn, *args) -> None:  # type: ignore[no-untyped-def]
+    """Calls ``fn(*args, stream)`` with ``device`` current, on its current stream."""
+    if torch.cuda.current_device() == device.index:
+        _check(fn(*args, _stream()), what)
+    else:
+        with torch.cuda.device(device):
+            _check(fn(*args, _stream()), what)
+
+
+def _fp8_pool_dims(what: str, key_pool: torch.Tensor, value_pool: torch.Tensor,
+                   key_scales: torch.Tensor, value_scales: torch.Tensor
+                   ) -> tuple[int, int, int, int]:  # fmt: skip
+    shape = key_pool.shape
+    for p in (key_pool, value_pool):
+        if (p.dtype != torch.float8_e4m3fn or len(shape) != 4 or p.shape != shape
+                or not p.is_contiguous()):  # fmt: skip
+            raise KernelError(f"{what}: 8-bit pools must be contiguous float8_e4m3fn "
+                              "[num_blocks, kv_heads, block_size, head_dim]")  # fmt: skip
+    for s in (key_scales, value_scales):
+        if s.dtype != torch.float32 or s.shape != shape[:3] or not s.is_contiguous():
+            raise KernelError(f"{what}: scales must be contiguous float32 "
+                              "[num_blocks, kv_heads, block_size]")  # fmt: skip
+    return shape[0], shape[1], shape[2], shape[3]
+
+
+def _int_array(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, n: int) -> None:
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise KernelError(f"{what}: {name} must be a contiguous {dtype} of {n} entries, got "
+                          f"{t.dtype} {tuple(t.shape)}")  # fmt: skip
+
+
+def _error_flag(what: str, t: torch.Tensor | None) -> None:
+    if t is not None and (t.dtype != torch.int32 or t.numel() < 1):
+        raise KernelError(f"{what}: error_flag must be an int32 tensor")
+
+
+def _tables(what: str, t: torch.Tensor, rows: int) -> int:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != rows or not t.is_contiguous():
+        raise KernelError(f"{what}: block_tables must be contiguous int32 [{rows}, max_blocks]")
+    return t.shape[1]
+
+
+def _attention_rows(what: str, out: torch.Tensor, query: torch.Tensor, kv_heads: int,
+                    head_dim: int) -> tuple[int, int]:  # fmt: skip
+    """Query heads and token stride of ``query [T, Hq, D]``, checked against ``out``."""
+    if query.dim() != 3 or query.shape[1] == 0 or query.shape[1] % kv_heads:
+        raise KernelError(f"{what}: query must be [tokens, heads, {head_dim}] with a multiple of "
+                          f"{kv_heads} heads, got {tuple(query.shape)}")  # fmt: skip
+    stride = _rows(query, query.shape[1], head_dim, f"{what}: query")
+    if out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+        raise KernelError(f"{what}: out must be contiguous, of the query's shape and dtype")
+    return query.shape[1], max(stride, query.shape[1] * head_dim) if query.shape[0] < 2 else stride
+
+
+def reshape_and_cache_fp8(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    *,
+    token_tags: torch.Tensor | None = None,
+    tag_pool: torch.Tensor | None = None,
+    error_flag: torch.Tensor | None = None,
+) -> None:
+    """K1 into an 8-bit cache: ``key/value [T, Hkv, D]`` are quantised row by row as they are
+    written at ``slot_mapping [T]`` (int64, distinct; negative: skipped)."""
+    what = "reshape_and_cache_fp8"
+    nb, h, bs, d = _fp8_pool_dims(what, key_pool, value_pool, key_scales, value_scales)
+    dev = _cuda(what, key, value, key_pool, value_pool, key_scales, value_scales, slot_mapping,
+                token_tags, tag_pool, error_flag)  # fmt: skip
+    if key.dtype != value.dtype or key.shape != value.shape:
+        raise KernelError(f"{what}: key and value must have one shape and dtype")
+    n = key.shape[0]
+    ks, vs = _rows(key, h, d, f"{what}: key"), _rows(value, h, d, f"{what}: value")
+    if n == 1:  # a single row's stride says nothing
+        ks, vs = max(ks, h * d), max(vs, h * d)
+    _int_array(what, "slot_mapping", slot_mapping, torch.int64, n)
+    if token_tags is not None:
+        _int_array(what, "token_tags", token_tags, torch.int32, n)
+    if tag_pool is not None:
+        _int_array(what, "tag_pool", tag_pool, torch.int32, nb * bs)
+    _error_flag(what, error_flag)
+    _launch(what, dev, load_library().ts_reshape_and_cache_fp8,
+            _ptr(key), _ptr(value), ks, vs, _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
+            _ptr(value_scales), _ptr(slot_mapping), n, h, d, bs, nb, _dtype(key),
+            _ptr(token_tags), _ptr(tag_pool), _ptr(error_flag))  # fmt: skip
+
+
+def rotary_and_cache(
+    qkv: torch.Tensor,
+    q_out: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    num_q_heads: int,
+    num_kv_heads: int,
+    *,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
+    interleaved: bool = False,
+    attention_scaling: float = 1.0,
+    error_flag: torch.Tensor | None = None,
+) -> None:
+    """Rotary positions on q and k of fused ``qkv [T, (Hq + 2 Hkv) * D]``; q -> ``q_out [T, Hq,
+    D]``, k and v -> the pools, quantised where ``key_scales`` and ``value_scales`` are given.
+
+    The first ``2 * len(inv_freq)`` dims of each head turn by ``positions * inv_freq`` (any
+    frequencies), in pairs ``(i, i + len)`` or, ``interleaved``, ``(2i, 2i + 1)``;
+    ``attention_scaling`` multiplies cos and sin. Computed in fp32, rounded once.
+    """
+    what = "rotary_and_cache"
+    if (key_scales is None) != (value_scales is None):
+        raise KernelError(f"{what}: key_scales and value_scales go together")
+    if key_scales is not None:
+        nb, hkv, bs, d = _fp8_pool_dims(what, key_pool, value_pool, key_scales, value_scales)
+    else:
+        nb, hkv, bs, d = _pool_dims(key_pool)
+        if (value_pool.shape != key_pool.shape or not value_pool.is_contiguous()
+                or key_pool.dtype != qkv.dtype or value_pool.dtype != qkv.dtype):  # fmt: skip
+            raise KernelError(f"{what}: pools must be contiguous, of one shape and of qkv's dtype")
+    dev = _cuda(what, qkv, q_out, key_pool, value_pool, key_scales, value_scales, slot_mapping,
+                positions, inv_freq, error_flag)  # fmt: skip
+    n, width = qkv.shape if qkv.dim() == 2 else (-1, -1)
+    if hkv != num_kv_heads or num_q_heads <= 0 or width != (num_q_heads + 2 * hkv) * d or (
+            qkv.stride(1) != 1):  # fmt: skip
+        raise KernelError(f"{what}: qkv must be [tokens, (q heads + 2 kv heads) * head_dim] with "
+                          "contiguous rows and the pool's kv heads")  # fmt: skip
+    if q_out.shape != (n, num_q_heads, d) or q_out.dtype != qkv.dtype or not q_out.is_contiguous():
+        raise KernelError(f"{what}: q_out must be a contiguous [tokens, q heads, head_dim] of "
+                          "qkv's dtype")  # fmt: skip
+    _int_array(what, "slot_mapping", slot_mapping, torch.int64, n)
+    _int_array(what, "positions", positions, torch.int64, n)
+    half = inv_freq.numel()
+    _int_array(what, "inv_freq", inv_freq, torch.float32, half)
+    _error_flag(what, error_flag)
+    _launch(what, dev, load_library().ts_rotary_and_cache,
+            _ptr(qkv), qkv.stride(0) if n > 1 else width, _ptr(q_out), _ptr(key_pool),
+            _ptr(value_pool), _ptr(key_scales), _ptr(value_scales), _ptr(slot_mapping),
+            _ptr(positions), _ptr(inv_freq), n, num_q_heads, hkv, d, 2 * half, int(interleaved),
+            float(attention_scaling), bs, nb, _dtype(qkv), _ptr(error_flag))  # fmt: skip
+
+
+def read_cache_fp8(
+    key_out: torch.Tensor,
+    value_out: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    token_start_loc: torch.Tensor,
+    error_flag: torch.Tensor | None = None,
+) -> None:
+    """Reads an 8-bit cache back: position p of sequence s -> row ``token_start_loc[s] + p`` of
+    ``key_out`` and ``value_out [T, Hkv, D]`` (float32, float16 or bfloat16)."""
+    what = "read_cache_fp8"
+    nb, h, bs, d = _fp8_pool_dims(what, key_pool, value_pool, key_scales, value_scales)
+    dev = _cuda(what, key_out, value_out, key_pool, value_pool, key_scales, value_scales,
+                block_tables, token_start_loc, error_flag)  # fmt: skip
+    n = key_out.shape[0] if key_out.dim() == 3 else -1
+    for t in (key_out, value_out):
+        if t.shape != (n, h, d) or t.dtype != key_out.dtype or not t.is_contiguous():
+            raise KernelError(f"{what}: outputs must be contiguous [tokens, {h}, {d}] of one dtype")
+    seqs = block_tables.shape[0]
+    width = _tables(what, block_tables, seqs)
+    _int_array(what, "token_start_loc", token_start_loc, torch.int32, seqs + 1)
+    _error_flag(what, error_flag)
+    _launch(what, dev, load_library().ts_read_cache_fp8,
+            _ptr(key_out), _ptr(value_out), _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
+            _ptr(value_scales), _ptr(block_tables), width, _ptr(token_start_loc), seqs, n, h, d,
+            bs, nb, _dtype(key_out), _ptr(error_flag))  # fmt: skip
+
+
+def paged_decode_fp8(
+    out: torch.Tensor,
+    query: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    scale: float,
+    workspace: torch.Tensor | None,
+    reuse_plan: bool = False,
+) -> None:
+    """K2 over an 8-bit cache: ``query [B, Hq, D]`` -> ``out``; see :func:`paged_decode`. The
+    workspace is sized by :func:`decode_workspace_size` with the query's dtype."""
+    what = "paged_decode_fp8"
+    nb, hkv, bs, d = _fp8_pool_dims(what, key_pool, value_pool, key_scales, value_scales)
+    dev = _cuda(what, out, query, key_pool, value_pool, key_scales, value_scales, block_tables,
+                context_lens, workspace)  # fmt: skip
+    hq, qs = _attention_rows(what, out, query, hkv, d)
+    b = query.shape[0]
+    width = _tables(what, block_tables, b)
+    _int_array(what, "context_lens", context_lens, torch.int32, b)
+    if workspace is not None and not workspace.is_contiguous():
+        raise KernelError(f"{what}: workspace must be contiguous")
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _launch(what, dev, load_library().ts_paged_decode_fp8,
+            _ptr(out), _ptr(query), qs, _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
+            _ptr(value_scales), _ptr(block_tables), width, _ptr(context_lens), b, hq, hkv, d, bs,
+            nb, float(scale), _dtype(query), _ptr(workspace), ws_bytes,
+            int(reuse_plan))  # fmt: skip
+
+
+def paged_prefill_fp8(
+    out: torch.Tensor,
+    query: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    context_lens: torch.Tensor,
+    max_query_len: int,
+    scale: float,
+) -> None:
+    """K3 over an 8-bit cache: causal chunk attention, ``query [T, Hq, D]`` -> ``out``."""
+    what = "paged_prefill_fp8"
+    nb, hkv, bs, d = _fp8_pool_dims(what, key_pool, value_pool, key_scales, value_scales)
+    dev = _cuda(what, out, query, key_pool, value_pool, key_scales, value_scales, block_tables,
+                query_start_loc, context_lens)  # fmt: skip
+    hq, qs = _attention_rows(what, out, query, hkv, d)
+    seqs = context_lens.numel()
+    width = _tables(what, block_tables, seqs)
+    _int_array(what, "context_lens", context_lens, torch.int32, seqs)
+    _int_array(what, "query_start_loc", query_start_loc, torch.int32, seqs + 1)
+    _launch(what, dev, load_library().ts_paged_prefill_fp8,
+            _ptr(out), _ptr(query), qs, _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
+            _ptr(value_scales), _ptr(block_tables), width, _ptr(query_start_loc),
+            _ptr(context_lens), seqs, query.shape[0], int(max_query_len), hq, hkv, d, bs, nb,
+            float(scale), _dtype(query))  # fmt: skip
