@@ -1,5 +1,31 @@
 // Chunked-prefill attention (causal) over the 8-bit paged cache (fp8.cuh).
-#include "common.cuh"
+//
+// Query row j of a sequence whose step ends at context_lens[s] sits at position
+// context_lens[s] - q_len + j and sees positions 0..that one; out = softmax(q k^T scale) v.
+//
+// bf16/fp16 queries, head_dim 64 or 128, block 16: tcgen05 kernel. It is bound by the tensor cores
+// and by the exponentials (one per score), so the cache's 8 bits must cost neither of them:
+//   * CTA = (sequence, KV head, pair of query tiles); a tile's 128 rows are 128/G tokens x the G
+//     query heads of the KV head, so a converted K/V tile serves 256 rows.
+//   * warps 8-11 (converters): read a 128-token tile's codes and scales from global memory a tile
+//     ahead into registers, multiply each row by its scale and store it as fp16 in the swizzled
+//     layout the MMAs read. Values are taken relative to the tile's largest scale (K) or the
+//     largest so far (V) times 2^-7, so they fill fp16's range whatever their magnitude; the
+//     scale is split into two fp16 parts, so a value is rounded once, to 2^-11 of itself. K's
+//     reference is a factor on the tile's scores; when V's grows, O is rescaled.
+//   * warps 0-3 / 4-7 (softmax, one warpgroup per query tile, thread = row): q's row is scaled by a
+//     power of two into fp16's range and written to shared memory; then per tile S from TMEM, the
+//     row's maximum, 2^(s - m), P in fp16 (11 bits) back to TMEM over S. The maximum is kept while
+//     no score exceeds it by 2^8, so O is rarely rescaled; sums are fp32.
+//   * warp 13, one lane: tcgen05.mma, S_x = Q_x K^T and O_x += P_x V, in the order PV_A(j),
+//     QK_A(j+1), PV_B(j), QK_B(j+1), so one tile's softmax runs under the other's MMAs. A QK's
+//     commit covers the PV before it, so S of tile j + 1 also says that O holds tile j.
+// A page outside the pool is skipped (its columns are masked). A V row with a NaN scale is stored
+// as zeros and its column's weight set to NaN for the rows that see it, so rows before it in the
+// chunk stay clean. Tokens past the last visible key are stored as zeros: their slots may hold
+// anything. Other shapes and fp32 queries run on CUDA cores (attention_portable.cu).
+#include "fp8.cuh"
+#include "tcgen05.cuh"
 
 namespace ts {
 int paged_attention_portable(void* out, const void* query, int64_t q_stride, const void* kp,
@@ -8,6 +34,564 @@ int paged_attention_portable(void* out, const void* query, int64_t q_stride, con
                              int hq, int hkv, int hd, int bs, int64_t nb, float scale, int dtype,
                              cudaStream_t s, const float* k_scales, const float* v_scales);
 }
+
+namespace {
+
+constexpr int kRows = 128;    // query rows per tile (M)
+constexpr int kKvTile = 128;  // KV tokens per tile (N of QK, K of PV)
+constexpr int kBlock = 16;    // tokens per KV block
+constexpr int kHalfBytes = 128 * 128;  // 128 rows x 64 fp16 columns
+constexpr int kQTiles = 2;
+constexpr int kStages = 2;  // K ring, and V ring
+constexpr int kInfos = 4;   // tile descriptions: a softmax trails the converters by under 4 tiles
+constexpr int kThreads = 512;
+// Registers a thread after setmaxnreg: two softmax warpgroups, the converters, the rest. Their sum
+// is what the block is launched with, 4 x 128.
+constexpr int kRegsSoftmax = 176, kRegsConvert = 112, kRegsRest = 48;
+static_assert(2 * kRegsSoftmax + kRegsConvert + kRegsRest <= 4 * 128, "register split");
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleSlack = 8.f;  // keep a stale row max unless exceeded by 2^8
+constexpr uint32_t kTmemCols = 512;   // S_A [0,128), S_B [128,256), O_A [256,384), O_B [384,512)
+constexpr float kRefScale = 128.f;    // fp16 values are code * scale / ref * 128 <= 57344
+
+struct Args {
+  void* out;
+  const void* query;
+  int64_t q_stride;
+  const uint8_t* key_pool;
+  const uint8_t* value_pool;
+  const float* key_scales;
+  const float* value_scales;
+  const int32_t* block_tables;
+  const int32_t* qsl;
+  const int32_t* context_lens;
+  int max_blocks, num_q_heads, num_kv_heads, group;
+  int tq;  // query tokens per tile
+  int64_t num_blocks;
+  float scale_log2;
+};
+
+// What the softmax of a KV tile has to know: references of K and V, and the columns to mask (page
+// outside the pool) or to spoil (V row NaN), if any.
+struct TileInfo {
+  float ref_k, ref_v;
+  uint32_t any, pad;
+  uint32_t skip[4], spoil[4];
+};
+
+struct Shared {
+  uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+  uint64_t s_full[kQTiles], p_full[kQTiles], pv_done[kQTiles], drain;
+  TileInfo info[kInfos];
+  uint32_t tmem;
+  int abort;
+};
+
+template <int D>
+struct Geo {
+  static constexpr int kTileBytes = 128 * D * 2;
+  static constexpr int kTiles = (kQTiles + 2 * kStages) * kTileBytes;
+  static constexpr int kSmemBytes = kTiles + int(sizeof(Shared)) + 1024;
+};
+
+// Bounded wait that also gives up as soon as another role has aborted.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, volatile int* abort) {
+  for (long long i = 0; i < ts::kMaxSpins; ++i) {
+    if (ts::mbar_try_wait(bar, phase)) return true;
+    if ((i & 255) == 255 && *abort) return false;
+  }
+  *abort = 1;
+  return false;
+}
+
+// The same for a whole warp, with one answer.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase, volatile int* abort) {
+  return __all_sync(0xffffffffu, wait_bar(bar, phase, abort));
+}
+
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// One converter warp's view of the KV tiles of a (sequence, KV head): it converts tokens 32 w ..
+// 32 w + 31 of every tile.
+template <int D>
+struct Converter {
+  static constexpr int kLanes = D / 16;        // lanes per row, 16 codes each
+  static constexpr int kRpi = 32 / kLanes;     // rows per load instruction
+  static constexpr int kLoads = 32 / kRpi;     // load instructions per item
+  const Args& a;
+  const int32_t* table;
+  int h, n_kv, total_blk, w, lane;
+  int next_table;        // lane b < 8: block b of the next tile to be looked up (-1 none, -2 bad)
+  uint4 raw_k[kLoads], raw_v[kLoads];
+  float ks[4], vs[4];    // scales of token 32 ((w + i) % 4) + lane: [0] is this lane's own row
+  uint32_t bad;          // bit i: that token is in a page outside the pool
+  float ref_v;           // largest V scale so far
+
+  __device__ __forceinline__ void look_up(int t) {
+    const int b = t * (kKvTile / kBlock) + lane;
+    next_table = -1;
+    if (lane < kKvTile / kBlock && b < total_blk) {
+      const int phys = __ldg(table + b);
+      next_table = phys >= 0 && int64_t(phys) < a.num_blocks ? phys : -2;
+    }
+  }
+  // Row of this KV head at block `phys`, offset `off`.
+  __device__ __forceinline__ int64_t row(int phys, int off) const {
+    return (int64_t(phys) * a.num_kv_heads + h) * kBlock + off;
+  }
+  __device__ __forceinline__ void load_codes(const uint8_t* pool, const int tab, uint4 (&raw)[kLoads]) {
+    const int own[2] = {__shfl_sync(0xffffffffu, tab, 2 * w), __shfl_sync(0xffffffffu, tab, 2 * w + 1)};
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * kRpi + lane / kLanes;  // row of the warp's 32
+      const int phys = own[(i * kRpi) / kBlock];
+      raw[i] = phys >= 0 ? __ldg(reinterpret_cast<const uint4*>(pool + row(phys, r % kBlock) * D) +
+                                 lane % kLanes)
+                         : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void load_scales(int t, const int tab) {
+    bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int g = (w + i) & 3;
+      const int phys = __shfl_sync(0xffffffffu, tab, 2 * g + lane / kBlock);
+      const bool in = t * kKvTile + 32 * g + lane < n_kv;
+      if (in && phys == -2) bad |= 1u << i;
+      const int64_t r = row(phys, lane % kBlock);
+      ks[i] = in && phys >= 0 ? __ldg(a.key_scales + r) : 0.f;
+      vs[i] = in && phys >= 0 ? __ldg(a.value_scales + r) : 0.f;
+    }
+  }
+  // Largest finite scale of the tile.
+  __device__ __forceinline__ float top(const float (&sc)[4]) const {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, isfinite(sc[i]) ? sc[i] : 0.f);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+  }
+  // raw -> fp16 rows at `dst` (a tile in shared memory, 128-byte swizzled halves of 64 columns).
+  // `f`: this lane's row's factor; `zero`: its codes are dropped.
+  __device__ __forceinline__ void convert(const uint4 (&raw)[kLoads], float f, bool zero, uint8_t* dst) {
+    const __half hi = __float2half_rn(f);
+    const __half lo = __float2half_rn(f - __half2float(hi));
+    const uint32_t my = uint32_t(__half_as_ushort(hi)) | (uint32_t(__half_as_ushort(lo)) << 16);
+    const uint32_t dropped = __ballot_sync(0xffffffffu, zero);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * kRpi + lane / kLanes;
+      const uint32_t s2 = __shfl_sync(0xffffffffu, my, r);
+      const __half2 h2 = __half2half2(__ushort_as_half(static_cast<unsigned short>(s2 & 0xffffu)));
+      const __half2 l2 = __half2half2(__ushort_as_half(static_cast<unsigned short>(s2 >> 16)));
+      uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      if (dropped >> r & 1) word[0] = word[1] = word[2] = word[3] = 0;
+      uint32_t v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const __half2 c = ts::fp8_half2(word[k / 2] >> (16 * (k & 1)));
+        const __half2 x = __hfma2(c, h2, __hmul2(c, l2));
+        v[k] = *reinterpret_cast<const uint32_t*>(&x);
+      }
+      const int c = lane % kLanes, row_in_tile = 32 * w + r;
+      // Chunks 2 (c % 4) and + 1 of half c / 4; the halves' lanes store them in opposite order, so
+      // the eight lanes of a row never meet in a bank.
+      const int first = c / 4;
+      uint8_t* base = dst + (c / 4) * kHalfBytes + row_in_tile * 128;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bool second = (u ^ first) != 0;
+        const int chunk = (2 * (c % 4) + int(second)) ^ (row_in_tile & 7);
+        *reinterpret_cast<uint4*>(base + chunk * 16) =
+            second ? make_uint4(v[4], v[5], v[6], v[7]) : make_uint4(v[0], v[1], v[2], v[3]);
+      }
+    }
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Args a) {
+  using G = Geo<D>;
+  using Mma = ts::MmaOp<T>;
+  const int pair = blockIdx.x, h = blockIdx.y, seq = blockIdx.z;
+  const int q0 = a.qsl[seq];
+  const int q_len = a.qsl[seq + 1] - q0;
+  const int tile0 = pair * kQTiles;
+  if (tile0 * a.tq >= q_len) return;
+  const int ctx = min(a.context_lens[seq], a.max_blocks * kBlock);
+  const int p0 = ctx - q_len;  // position of the first query row; negative rows see nothing
+  int n_t[kQTiles];            // KV tiles each query tile needs
+  int n_kv = 0;                // keys the CTA's last query row sees
+#pragma unroll
+  for (int x = 0; x < kQTiles; ++x) {
+    const int first = (tile0 + x) * a.tq;
+    const int n = first < q_len ? max(0, p0 + min(q_len, first + a.tq)) : 0;
+    n_t[x] = (n + kKvTile - 1) / kKvTile;
+    n_kv = max(n_kv, n);
+  }
+  const int n_max = (n_kv + kKvTile - 1) / kKvTile;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = ts::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023) & ~1023u) - raw_addr);
+  auto sQ = [&](int x) { return smem + x * G::kTileBytes; };
+  auto sK = [&](int st) { return smem + (kQTiles + st) * G::kTileBytes; };
+  auto sV = [&](int st) { return smem + (kQTiles + kStages + st) * G::kTileBytes; };
+  Shared* sh = reinterpret_cast<Shared*>(smem + G::kTiles);
+  volatile int* abort = &sh->abort;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    ts::mbar_init(&sh->q_full, 128 * kQTiles);
+    for (int i = 0; i < kStages; ++i) {
+      ts::mbar_init(&sh->k_full[i], 128);
+      ts::mbar_init(&sh->k_empty[i], 1);
+      ts::mbar_init(&sh->v_full[i], 128);
+      ts::mbar_init(&sh->v_empty[i], 1);
+    }
+    for (int x = 0; x < kQTiles; ++x) {
+      ts::mbar_init(&sh->s_full[x], 1);
+      ts::mbar_init(&sh->p_full[x], 128);
+      ts::mbar_init(&sh->pv_done[x], 1);
+    }
+    ts::mbar_init(&sh->drain, 1);
+    sh->abort = 0;
+    ts::fence_mbar_init();
+  }
+  if (warp == 0) {
+    ts::tc::tmem_alloc(&sh->tmem, kTmemCols);
+    ts::tc::tmem_relinquish();
+  }
+  ts::tc::fence_before_sync();
+  __syncthreads();
+  ts::tc::fence_after_sync();
+  const uint32_t tmem = sh->tmem;
+
+  if (warp >= 12) {
+    regs_dec<kRegsRest>();
+    if (warp == 13 && lane == 0 && n_max > 0) {
+      // ---------------------------------------------------------- MMA issuer
+      constexpr uint32_t idesc_qk = ts::tc::idesc_f16(false, kRows, kKvTile, false);
+      constexpr uint32_t idesc_pv = ts::tc::idesc_f16(false, kRows, D, true);
+      // The last query tile to use KV tile j releases its K (after QK) and V (after PV).
+      auto last_user = [&](int j) { return j < n_t[1] ? 1 : 0; };
+      const uint64_t dq0 = ts::tc::smem_desc_sw128(ts::smem_u32(sQ(0)), 16, 1024);
+      const uint64_t dk0 = ts::tc::smem_desc_sw128(ts::smem_u32(sK(0)), 16, 1024);
+      const uint64_t dv0 = ts::tc::smem_desc_sw128(ts::smem_u32(sV(0)), kHalfBytes, 1024);
+      auto issue_qk = [&](int x, int j) -> bool {
+        const int st = j % kStages;
+        if (!wait_bar(&sh->k_full[st], (j / kStages) & 1, abort)) return false;
+        ts::tc::fence_after_sync();
+        const uint64_t dq = dq0 + uint64_t((x * G::kTileBytes) >> 4);
+        const uint64_t dk = dk0 + uint64_t((st * G::kTileBytes) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off16 = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
+          ts::tc::mma_ss(tmem + x * 128, dq + off16, dk + off16, idesc_qk, kk > 0);
+        }
+        ts::tc::commit(&sh->s_full[x]);
+        if (x == last_user(j) && j + kStages < n_max) ts::tc::commit(&sh->k_empty[st]);
+        return true;
+      };
+      bool ok = wait_bar(&sh->q_full, 0, abort);
+      for (int x = 0; ok && x < kQTiles; ++x)
+        if (n_t[x] > 0) ok = issue_qk(x, 0);
+      for (int j = 0; ok && j < n_max; ++j) {
+        const int st = j % kStages;
+        for (int x = 0; ok && x < kQTiles; ++x) {
+          if (j >= n_t[x]) continue;
+          if (!wait_bar(&sh->p_full[x], j & 1, abort) ||
+              !wait_bar(&sh->v_full[st], (j / kStages) & 1, abort)) {
+            ok = false;
+            break;
+          }
+          ts::tc::fence_after_sync();
+          const uint64_t dv = dv0 + uint64_t((st * G::kTileBytes) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kKvTile / 16; ++kk)
+            ts::tc::mma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8,
+                           dv + uint64_t((kk * 2048) >> 4), idesc_pv, j > 0 || kk > 0);
+          if (j + 1 == n_t[x]) ts::tc::commit(&sh->pv_done[x]);
+          if (x == last_user(j) && j + kStages < n_max) ts::tc::commit(&sh->v_empty[st]);
+          if (j + 1 < n_t[x]) ok = issue_qk(x, j + 1);
+        }
+      }
+      if (*abort) {  // the MMAs in flight end before shared and tensor memory are released
+        ts::tc::commit(&sh->drain);
+        ts::mbar_wait_bounded(&sh->drain, 0);
+      }
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------ converters
+    regs_dec<kRegsConvert>();
+    Converter<D> cv{a, a.block_tables + int64_t(seq) * a.max_blocks, h, n_kv,
+                    (n_kv + kBlock - 1) / kBlock, warp - 8, lane};
+    cv.ref_v = 0.f;
+    if (n_max > 0) {
+      cv.look_up(0);
+      cv.load_scales(0, cv.next_table);
+      cv.load_codes(a.key_pool, cv.next_table, cv.raw_k);
+      cv.load_codes(a.value_pool, cv.next_table, cv.raw_v);
+      cv.look_up(1);
+    }
+    for (int t = 0; t < n_max; ++t) {
+      const int st = t % kStages;
+      const float ref_k = cv.top(cv.ks);
+      cv.ref_v = fmaxf(cv.ref_v, cv.top(cv.vs));
+      const float k_own = cv.ks[0], v_own = cv.vs[0];
+      const bool out_of_reach = t * kKvTile + 32 * cv.w + lane >= n_kv;
+      if (cv.w == 0) {
+        TileInfo* info = &sh->info[t % kInfos];
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t skip = __ballot_sync(0xffffffffu, cv.bad >> i & 1);
+          const uint32_t spoil = __ballot_sync(0xffffffffu, !isfinite(cv.vs[i]));
+          any |= skip | spoil;
+          if (lane == 0) {
+            info->skip[i] = skip;
+            info->spoil[i] = spoil;
+          }
+        }
+        if (lane == 0) {
+          info->ref_k = ref_k;
+          info->ref_v = cv.ref_v;
+          info->any = any;
+        }
+      }
+      const int tab = cv.next_table;  // of tile t + 1
+      if (t >= kStages && !wait_warp(&sh->k_empty[st], ((t - kStages) / kStages) & 1, abort)) break;
+      cv.convert(cv.raw_k, ref_k > 0.f ? k_own / ref_k * kRefScale : k_own, out_of_reach, sK(st));
+      ts::fence_proxy_async_smem();
+      ts::mbar_arrive(&sh->k_full[st]);
+      if (t + 1 < n_max) {
+        cv.load_scales(t + 1, tab);
+        cv.load_codes(a.key_pool, tab, cv.raw_k);
+        cv.look_up(t + 2);
+      }
+      if (t >= kStages && !wait_warp(&sh->v_empty[st], ((t - kStages) / kStages) & 1, abort)) break;
+      const bool drop = out_of_reach || !isfinite(v_own);
+      cv.convert(cv.raw_v, drop || cv.ref_v == 0.f ? 0.f : v_own / cv.ref_v * kRefScale, drop, sV(st));
+      ts::fence_proxy_async_smem();
+      ts::mbar_arrive(&sh->v_full[st]);
+      if (t + 1 < n_max) cv.load_codes(a.value_pool, tab, cv.raw_v);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax / epilogue
+    regs_inc<kRegsSoftmax>();
+    const int x = warp / 4;               // query tile of this warpgroup
+    const int r = threadIdx.x - 128 * x;  // tile row == TMEM lane
+    const int n_x = n_t[x];
+    const int i = r / a.group, g = r - i * a.group;
+    const int qi = (tile0 + x) * a.tq + i;
+    const bool row_valid = i < a.tq && qi < q_len;
+    const int pos = row_valid ? p0 + qi : p0 + q_len - 1;
+    const int64_t orow = int64_t(q0 + qi) * a.num_q_heads + h * a.group + g;
+    const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t s_col = x * 128, o_col = 256 + x * 128;
+
+    // q's row times 2^(14 - exponent of its amax), in fp16; `sl` undoes it (times the softmax
+    // scale, whose sign goes with q).
+    float sl;
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(
+          static_cast<const T*>(a.query) + int64_t(q0 + qi) * a.q_stride +
+          int64_t(h * a.group + g) * D);
+      uint4 v[D / 8];
+      uint32_t m = 0;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        v[c] = row_valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        const uint32_t wds[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = Mma::unpack(wds[k]);
+          m = max(m, max(ts::abs_bits(f.x), ts::abs_bits(f.y)));
+        }
+      }
+      const int e = max(int(m >> 23), 27);  // biased exponent; tiny rows keep a finite factor
+      const float up = copysignf(__uint_as_float(uint32_t(127 + 14 + 127 - e) << 23), a.scale_log2);
+      sl = ldexpf(fabsf(a.scale_log2) / kRefScale, e - 127 - 14);
+      uint8_t* dst = sQ(x) + r * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint32_t wds[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = Mma::unpack(wds[k]);
+          o[k] = pack_half2(f.x * up, f.y * up);
+        }
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalfBytes + (((c & 7) ^ (r & 7)) << 4)) =
+            make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      ts::fence_proxy_async_smem();
+      ts::mbar_arrive(&sh->q_full);
+    }
+
+    float m_run = -INFINITY, l_run = 0.f, ref_v = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n_x; ++j) {
+      if (!wait_warp(&sh->s_full[x], j & 1, abort)) {
+        ok = false;
+        break;
+      }
+      ts::tc::fence_after_sync();
+      uint32_t sr[128];
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4) {
+        uint32_t (&chunk)[32] = *reinterpret_cast<uint32_t(*)[32]>(sr + 32 * c4);
+        ts::tc::tmem_ld32(lane_base + s_col + c4 * 32, chunk);
+      }
+      const volatile TileInfo* info = &sh->info[j % kInfos];
+      const float slj = fmaxf(sl * info->ref_k, 0x1p-126f);  // > 0, so that -inf stays -inf
+      const float ref_old = ref_v;
+      ref_v = info->ref_v;
+      const bool odd_columns = info->any != 0;
+      ts::tc::wait_ld();
+      const int limit = pos - j * kKvTile;  // columns c <= limit are visible
+      if (limit < kKvTile - 1) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (c > limit) sr[c] = __float_as_uint(-INFINITY);
+      }
+      if (odd_columns) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) {
+          if (info->skip[c / 32] >> (c % 32) & 1) sr[c] = __float_as_uint(-INFINITY);
+          if ((info->spoil[c / 32] >> (c % 32) & 1) && c <= limit) sr[c] = 0x7fc00000u;
+        }
+      }
+      float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 128; c += 4) {
+        mx = max3f(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        my = max3f(my, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+      }
+      const float m_tile = fmaxf(mx, my) * slj;
+      float corr = 1.f;
+      if (m_tile > m_run + kRescaleSlack || m_run == -INFINITY) {
+        corr = m_run == -INFINITY ? 1.f : ex2(m_run - m_tile);  // nothing summed yet: 0 either way
+        m_run = m_tile;
+      }
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+      float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+      for (int c = 0; c < 128; c += 2) {
+        const float p = ex2(fmaf(__uint_as_float(sr[c]), slj, -m_use));
+        const float q = ex2(fmaf(__uint_as_float(sr[c + 1]), slj, -m_use));
+        sum0 += p;
+        sum1 += q;
+        sr[c / 2] = pack_half2(p, q);
+      }
+#pragma unroll
+      for (int c2 = 0; c2 < 2; ++c2) {
+        const uint32_t (&chunk)[32] = *reinterpret_cast<const uint32_t(*)[32]>(sr + 32 * c2);
+        ts::tc::tmem_st32(lane_base + s_col + c2 * 32, chunk);
+      }
+      l_run = l_run * corr + (sum0 + sum1);
+      // O is in units of V's reference: it shrinks when that grows.
+      const float corr_o = j > 0 && ref_v != ref_old ? corr * (ref_old / ref_v) : corr;
+      if (j > 0 && __any_sync(0xffffffffu, corr_o != 1.f)) {
+#pragma unroll
+        for (int c4 = 0; c4 < D / 32; ++c4) {
+          uint32_t rr[32];
+          ts::tc::tmem_ld32(lane_base + o_col + c4 * 32, rr);
+          ts::tc::wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) rr[c] = __float_as_uint(__uint_as_float(rr[c]) * corr_o);
+          ts::tc::tmem_st32(lane_base + o_col + c4 * 32, rr);
+        }
+      }
+      ts::tc::wait_st();
+      ts::tc::fence_before_sync();
+      ts::mbar_arrive(&sh->p_full[x]);
+    }
+    if (ok && n_x > 0) ok = wait_warp(&sh->pv_done[x], 0, abort);
+    ts::tc::fence_after_sync();
+    if (ok) {
+      const float inv = l_run > 0.f ? ref_v / (kRefScale * l_run) : l_run;
+#pragma unroll
+      for (int c4 = 0; c4 < D / 32; ++c4) {
+        uint32_t rr[32];
+        if (n_x > 0) {
+          ts::tc::tmem_ld32(lane_base + o_col + c4 * 32, rr);
+          ts::tc::wait_ld();
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) rr[c] = 0;
+        }
+        if (row_valid) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + orow * D + c4 * 32);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              pk[k] = Mma::pack(__uint_as_float(rr[8 * c + 2 * k]) * inv,
+                                __uint_as_float(rr[8 * c + 2 * k + 1]) * inv);
+            dst[c] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          }
+        }
+      }
+    }
+  }
+  ts::tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    ts::tc::fence_after_sync();
+    ts::tc::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+bool tc_path(int group, int hkv, int hd, int bs, int dtype, const void* kp, const void* vp,
+             const void* q, int64_t q_stride, const void* out, int num_seqs) {
+  if (dtype != TS_BFLOAT16 && dtype != TS_FLOAT16) return false;
+  if ((hd != 64 && hd != 128) || bs != kBlock || group > kRows) return false;
+  if (num_seqs > 65535 || hkv > 65535) return false;
+  if ((reinterpret_cast<uint64_t>(kp) | reinterpret_cast<uint64_t>(vp) |
+       reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(out)) % 16)
+    return false;
+  return (q_stride * 2) % 16 == 0;
+}
+
+template <typename T, int D>
+int launch(const Args& a, dim3 grid, cudaStream_t s) {
+  auto kern = paged_prefill_fp8_kernel<T, D>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             Geo<D>::kSmemBytes);
+  if (e != cudaSuccess)
+    return ts::set_error(static_cast<int>(e), "paged_prefill_fp8: %s", cudaGetErrorString(e));
+  kern<<<grid, kThreads, Geo<D>::kSmemBytes, s>>>(a);
+  return ts::launch_status("paged_prefill_fp8");
+}
+
+}  // namespace
 
 extern "C" int ts_paged_prefill_fp8(void* out, const void* query, int64_t query_token_stride,
                                     const void* key_pool, const void* value_pool,
@@ -38,9 +622,38 @@ extern "C" int ts_paged_prefill_fp8(void* out, const void* query, int64_t query_
   if ((reinterpret_cast<uint64_t>(key_scales) | reinterpret_cast<uint64_t>(value_scales)) % 4 ||
       (reinterpret_cast<uint64_t>(query) | reinterpret_cast<uint64_t>(out)) % es)
     return ts::set_error(TS_ERR_MISALIGNED, "paged_prefill_fp8: pointers not element-aligned");
-  return ts::paged_attention_portable(out, query, query_token_stride, key_pool, value_pool,
-                                      block_tables, max_blocks_per_seq, query_start_loc,
-                                      context_lens, num_seqs, num_query_tokens, num_q_heads,
-                                      num_kv_heads, head_dim, block_size, num_blocks, scale, dtype,
-                                      static_cast<cudaStream_t>(stream), key_scales, value_scales);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int group = num_q_heads / num_kv_heads;
+  if (!tc_path(group, num_kv_heads, head_dim, block_size, dtype, key_pool, value_pool, query,
+               query_token_stride, out, num_seqs))
+    return ts::paged_attention_portable(out, query, query_token_stride, key_pool, value_pool,
+                                        block_tables, max_blocks_per_seq, query_start_loc,
+                                        context_lens, num_seqs, num_query_tokens, num_q_heads,
+                                        num_kv_heads, head_dim, block_size, num_blocks, scale,
+                                        dtype, s, key_scales, value_scales);
+  Args a;
+  a.out = out;
+  a.query = query;
+  a.q_stride = query_token_stride;
+  a.key_pool = static_cast<const uint8_t*>(key_pool);
+  a.value_pool = static_cast<const uint8_t*>(value_pool);
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.block_tables = block_tables;
+  a.qsl = query_start_loc;
+  a.context_lens = context_lens;
+  a.max_blocks = max_blocks_per_seq;
+  a.num_q_heads = num_q_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.group = group;
+  a.tq = kRows / group;
+  a.num_blocks = num_blocks;
+  a.scale_log2 = scale * kLog2e;
+  const int longest = max_query_len < num_query_tokens ? max_query_len : num_query_tokens;
+  const int tiles = (longest + a.tq - 1) / a.tq;
+  const dim3 grid((tiles + kQTiles - 1) / kQTiles, num_kv_heads, num_seqs);
+  if (dtype == TS_BFLOAT16)
+    return head_dim == 128 ? launch<__nv_bfloat16, 128>(a, grid, s)
+                           : launch<__nv_bfloat16, 64>(a, grid, s);
+  return head_dim == 128 ? launch<__half, 128>(a, grid, s) : launch<__half, 64>(a, grid, s);
 }
