@@ -7,12 +7,14 @@
 // and by the exponentials (one per score), so the cache's 8 bits must cost neither of them:
 //   * CTA = (sequence, KV head, pair of query tiles); a tile's 128 rows are 128/G tokens x the G
 //     query heads of the KV head, so a converted K/V tile serves 256 rows.
-//   * warps 8-11 (converters): read a 128-token tile's codes and scales from global memory a tile
-//     ahead into registers, multiply each row by its scale and store it as fp16 in the swizzled
-//     layout the MMAs read. Values are taken relative to the tile's largest scale (K) or the
-//     largest so far (V) times 2^-7, so they fill fp16's range whatever their magnitude; the
-//     scale is split into two fp16 parts, so a value is rounded once, to 2^-11 of itself. K's
-//     reference is a factor on the tile's scores; when V's grows, O is rescaled.
+//   * warp 12 (scout) runs up to four KV tiles (128 tokens) ahead: block table, the tile's scales,
+//     each row's factor and the tile's references, left in shared memory.
+//   * warps 8-11, 14, 15 (converters) take a tile's 16 blocks (8 of K, 8 of V) in turn: codes from
+//     global memory two blocks ahead into registers, times the row's factor, as fp16 into the
+//     swizzled layout the MMAs read. Values are relative to the tile's largest scale (K) or the
+//     largest so far (V) times 2^-7, so they fill fp16's range whatever their magnitude; a factor
+//     is two fp16 parts, so a value is rounded once, to 2^-11 of itself. K's reference is a factor
+//     on the tile's scores; when V's grows, O is rescaled.
 //   * warps 0-3 / 4-7 (softmax, one warpgroup per query tile, thread = row): q's row is scaled by a
 //     power of two into fp16's range and written to shared memory; then per tile S from TMEM, the
 //     row's maximum, 2^(s - m), P in fp16 (11 bits) back to TMEM over S. The maximum is kept while
@@ -43,12 +45,18 @@ constexpr int kBlock = 16;    // tokens per KV block
 constexpr int kHalfBytes = 128 * 128;  // 128 rows x 64 fp16 columns
 constexpr int kQTiles = 2;
 constexpr int kStages = 2;  // K ring, and V ring
-constexpr int kInfos = 4;   // tile descriptions: a softmax trails the converters by under 4 tiles
+// Tile descriptions. The scout writes tile t once the converters are done with t - kAhead, when
+// the MMAs, and so the softmaxes, are done with t - kAhead - kStages.
+constexpr int kInfos = 8, kAhead = 4;
+static_assert(kAhead + kStages <= kInfos, "a description outlives its readers");
+constexpr int kConverters = 6;  // converter warps
+constexpr int kUnits = 2 * kKvTile / kBlock;  // blocks of a tile, K then V
 constexpr int kThreads = 512;
-// Registers a thread after setmaxnreg: two softmax warpgroups, the converters, the rest. Their sum
-// is what the block is launched with, 4 x 128.
-constexpr int kRegsSoftmax = 176, kRegsConvert = 112, kRegsRest = 48;
-static_assert(2 * kRegsSoftmax + kRegsConvert + kRegsRest <= 4 * 128, "register split");
+// Registers a thread after setmaxnreg: two softmax warpgroups, and the two others. Their sum is
+// what the block is launched with, 4 x 128.
+constexpr int kRegsSoftmax = 168, kRegsRest = 88;
+static_assert(2 * kRegsSoftmax + 2 * kRegsRest <= 4 * 128, "register split");
+constexpr uint32_t kDropped = 0x80008000u;  // factor of a row whose codes are not used
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;  // keep a stale row max unless exceeded by 2^8
 constexpr uint32_t kTmemCols = 512;   // S_A [0,128), S_B [128,256), O_A [256,384), O_B [384,512)
@@ -71,17 +79,21 @@ struct Args {
   float scale_log2;
 };
 
-// What the softmax of a KV tile has to know: references of K and V, and the columns to mask (page
-// outside the pool) or to spoil (V row NaN), if any.
+// A KV tile as the scout leaves it: references of K and V, the columns to mask (page outside the
+// pool) or to spoil (V row NaN), if any; the blocks (negative: none); each row's factor for K and
+// for V, fp16 high and low part, or kDropped.
 struct TileInfo {
   float ref_k, ref_v;
   uint32_t any, pad;
   uint32_t skip[4], spoil[4];
+  int block[kKvTile / kBlock];
+  uint32_t factor[2][kKvTile];
 };
 
 struct Shared {
   uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[kQTiles], p_full[kQTiles], pv_done[kQTiles], drain;
+  uint64_t info_full[kInfos], converted[kAhead];
   TileInfo info[kInfos];
   uint32_t tmem;
   int abort;
@@ -135,101 +147,121 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// One converter warp's view of the KV tiles of a (sequence, KV head): it converts tokens 32 w ..
-// 32 w + 31 of every tile.
-template <int D>
-struct Converter {
-  static constexpr int kLanes = D / 16;        // lanes per row, 16 codes each
-  static constexpr int kRpi = 32 / kLanes;     // rows per load instruction
-  static constexpr int kLoads = 32 / kRpi;     // load instructions per item
-  const Args& a;
-  const int32_t* table;
-  int h, n_kv, total_blk, w, lane;
-  int next_table;        // lane b < 8: block b of the next tile to be looked up (-1 none, -2 bad)
-  uint4 raw_k[kLoads], raw_v[kLoads];
-  float ks[4], vs[4];    // scales of token 32 ((w + i) % 4) + lane: [0] is this lane's own row
-  uint32_t bad;          // bit i: that token is in a page outside the pool
-  float ref_v;           // largest V scale so far
+// Two fp16 parts of a row's factor, hi + lo = f to 2^-22 of it.
+__device__ __forceinline__ uint32_t split_factor(float f) {
+  const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
+  return uint32_t(__half_as_ushort(hi)) | (uint32_t(__half_as_ushort(lo)) << 16);
+}
 
-  __device__ __forceinline__ void look_up(int t) {
-    const int b = t * (kKvTile / kBlock) + lane;
-    next_table = -1;
-    if (lane < kKvTile / kBlock && b < total_blk) {
-      const int phys = __ldg(table + b);
-      next_table = phys >= 0 && int64_t(phys) < a.num_blocks ? phys : -2;
-    }
-  }
-  // Row of this KV head at block `phys`, offset `off`.
-  __device__ __forceinline__ int64_t row(int phys, int off) const {
-    return (int64_t(phys) * a.num_kv_heads + h) * kBlock + off;
-  }
-  __device__ __forceinline__ void load_codes(const uint8_t* pool, const int tab, uint4 (&raw)[kLoads]) {
-    const int own[2] = {__shfl_sync(0xffffffffu, tab, 2 * w), __shfl_sync(0xffffffffu, tab, 2 * w + 1)};
+// Largest finite value over the warp's 4 x 32 scales.
+__device__ __forceinline__ float top(const float (&sc)[4]) {
+  float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int r = i * kRpi + lane / kLanes;  // row of the warp's 32
-      const int phys = own[(i * kRpi) / kBlock];
-      raw[i] = phys >= 0 ? __ldg(reinterpret_cast<const uint4*>(pool + row(phys, r % kBlock) * D) +
-                                 lane % kLanes)
-                         : make_uint4(0, 0, 0, 0);
-    }
-  }
-  __device__ __forceinline__ void load_scales(int t, const int tab) {
-    bad = 0;
+  for (int i = 0; i < 4; ++i) m = fmaxf(m, isfinite(sc[i]) ? sc[i] : 0.f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int g = (w + i) & 3;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
+// The scout warp: describes the n_max KV tiles of (table, KV head h), n_kv visible keys.
+__device__ void scout(const Args& a, Shared* sh, const int32_t* table, int h, int n_kv, int n_max,
+                      int lane, volatile int* abort) {
+  constexpr int kBlocks = kKvTile / kBlock;
+  const int total_blk = (n_kv + kBlock - 1) / kBlock;
+  float run_v = 0.f;  // largest V scale so far
+  auto look_up = [&](int t) -> int {  // lane b < 8: block b of tile t (-1 none, -2 not in the pool)
+    const int b = t * kBlocks + lane;
+    if (lane >= kBlocks || b >= total_blk) return -1;
+    const int phys = __ldg(table + b);
+    return phys >= 0 && int64_t(phys) < a.num_blocks ? phys : -2;
+  };
+  int tab = look_up(0);
+  for (int t = 0; t < n_max; ++t) {
+    const int next = look_up(t + 1);
+    float ks[4], vs[4];
+    uint32_t skip[4], reach[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {  // tokens 32 g + lane
       const int phys = __shfl_sync(0xffffffffu, tab, 2 * g + lane / kBlock);
       const bool in = t * kKvTile + 32 * g + lane < n_kv;
-      if (in && phys == -2) bad |= 1u << i;
-      const int64_t r = row(phys, lane % kBlock);
-      ks[i] = in && phys >= 0 ? __ldg(a.key_scales + r) : 0.f;
-      vs[i] = in && phys >= 0 ? __ldg(a.value_scales + r) : 0.f;
+      const int64_t r = (int64_t(phys) * a.num_kv_heads + h) * kBlock + lane % kBlock;
+      ks[g] = in && phys >= 0 ? __ldg(a.key_scales + r) : 0.f;
+      vs[g] = in && phys >= 0 ? __ldg(a.value_scales + r) : 0.f;
+      skip[g] = __ballot_sync(0xffffffffu, in && phys == -2);
+      reach[g] = in;
     }
-  }
-  // Largest finite scale of the tile.
-  __device__ __forceinline__ float top(const float (&sc)[4]) const {
-    float m = 0.f;
+    if (t >= kAhead && !wait_warp(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1, abort))
+      return;
+    TileInfo* info = &sh->info[t % kInfos];
+    const float ref_k = top(ks);
+    run_v = fmaxf(run_v, top(vs));
+    uint32_t any = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = fmaxf(m, isfinite(sc[i]) ? sc[i] : 0.f);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m;
+    for (int g = 0; g < 4; ++g) {
+      const uint32_t spoil = __ballot_sync(0xffffffffu, !isfinite(vs[g]));
+      any |= skip[g] | spoil;
+      if (lane == 0) {
+        info->skip[g] = skip[g];
+        info->spoil[g] = spoil;
+      }
+      // A NaN K row makes NaN scores; a NaN V row is stored as zeros (see the head of the file).
+      const float fk = ref_k > 0.f ? ks[g] / ref_k * kRefScale : ks[g];
+      const float fv = run_v > 0.f ? vs[g] / run_v * kRefScale : 0.f;
+      info->factor[0][32 * g + lane] = reach[g] ? split_factor(fk) : kDropped;
+      info->factor[1][32 * g + lane] = reach[g] && isfinite(vs[g]) ? split_factor(fv) : kDropped;
+    }
+    if (lane < kBlocks) info->block[lane] = tab;
+    if (lane == 0) {
+      info->ref_k = ref_k;
+      info->ref_v = run_v;
+      info->any = any;
+    }
+    __syncwarp();
+    if (lane == 0) ts::mbar_arrive(&sh->info_full[t % kInfos]);
+    tab = next;
   }
-  // raw -> fp16 rows at `dst` (a tile in shared memory, 128-byte swizzled halves of 64 columns).
-  // `f`: this lane's row's factor; `zero`: its codes are dropped.
-  __device__ __forceinline__ void convert(const uint4 (&raw)[kLoads], float f, bool zero, uint8_t* dst) {
-    const __half hi = __float2half_rn(f);
-    const __half lo = __float2half_rn(f - __half2float(hi));
-    const uint32_t my = uint32_t(__half_as_ushort(hi)) | (uint32_t(__half_as_ushort(lo)) << 16);
-    const uint32_t dropped = __ballot_sync(0xffffffffu, zero);
+}
+
+// One block of codes (16 rows of a KV head) in a converter warp's registers.
+template <int D>
+struct Codes {
+  static constexpr int kLanes = D / 16;          // lanes per row, 16 codes each
+  static constexpr int kRpi = 32 / kLanes;       // rows per load instruction
+  static constexpr int kLoads = kBlock / kRpi;
+  uint4 raw[kLoads];
+
+  __device__ __forceinline__ void load(const uint8_t* block, int lane) {  // nullptr: zeros
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      raw[i] = block != nullptr ? __ldg(reinterpret_cast<const uint4*>(block) + i * 32 + lane)
+                                : make_uint4(0, 0, 0, 0);
+  }
+  // Rows row0 .. row0 + 15 of the fp16 tile at `dst` (128-byte swizzled halves of 64 columns).
+  __device__ __forceinline__ void store(uint8_t* dst, const uint32_t* factor, int row0, int lane) {
+    const int c = lane % kLanes;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = i * kRpi + lane / kLanes;
-      const uint32_t s2 = __shfl_sync(0xffffffffu, my, r);
-      const __half2 h2 = __half2half2(__ushort_as_half(static_cast<unsigned short>(s2 & 0xffffu)));
-      const __half2 l2 = __half2half2(__ushort_as_half(static_cast<unsigned short>(s2 >> 16)));
+      const int row = row0 + i * kRpi + lane / kLanes;
+      const uint32_t f = factor[row];
+      const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
+      const __half2 h2 = __low2half2(f2), l2 = __high2half2(f2);
       uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-      if (dropped >> r & 1) word[0] = word[1] = word[2] = word[3] = 0;
+      if (f == kDropped) word[0] = word[1] = word[2] = word[3] = 0;
       uint32_t v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const __half2 c = ts::fp8_half2(word[k / 2] >> (16 * (k & 1)));
-        const __half2 x = __hfma2(c, h2, __hmul2(c, l2));
-        v[k] = *reinterpret_cast<const uint32_t*>(&x);
+        const __half2 x = ts::fp8_half2(word[k / 2] >> (16 * (k & 1)));
+        const __half2 y = __hfma2(x, h2, __hmul2(x, l2));
+        v[k] = *reinterpret_cast<const uint32_t*>(&y);
       }
-      const int c = lane % kLanes, row_in_tile = 32 * w + r;
-      // Chunks 2 (c % 4) and + 1 of half c / 4; the halves' lanes store them in opposite order, so
-      // the eight lanes of a row never meet in a bank.
-      const int first = c / 4;
-      uint8_t* base = dst + (c / 4) * kHalfBytes + row_in_tile * 128;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const bool second = (u ^ first) != 0;
-        const int chunk = (2 * (c % 4) + int(second)) ^ (row_in_tile & 7);
-        *reinterpret_cast<uint4*>(base + chunk * 16) =
-            second ? make_uint4(v[4], v[5], v[6], v[7]) : make_uint4(v[0], v[1], v[2], v[3]);
-      }
+      // Chunks 2 (c % 4) and + 1 of half c / 4; the two halves' lanes store them in opposite
+      // order, so the eight lanes of a row never meet in a bank.
+      const bool flip = c >= 4;
+      uint8_t* base = dst + (c / 4) * kHalfBytes + row * 128;
+      const int at = (2 * (c % 4)) ^ (row & 7);
+      const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
+      *reinterpret_cast<uint4*>(base + (flip ? at ^ 1 : at) * 16) = flip ? hi : lo;
+      *reinterpret_cast<uint4*>(base + (flip ? at : at ^ 1) * 16) = flip ? lo : hi;
     }
   }
 };
@@ -269,11 +301,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   if (threadIdx.x == 0) {
     ts::mbar_init(&sh->q_full, 128 * kQTiles);
     for (int i = 0; i < kStages; ++i) {
-      ts::mbar_init(&sh->k_full[i], 128);
+      ts::mbar_init(&sh->k_full[i], kUnits / 2);
       ts::mbar_init(&sh->k_empty[i], 1);
-      ts::mbar_init(&sh->v_full[i], 128);
+      ts::mbar_init(&sh->v_full[i], kUnits / 2);
       ts::mbar_init(&sh->v_empty[i], 1);
     }
+    for (int i = 0; i < kInfos; ++i) ts::mbar_init(&sh->info_full[i], 1);
+    for (int i = 0; i < kAhead; ++i) ts::mbar_init(&sh->converted[i], kUnits);
     for (int x = 0; x < kQTiles; ++x) {
       ts::mbar_init(&sh->s_full[x], 1);
       ts::mbar_init(&sh->p_full[x], 128);
@@ -292,9 +326,49 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   ts::tc::fence_after_sync();
   const uint32_t tmem = sh->tmem;
 
-  if (warp >= 12) {
+  if (warp >= 8) {
     regs_dec<kRegsRest>();
-    if (warp == 13 && lane == 0 && n_max > 0) {
+    if (warp == 12) {
+      scout(a, sh, a.block_tables + int64_t(seq) * a.max_blocks, h, n_kv, n_max, lane, abort);
+    } else if (warp != 13) {
+      // ---------------------------------------------------------- converters
+      const int total = n_max * kUnits;
+      const int64_t block_bytes = int64_t(a.num_kv_heads) * kBlock * D;
+      Codes<D> codes[2];
+      auto fetch = [&](Codes<D>& c, int u) -> bool {
+        if (u >= total) return true;
+        const int t = u / kUnits, k = u % kUnits;
+        if (!wait_warp(&sh->info_full[t % kInfos], (t / kInfos) & 1, abort)) return false;
+        const int phys = sh->info[t % kInfos].block[k % (kUnits / 2)];
+        const uint8_t* pool = (k < kUnits / 2 ? a.key_pool : a.value_pool) + h * kBlock * D;
+        c.load(phys >= 0 ? pool + phys * block_bytes : nullptr, lane);
+        return true;
+      };
+      auto convert = [&](Codes<D>& c, int u) -> bool {
+        const int t = u / kUnits, k = u % kUnits, st = t % kStages;
+        const bool is_v = k >= kUnits / 2;
+        if (t >= kStages && !wait_warp(is_v ? &sh->v_empty[st] : &sh->k_empty[st],
+                                       ((t - kStages) / kStages) & 1, abort))
+          return false;
+        c.store(is_v ? sV(st) : sK(st), sh->info[t % kInfos].factor[is_v],
+                k % (kUnits / 2) * kBlock, lane);
+        ts::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          ts::mbar_arrive(is_v ? &sh->v_full[st] : &sh->k_full[st]);
+          ts::mbar_arrive(&sh->converted[t % kAhead]);
+        }
+        return true;
+      };
+      int u = warp < 12 ? warp - 8 : warp - 10;
+      bool ok = fetch(codes[0], u) && fetch(codes[1], u + kConverters);
+      while (ok && u < total) {
+        ok = convert(codes[0], u) && fetch(codes[0], u + 2 * kConverters);
+        u += kConverters;
+        if (ok && u < total) ok = convert(codes[1], u) && fetch(codes[1], u + 2 * kConverters);
+        u += kConverters;
+      }
+    } else if (lane == 0 && n_max > 0) {
       // ---------------------------------------------------------- MMA issuer
       constexpr uint32_t idesc_qk = ts::tc::idesc_f16(false, kRows, kKvTile, false);
       constexpr uint32_t idesc_pv = ts::tc::idesc_f16(false, kRows, D, true);
@@ -345,61 +419,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         ts::tc::commit(&sh->drain);
         ts::mbar_wait_bounded(&sh->drain, 0);
       }
-    }
-  } else if (warp >= 8) {
-    // ------------------------------------------------------------ converters
-    regs_dec<kRegsConvert>();
-    Converter<D> cv{a, a.block_tables + int64_t(seq) * a.max_blocks, h, n_kv,
-                    (n_kv + kBlock - 1) / kBlock, warp - 8, lane};
-    cv.ref_v = 0.f;
-    if (n_max > 0) {
-      cv.look_up(0);
-      cv.load_scales(0, cv.next_table);
-      cv.load_codes(a.key_pool, cv.next_table, cv.raw_k);
-      cv.load_codes(a.value_pool, cv.next_table, cv.raw_v);
-      cv.look_up(1);
-    }
-    for (int t = 0; t < n_max; ++t) {
-      const int st = t % kStages;
-      const float ref_k = cv.top(cv.ks);
-      cv.ref_v = fmaxf(cv.ref_v, cv.top(cv.vs));
-      const float k_own = cv.ks[0], v_own = cv.vs[0];
-      const bool out_of_reach = t * kKvTile + 32 * cv.w + lane >= n_kv;
-      if (cv.w == 0) {
-        TileInfo* info = &sh->info[t % kInfos];
-        uint32_t any = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t skip = __ballot_sync(0xffffffffu, cv.bad >> i & 1);
-          const uint32_t spoil = __ballot_sync(0xffffffffu, !isfinite(cv.vs[i]));
-          any |= skip | spoil;
-          if (lane == 0) {
-            info->skip[i] = skip;
-            info->spoil[i] = spoil;
-          }
-        }
-        if (lane == 0) {
-          info->ref_k = ref_k;
-          info->ref_v = cv.ref_v;
-          info->any = any;
-        }
-      }
-      const int tab = cv.next_table;  // of tile t + 1
-      if (t >= kStages && !wait_warp(&sh->k_empty[st], ((t - kStages) / kStages) & 1, abort)) break;
-      cv.convert(cv.raw_k, ref_k > 0.f ? k_own / ref_k * kRefScale : k_own, out_of_reach, sK(st));
-      ts::fence_proxy_async_smem();
-      ts::mbar_arrive(&sh->k_full[st]);
-      if (t + 1 < n_max) {
-        cv.load_scales(t + 1, tab);
-        cv.load_codes(a.key_pool, tab, cv.raw_k);
-        cv.look_up(t + 2);
-      }
-      if (t >= kStages && !wait_warp(&sh->v_empty[st], ((t - kStages) / kStages) & 1, abort)) break;
-      const bool drop = out_of_reach || !isfinite(v_own);
-      cv.convert(cv.raw_v, drop || cv.ref_v == 0.f ? 0.f : v_own / cv.ref_v * kRefScale, drop, sV(st));
-      ts::fence_proxy_async_smem();
-      ts::mbar_arrive(&sh->v_full[st]);
-      if (t + 1 < n_max) cv.load_codes(a.value_pool, tab, cv.raw_v);
     }
   } else {
     // ------------------------------------------------------------ softmax / epilogue
@@ -487,13 +506,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           if ((info->spoil[c / 32] >> (c % 32) & 1) && c <= limit) sr[c] = 0x7fc00000u;
         }
       }
-      float mx = -INFINITY, my = -INFINITY;
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 128; c += 4) {
-        mx = max3f(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-        my = max3f(my, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
-      }
-      const float m_tile = fmaxf(mx, my) * slj;
+      for (int c = 0; c < 128; c += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mx[k] = max3f(mx[k], __uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1]));
+      const float m_tile = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * slj;
       float corr = 1.f;
       if (m_tile > m_run + kRescaleSlack || m_run == -INFINITY) {
         corr = m_run == -INFINITY ? 1.f : ex2(m_run - m_tile);  // nothing summed yet: 0 either way
