@@ -16,9 +16,11 @@
 //     is two fp16 parts, so a value is rounded once, to 2^-11 of itself. K's reference is a factor
 //     on the tile's scores; when V's grows, O is rescaled.
 //   * warps 0-3 / 4-7 (softmax, one warpgroup per query tile, thread = row): q's row is scaled by a
-//     power of two into fp16's range and written to shared memory; then per tile S from TMEM, the
-//     row's maximum, 2^(s - m), P in fp16 (11 bits) back to TMEM over S. The maximum is kept while
-//     no score exceeds it by 2^8, so O is rarely rescaled; sums are fp32.
+//     power of two into fp16's range and written to shared memory; then per tile, 32 columns at a
+//     time: the row's maximum, then 2^(s - m), P in fp16 (11 bits) back to TMEM over S. The maximum
+//     is kept while no score exceeds it by 2^8, so O is rarely rescaled; sums are fp32. Columns no
+//     row of a warp sees are skipped. Everything is in loops over few columns: unrolled over a
+//     whole row, the roles' code outgrew the instruction caches (a quarter of the stalls).
 //   * warp 13, one lane: tcgen05.mma, S_x = Q_x K^T and O_x += P_x V, in the order PV_A(j),
 //     QK_A(j+1), PV_B(j), QK_B(j+1), so one tile's softmax runs under the other's MMAs. A QK's
 //     commit covers the PV before it, so S of tile j + 1 also says that O holds tile j.
@@ -52,15 +54,14 @@ static_assert(kAhead + kStages <= kInfos, "a description outlives its readers");
 constexpr int kConverters = 6;  // converter warps
 constexpr int kUnits = 2 * kKvTile / kBlock;  // blocks of a tile, K then V
 constexpr int kThreads = 512;
-// Registers a thread after setmaxnreg: two softmax warpgroups, and the two others. Their sum is
-// what the block is launched with, 4 x 128.
-constexpr int kRegsSoftmax = 168, kRegsRest = 88;
-static_assert(2 * kRegsSoftmax + 2 * kRegsRest <= 4 * 128, "register split");
+constexpr int kMaxTries = 1 << 22;  // of a bounded wait
 constexpr uint32_t kDropped = 0x80008000u;  // factor of a row whose codes are not used
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;  // keep a stale row max unless exceeded by 2^8
 constexpr uint32_t kTmemCols = 512;   // S_A [0,128), S_B [128,256), O_A [256,384), O_B [384,512)
 constexpr float kRefScale = 128.f;    // fp16 values are code * scale / ref * 128 <= 57344
+// V's reference starts, and grows, to this times the scales seen, so that it seldom grows.
+constexpr float kRefRoom = 8.f;
 
 struct Args {
   void* out;
@@ -84,7 +85,7 @@ struct Args {
 // for V, fp16 high and low part, or kDropped.
 struct TileInfo {
   float ref_k, ref_v;
-  uint32_t any, pad;
+  uint32_t any, dropped;  // dropped: bit b, 8 + b: block b of K, of V has rows of factor kDropped
   uint32_t skip[4], spoil[4];
   int block[kKvTile / kBlock];
   uint32_t factor[2][kKvTile];
@@ -106,16 +107,26 @@ struct Geo {
   static constexpr int kSmemBytes = kTiles + int(sizeof(Shared)) + 1024;
 };
 
-// Bounded wait that also gives up as soon as another role has aborted.
+// Bounded wait (a try sleeps for some time, so the tries last about a second); sets *abort when it
+// gives up. A loop of few instructions: there are many waits, and all roles share the caches.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, volatile int* abort) {
-  for (long long i = 0; i < ts::kMaxSpins; ++i) {
-    if (ts::mbar_try_wait(bar, phase)) return true;
-    if ((i & 255) == 255 && *abort) return false;
-  }
-  *abort = 1;
-  return false;
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %3;\n"
+      "TRY:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.ne.u32 q, n, 0;\n\t"
+      "@q bra TRY;\n"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(ts::smem_u32(bar)), "r"(phase), "n"(kMaxTries)
+      : "memory");
+  if (!ok) *abort = 1;
+  return ok != 0;
 }
-
 // The same for a whole warp, with one answer.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase, volatile int* abort) {
   return __all_sync(0xffffffffu, wait_bar(bar, phase, abort));
@@ -133,18 +144,23 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// (d0, d1) = (a0, a1) * b + c, and (s0, s1) += (a0, a1): one packed instruction each.
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b, float c) {
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\t"
+      "mov.b64 z, {%5, %5};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b), "f"(c));
+}
+__device__ __forceinline__ void add2(float& s0, float& s1, float a0, float a1) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(s0), "+f"(s1)
+      : "f"(a0), "f"(a1));
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-template <int N>
-__device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Two fp16 parts of a row's factor, hi + lo = f to 2^-22 of it.
@@ -168,7 +184,7 @@ __device__ void scout(const Args& a, Shared* sh, const int32_t* table, int h, in
                       int lane, volatile int* abort) {
   constexpr int kBlocks = kKvTile / kBlock;
   const int total_blk = (n_kv + kBlock - 1) / kBlock;
-  float run_v = 0.f;  // largest V scale so far
+  float run_v = 0x1p-126f;  // V's reference: never below the scales seen
   auto look_up = [&](int t) -> int {  // lane b < 8: block b of tile t (-1 none, -2 not in the pool)
     const int b = t * kBlocks + lane;
     if (lane >= kBlocks || b >= total_blk) return -1;
@@ -193,9 +209,10 @@ __device__ void scout(const Args& a, Shared* sh, const int32_t* table, int h, in
     if (t >= kAhead && !wait_warp(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1, abort))
       return;
     TileInfo* info = &sh->info[t % kInfos];
-    const float ref_k = top(ks);
-    run_v = fmaxf(run_v, top(vs));
-    uint32_t any = 0;
+    const float ref_k = fmaxf(top(ks), 0x1p-126f), top_v = top(vs);
+    if (top_v > run_v) run_v = fminf(top_v * kRefRoom, 0x1p127f);
+    const float inv_k = 1.f / ref_k, inv_v = 1.f / run_v;
+    uint32_t any = 0, dropped = 0;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const uint32_t spoil = __ballot_sync(0xffffffffu, !isfinite(vs[g]));
@@ -205,16 +222,23 @@ __device__ void scout(const Args& a, Shared* sh, const int32_t* table, int h, in
         info->spoil[g] = spoil;
       }
       // A NaN K row makes NaN scores; a NaN V row is stored as zeros (see the head of the file).
-      const float fk = ref_k > 0.f ? ks[g] / ref_k * kRefScale : ks[g];
-      const float fv = run_v > 0.f ? vs[g] / run_v * kRefScale : 0.f;
+      const float fk = ks[g] * inv_k * kRefScale, fv = vs[g] * inv_v * kRefScale;
+      const bool keep_v = reach[g] && isfinite(vs[g]);
       info->factor[0][32 * g + lane] = reach[g] ? split_factor(fk) : kDropped;
-      info->factor[1][32 * g + lane] = reach[g] && isfinite(vs[g]) ? split_factor(fv) : kDropped;
+      info->factor[1][32 * g + lane] = keep_v ? split_factor(fv) : kDropped;
+      const uint32_t dk = ~__ballot_sync(0xffffffffu, reach[g]);
+      const uint32_t dv = ~__ballot_sync(0xffffffffu, keep_v);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        dropped |= uint32_t((dk >> 16 * b & 0xffffu) != 0) << (2 * g + b) |
+                   uint32_t((dv >> 16 * b & 0xffffu) != 0) << (8 + 2 * g + b);
     }
     if (lane < kBlocks) info->block[lane] = tab;
     if (lane == 0) {
       info->ref_k = ref_k;
       info->ref_v = run_v;
       info->any = any;
+      info->dropped = dropped;
     }
     __syncwarp();
     if (lane == 0) ts::mbar_arrive(&sh->info_full[t % kInfos]);
@@ -222,46 +246,45 @@ __device__ void scout(const Args& a, Shared* sh, const int32_t* table, int h, in
   }
 }
 
-// One block of codes (16 rows of a KV head) in a converter warp's registers.
+// One block of codes (16 rows of a KV head) in a converter warp's registers: a row in 8 lanes, each
+// with 8 codes of every 64 columns, so a lane's values are one 16-byte chunk of each half tile.
 template <int D>
 struct Codes {
-  static constexpr int kLanes = D / 16;          // lanes per row, 16 codes each
-  static constexpr int kRpi = 32 / kLanes;       // rows per load instruction
-  static constexpr int kLoads = kBlock / kRpi;
-  uint4 raw[kLoads];
+  static constexpr int kHalves = D / 64;
+  static constexpr int kLoads = kBlock / 4;  // 4 rows per load instruction
+  uint2 raw[kLoads][kHalves];
 
   __device__ __forceinline__ void load(const uint8_t* block, int lane) {  // nullptr: zeros
+    const uint2* src = reinterpret_cast<const uint2*>(block) + lane / 8 * (D / 8) + lane % 8;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-      raw[i] = block != nullptr ? __ldg(reinterpret_cast<const uint4*>(block) + i * 32 + lane)
-                                : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int hf = 0; hf < kHalves; ++hf)
+        raw[i][hf] = block != nullptr ? __ldg(src + i * (D / 2) + hf * 8) : make_uint2(0, 0);
   }
   // Rows row0 .. row0 + 15 of the fp16 tile at `dst` (128-byte swizzled halves of 64 columns).
-  __device__ __forceinline__ void store(uint8_t* dst, const uint32_t* factor, int row0, int lane) {
-    const int c = lane % kLanes;
+  __device__ __forceinline__ void store(uint8_t* dst, const uint32_t* factor, int row0, bool dropped,
+                                        int lane) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int row = row0 + i * kRpi + lane / kLanes;
+      const int row = row0 + i * 4 + lane / 8;
       const uint32_t f = factor[row];
       const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
       const __half2 h2 = __low2half2(f2), l2 = __high2half2(f2);
-      uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-      if (f == kDropped) word[0] = word[1] = word[2] = word[3] = 0;
-      uint32_t v[8];
+      uint8_t* base = dst + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const __half2 x = ts::fp8_half2(word[k / 2] >> (16 * (k & 1)));
-        const __half2 y = __hfma2(x, h2, __hmul2(x, l2));
-        v[k] = *reinterpret_cast<const uint32_t*>(&y);
+      for (int hf = 0; hf < kHalves; ++hf) {
+        uint2 w = raw[i][hf];
+        if (dropped && f == kDropped) w = make_uint2(0, 0);
+        uint32_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const __half2 x = ts::fp8_half2((k < 2 ? w.x : w.y) >> (16 * (k & 1)));
+          const __half2 y = __hfma2(x, h2, __hmul2(x, l2));
+          v[k] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        *reinterpret_cast<uint4*>(base + hf * kHalfBytes) = make_uint4(v[0], v[1], v[2], v[3]);
       }
-      // Chunks 2 (c % 4) and + 1 of half c / 4; the two halves' lanes store them in opposite
-      // order, so the eight lanes of a row never meet in a bank.
-      const bool flip = c >= 4;
-      uint8_t* base = dst + (c / 4) * kHalfBytes + row * 128;
-      const int at = (2 * (c % 4)) ^ (row & 7);
-      const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
-      *reinterpret_cast<uint4*>(base + (flip ? at ^ 1 : at) * 16) = flip ? hi : lo;
-      *reinterpret_cast<uint4*>(base + (flip ? at : at ^ 1) * 16) = flip ? lo : hi;
     }
   }
 };
@@ -327,7 +350,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   const uint32_t tmem = sh->tmem;
 
   if (warp >= 8) {
-    regs_dec<kRegsRest>();
     if (warp == 12) {
       scout(a, sh, a.block_tables + int64_t(seq) * a.max_blocks, h, n_kv, n_max, lane, abort);
     } else if (warp != 13) {
@@ -350,8 +372,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         if (t >= kStages && !wait_warp(is_v ? &sh->v_empty[st] : &sh->k_empty[st],
                                        ((t - kStages) / kStages) & 1, abort))
           return false;
-        c.store(is_v ? sV(st) : sK(st), sh->info[t % kInfos].factor[is_v],
-                k % (kUnits / 2) * kBlock, lane);
+        const TileInfo& info = sh->info[t % kInfos];
+        c.store(is_v ? sV(st) : sK(st), info.factor[is_v], k % (kUnits / 2) * kBlock,
+                info.dropped >> k & 1, lane);
         ts::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -422,52 +445,62 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     }
   } else {
     // ------------------------------------------------------------ softmax / epilogue
-    regs_inc<kRegsSoftmax>();
     const int x = warp / 4;               // query tile of this warpgroup
     const int r = threadIdx.x - 128 * x;  // tile row == TMEM lane
     const int n_x = n_t[x];
-    const int i = r / a.group, g = r - i * a.group;
+    const int i = r / a.group;
     const int qi = (tile0 + x) * a.tq + i;
     const bool row_valid = i < a.tq && qi < q_len;
     const int pos = row_valid ? p0 + qi : p0 + q_len - 1;
-    const int64_t orow = int64_t(q0 + qi) * a.num_q_heads + h * a.group + g;
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t s_col = x * 128, o_col = 256 + x * 128;
 
-    // q's row times 2^(14 - exponent of its amax), in fp16; `sl` undoes it (times the softmax
-    // scale, whose sign goes with q).
-    float sl;
+    // q's rows times 2^(14 - exponent of their amax), in fp16; `sl` undoes it (times the softmax
+    // scale, whose sign goes with q). A warp loads its 32 rows 16 bytes a lane, D / 8 lanes a row.
+    float sl = 0.f;
     {
-      const uint4* src = reinterpret_cast<const uint4*>(
-          static_cast<const T*>(a.query) + int64_t(q0 + qi) * a.q_stride +
-          int64_t(h * a.group + g) * D);
-      uint4 v[D / 8];
-      uint32_t m = 0;
+      constexpr int kLanes = D / 8, kRpi = 32 / kLanes;
+      const int c = lane % kLanes;
+      auto load_row = [&](int it) -> uint4 {
+        const int rr = (warp & 3) * 32 + it * kRpi + lane / kLanes;
+        const int ri = rr / a.group, qr = (tile0 + x) * a.tq + ri;
+        if (ri >= a.tq || qr >= q_len) return make_uint4(0, 0, 0, 0);
+        return __ldg(reinterpret_cast<const uint4*>(
+                         static_cast<const T*>(a.query) + int64_t(q0 + qr) * a.q_stride +
+                         int64_t(h * a.group + rr - ri * a.group) * D) + c);
+      };
+      constexpr int kBatch = 4;  // loads in flight
+#pragma unroll 1
+      for (int it0 = 0; it0 < kLanes; it0 += kBatch) {  // 32 / kRpi = kLanes load instructions
+        uint4 v[kBatch];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        v[c] = row_valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-        const uint32_t wds[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+        for (int b = 0; b < kBatch; ++b) v[b] = load_row(it0 + b);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 f = Mma::unpack(wds[k]);
-          m = max(m, max(ts::abs_bits(f.x), ts::abs_bits(f.y)));
+        for (int b = 0; b < kBatch; ++b) {
+          const uint32_t wds[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+          uint32_t m = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = Mma::unpack(wds[k]);
+            m = max(m, max(ts::abs_bits(f.x), ts::abs_bits(f.y)));
+          }
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const int e = max(int(m >> 23), 27);  // biased exponent; tiny rows keep a finite factor
+          const float up =
+              copysignf(__uint_as_float(uint32_t(127 + 14 + 127 - e) << 23), a.scale_log2);
+          const int my = __shfl_sync(0xffffffffu, e, lane % kRpi * kLanes);
+          if (lane / kRpi == it0 + b) sl = ldexpf(fabsf(a.scale_log2) / kRefScale, my - 127 - 14);
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = Mma::unpack(wds[k]);
+            o[k] = pack_half2(f.x * up, f.y * up);
+          }
+          const int rr = (warp & 3) * 32 + (it0 + b) * kRpi + lane / kLanes;
+          *reinterpret_cast<uint4*>(sQ(x) + rr * 128 + (c >> 3) * kHalfBytes +
+                                    (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
-      }
-      const int e = max(int(m >> 23), 27);  // biased exponent; tiny rows keep a finite factor
-      const float up = copysignf(__uint_as_float(uint32_t(127 + 14 + 127 - e) << 23), a.scale_log2);
-      sl = ldexpf(fabsf(a.scale_log2) / kRefScale, e - 127 - 14);
-      uint8_t* dst = sQ(x) + r * 128;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        const uint32_t wds[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-        uint32_t o[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 f = Mma::unpack(wds[k]);
-          o[k] = pack_half2(f.x * up, f.y * up);
-        }
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalfBytes + (((c & 7) ^ (r & 7)) << 4)) =
-            make_uint4(o[0], o[1], o[2], o[3]);
       }
       ts::fence_proxy_async_smem();
       ts::mbar_arrive(&sh->q_full);
@@ -481,67 +514,85 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         break;
       }
       ts::tc::fence_after_sync();
-      uint32_t sr[128];
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4) {
-        uint32_t (&chunk)[32] = *reinterpret_cast<uint32_t(*)[32]>(sr + 32 * c4);
-        ts::tc::tmem_ld32(lane_base + s_col + c4 * 32, chunk);
-      }
       const volatile TileInfo* info = &sh->info[j % kInfos];
       const float slj = fmaxf(sl * info->ref_k, 0x1p-126f);  // > 0, so that -inf stays -inf
+      // O is in units of V's reference: it shrinks when that grows.
       const float ref_old = ref_v;
       ref_v = info->ref_v;
       const bool odd_columns = info->any != 0;
-      ts::tc::wait_ld();
+      float corr_o = ref_v != ref_old && j > 0 ? ref_old / ref_v : 1.f;
       const int limit = pos - j * kKvTile;  // columns c <= limit are visible
-      if (limit < kKvTile - 1) {
+      // Column groups of 32 that some row of the warp sees, and those every row sees whole.
+      const int n_some = min(4, max(0, __reduce_max_sync(0xffffffffu, limit) + 32) / 32);
+      const int n_whole = odd_columns ? 0 : max(0, __reduce_min_sync(0xffffffffu, limit) + 1) / 32;
+      auto mask = [&](uint32_t (&r)[32], int c) {
+        const int lim = limit - 32 * c;
+        const uint32_t seen = lim >= 31 ? ~0u : lim < 0 ? 0u : (2u << lim) - 1;
+        const uint32_t keep = seen & ~info->skip[c], spoil = seen & info->spoil[c];
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c > limit) sr[c] = __float_as_uint(-INFINITY);
-      }
-      if (odd_columns) {
-#pragma unroll
-        for (int c = 0; c < 128; ++c) {
-          if (info->skip[c / 32] >> (c % 32) & 1) sr[c] = __float_as_uint(-INFINITY);
-          if ((info->spoil[c / 32] >> (c % 32) & 1) && c <= limit) sr[c] = 0x7fc00000u;
+        for (int k = 0; k < 32; ++k) {
+          const uint32_t z = spoil >> k & 1 ? 0x7fc00000u : r[k];
+          r[k] = keep >> k & 1 ? z : __float_as_uint(-INFINITY);
         }
-      }
+      };
+      uint32_t sa[32], sb[32];
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      ts::tc::tmem_ld32(lane_base + s_col, sa);
+#pragma unroll 1
+      for (int c = 0; c < n_some; ++c) {
+        ts::tc::wait_ld(sa);
+        if (c >= n_whole) mask(sa, c);
 #pragma unroll
-      for (int c = 0; c < 128; c += 8)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mx[k] = max3f(mx[k], __uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1]));
+        for (int k = 0; k < 32; k += 2)
+          mx[k / 2 % 4] = max3f(mx[k / 2 % 4], __uint_as_float(sa[k]), __uint_as_float(sa[k + 1]));
+        ts::tc::tmem_ld32(lane_base + s_col + (c + 1 < n_some ? c + 1 : 0) * 32, sa);
+      }
       const float m_tile = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * slj;
-      float corr = 1.f;
       if (m_tile > m_run + kRescaleSlack || m_run == -INFINITY) {
-        corr = m_run == -INFINITY ? 1.f : ex2(m_run - m_tile);  // nothing summed yet: 0 either way
+        const float f = m_run == -INFINITY ? 1.f : ex2(m_run - m_tile);  // all so far is 0
+        l_run *= f;
+        corr_o *= f;
         m_run = m_tile;
       }
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
       float sum0 = 0.f, sum1 = 0.f;
+      auto columns = [&](uint32_t (&r)[32], int c) {  // P of columns 32 c .. 32 c + 31
+        if (c >= n_whole) mask(r, c);
+        uint32_t pw[16];
 #pragma unroll
-      for (int c = 0; c < 128; c += 2) {
-        const float p = ex2(fmaf(__uint_as_float(sr[c]), slj, -m_use));
-        const float q = ex2(fmaf(__uint_as_float(sr[c + 1]), slj, -m_use));
-        sum0 += p;
-        sum1 += q;
-        sr[c / 2] = pack_half2(p, q);
+        for (int k = 0; k < 32; k += 2) {
+          float p, q;
+          fma2(p, q, __uint_as_float(r[k]), __uint_as_float(r[k + 1]), slj, -m_use);
+          p = ex2(p);
+          q = ex2(q);
+          add2(sum0, sum1, p, q);
+          pw[k / 2] = pack_half2(p, q);
+        }
+        ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
+      };
+      ts::tc::wait_ld(sa);
+#pragma unroll 1
+      for (int c = 0; c < n_some; c += 2) {
+        if (c + 1 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 1) * 32, sb);
+        columns(sa, c);
+        if (c + 1 == n_some) break;
+        ts::tc::wait_ld(sb);
+        if (c + 2 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 2) * 32, sa);
+        columns(sb, c + 1);
+        if (c + 2 < n_some) ts::tc::wait_ld(sa);
       }
-#pragma unroll
-      for (int c2 = 0; c2 < 2; ++c2) {
-        const uint32_t (&chunk)[32] = *reinterpret_cast<const uint32_t(*)[32]>(sr + 32 * c2);
-        ts::tc::tmem_st32(lane_base + s_col + c2 * 32, chunk);
+#pragma unroll 1
+      for (int c = n_some; c < 4; ++c) {
+        uint32_t pw[16] = {};
+        ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
       }
-      l_run = l_run * corr + (sum0 + sum1);
-      // O is in units of V's reference: it shrinks when that grows.
-      const float corr_o = j > 0 && ref_v != ref_old ? corr * (ref_old / ref_v) : corr;
+      l_run += sum0 + sum1;
       if (j > 0 && __any_sync(0xffffffffu, corr_o != 1.f)) {
-#pragma unroll
+#pragma unroll 1
         for (int c4 = 0; c4 < D / 32; ++c4) {
           uint32_t rr[32];
           ts::tc::tmem_ld32(lane_base + o_col + c4 * 32, rr);
-          ts::tc::wait_ld();
+          ts::tc::wait_ld(rr);
 #pragma unroll
           for (int c = 0; c < 32; ++c) rr[c] = __float_as_uint(__uint_as_float(rr[c]) * corr_o);
           ts::tc::tmem_st32(lane_base + o_col + c4 * 32, rr);
@@ -555,28 +606,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     ts::tc::fence_after_sync();
     if (ok) {
       const float inv = l_run > 0.f ? ref_v / (kRefScale * l_run) : l_run;
-#pragma unroll
+      // The row goes to the warp's part of its Q tile (no MMA reads it any more), 16 bytes at a
+      // time in swizzled places, and from there to memory in whole rows.
+      uint8_t* stage = sQ(x) + (warp & 3) * 32 * D * 2;
+      constexpr int kChunks = D / 8;
+#pragma unroll 1
       for (int c4 = 0; c4 < D / 32; ++c4) {
-        uint32_t rr[32];
+        uint32_t rr[32] = {};
         if (n_x > 0) {
           ts::tc::tmem_ld32(lane_base + o_col + c4 * 32, rr);
-          ts::tc::wait_ld();
-        } else {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) rr[c] = 0;
+          ts::tc::wait_ld(rr);
         }
-        if (row_valid) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + orow * D + c4 * 32);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[4];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              pk[k] = Mma::pack(__uint_as_float(rr[8 * c + 2 * k]) * inv,
-                                __uint_as_float(rr[8 * c + 2 * k + 1]) * inv);
-            dst[c] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-          }
+          for (int k = 0; k < 4; ++k)
+            pk[k] = Mma::pack(__uint_as_float(rr[8 * c + 2 * k]) * inv,
+                              __uint_as_float(rr[8 * c + 2 * k + 1]) * inv);
+          *reinterpret_cast<uint4*>(stage + lane * D * 2 + ((c4 * 4 + c) ^ (lane & 7)) * 16) =
+              make_uint4(pk[0], pk[1], pk[2], pk[3]);
         }
+      }
+      __syncwarp();
+#pragma unroll 4
+      for (int k = lane; k < 32 * kChunks; k += 32) {
+        const int w = k / kChunks, c = k % kChunks;
+        const int rr = (warp & 3) * 32 + w, ri = rr / a.group, qr = (tile0 + x) * a.tq + ri;
+        if (ri >= a.tq || qr >= q_len) continue;
+        const int64_t row = int64_t(q0 + qr) * a.num_q_heads + h * a.group + rr - ri * a.group;
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * D + c * 8) =
+            *reinterpret_cast<const uint4*>(stage + w * D * 2 + (c ^ (w & 7)) * 16);
       }
     }
   }
