@@ -21,7 +21,7 @@
 //     is kept while no score exceeds it by 2^8, so O is rarely rescaled; sums are fp32. Columns no
 //     row of a warp sees are skipped. Everything is in loops over few columns: unrolled over a
 //     whole row, the roles' code outgrew the instruction caches (a quarter of the stalls).
-//   * warp 13, one lane: tcgen05.mma, S_x = Q_x K^T and O_x += P_x V, in the order PV_A(j),
+//   * warp 13: tcgen05.mma, S_x = Q_x K^T and O_x += P_x V, in the order PV_A(j),
 //     QK_A(j+1), PV_B(j), QK_B(j+1), so one tile's softmax runs under the other's MMAs. A QK's
 //     commit covers the PV before it, so S of tile j + 1 also says that O holds tile j.
 // A page outside the pool is skipped (its columns are masked). A V row with a NaN scale is stored
@@ -85,7 +85,7 @@ struct Args {
 // for V, fp16 high and low part, or kDropped.
 struct TileInfo {
   float ref_k, ref_v;
-  uint32_t any, dropped;  // dropped: bit b, 8 + b: block b of K, of V has rows of factor kDropped
+  uint32_t any, dropped;  // dropped: bit 0, 1: K, V has rows of factor kDropped
   uint32_t skip[4], spoil[4];
   int block[kKvTile / kBlock];
   uint32_t factor[2][kKvTile];
@@ -169,42 +169,44 @@ __device__ __forceinline__ uint32_t split_factor(float f) {
   return uint32_t(__half_as_ushort(hi)) | (uint32_t(__half_as_ushort(lo)) << 16);
 }
 
-// Largest finite value over the warp's 4 x 32 scales.
-__device__ __forceinline__ float top(const float (&sc)[4]) {
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = fmaxf(m, isfinite(sc[i]) ? sc[i] : 0.f);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
+// Largest finite value of the warp's 128 scales.
+__device__ __forceinline__ float top(const float4& sc) {
+  auto fin = [](float v) { return isfinite(v) ? v : 0.f; };
+  const float m = fmaxf(fmaxf(fin(sc.x), fin(sc.y)), fmaxf(fin(sc.z), fin(sc.w)));
+  // Not negative, so they order like their bits.
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(m, 0.f))));
 }
 
-// The scout warp: describes the n_max KV tiles of (table, KV head h), n_kv visible keys.
-__device__ void scout(const Args& a, Shared* sh, const int32_t* table, int h, int n_kv, int n_max,
-                      int lane, volatile int* abort) {
+// The scout warp: describes the n_max KV tiles of (table, KV head h), n_kv visible keys. Lane l
+// looks after tokens 4 l .. 4 l + 3 of each tile, in block l / 4.
+__device__ __forceinline__ void scout(const Args& a, Shared* sh, const int32_t* table, int h,
+                                      int n_kv, int n_max, int lane, volatile int* abort) {
   constexpr int kBlocks = kKvTile / kBlock;
   const int total_blk = (n_kv + kBlock - 1) / kBlock;
+  const int64_t stride = int64_t(a.num_kv_heads) * kBlock;  // scales of a block, all heads
+  const int64_t mine = int64_t(h) * kBlock + lane % 4 * 4;
   float run_v = 0x1p-126f;  // V's reference: never below the scales seen
-  auto look_up = [&](int t) -> int {  // lane b < 8: block b of tile t (-1 none, -2 not in the pool)
-    const int b = t * kBlocks + lane;
-    if (lane >= kBlocks || b >= total_blk) return -1;
+  auto look_up = [&](int t) -> int {  // this lane's block of tile t (-1 none, -2 not in the pool)
+    const int b = t * kBlocks + lane / 4;
+    if (b >= total_blk) return -1;
     const int phys = __ldg(table + b);
     return phys >= 0 && int64_t(phys) < a.num_blocks ? phys : -2;
   };
-  int tab = look_up(0);
+  int phys = look_up(0);
+#pragma unroll 1
   for (int t = 0; t < n_max; ++t) {
     const int next = look_up(t + 1);
-    float ks[4], vs[4];
-    uint32_t skip[4], reach[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {  // tokens 32 g + lane
-      const int phys = __shfl_sync(0xffffffffu, tab, 2 * g + lane / kBlock);
-      const bool in = t * kKvTile + 32 * g + lane < n_kv;
-      const int64_t r = (int64_t(phys) * a.num_kv_heads + h) * kBlock + lane % kBlock;
-      ks[g] = in && phys >= 0 ? __ldg(a.key_scales + r) : 0.f;
-      vs[g] = in && phys >= 0 ? __ldg(a.value_scales + r) : 0.f;
-      skip[g] = __ballot_sync(0xffffffffu, in && phys == -2);
-      reach[g] = in;
+    float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;
+    if (phys >= 0) {
+      ks = __ldg(reinterpret_cast<const float4*>(a.key_scales + phys * stride + mine));
+      vs = __ldg(reinterpret_cast<const float4*>(a.value_scales + phys * stride + mine));
+    }
+    const int reach = n_kv - t * kKvTile - 4 * lane;  // of its tokens, those below n_kv
+    if (reach < 4) {
+      if (reach < 1) ks.x = vs.x = 0.f;
+      if (reach < 2) ks.y = vs.y = 0.f;
+      if (reach < 3) ks.z = vs.z = 0.f;
+      ks.w = vs.w = 0.f;
     }
     if (t >= kAhead && !wait_warp(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1, abort))
       return;
@@ -212,37 +214,46 @@ __device__ void scout(const Args& a, Shared* sh, const int32_t* table, int h, in
     const float ref_k = fmaxf(top(ks), 0x1p-126f), top_v = top(vs);
     if (top_v > run_v) run_v = fminf(top_v * kRefRoom, 0x1p127f);
     const float inv_k = 1.f / ref_k, inv_v = 1.f / run_v;
-    uint32_t any = 0, dropped = 0;
+    // A NaN K row makes NaN scores; a NaN V row is stored as zeros (see the head of the file).
+    uint32_t spoil = 0;
+    uint32_t fk[4], fv[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const uint32_t spoil = __ballot_sync(0xffffffffu, !isfinite(vs[g]));
-      any |= skip[g] | spoil;
-      if (lane == 0) {
-        info->skip[g] = skip[g];
-        info->spoil[g] = spoil;
-      }
-      // A NaN K row makes NaN scores; a NaN V row is stored as zeros (see the head of the file).
-      const float fk = ks[g] * inv_k * kRefScale, fv = vs[g] * inv_v * kRefScale;
-      const bool keep_v = reach[g] && isfinite(vs[g]);
-      info->factor[0][32 * g + lane] = reach[g] ? split_factor(fk) : kDropped;
-      info->factor[1][32 * g + lane] = keep_v ? split_factor(fv) : kDropped;
-      const uint32_t dk = ~__ballot_sync(0xffffffffu, reach[g]);
-      const uint32_t dv = ~__ballot_sync(0xffffffffu, keep_v);
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-        dropped |= uint32_t((dk >> 16 * b & 0xffffu) != 0) << (2 * g + b) |
-                   uint32_t((dv >> 16 * b & 0xffffu) != 0) << (8 + 2 * g + b);
+    for (int i = 0; i < 4; ++i) {
+      const float k = i == 0 ? ks.x : i == 1 ? ks.y : i == 2 ? ks.z : ks.w;
+      const float v = i == 0 ? vs.x : i == 1 ? vs.y : i == 2 ? vs.z : vs.w;
+      if (!isfinite(v)) spoil |= 1u << i;
+      fk[i] = i < reach ? split_factor(k * inv_k * kRefScale) : kDropped;
+      fv[i] = i < reach && isfinite(v) ? split_factor(v * inv_v * kRefScale) : kDropped;
     }
-    if (lane < kBlocks) info->block[lane] = tab;
+    *reinterpret_cast<uint4*>(&info->factor[0][4 * lane]) = make_uint4(fk[0], fk[1], fk[2], fk[3]);
+    *reinterpret_cast<uint4*>(&info->factor[1][4 * lane]) = make_uint4(fv[0], fv[1], fv[2], fv[3]);
+    if (lane % 4 == 0) info->block[lane / 4] = phys;
+    const bool any = __any_sync(0xffffffffu, spoil != 0 || phys == -2);
+    const bool past = __any_sync(0xffffffffu, reach < 4);
+    if (any) {
+      uint32_t skip = (phys == -2 ? 0xfu : 0u) << lane % 8 * 4;
+      spoil <<= lane % 8 * 4;
+#pragma unroll 1
+      for (int o = 1; o < 8; o <<= 1) {
+        skip |= __shfl_xor_sync(0xffffffffu, skip, o);
+        spoil |= __shfl_xor_sync(0xffffffffu, spoil, o);
+      }
+      if (lane % 8 == 0) {
+        info->skip[lane / 8] = skip;
+        info->spoil[lane / 8] = spoil;
+      }
+    } else if (lane < 4) {
+      info->skip[lane] = info->spoil[lane] = 0;
+    }
     if (lane == 0) {
       info->ref_k = ref_k;
       info->ref_v = run_v;
       info->any = any;
-      info->dropped = dropped;
+      info->dropped = uint32_t(past) | uint32_t(past || any) << 1;
     }
     __syncwarp();
     if (lane == 0) ts::mbar_arrive(&sh->info_full[t % kInfos]);
-    tab = next;
+    phys = next;
   }
 }
 
@@ -374,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           return false;
         const TileInfo& info = sh->info[t % kInfos];
         c.store(is_v ? sV(st) : sK(st), info.factor[is_v], k % (kUnits / 2) * kBlock,
-                info.dropped >> k & 1, lane);
+                info.dropped >> int(is_v) & 1, lane);
         ts::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -391,55 +402,58 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         if (ok && u < total) ok = convert(codes[1], u) && fetch(codes[1], u + 2 * kConverters);
         u += kConverters;
       }
-    } else if (lane == 0 && n_max > 0) {
+    } else if (n_max > 0) {
       // ---------------------------------------------------------- MMA issuer
+      // The whole warp runs it, so addresses and descriptors stay in uniform registers, and one
+      // elected lane issues.
       constexpr uint32_t idesc_qk = ts::tc::idesc_f16(false, kRows, kKvTile, false);
       constexpr uint32_t idesc_pv = ts::tc::idesc_f16(false, kRows, D, true);
+      // Low words of the shared-memory descriptors: address / 16, and V's distance between halves.
+      const uint32_t q_lo = ts::smem_u32(sQ(0)) >> 4 | 1u << 16;
+      const uint32_t k_lo = ts::smem_u32(sK(0)) >> 4 | 1u << 16;
+      const uint32_t v_lo = ts::smem_u32(sV(0)) >> 4 | uint32_t(kHalfBytes >> 4) << 16;
       // The last query tile to use KV tile j releases its K (after QK) and V (after PV).
       auto last_user = [&](int j) { return j < n_t[1] ? 1 : 0; };
-      const uint64_t dq0 = ts::tc::smem_desc_sw128(ts::smem_u32(sQ(0)), 16, 1024);
-      const uint64_t dk0 = ts::tc::smem_desc_sw128(ts::smem_u32(sK(0)), 16, 1024);
-      const uint64_t dv0 = ts::tc::smem_desc_sw128(ts::smem_u32(sV(0)), kHalfBytes, 1024);
-      auto issue_qk = [&](int x, int j) -> bool {
-        const int st = j % kStages;
-        if (!wait_bar(&sh->k_full[st], (j / kStages) & 1, abort)) return false;
-        ts::tc::fence_after_sync();
-        const uint64_t dq = dq0 + uint64_t((x * G::kTileBytes) >> 4);
-        const uint64_t dk = dk0 + uint64_t((st * G::kTileBytes) >> 4);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off16 = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
-          ts::tc::mma_ss(tmem + x * 128, dq + off16, dk + off16, idesc_qk, kk > 0);
-        }
-        ts::tc::commit(&sh->s_full[x]);
-        if (x == last_user(j) && j + kStages < n_max) ts::tc::commit(&sh->k_empty[st]);
-        return true;
-      };
-      bool ok = wait_bar(&sh->q_full, 0, abort);
-      for (int x = 0; ok && x < kQTiles; ++x)
-        if (n_t[x] > 0) ok = issue_qk(x, 0);
-      for (int j = 0; ok && j < n_max; ++j) {
-        const int st = j % kStages;
+      bool ok = wait_warp(&sh->q_full, 0, abort);
+      // Step j: PV(j - 1) then QK(j), of each query tile in turn.
+#pragma unroll 1
+      for (int j = 0; ok && j <= n_max; ++j) {
+        const int sk = j % kStages, sv = (j - 1) % kStages;
+#pragma unroll 1
         for (int x = 0; ok && x < kQTiles; ++x) {
-          if (j >= n_t[x]) continue;
-          if (!wait_bar(&sh->p_full[x], j & 1, abort) ||
-              !wait_bar(&sh->v_full[st], (j / kStages) & 1, abort)) {
-            ok = false;
-            break;
-          }
-          ts::tc::fence_after_sync();
-          const uint64_t dv = dv0 + uint64_t((st * G::kTileBytes) >> 4);
+          const int n_x = x ? n_t[1] : n_t[0];
+          if (j > 0 && j <= n_x) {
+            ok = wait_warp(&sh->p_full[x], (j - 1) & 1, abort) &&
+                 wait_warp(&sh->v_full[sv], ((j - 1) / kStages) & 1, abort);
+            if (!ok) break;
+            ts::tc::fence_after_sync();
+            const uint32_t dv = v_lo + sv * (G::kTileBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kKvTile / 16; ++kk)
-            ts::tc::mma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8,
-                           dv + uint64_t((kk * 2048) >> 4), idesc_pv, j > 0 || kk > 0);
-          if (j + 1 == n_t[x]) ts::tc::commit(&sh->pv_done[x]);
-          if (x == last_user(j) && j + kStages < n_max) ts::tc::commit(&sh->v_empty[st]);
-          if (j + 1 < n_t[x]) ok = issue_qk(x, j + 1);
+            for (int kk = 0; kk < kKvTile / 16; ++kk)
+              ts::tc::mma_ts_elect(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, dv + kk * 128,
+                                   idesc_pv, j > 1 || kk > 0);
+            if (j == n_x) ts::tc::commit_elect(&sh->pv_done[x]);
+            if (x == last_user(j - 1) && j - 1 + kStages < n_max)
+              ts::tc::commit_elect(&sh->v_empty[sv]);
+          }
+          if (j < n_x) {
+            ok = wait_warp(&sh->k_full[sk], (j / kStages) & 1, abort);
+            if (!ok) break;
+            ts::tc::fence_after_sync();
+            const uint32_t dq = q_lo + x * (G::kTileBytes >> 4);
+            const uint32_t dk = k_lo + sk * (G::kTileBytes >> 4);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
+              ts::tc::mma_ss_elect(tmem + x * 128, dq + off, dk + off, idesc_qk, kk > 0);
+            }
+            ts::tc::commit_elect(&sh->s_full[x]);
+            if (x == last_user(j) && j + kStages < n_max) ts::tc::commit_elect(&sh->k_empty[sk]);
+          }
         }
       }
-      if (*abort) {  // the MMAs in flight end before shared and tensor memory are released
-        ts::tc::commit(&sh->drain);
+      if (!ok) {  // the MMAs in flight end before shared and tensor memory are released
+        ts::tc::commit_elect(&sh->drain);
         ts::mbar_wait_bounded(&sh->drain, 0);
       }
     }
@@ -448,7 +462,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     const int x = warp / 4;               // query tile of this warpgroup
     const int r = threadIdx.x - 128 * x;  // tile row == TMEM lane
     const int n_x = n_t[x];
-    const int i = r / a.group;
+    // Token of a tile row, rr / group: exact in fp32 for rows below 128.
+    const float inv_group = 1.f / float(a.group);
+    auto row_token = [&](int rr) { return int((float(rr) + 0.5f) * inv_group); };
+    const int i = row_token(r);
     const int qi = (tile0 + x) * a.tq + i;
     const bool row_valid = i < a.tq && qi < q_len;
     const int pos = row_valid ? p0 + qi : p0 + q_len - 1;
@@ -461,46 +478,43 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     {
       constexpr int kLanes = D / 8, kRpi = 32 / kLanes;
       const int c = lane % kLanes;
-      auto load_row = [&](int it) -> uint4 {
-        const int rr = (warp & 3) * 32 + it * kRpi + lane / kLanes;
-        const int ri = rr / a.group, qr = (tile0 + x) * a.tq + ri;
-        if (ri >= a.tq || qr >= q_len) return make_uint4(0, 0, 0, 0);
-        return __ldg(reinterpret_cast<const uint4*>(
-                         static_cast<const T*>(a.query) + int64_t(q0 + qr) * a.q_stride +
-                         int64_t(h * a.group + rr - ri * a.group) * D) + c);
-      };
-      constexpr int kBatch = 4;  // loads in flight
+      uint8_t* q_warp = sQ(x) + (warp & 3) * 32 * 128 + (c >> 3) * kHalfBytes;
+      auto place = [&](int w) { return q_warp + w * 128 + (((c & 7) ^ (w & 7)) << 4); };
+      // Rows as they are, all loads in flight at once, then converted in place.
 #pragma unroll 1
-      for (int it0 = 0; it0 < kLanes; it0 += kBatch) {  // 32 / kRpi = kLanes load instructions
-        uint4 v[kBatch];
+      for (int w = lane / kLanes; w < 32; w += kRpi) {
+        const int rr = (warp & 3) * 32 + w, ri = row_token(rr), qr = (tile0 + x) * a.tq + ri;
+        const bool in = ri < a.tq && qr < q_len;
+        const T* src = static_cast<const T*>(a.query);
+        if (in) src += int64_t(q0 + qr) * a.q_stride + int64_t(h * a.group + rr - ri * a.group) * D + c * 8;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ts::smem_u32(place(w))),
+                     "l"(src), "r"(in ? 16 : 0)
+                     : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      const float base = fabsf(a.scale_log2) / kRefScale;
+#pragma unroll 2
+      for (int w = lane / kLanes; w < 32; w += kRpi) {
+        uint4* at = reinterpret_cast<uint4*>(place(w));
+        const uint4 v = *at;
+        const uint32_t wds[4] = {v.x, v.y, v.z, v.w};
+        float f[8];
+        uint32_t m = 0;
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) v[b] = load_row(it0 + b);
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-          const uint32_t wds[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
-          uint32_t m = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = Mma::unpack(wds[k]);
-            m = max(m, max(ts::abs_bits(f.x), ts::abs_bits(f.y)));
-          }
-#pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const int e = max(int(m >> 23), 27);  // biased exponent; tiny rows keep a finite factor
-          const float up =
-              copysignf(__uint_as_float(uint32_t(127 + 14 + 127 - e) << 23), a.scale_log2);
-          const int my = __shfl_sync(0xffffffffu, e, lane % kRpi * kLanes);
-          if (lane / kRpi == it0 + b) sl = ldexpf(fabsf(a.scale_log2) / kRefScale, my - 127 - 14);
-          uint32_t o[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = Mma::unpack(wds[k]);
-            o[k] = pack_half2(f.x * up, f.y * up);
-          }
-          const int rr = (warp & 3) * 32 + (it0 + b) * kRpi + lane / kLanes;
-          *reinterpret_cast<uint4*>(sQ(x) + rr * 128 + (c >> 3) * kHalfBytes +
-                                    (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int k = 0; k < 4; ++k) {
+          const float2 u = Mma::unpack(wds[k]);
+          f[2 * k] = u.x;
+          f[2 * k + 1] = u.y;
+          m = max(m, max(ts::abs_bits(u.x), ts::abs_bits(u.y)));
         }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int e = max(int(m >> 23), 27);  // biased exponent; tiny rows keep a finite factor
+        const float up = copysignf(__uint_as_float(uint32_t(127 + 14 + 127 - e) << 23), a.scale_log2);
+        const int my = __shfl_sync(0xffffffffu, e, lane % kRpi * kLanes);
+        if (lane / kRpi == w / kRpi) sl = base * __uint_as_float(uint32_t(my - 14) << 23);
+        *at = make_uint4(pack_half2(f[0] * up, f[1] * up), pack_half2(f[2] * up, f[3] * up),
+                         pack_half2(f[4] * up, f[5] * up), pack_half2(f[6] * up, f[7] * up));
       }
       ts::fence_proxy_async_smem();
       ts::mbar_arrive(&sh->q_full);
@@ -535,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           r[k] = keep >> k & 1 ? z : __float_as_uint(-INFINITY);
         }
       };
-      uint32_t sa[32], sb[32];
+      uint32_t sa[32];
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       ts::tc::tmem_ld32(lane_base + s_col, sa);
 #pragma unroll 1
@@ -556,30 +570,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       }
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
       float sum0 = 0.f, sum1 = 0.f;
-      auto columns = [&](uint32_t (&r)[32], int c) {  // P of columns 32 c .. 32 c + 31
-        if (c >= n_whole) mask(r, c);
+#pragma unroll 1
+      for (int c = 0; c < n_some; ++c) {  // P of columns 32 c .. 32 c + 31
+        ts::tc::wait_ld(sa);
+        if (c >= n_whole) mask(sa, c);
+        float e[32];
+#pragma unroll
+        for (int k = 0; k < 32; k += 2)
+          fma2(e[k], e[k + 1], __uint_as_float(sa[k]), __uint_as_float(sa[k + 1]), slj, -m_use);
+        if (c + 1 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 1) * 32, sa);
         uint32_t pw[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          float p, q;
-          fma2(p, q, __uint_as_float(r[k]), __uint_as_float(r[k + 1]), slj, -m_use);
-          p = ex2(p);
-          q = ex2(q);
+          const float p = ex2(e[k]), q = ex2(e[k + 1]);
           add2(sum0, sum1, p, q);
           pw[k / 2] = pack_half2(p, q);
         }
         ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
-      };
-      ts::tc::wait_ld(sa);
-#pragma unroll 1
-      for (int c = 0; c < n_some; c += 2) {
-        if (c + 1 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 1) * 32, sb);
-        columns(sa, c);
-        if (c + 1 == n_some) break;
-        ts::tc::wait_ld(sb);
-        if (c + 2 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 2) * 32, sa);
-        columns(sb, c + 1);
-        if (c + 2 < n_some) ts::tc::wait_ld(sa);
       }
 #pragma unroll 1
       for (int c = n_some; c < 4; ++c) {
@@ -629,10 +636,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         }
       }
       __syncwarp();
-#pragma unroll 4
+#pragma unroll 2
       for (int k = lane; k < 32 * kChunks; k += 32) {
         const int w = k / kChunks, c = k % kChunks;
-        const int rr = (warp & 3) * 32 + w, ri = rr / a.group, qr = (tile0 + x) * a.tq + ri;
+        const int rr = (warp & 3) * 32 + w, ri = row_token(rr), qr = (tile0 + x) * a.tq + ri;
         if (ri >= a.tq || qr >= q_len) continue;
         const int64_t row = int64_t(q0 + qr) * a.num_q_heads + h * a.group + rr - ri * a.group;
         *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * D + c * 8) =
@@ -649,11 +656,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
 }
 
 bool tc_path(int group, int hkv, int hd, int bs, int dtype, const void* kp, const void* vp,
-             const void* q, int64_t q_stride, const void* out, int num_seqs) {
+             const void* ks, const void* vs, const void* q, int64_t q_stride, const void* out, int num_seqs) {
   if (dtype != TS_BFLOAT16 && dtype != TS_FLOAT16) return false;
   if ((hd != 64 && hd != 128) || bs != kBlock || group > kRows) return false;
   if (num_seqs > 65535 || hkv > 65535) return false;
   if ((reinterpret_cast<uint64_t>(kp) | reinterpret_cast<uint64_t>(vp) |
+       reinterpret_cast<uint64_t>(ks) | reinterpret_cast<uint64_t>(vs) |
        reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(out)) % 16)
     return false;
   return (q_stride * 2) % 16 == 0;
@@ -703,8 +711,8 @@ extern "C" int ts_paged_prefill_fp8(void* out, const void* query, int64_t query_
     return ts::set_error(TS_ERR_MISALIGNED, "paged_prefill_fp8: pointers not element-aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int group = num_q_heads / num_kv_heads;
-  if (!tc_path(group, num_kv_heads, head_dim, block_size, dtype, key_pool, value_pool, query,
-               query_token_stride, out, num_seqs))
+  if (!tc_path(group, num_kv_heads, head_dim, block_size, dtype, key_pool, value_pool,
+               key_scales, value_scales, query, query_token_stride, out, num_seqs))
     return ts::paged_attention_portable(out, query, query_token_stride, key_pool, value_pool,
                                         block_tables, max_blocks_per_seq, query_start_loc,
                                         context_lens, num_seqs, num_query_tokens, num_q_heads,
