@@ -17,9 +17,10 @@
 //     on the tile's scores; when V's grows, O is rescaled.
 //   * warps 0-3 / 4-7 (softmax, one warpgroup per query tile, thread = row): q's row is scaled by a
 //     power of two into fp16's range and written to shared memory; then per tile, 32 columns at a
-//     time: the row's maximum, then 2^(s - m), P in fp16 (11 bits) back to TMEM over S. The maximum
-//     is kept while no score exceeds it by 2^8, so O is rarely rescaled; sums are fp32. Columns no
-//     row of a warp sees are skipped. Everything is in loops over few columns: unrolled over a
+//     time: 2^(s - m), P in fp16 (11 bits) back to TMEM over S, sums in fp32. m is the maximum of
+//     the row's first tile and is kept while no score exceeds it by 2^8, so the exponentials wait
+//     for no maximum; a warp with a row past that takes the columns, and all before them, to the
+//     new maximum. Columns no row of a warp sees are skipped. Everything is in loops over few columns: unrolled over a
 //     whole row, the roles' code outgrew the instruction caches (a quarter of the stalls).
 //   * warp 13: tcgen05.mma, S_x = Q_x K^T and O_x += P_x V, in the order PV_A(j),
 //     QK_A(j+1), PV_B(j), QK_B(j+1), so one tile's softmax runs under the other's MMAs. A QK's
@@ -144,12 +145,22 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// (d0, d1) = (a0, a1) * b + c, and (s0, s1) += (a0, a1): one packed instruction each.
-__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b, float c) {
+// Maximum of 32 floats given as bits.
+__device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int k = 0; k < 32; k += 2)
+    m[k / 2 % 4] = max3f(m[k / 2 % 4], __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
+  return fmaxf(max3f(m[0], m[1], m[2]), m[3]);
+}
+
+// (d0, d1) = (a0, a1) * b + c on bits, and (s0, s1) += (a0, a1): one packed instruction each.
+__device__ __forceinline__ void fma2(uint32_t& d0, uint32_t& d1, uint32_t a0, uint32_t a1, float b,
+                                     float c) {
   asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\t"
       "mov.b64 z, {%5, %5};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=f"(d0), "=f"(d1)
-      : "f"(a0), "f"(a1), "f"(b), "f"(c));
+      : "=r"(d0), "=r"(d1)
+      : "r"(a0), "r"(a1), "f"(b), "f"(c));
 }
 __device__ __forceinline__ void add2(float& s0, float& s1, float a0, float a1) {
   asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
@@ -481,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       uint8_t* q_warp = sQ(x) + (warp & 3) * 32 * 128 + (c >> 3) * kHalfBytes;
       auto place = [&](int w) { return q_warp + w * 128 + (((c & 7) ^ (w & 7)) << 4); };
       // Rows as they are, all loads in flight at once, then converted in place.
-#pragma unroll 1
+#pragma unroll 4
       for (int w = lane / kLanes; w < 32; w += kRpi) {
         const int rr = (warp & 3) * 32 + w, ri = row_token(rr), qr = (tile0 + x) * a.tq + ri;
         const bool in = ri < a.tq && qr < q_len;
@@ -493,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       const float base = fabsf(a.scale_log2) / kRefScale;
-#pragma unroll 2
+#pragma unroll 4
       for (int w = lane / kLanes; w < 32; w += kRpi) {
         uint4* at = reinterpret_cast<uint4*>(place(w));
         const uint4 v = *at;
@@ -550,39 +561,58 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         }
       };
       uint32_t sa[32];
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       ts::tc::tmem_ld32(lane_base + s_col, sa);
+      if (__any_sync(0xffffffffu, m_run == -INFINITY)) {  // a row that has seen nothing yet
+        float m = -INFINITY;
 #pragma unroll 1
-      for (int c = 0; c < n_some; ++c) {
-        ts::tc::wait_ld(sa);
-        if (c >= n_whole) mask(sa, c);
-#pragma unroll
-        for (int k = 0; k < 32; k += 2)
-          mx[k / 2 % 4] = max3f(mx[k / 2 % 4], __uint_as_float(sa[k]), __uint_as_float(sa[k + 1]));
-        ts::tc::tmem_ld32(lane_base + s_col + (c + 1 < n_some ? c + 1 : 0) * 32, sa);
+        for (int c = 0; c < n_some; ++c) {
+          ts::tc::wait_ld(sa);
+          if (c >= n_whole) mask(sa, c);
+          m = fmaxf(m, max32(sa));
+          ts::tc::tmem_ld32(lane_base + s_col + (c + 1 < n_some ? c + 1 : 0) * 32, sa);
+        }
+        if (m_run == -INFINITY) m_run = m * slj;
       }
-      const float m_tile = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * slj;
-      if (m_tile > m_run + kRescaleSlack || m_run == -INFINITY) {
-        const float f = m_run == -INFINITY ? 1.f : ex2(m_run - m_tile);  // all so far is 0
-        l_run *= f;
-        corr_o *= f;
-        m_run = m_tile;
-      }
-      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+      float m_use = m_run == -INFINITY ? 0.f : m_run;
       float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll 1
       for (int c = 0; c < n_some; ++c) {  // P of columns 32 c .. 32 c + 31
         ts::tc::wait_ld(sa);
         if (c >= n_whole) mask(sa, c);
-        float e[32];
+        uint32_t e[32];  // log2 of P
 #pragma unroll
         for (int k = 0; k < 32; k += 2)
-          fma2(e[k], e[k + 1], __uint_as_float(sa[k]), __uint_as_float(sa[k + 1]), slj, -m_use);
+          fma2(e[k], e[k + 1], sa[k], sa[k + 1], slj, -m_use);
         if (c + 1 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 1) * 32, sa);
+        const float over = max32(e);
+        if (__any_sync(0xffffffffu, over > kRescaleSlack)) {
+          const float up = over > kRescaleSlack ? over : 0.f, f = ex2(-up);
+          m_run += up;
+          m_use = m_run;
+          l_run *= f;
+          sum0 *= f;
+          sum1 *= f;
+          corr_o *= f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) e[k] = __float_as_uint(__uint_as_float(e[k]) - up);
+#pragma unroll 1
+          for (int b = 0; b < c; ++b) {  // the tile's P so far
+            uint32_t pw[16];
+            ts::tc::wait_st();
+            ts::tc::tmem_ld16(lane_base + s_col + b * 16, pw);
+            ts::tc::wait_ld(pw);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&pw[k]));
+              pw[k] = pack_half2(v.x * f, v.y * f);
+            }
+            ts::tc::tmem_st16(lane_base + s_col + b * 16, pw);
+          }
+        }
         uint32_t pw[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          const float p = ex2(e[k]), q = ex2(e[k + 1]);
+          const float p = ex2(__uint_as_float(e[k])), q = ex2(__uint_as_float(e[k + 1]));
           add2(sum0, sum1, p, q);
           pw[k / 2] = pack_half2(p, q);
         }
@@ -636,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         }
       }
       __syncwarp();
-#pragma unroll 2
+#pragma unroll 4
       for (int k = lane; k < 32 * kChunks; k += 32) {
         const int w = k / kChunks, c = k % kChunks;
         const int rr = (warp & 3) * 32 + w, ri = row_token(rr), qr = (tile0 + x) * a.tq + ri;
