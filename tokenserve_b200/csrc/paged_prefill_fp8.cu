@@ -343,6 +343,33 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   volatile int* abort = &sh->abort;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  // Token of a tile row, row / group: exact in fp32 for rows below 128.
+  const float inv_group = 1.f / float(a.group);
+  auto row_token = [&](int row) { return int((float(row) + 0.5f) * inv_group); };
+  // The softmax warps' queries as they are, 16 bytes a lane and D / 8 lanes a row, on their way
+  // while the barriers and tensor memory are set up.
+  constexpr int kQLanes = D / 8, kQRows = 32 / kQLanes;
+  auto q_place = [&](int w) {  // this lane's 16 bytes of row w of the warp's 32
+    const int c = lane % kQLanes;
+    return sQ(warp / 4 & 1) + (warp & 3) * 32 * 128 + (c >> 3) * kHalfBytes + w * 128 +
+           (((c & 7) ^ (w & 7)) << 4);
+  };
+  if (warp < 4 * kQTiles) {
+#pragma unroll 4
+    for (int w = lane / kQLanes; w < 32; w += kQRows) {
+      const int row = (warp & 3) * 32 + w, token = row_token(row);
+      const int q = (tile0 + warp / 4) * a.tq + token;
+      const bool in = token < a.tq && q < q_len;
+      const T* src = static_cast<const T*>(a.query);
+      if (in)
+        src += int64_t(q0 + q) * a.q_stride + (h * a.group + row - token * a.group) * D +
+               lane % kQLanes * 8;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ts::smem_u32(q_place(w))),
+                   "l"(src), "r"(in ? 16 : 0)
+                   : "memory");
+    }
+  }
   if (threadIdx.x == 0) {
     ts::mbar_init(&sh->q_full, 128 * kQTiles);
     for (int i = 0; i < kStages; ++i) {
@@ -473,9 +500,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     const int x = warp / 4;               // query tile of this warpgroup
     const int r = threadIdx.x - 128 * x;  // tile row == TMEM lane
     const int n_x = n_t[x];
-    // Token of a tile row, rr / group: exact in fp32 for rows below 128.
-    const float inv_group = 1.f / float(a.group);
-    auto row_token = [&](int rr) { return int((float(rr) + 0.5f) * inv_group); };
     const int i = row_token(r);
     const int qi = (tile0 + x) * a.tq + i;
     const bool row_valid = i < a.tq && qi < q_len;
@@ -487,45 +511,44 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     // scale, whose sign goes with q). A warp loads its 32 rows 16 bytes a lane, D / 8 lanes a row.
     float sl = 0.f;
     {
-      constexpr int kLanes = D / 8, kRpi = 32 / kLanes;
-      const int c = lane % kLanes;
-      uint8_t* q_warp = sQ(x) + (warp & 3) * 32 * 128 + (c >> 3) * kHalfBytes;
-      auto place = [&](int w) { return q_warp + w * 128 + (((c & 7) ^ (w & 7)) << 4); };
-      // Rows as they are, all loads in flight at once, then converted in place.
-#pragma unroll 4
-      for (int w = lane / kLanes; w < 32; w += kRpi) {
-        const int rr = (warp & 3) * 32 + w, ri = row_token(rr), qr = (tile0 + x) * a.tq + ri;
-        const bool in = ri < a.tq && qr < q_len;
-        const T* src = static_cast<const T*>(a.query);
-        if (in) src += int64_t(q0 + qr) * a.q_stride + int64_t(h * a.group + rr - ri * a.group) * D + c * 8;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ts::smem_u32(place(w))),
-                     "l"(src), "r"(in ? 16 : 0)
-                     : "memory");
-      }
       asm volatile("cp.async.wait_all;" ::: "memory");
       const float base = fabsf(a.scale_log2) / kRefScale;
-#pragma unroll 4
-      for (int w = lane / kLanes; w < 32; w += kRpi) {
-        uint4* at = reinterpret_cast<uint4*>(place(w));
-        const uint4 v = *at;
-        const uint32_t wds[4] = {v.x, v.y, v.z, v.w};
-        float f[8];
-        uint32_t m = 0;
+      constexpr int kBatch = 4;  // rows of a lane at a time
+#pragma unroll 1
+      for (int w0 = lane / kQLanes; w0 < 32; w0 += kBatch * kQRows) {
+        uint4 v[kBatch];
+        uint32_t m[kBatch];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 u = Mma::unpack(wds[k]);
-          f[2 * k] = u.x;
-          f[2 * k + 1] = u.y;
-          m = max(m, max(ts::abs_bits(u.x), ts::abs_bits(u.y)));
+        for (int b = 0; b < kBatch; ++b) v[b] = *reinterpret_cast<const uint4*>(q_place(w0 + b * kQRows));
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          const uint32_t wds[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+          m[b] = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 u = Mma::unpack(wds[k]);
+            m[b] = max(m[b], max(ts::abs_bits(u.x), ts::abs_bits(u.y)));
+          }
         }
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const int e = max(int(m >> 23), 27);  // biased exponent; tiny rows keep a finite factor
-        const float up = copysignf(__uint_as_float(uint32_t(127 + 14 + 127 - e) << 23), a.scale_log2);
-        const int my = __shfl_sync(0xffffffffu, e, lane % kRpi * kLanes);
-        if (lane / kRpi == w / kRpi) sl = base * __uint_as_float(uint32_t(my - 14) << 23);
-        *at = make_uint4(pack_half2(f[0] * up, f[1] * up), pack_half2(f[2] * up, f[3] * up),
-                         pack_half2(f[4] * up, f[5] * up), pack_half2(f[6] * up, f[7] * up));
+        for (int o = kQLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) m[b] = max(m[b], __shfl_xor_sync(0xffffffffu, m[b], o));
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          const int e = max(int(m[b] >> 23), 27);  // biased exponent; tiny rows keep a finite factor
+          const float up = copysignf(__uint_as_float(uint32_t(127 + 14 + 127 - e) << 23), a.scale_log2);
+          const int my = __shfl_sync(0xffffffffu, e, lane % kQRows * kQLanes);
+          if (lane / kQRows == w0 / kQRows + b) sl = base * __uint_as_float(uint32_t(my - 14) << 23);
+          const uint32_t wds[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 u = Mma::unpack(wds[k]);
+            o[k] = pack_half2(u.x * up, u.y * up);
+          }
+          *reinterpret_cast<uint4*>(q_place(w0 + b * kQRows)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
       }
       ts::fence_proxy_async_smem();
       ts::mbar_arrive(&sh->q_full);
@@ -666,14 +689,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         }
       }
       __syncwarp();
-#pragma unroll 4
-      for (int k = lane; k < 32 * kChunks; k += 32) {
-        const int w = k / kChunks, c = k % kChunks;
-        const int rr = (warp & 3) * 32 + w, ri = row_token(rr), qr = (tile0 + x) * a.tq + ri;
-        if (ri >= a.tq || qr >= q_len) continue;
-        const int64_t row = int64_t(q0 + qr) * a.num_q_heads + h * a.group + rr - ri * a.group;
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * D + c * 8) =
-            *reinterpret_cast<const uint4*>(stage + w * D * 2 + (c ^ (w & 7)) * 16);
+#pragma unroll 1
+      for (int w0 = lane / kChunks; w0 < 32; w0 += 4 * kQRows) {
+        uint4 v[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int w = w0 + b * kQRows;
+          v[b] = *reinterpret_cast<const uint4*>(stage + w * D * 2 + (lane % kChunks ^ (w & 7)) * 16);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int row = (warp & 3) * 32 + w0 + b * kQRows, token = row_token(row);
+          const int q = (tile0 + x) * a.tq + token;
+          if (token < a.tq && q < q_len)
+            *reinterpret_cast<uint4*>(
+                static_cast<T*>(a.out) +
+                (int64_t(q0 + q) * a.num_q_heads + h * a.group + row - token * a.group) * D +
+                lane % kChunks * 8) = v[b];
+        }
       }
     }
   }
