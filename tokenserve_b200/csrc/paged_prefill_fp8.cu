@@ -7,24 +7,25 @@
 // and by the exponentials (one per score), so the cache's 8 bits must cost neither of them:
 //   * CTA = (sequence, KV head, pair of query tiles); a tile's 128 rows are 128/G tokens x the G
 //     query heads of the KV head, so a converted K/V tile serves 256 rows.
-//   * warp 12 (scout) runs up to four KV tiles (128 tokens) ahead: block table, the tile's scales,
-//     each row's factor and the tile's references, left in shared memory.
-//   * warps 8-11, 14, 15 (converters) take a tile's 16 blocks (8 of K, 8 of V) in turn: codes from
+//   * warp 12 (scout) runs up to four spans of 128 tokens ahead: block table, the span's scales,
+//     each row's factor and the span's references, left in shared memory.
+//   * warps 8-11, 14, 15 (converters) take the blocks of 64-token tiles (4 of K, 4 of V) in turn: codes from
 //     global memory two blocks ahead into registers, times the row's factor, as fp16 into the
-//     swizzled layout the MMAs read. Values are relative to the tile's largest scale (K) or the
+//     swizzled layout the MMAs read. Values are relative to the span's largest scale (K) or the
 //     largest so far (V) times 2^-7, so they fill fp16's range whatever their magnitude; a factor
 //     is two fp16 parts, so a value is rounded once, to 2^-11 of itself. K's reference is a factor
 //     on the tile's scores; when V's grows, O is rescaled.
 //   * warps 0-3 / 4-7 (softmax, one warpgroup per query tile, thread = row): q's row is scaled by a
 //     power of two into fp16's range and written to shared memory; then per tile, 32 columns at a
 //     time: 2^(s - m), P in fp16 (11 bits) back to TMEM over S, sums in fp32. m is the maximum of
-//     the row's first tile and is kept while no score exceeds it by 2^8, so the exponentials wait
+//     the row's first tile and is kept while no score exceeds it by 2^14, so the exponentials wait
 //     for no maximum; a warp with a row past that takes the columns, and all before them, to the
 //     new maximum. Columns no row of a warp sees are skipped. Everything is in loops over few columns: unrolled over a
 //     whole row, the roles' code outgrew the instruction caches (a quarter of the stalls).
-//   * warp 13: tcgen05.mma, S_x = Q_x K^T and O_x += P_x V, in the order PV_A(j),
-//     QK_A(j+1), PV_B(j), QK_B(j+1), so one tile's softmax runs under the other's MMAs. A QK's
-//     commit covers the PV before it, so S of tile j + 1 also says that O holds tile j.
+//   * warp 13: tcgen05.mma, S_x = Q_x K^T and O_x += P_x V, in the order PV_A(j), QK_A(j+2),
+//     PV_B(j), QK_B(j+2): each query tile has two S buffers of 64 columns, so its softmax finds the
+//     next tile's scores ready and waits for no MMA (with one buffer of 128 columns a tile's
+//     softmax, PV and QK took turns: 5,000 clocks per 128 tokens).
 // A page outside the pool is skipped (its columns are masked). A V row with a NaN scale is stored
 // as zeros and its column's weight set to NaN for the rows that see it, so rows before it in the
 // chunk stay clean. Tokens past the last visible key are stored as zeros: their slots may hold
@@ -43,23 +44,29 @@ int paged_attention_portable(void* out, const void* query, int64_t q_stride, con
 namespace {
 
 constexpr int kRows = 128;    // query rows per tile (M)
-constexpr int kKvTile = 128;  // KV tokens per tile (N of QK, K of PV)
+constexpr int kKvTile = 64;   // KV tokens per tile (N of QK, K of PV)
+constexpr int kSpan = 128;    // KV tokens the scout describes at a time
 constexpr int kBlock = 16;    // tokens per KV block
-constexpr int kHalfBytes = 128 * 128;  // 128 rows x 64 fp16 columns
+constexpr int kQHalf = kRows * 128;     // bytes of 64 fp16 columns of a query tile
+constexpr int kKvHalf = kKvTile * 128;  // and of a KV tile
 constexpr int kQTiles = 2;
-constexpr int kStages = 2;  // K ring, and V ring
-// Tile descriptions. The scout writes tile t once the converters are done with t - kAhead, when
-// the MMAs, and so the softmaxes, are done with t - kAhead - kStages.
+constexpr int kStages = 4;  // K ring, and V ring
+constexpr int kTilesPerSpan = kSpan / kKvTile;
+// Span descriptions. The scout writes span t once the converters are done with t - kAhead, when
+// the MMAs, and so the softmaxes, are done with kStages tiles before that.
 constexpr int kInfos = 8, kAhead = 4;
-static_assert(kAhead + kStages <= kInfos, "a description outlives its readers");
+static_assert(kAhead + kStages / kTilesPerSpan < kInfos, "a description outlives its readers");
 constexpr int kConverters = 6;  // converter warps
 constexpr int kUnits = 2 * kKvTile / kBlock;  // blocks of a tile, K then V
 constexpr int kThreads = 512;
-constexpr int kMaxTries = 1 << 22;  // of a bounded wait
+constexpr int kMaxTries = 1 << 22, kMaxNaps = 1 << 22;  // of a bounded wait
 constexpr uint32_t kDropped = 0x80008000u;  // factor of a row whose codes are not used
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescaleSlack = 8.f;  // keep a stale row max unless exceeded by 2^8
-constexpr uint32_t kTmemCols = 512;   // S_A [0,128), S_B [128,256), O_A [256,384), O_B [384,512)
+// A stale row max is kept unless exceeded by 2^14: P stays below fp16's 2^16, and weights near the
+// true maximum, at least 1, well inside its normal range.
+constexpr float kRescaleSlack = 14.f;
+// S_A [0,128) and S_B [128,256), two buffers each, O_A [256,384), O_B [384,512).
+constexpr uint32_t kTmemCols = 512;
 constexpr float kRefScale = 128.f;    // fp16 values are code * scale / ref * 128 <= 57344
 // V's reference starts, and grows, to this times the scales seen, so that it seldom grows.
 constexpr float kRefRoom = 8.f;
@@ -81,20 +88,20 @@ struct Args {
   float scale_log2;
 };
 
-// A KV tile as the scout leaves it: references of K and V, the columns to mask (page outside the
+// A span as the scout leaves it: references of K and V, the columns to mask (page outside the
 // pool) or to spoil (V row NaN), if any; the blocks (negative: none); each row's factor for K and
 // for V, fp16 high and low part, or kDropped.
 struct TileInfo {
   float ref_k, ref_v;
   uint32_t any, dropped;  // dropped: bit 0, 1: K, V has rows of factor kDropped
   uint32_t skip[4], spoil[4];
-  int block[kKvTile / kBlock];
-  uint32_t factor[2][kKvTile];
+  int block[kSpan / kBlock];
+  uint32_t factor[2][kSpan];
 };
 
 struct Shared {
   uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[kQTiles], p_full[kQTiles], pv_done[kQTiles], drain;
+  uint64_t s_full[kQTiles][2], p_full[kQTiles][2], pv_done[kQTiles], o_full[kQTiles], drain;
   uint64_t info_full[kInfos], converted[kAhead];
   TileInfo info[kInfos];
   uint32_t tmem;
@@ -103,8 +110,8 @@ struct Shared {
 
 template <int D>
 struct Geo {
-  static constexpr int kTileBytes = 128 * D * 2;
-  static constexpr int kTiles = (kQTiles + 2 * kStages) * kTileBytes;
+  static constexpr int kQBytes = kRows * D * 2, kKvBytes = kKvTile * D * 2;
+  static constexpr int kTiles = kQTiles * kQBytes + 2 * kStages * kKvBytes;
   static constexpr int kSmemBytes = kTiles + int(sizeof(Shared)) + 1024;
 };
 
@@ -112,9 +119,16 @@ struct Geo {
 // gives up. A loop of few instructions: there are many waits, and all roles share the caches.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, volatile int* abort) {
   uint32_t ok;
+  // Four tries a turn of the loop: two instructions a try instead of six.
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %3;\n"
       "TRY:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "@p bra DONE;\n\t"
       "sub.u32 n, n, 1;\n\t"
@@ -123,10 +137,21 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, volatile
       "DONE:\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(ts::smem_u32(bar)), "r"(phase), "n"(kMaxTries)
+      : "r"(ts::smem_u32(bar)), "r"(phase), "n"(kMaxTries / 4)
       : "memory");
   if (!ok) *abort = 1;
   return ok != 0;
+}
+// For the warps that run ahead: naps between tries leave the issue slots to the others.
+__device__ __forceinline__ bool wait_ahead(uint64_t* bar, uint32_t phase, volatile int* abort) {
+  bool ok = ts::mbar_try_wait(bar, phase);
+#pragma unroll 1
+  for (int i = 0; !ok && i < kMaxNaps; ++i) {
+    __nanosleep(100);
+    ok = ts::mbar_try_wait(bar, phase);
+  }
+  if (!ok) *abort = 1;
+  return __all_sync(0xffffffffu, ok);
 }
 // The same for a whole warp, with one answer.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase, volatile int* abort) {
@@ -154,19 +179,31 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
   return fmaxf(max3f(m[0], m[1], m[2]), m[3]);
 }
 
-// (d0, d1) = (a0, a1) * b + c on bits, and (s0, s1) += (a0, a1): one packed instruction each.
-__device__ __forceinline__ void fma2(uint32_t& d0, uint32_t& d1, uint32_t a0, uint32_t a1, float b,
-                                     float c) {
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\t"
-      "mov.b64 z, {%5, %5};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=r"(d0), "=r"(d1)
-      : "r"(a0), "r"(a1), "f"(b), "f"(c));
+// Pairs of floats, for the packed fp32 instructions.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
 }
-__device__ __forceinline__ void add2(float& s0, float& s1, float a0, float a1) {
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
-      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(s0), "+f"(s1)
-      : "f"(a0), "f"(a1));
+__device__ __forceinline__ uint64_t two(uint32_t a, uint32_t b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+  return v;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -188,16 +225,17 @@ __device__ __forceinline__ float top(const float4& sc) {
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(m, 0.f))));
 }
 
-// The scout warp: describes the n_max KV tiles of (table, KV head h), n_kv visible keys. Lane l
-// looks after tokens 4 l .. 4 l + 3 of each tile, in block l / 4.
+// The scout warp: describes the spans of (table, KV head h), n_kv visible keys. Lane l looks after
+// tokens 4 l .. 4 l + 3 of each span, in block l / 4.
 __device__ __forceinline__ void scout(const Args& a, Shared* sh, const int32_t* table, int h,
-                                      int n_kv, int n_max, int lane, volatile int* abort) {
-  constexpr int kBlocks = kKvTile / kBlock;
+                                      int n_kv, int lane, volatile int* abort) {
+  constexpr int kBlocks = kSpan / kBlock;
+  const int spans = (n_kv + kSpan - 1) / kSpan;
   const int total_blk = (n_kv + kBlock - 1) / kBlock;
   const int64_t stride = int64_t(a.num_kv_heads) * kBlock;  // scales of a block, all heads
   const int64_t mine = int64_t(h) * kBlock + lane % 4 * 4;
   float run_v = 0x1p-126f;  // V's reference: never below the scales seen
-  auto look_up = [&](int t) -> int {  // this lane's block of tile t (-1 none, -2 not in the pool)
+  auto look_up = [&](int t) -> int {  // this lane's block of span t (-1 none, -2 not in the pool)
     const int b = t * kBlocks + lane / 4;
     if (b >= total_blk) return -1;
     const int phys = __ldg(table + b);
@@ -205,21 +243,21 @@ __device__ __forceinline__ void scout(const Args& a, Shared* sh, const int32_t* 
   };
   int phys = look_up(0);
 #pragma unroll 1
-  for (int t = 0; t < n_max; ++t) {
+  for (int t = 0; t < spans; ++t) {
     const int next = look_up(t + 1);
     float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;
     if (phys >= 0) {
       ks = __ldg(reinterpret_cast<const float4*>(a.key_scales + phys * stride + mine));
       vs = __ldg(reinterpret_cast<const float4*>(a.value_scales + phys * stride + mine));
     }
-    const int reach = n_kv - t * kKvTile - 4 * lane;  // of its tokens, those below n_kv
+    const int reach = n_kv - t * kSpan - 4 * lane;  // of its tokens, those below n_kv
     if (reach < 4) {
       if (reach < 1) ks.x = vs.x = 0.f;
       if (reach < 2) ks.y = vs.y = 0.f;
       if (reach < 3) ks.z = vs.z = 0.f;
       ks.w = vs.w = 0.f;
     }
-    if (t >= kAhead && !wait_warp(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1, abort))
+    if (t >= kAhead && !wait_ahead(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1, abort))
       return;
     TileInfo* info = &sh->info[t % kInfos];
     const float ref_k = fmaxf(top(ks), 0x1p-126f), top_v = top(vs);
@@ -284,13 +322,14 @@ struct Codes {
       for (int hf = 0; hf < kHalves; ++hf)
         raw[i][hf] = block != nullptr ? __ldg(src + i * (D / 2) + hf * 8) : make_uint2(0, 0);
   }
-  // Rows row0 .. row0 + 15 of the fp16 tile at `dst` (128-byte swizzled halves of 64 columns).
+  // Rows row0 .. row0 + 15 of the fp16 tile at `dst` (128-byte swizzled halves of 64 columns);
+  // `factor`: of those rows.
   __device__ __forceinline__ void store(uint8_t* dst, const uint32_t* factor, int row0, bool dropped,
                                         int lane) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = row0 + i * 4 + lane / 8;
-      const uint32_t f = factor[row];
+      const uint32_t f = factor[i * 4 + lane / 8];
       const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
       const __half2 h2 = __low2half2(f2), l2 = __high2half2(f2);
       uint8_t* base = dst + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
@@ -305,7 +344,7 @@ struct Codes {
           const __half2 y = __hfma2(x, h2, __hmul2(x, l2));
           v[k] = *reinterpret_cast<const uint32_t*>(&y);
         }
-        *reinterpret_cast<uint4*>(base + hf * kHalfBytes) = make_uint4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<uint4*>(base + hf * kKvHalf) = make_uint4(v[0], v[1], v[2], v[3]);
       }
     }
   }
@@ -336,9 +375,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ts::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023) & ~1023u) - raw_addr);
-  auto sQ = [&](int x) { return smem + x * G::kTileBytes; };
-  auto sK = [&](int st) { return smem + (kQTiles + st) * G::kTileBytes; };
-  auto sV = [&](int st) { return smem + (kQTiles + kStages + st) * G::kTileBytes; };
+  auto sQ = [&](int x) { return smem + x * G::kQBytes; };
+  auto sK = [&](int st) { return smem + kQTiles * G::kQBytes + st * G::kKvBytes; };
+  auto sV = [&](int st) { return sK(kStages + st); };
   Shared* sh = reinterpret_cast<Shared*>(smem + G::kTiles);
   volatile int* abort = &sh->abort;
 
@@ -352,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   constexpr int kQLanes = D / 8, kQRows = 32 / kQLanes;
   auto q_place = [&](int w) {  // this lane's 16 bytes of row w of the warp's 32
     const int c = lane % kQLanes;
-    return sQ(warp / 4 & 1) + (warp & 3) * 32 * 128 + (c >> 3) * kHalfBytes + w * 128 +
+    return sQ(warp / 4 & 1) + (warp & 3) * 32 * 128 + (c >> 3) * kQHalf + w * 128 +
            (((c & 7) ^ (w & 7)) << 4);
   };
   if (warp < 4 * kQTiles) {
@@ -379,11 +418,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       ts::mbar_init(&sh->v_empty[i], 1);
     }
     for (int i = 0; i < kInfos; ++i) ts::mbar_init(&sh->info_full[i], 1);
-    for (int i = 0; i < kAhead; ++i) ts::mbar_init(&sh->converted[i], kUnits);
+    for (int i = 0; i < kAhead; ++i) ts::mbar_init(&sh->converted[i], kUnits * kTilesPerSpan);
     for (int x = 0; x < kQTiles; ++x) {
-      ts::mbar_init(&sh->s_full[x], 1);
-      ts::mbar_init(&sh->p_full[x], 128);
+      for (int b = 0; b < 2; ++b) {
+        ts::mbar_init(&sh->s_full[x][b], 1);
+        ts::mbar_init(&sh->p_full[x][b], 128);
+      }
       ts::mbar_init(&sh->pv_done[x], 1);
+      ts::mbar_init(&sh->o_full[x], 1);
     }
     ts::mbar_init(&sh->drain, 1);
     sh->abort = 0;
@@ -396,11 +438,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   ts::tc::fence_before_sync();
   __syncthreads();
   ts::tc::fence_after_sync();
-  const uint32_t tmem = sh->tmem;
+  constexpr uint32_t tmem = 0;  // all 512 columns: the allocation starts at the first
 
   if (warp >= 8) {
     if (warp == 12) {
-      scout(a, sh, a.block_tables + int64_t(seq) * a.max_blocks, h, n_kv, n_max, lane, abort);
+      scout(a, sh, a.block_tables + int64_t(seq) * a.max_blocks, h, n_kv, lane, abort);
     } else if (warp != 13) {
       // ---------------------------------------------------------- converters
       const int total = n_max * kUnits;
@@ -408,21 +450,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       Codes<D> codes[2];
       auto fetch = [&](Codes<D>& c, int u) -> bool {
         if (u >= total) return true;
-        const int t = u / kUnits, k = u % kUnits;
-        if (!wait_warp(&sh->info_full[t % kInfos], (t / kInfos) & 1, abort)) return false;
-        const int phys = sh->info[t % kInfos].block[k % (kUnits / 2)];
+        const int j = u / kUnits, k = u % kUnits, t = j / kTilesPerSpan;
+        if (!wait_ahead(&sh->info_full[t % kInfos], (t / kInfos) & 1, abort)) return false;
+        const int phys =
+            sh->info[t % kInfos].block[j % kTilesPerSpan * (kUnits / 2) + k % (kUnits / 2)];
         const uint8_t* pool = (k < kUnits / 2 ? a.key_pool : a.value_pool) + h * kBlock * D;
         c.load(phys >= 0 ? pool + phys * block_bytes : nullptr, lane);
         return true;
       };
       auto convert = [&](Codes<D>& c, int u) -> bool {
-        const int t = u / kUnits, k = u % kUnits, st = t % kStages;
+        const int j = u / kUnits, k = u % kUnits, st = j % kStages, t = j / kTilesPerSpan;
         const bool is_v = k >= kUnits / 2;
-        if (t >= kStages && !wait_warp(is_v ? &sh->v_empty[st] : &sh->k_empty[st],
-                                       ((t - kStages) / kStages) & 1, abort))
+        if (j >= kStages && !wait_ahead(is_v ? &sh->v_empty[st] : &sh->k_empty[st],
+                                       ((j - kStages) / kStages) & 1, abort))
           return false;
         const TileInfo& info = sh->info[t % kInfos];
-        c.store(is_v ? sV(st) : sK(st), info.factor[is_v], k % (kUnits / 2) * kBlock,
+        const int row0 = k % (kUnits / 2) * kBlock;
+        c.store(is_v ? sV(st) : sK(st), info.factor[is_v] + j % kTilesPerSpan * kKvTile + row0, row0,
                 info.dropped >> int(is_v) & 1, lane);
         ts::fence_proxy_async_smem();
         __syncwarp();
@@ -449,44 +493,44 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       // Low words of the shared-memory descriptors: address / 16, and V's distance between halves.
       const uint32_t q_lo = ts::smem_u32(sQ(0)) >> 4 | 1u << 16;
       const uint32_t k_lo = ts::smem_u32(sK(0)) >> 4 | 1u << 16;
-      const uint32_t v_lo = ts::smem_u32(sV(0)) >> 4 | uint32_t(kHalfBytes >> 4) << 16;
+      const uint32_t v_lo = ts::smem_u32(sV(0)) >> 4 | uint32_t(kKvHalf >> 4) << 16;
       // The last query tile to use KV tile j releases its K (after QK) and V (after PV).
       auto last_user = [&](int j) { return j < n_t[1] ? 1 : 0; };
       bool ok = wait_warp(&sh->q_full, 0, abort);
-      // Step j: PV(j - 1) then QK(j), of each query tile in turn.
+      // Step i: PV(i - 2) then QK(i), of each query tile in turn.
 #pragma unroll 1
-      for (int j = 0; ok && j <= n_max; ++j) {
-        const int sk = j % kStages, sv = (j - 1) % kStages;
+      for (int i = 0; ok && i < n_max + 2; ++i) {
+        const int j = i - 2, b = i & 1, sk = i % kStages, sv = j & (kStages - 1);
 #pragma unroll 1
         for (int x = 0; ok && x < kQTiles; ++x) {
           const int n_x = x ? n_t[1] : n_t[0];
-          if (j > 0 && j <= n_x) {
-            ok = wait_warp(&sh->p_full[x], (j - 1) & 1, abort) &&
-                 wait_warp(&sh->v_full[sv], ((j - 1) / kStages) & 1, abort);
+          const uint32_t s_tmem = tmem + x * 128 + b * kKvTile;
+          if (j >= 0 && j < n_x) {
+            ok = wait_warp(&sh->p_full[x][b], (j / 2) & 1, abort) &&
+                 wait_warp(&sh->v_full[sv], (j / kStages) & 1, abort);
             if (!ok) break;
             ts::tc::fence_after_sync();
-            const uint32_t dv = v_lo + sv * (G::kTileBytes >> 4);
+            const uint32_t dv = v_lo + sv * (G::kKvBytes >> 4);
 #pragma unroll
             for (int kk = 0; kk < kKvTile / 16; ++kk)
-              ts::tc::mma_ts_elect(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, dv + kk * 128,
-                                   idesc_pv, j > 1 || kk > 0);
-            if (j == n_x) ts::tc::commit_elect(&sh->pv_done[x]);
-            if (x == last_user(j - 1) && j - 1 + kStages < n_max)
-              ts::tc::commit_elect(&sh->v_empty[sv]);
+              ts::tc::mma_ts_elect(tmem + 256 + x * 128, s_tmem + kk * 8, dv + kk * 128, idesc_pv,
+                                   j > 0 || kk > 0);
+            ts::tc::commit_elect(j + 1 == n_x ? &sh->o_full[x] : &sh->pv_done[x]);
+            if (x == last_user(j) && j + kStages < n_max) ts::tc::commit_elect(&sh->v_empty[sv]);
           }
-          if (j < n_x) {
-            ok = wait_warp(&sh->k_full[sk], (j / kStages) & 1, abort);
+          if (i < n_x) {
+            ok = wait_warp(&sh->k_full[sk], (i / kStages) & 1, abort);
             if (!ok) break;
             ts::tc::fence_after_sync();
-            const uint32_t dq = q_lo + x * (G::kTileBytes >> 4);
-            const uint32_t dk = k_lo + sk * (G::kTileBytes >> 4);
+            const uint32_t dq = q_lo + x * (G::kQBytes >> 4);
+            const uint32_t dk = k_lo + sk * (G::kKvBytes >> 4);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
-              ts::tc::mma_ss_elect(tmem + x * 128, dq + off, dk + off, idesc_qk, kk > 0);
-            }
-            ts::tc::commit_elect(&sh->s_full[x]);
-            if (x == last_user(j) && j + kStages < n_max) ts::tc::commit_elect(&sh->k_empty[sk]);
+            for (int kk = 0; kk < D / 16; ++kk)
+              ts::tc::mma_ss_elect(s_tmem, dq + (((kk >> 2) * kQHalf + (kk & 3) * 32) >> 4),
+                                   dk + (((kk >> 2) * kKvHalf + (kk & 3) * 32) >> 4), idesc_qk,
+                                   kk > 0);
+            ts::tc::commit_elect(&sh->s_full[x][b]);
+            if (x == last_user(i) && i + kStages < n_max) ts::tc::commit_elect(&sh->k_empty[sk]);
           }
         }
       }
@@ -505,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     const bool row_valid = i < a.tq && qi < q_len;
     const int pos = row_valid ? p0 + qi : p0 + q_len - 1;
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t s_col = x * 128, o_col = 256 + x * 128;
+    const uint32_t o_col = 256 + x * 128;
 
     // q's rows times 2^(14 - exponent of their amax), in fp16; `sl` undoes it (times the softmax
     // scale, whose sign goes with q). A warp loads its 32 rows 16 bytes a lane, D / 8 lanes a row.
@@ -557,12 +601,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     float m_run = -INFINITY, l_run = 0.f, ref_v = 0.f;
     bool ok = true;
     for (int j = 0; j < n_x; ++j) {
-      if (!wait_warp(&sh->s_full[x], j & 1, abort)) {
+      if (!wait_warp(&sh->s_full[x][j & 1], (j / 2) & 1, abort)) {
         ok = false;
         break;
       }
       ts::tc::fence_after_sync();
-      const volatile TileInfo* info = &sh->info[j % kInfos];
+      const uint32_t s_col = x * 128 + (j & 1) * kKvTile;
+      constexpr int kGroups = kKvTile / 32;  // of 32 columns
+      const volatile TileInfo* info = &sh->info[j / kTilesPerSpan % kInfos];
+      const int word = j % kTilesPerSpan * kGroups;  // of the span's column masks
       const float slj = fmaxf(sl * info->ref_k, 0x1p-126f);  // > 0, so that -inf stays -inf
       // O is in units of V's reference: it shrinks when that grows.
       const float ref_old = ref_v;
@@ -571,12 +618,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       float corr_o = ref_v != ref_old && j > 0 ? ref_old / ref_v : 1.f;
       const int limit = pos - j * kKvTile;  // columns c <= limit are visible
       // Column groups of 32 that some row of the warp sees, and those every row sees whole.
-      const int n_some = min(4, max(0, __reduce_max_sync(0xffffffffu, limit) + 32) / 32);
+      const int n_some = min(kGroups, max(0, __reduce_max_sync(0xffffffffu, limit) + 32) / 32);
       const int n_whole = odd_columns ? 0 : max(0, __reduce_min_sync(0xffffffffu, limit) + 1) / 32;
       auto mask = [&](uint32_t (&r)[32], int c) {
         const int lim = limit - 32 * c;
         const uint32_t seen = lim >= 31 ? ~0u : lim < 0 ? 0u : (2u << lim) - 1;
-        const uint32_t keep = seen & ~info->skip[c], spoil = seen & info->spoil[c];
+        const uint32_t keep = seen & ~info->skip[word + c],
+                       spoil = seen & info->spoil[word + c];
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
           const uint32_t z = spoil >> k & 1 ? 0x7fc00000u : r[k];
@@ -596,28 +644,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         }
         if (m_run == -INFINITY) m_run = m * slj;
       }
-      float m_use = m_run == -INFINITY ? 0.f : m_run;
-      float sum0 = 0.f, sum1 = 0.f;
+      const uint64_t slj2 = two(slj, slj);
+      float less = m_run == -INFINITY ? 0.f : -m_run;
+      uint64_t less2 = two(less, less), sum2 = two(0.f, 0.f);
 #pragma unroll 1
       for (int c = 0; c < n_some; ++c) {  // P of columns 32 c .. 32 c + 31
         ts::tc::wait_ld(sa);
         if (c >= n_whole) mask(sa, c);
-        uint32_t e[32];  // log2 of P
+        uint64_t e[16];  // log2 of P, two columns each
 #pragma unroll
-        for (int k = 0; k < 32; k += 2)
-          fma2(e[k], e[k + 1], sa[k], sa[k + 1], slj, -m_use);
+        for (int k = 0; k < 16; ++k) e[k] = fma2(two(sa[2 * k], sa[2 * k + 1]), slj2, less2);
         if (c + 1 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 1) * 32, sa);
-        const float over = max32(e);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float2 v = halves(e[k]);
+          mx[k % 4] = max3f(mx[k % 4], v.x, v.y);
+        }
+        const float over = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]);
         if (__any_sync(0xffffffffu, over > kRescaleSlack)) {
           const float up = over > kRescaleSlack ? over : 0.f, f = ex2(-up);
           m_run += up;
-          m_use = m_run;
+          less -= up;
+          less2 = two(less, less);
           l_run *= f;
-          sum0 *= f;
-          sum1 *= f;
           corr_o *= f;
+          const float2 v = halves(sum2);
+          sum2 = two(v.x * f, v.y * f);
+          const uint64_t up2 = two(-up, -up);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) e[k] = __float_as_uint(__uint_as_float(e[k]) - up);
+          for (int k = 0; k < 16; ++k) e[k] = add2(e[k], up2);
 #pragma unroll 1
           for (int b = 0; b < c; ++b) {  // the tile's P so far
             uint32_t pw[16];
@@ -626,28 +682,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
             ts::tc::wait_ld(pw);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&pw[k]));
-              pw[k] = pack_half2(v.x * f, v.y * f);
+              const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&pw[k]));
+              pw[k] = pack_half2(u.x * f, u.y * f);
             }
             ts::tc::tmem_st16(lane_base + s_col + b * 16, pw);
           }
         }
         uint32_t pw[16];
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          const float p = ex2(__uint_as_float(e[k])), q = ex2(__uint_as_float(e[k + 1]));
-          add2(sum0, sum1, p, q);
-          pw[k / 2] = pack_half2(p, q);
+        for (int k = 0; k < 16; ++k) {
+          const float2 v = halves(e[k]);
+          const float p = ex2(v.x), q = ex2(v.y);
+          sum2 = add2(sum2, two(p, q));
+          pw[k] = pack_half2(p, q);
         }
         ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
       }
 #pragma unroll 1
-      for (int c = n_some; c < 4; ++c) {
+      for (int c = n_some; c < kGroups; ++c) {
         uint32_t pw[16] = {};
         ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
       }
-      l_run += sum0 + sum1;
+      const float2 sums = halves(sum2);
+      l_run += sums.x + sums.y;
       if (j > 0 && __any_sync(0xffffffffu, corr_o != 1.f)) {
+        // O holds the tiles up to j - 1 (up to j - 2 it does since S of tile j was ready).
+        if (!wait_warp(&sh->pv_done[x], (j - 1) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        ts::tc::fence_after_sync();
 #pragma unroll 1
         for (int c4 = 0; c4 < D / 32; ++c4) {
           uint32_t rr[32];
@@ -660,9 +724,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       }
       ts::tc::wait_st();
       ts::tc::fence_before_sync();
-      ts::mbar_arrive(&sh->p_full[x]);
+      ts::mbar_arrive(&sh->p_full[x][j & 1]);
     }
-    if (ok && n_x > 0) ok = wait_warp(&sh->pv_done[x], 0, abort);
+    if (ok && n_x > 0) ok = wait_warp(&sh->o_full[x], 0, abort);
     ts::tc::fence_after_sync();
     if (ok) {
       const float inv = l_run > 0.f ? ref_v / (kRefScale * l_run) : l_run;
@@ -714,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   __syncthreads();
   if (warp == 0) {
     ts::tc::fence_after_sync();
-    ts::tc::tmem_dealloc(tmem, kTmemCols);
+    ts::tc::tmem_dealloc(sh->tmem, kTmemCols);
   }
 }
 
