@@ -355,11 +355,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   using G = Geo<D>;
   using Mma = ts::MmaOp<T>;
   const int pair = blockIdx.x, h = blockIdx.y, seq = blockIdx.z;
-  const int q0 = a.qsl[seq];
-  const int q_len = a.qsl[seq + 1] - q0;
+  const int q0 = __shfl_sync(0xffffffffu, a.qsl[seq], 0);
+  const int q_len = __shfl_sync(0xffffffffu, a.qsl[seq + 1], 0) - q0;
   const int tile0 = pair * kQTiles;
   if (tile0 * a.tq >= q_len) return;
-  const int ctx = min(a.context_lens[seq], a.max_blocks * kBlock);
+  const int ctx = min(__shfl_sync(0xffffffffu, a.context_lens[seq], 0), a.max_blocks * kBlock);
   const int p0 = ctx - q_len;  // position of the first query row; negative rows see nothing
   int n_t[kQTiles];            // KV tiles each query tile needs
   int n_kv = 0;                // keys the CTA's last query row sees
@@ -381,7 +381,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   Shared* sh = reinterpret_cast<Shared*>(smem + G::kTiles);
   volatile int* abort = &sh->abort;
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // Through a shuffle, so that the compiler knows a role's control flow to be uniform.
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
 
   // Token of a tile row, row / group: exact in fp32 for rows below 128.
   const float inv_group = 1.f / float(a.group);
