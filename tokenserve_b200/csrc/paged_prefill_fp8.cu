@@ -65,6 +65,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // A stale row max is kept unless exceeded by 2^14: P stays below fp16's 2^16, and weights near the
 // true maximum, at least 1, well inside its normal range.
 constexpr float kRescaleSlack = 14.f;
+// One of so many column pairs takes its 2^x from the FMA pipe (64 sequences of 512 new tokens: none
+// 928 us, one of 8 912, of 4 899, of 3 919, of 2 937).
+constexpr int kFmaEvery = 4;
 // S_A [0,128) and S_B [128,256), two buffers each, O_A [256,384), O_B [384,512).
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRefScale = 128.f;    // fp16 values are code * scale / ref * 128 <= 57344
@@ -83,7 +86,8 @@ struct Args {
   const int32_t* qsl;
   const int32_t* context_lens;
   int max_blocks, num_q_heads, num_kv_heads, group;
-  int tq;  // query tokens per tile
+  int tq;       // query tokens per tile
+  int q_tiles;  // query tiles per CTA, 1 or 2
   int64_t num_blocks;
   float scale_log2;
 };
@@ -206,6 +210,26 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
+// 2^x of two x <= 15 on the FMA pipe, for some of the columns: the exponential unit (16 a clock) is
+// what a tile's softmax waits for. x = n + f with n the nearest integer, 2^f by a polynomial of degree
+// 4 fitted to least relative error on [-1/2, 1/2] (2.9e-6, under fp16's 4.9e-4), n added to the
+// exponent. x below -126 gives 2^-126, which is 0 in fp16 and nothing beside a sum's 1. A NaN is lost.
+__device__ __forceinline__ float2 exp2_fma(uint64_t x2) {
+  float2 x = halves(x2);
+  x2 = two(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const uint64_t t2 = add2(x2, two(12582912.f, 12582912.f));  // 1.5 * 2^23: n in the low bits
+  const uint64_t n2 = add2(t2, two(-12582912.f, -12582912.f));
+  const uint64_t f2 = fma2(n2, two(-1.f, -1.f), x2);
+  uint64_t p2 = fma2(f2, two(0.009582851082086563f, 0.009582851082086563f),
+                     two(0.055906426161527634f, 0.055906426161527634f));
+  p2 = fma2(p2, f2, two(0.24024099111557007f, 0.24024099111557007f));
+  p2 = fma2(p2, f2, two(0.6931241750717163f, 0.6931241750717163f));
+  p2 = fma2(p2, f2, two(1.f, 1.f));
+  const float2 t = halves(t2), p = halves(p2);
+  return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(p.x)),
+                     __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(p.y)));
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -218,93 +242,103 @@ __device__ __forceinline__ uint32_t split_factor(float f) {
 }
 
 // Largest finite value of the warp's 128 scales.
-__device__ __forceinline__ float top(const float4& sc) {
+__device__ __forceinline__ float top(const float (&sc)[4]) {
   auto fin = [](float v) { return isfinite(v) ? v : 0.f; };
-  const float m = fmaxf(fmaxf(fin(sc.x), fin(sc.y)), fmaxf(fin(sc.z), fin(sc.w)));
+  const float m = fmaxf(fmaxf(fin(sc[0]), fin(sc[1])), fmaxf(fin(sc[2]), fin(sc[3])));
   // Not negative, so they order like their bits.
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(m, 0.f))));
 }
 
-// The scout warp: describes the spans of (table, KV head h), n_kv visible keys. Lane l looks after
-// tokens 4 l .. 4 l + 3 of each span, in block l / 4.
-__device__ __forceinline__ void scout(const Args& a, Shared* sh, const int32_t* table, int h,
-                                      int n_kv, int lane, volatile int* abort) {
-  constexpr int kBlocks = kSpan / kBlock;
-  const int spans = (n_kv + kSpan - 1) / kSpan;
-  const int total_blk = (n_kv + kBlock - 1) / kBlock;
-  const int64_t stride = int64_t(a.num_kv_heads) * kBlock;  // scales of a block, all heads
-  const int64_t mine = int64_t(h) * kBlock + lane % 4 * 4;
-  float run_v = 0x1p-126f;  // V's reference: never below the scales seen
-  auto look_up = [&](int t) -> int {  // this lane's block of span t (-1 none, -2 not in the pool)
-    const int b = t * kBlocks + lane / 4;
-    if (b >= total_blk) return -1;
-    const int phys = __ldg(table + b);
-    return phys >= 0 && int64_t(phys) < a.num_blocks ? phys : -2;
-  };
-  int phys = look_up(0);
-#pragma unroll 1
-  for (int t = 0; t < spans; ++t) {
-    const int next = look_up(t + 1);
-    float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;
+// The scout warp: describes the spans of a KV head's keys, n_kv of them visible. Lane l looks after
+// tokens 4 l .. 4 l + 3 of each span, in block l / 4; their scales are loaded a span ahead.
+struct Scout {
+  const Args& a;
+  const int32_t* table;
+  int n_kv, lane;
+  int64_t stride, mine;  // scales of a block over all heads; this lane's place among them
+  int phys;              // this lane's block of the next span (-1 none, -2 not in the pool)
+  float4 ks, vs;
+
+  __device__ __forceinline__ Scout(const Args& args, int seq, int h, int keys, int l)
+      : a(args), table(args.block_tables + int64_t(seq) * args.max_blocks), n_kv(keys), lane(l),
+        stride(int64_t(args.num_kv_heads) * kBlock), mine(int64_t(h) * kBlock + l % 4 * 4) {}
+
+  __device__ __forceinline__ int look_up(int t) const {
+    const int b = t * (kSpan / kBlock) + lane / 4;
+    if (b * kBlock >= n_kv) return -1;
+    const int p = __ldg(table + b);
+    return p >= 0 && int64_t(p) < a.num_blocks ? p : -2;
+  }
+  __device__ __forceinline__ void load(int block) {
+    phys = block;
+    ks = vs = make_float4(0.f, 0.f, 0.f, 0.f);
     if (phys >= 0) {
       ks = __ldg(reinterpret_cast<const float4*>(a.key_scales + phys * stride + mine));
       vs = __ldg(reinterpret_cast<const float4*>(a.value_scales + phys * stride + mine));
     }
-    const int reach = n_kv - t * kSpan - 4 * lane;  // of its tokens, those below n_kv
-    if (reach < 4) {
-      if (reach < 1) ks.x = vs.x = 0.f;
-      if (reach < 2) ks.y = vs.y = 0.f;
-      if (reach < 3) ks.z = vs.z = 0.f;
-      ks.w = vs.w = 0.f;
-    }
-    if (t >= kAhead && !wait_ahead(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1, abort))
-      return;
-    TileInfo* info = &sh->info[t % kInfos];
-    const float ref_k = fmaxf(top(ks), 0x1p-126f), top_v = top(vs);
-    if (top_v > run_v) run_v = fminf(top_v * kRefRoom, 0x1p127f);
-    const float inv_k = 1.f / ref_k, inv_v = 1.f / run_v;
-    // A NaN K row makes NaN scores; a NaN V row is stored as zeros (see the head of the file).
-    uint32_t spoil = 0;
-    uint32_t fk[4], fv[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float k = i == 0 ? ks.x : i == 1 ? ks.y : i == 2 ? ks.z : ks.w;
-      const float v = i == 0 ? vs.x : i == 1 ? vs.y : i == 2 ? vs.z : vs.w;
-      if (!isfinite(v)) spoil |= 1u << i;
-      fk[i] = i < reach ? split_factor(k * inv_k * kRefScale) : kDropped;
-      fv[i] = i < reach && isfinite(v) ? split_factor(v * inv_v * kRefScale) : kDropped;
-    }
-    *reinterpret_cast<uint4*>(&info->factor[0][4 * lane]) = make_uint4(fk[0], fk[1], fk[2], fk[3]);
-    *reinterpret_cast<uint4*>(&info->factor[1][4 * lane]) = make_uint4(fv[0], fv[1], fv[2], fv[3]);
-    if (lane % 4 == 0) info->block[lane / 4] = phys;
-    const bool any = __any_sync(0xffffffffu, spoil != 0 || phys == -2);
-    const bool past = __any_sync(0xffffffffu, reach < 4);
-    if (any) {
-      uint32_t skip = (phys == -2 ? 0xfu : 0u) << lane % 8 * 4;
-      spoil <<= lane % 8 * 4;
-#pragma unroll 1
-      for (int o = 1; o < 8; o <<= 1) {
-        skip |= __shfl_xor_sync(0xffffffffu, skip, o);
-        spoil |= __shfl_xor_sync(0xffffffffu, spoil, o);
-      }
-      if (lane % 8 == 0) {
-        info->skip[lane / 8] = skip;
-        info->spoil[lane / 8] = spoil;
-      }
-    } else if (lane < 4) {
-      info->skip[lane] = info->spoil[lane] = 0;
-    }
-    if (lane == 0) {
-      info->ref_k = ref_k;
-      info->ref_v = run_v;
-      info->any = any;
-      info->dropped = uint32_t(past) | uint32_t(past || any) << 1;
-    }
-    __syncwarp();
-    if (lane == 0) ts::mbar_arrive(&sh->info_full[t % kInfos]);
-    phys = next;
   }
-}
+
+  __device__ __forceinline__ void run(Shared* sh, volatile int* abort) {
+    const int spans = (n_kv + kSpan - 1) / kSpan;
+    float run_v = 0x1p-126f;  // V's reference: never below the scales seen
+#pragma unroll 1
+    for (int t = 0; t < spans; ++t) {
+      const int next = look_up(t + 1);
+      const int reach = n_kv - t * kSpan - 4 * lane;  // of its tokens, those below n_kv
+      float k[4] = {ks.x, ks.y, ks.z, ks.w}, v[4] = {vs.x, vs.y, vs.z, vs.w};
+      uint32_t spoil = 0;
+      bool k_odd = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= reach) k[i] = v[i] = 0.f;
+        k_odd |= !isfinite(k[i]);
+        if (!isfinite(v[i])) spoil |= 1u << i;
+      }
+      if (t >= kAhead && !wait_ahead(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1, abort))
+        return;
+      TileInfo* info = &sh->info[t % kInfos];
+      const float ref_k = fmaxf(top(k), 0x1p-126f), top_v = top(v);
+      if (top_v > run_v) run_v = fminf(top_v * kRefRoom, 0x1p127f);
+      const float inv_k = 1.f / ref_k, inv_v = 1.f / run_v;
+      // A NaN K row makes NaN scores; a NaN V row is stored as zeros (see the head of the file).
+      uint32_t fk[4], fv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        fk[i] = i < reach ? split_factor(k[i] * inv_k * kRefScale) : kDropped;
+        fv[i] = i < reach && !(spoil >> i & 1) ? split_factor(v[i] * inv_v * kRefScale) : kDropped;
+      }
+      *reinterpret_cast<uint4*>(&info->factor[0][4 * lane]) = make_uint4(fk[0], fk[1], fk[2], fk[3]);
+      *reinterpret_cast<uint4*>(&info->factor[1][4 * lane]) = make_uint4(fv[0], fv[1], fv[2], fv[3]);
+      if (lane % 4 == 0) info->block[lane / 4] = phys;
+      const bool any = __any_sync(0xffffffffu, spoil != 0 || k_odd || phys == -2);
+      const bool past = __any_sync(0xffffffffu, reach < 4);
+      if (any) {
+        uint32_t skip = (phys == -2 ? 0xfu : 0u) << lane % 8 * 4;
+        spoil <<= lane % 8 * 4;
+#pragma unroll 1
+        for (int o = 1; o < 8; o <<= 1) {
+          skip |= __shfl_xor_sync(0xffffffffu, skip, o);
+          spoil |= __shfl_xor_sync(0xffffffffu, spoil, o);
+        }
+        if (lane % 8 == 0) {
+          info->skip[lane / 8] = skip;
+          info->spoil[lane / 8] = spoil;
+        }
+      } else if (lane < 4) {
+        info->skip[lane] = info->spoil[lane] = 0;
+      }
+      if (lane == 0) {
+        info->ref_k = ref_k;
+        info->ref_v = run_v;
+        info->any = any;
+        info->dropped = uint32_t(past) | uint32_t(past || any) << 1;
+      }
+      __syncwarp();
+      if (lane == 0) ts::mbar_arrive(&sh->info_full[t % kInfos]);
+      load(next);
+    }
+  }
+};
 
 // One block of codes (16 rows of a KV head) in a converter warp's registers: a row in 8 lanes, each
 // with 8 codes of every 64 columns, so a lane's values are one 16-byte chunk of each half tile.
@@ -357,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   const int pair = blockIdx.x, h = blockIdx.y, seq = blockIdx.z;
   const int q0 = __shfl_sync(0xffffffffu, a.qsl[seq], 0);
   const int q_len = __shfl_sync(0xffffffffu, a.qsl[seq + 1], 0) - q0;
-  const int tile0 = pair * kQTiles;
+  const int tile0 = pair * a.q_tiles;
   if (tile0 * a.tq >= q_len) return;
   const int ctx = min(__shfl_sync(0xffffffffu, a.context_lens[seq], 0), a.max_blocks * kBlock);
   const int p0 = ctx - q_len;  // position of the first query row; negative rows see nothing
@@ -366,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
 #pragma unroll
   for (int x = 0; x < kQTiles; ++x) {
     const int first = (tile0 + x) * a.tq;
-    const int n = first < q_len ? max(0, p0 + min(q_len, first + a.tq)) : 0;
+    const int n = x < a.q_tiles && first < q_len ? max(0, p0 + min(q_len, first + a.tq)) : 0;
     n_t[x] = (n + kKvTile - 1) / kKvTile;
     n_kv = max(n_kv, n);
   }
@@ -410,7 +444,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
                    : "memory");
     }
   }
-  if (threadIdx.x == 0) {
+  Scout scout(a, seq, h, n_kv, lane);
+  if (warp == 12) scout.load(scout.look_up(0));
+  if (warp == 14 && lane == 0) {
     ts::mbar_init(&sh->q_full, 128 * kQTiles);
     for (int i = 0; i < kStages; ++i) {
       ts::mbar_init(&sh->k_full[i], kUnits / 2);
@@ -432,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     sh->abort = 0;
     ts::fence_mbar_init();
   }
-  if (warp == 0) {
+  if (warp == 13) {
     ts::tc::tmem_alloc(&sh->tmem, kTmemCols);
     ts::tc::tmem_relinquish();
   }
@@ -443,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
 
   if (warp >= 8) {
     if (warp == 12) {
-      scout(a, sh, a.block_tables + int64_t(seq) * a.max_blocks, h, n_kv, lane, abort);
+      scout.run(sh, abort);
     } else if (warp != 13) {
       // ---------------------------------------------------------- converters
       const int total = n_max * kUnits;
@@ -547,8 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     const int n_x = n_t[x];
     const int i = row_token(r);
     const int qi = (tile0 + x) * a.tq + i;
-    const bool row_valid = i < a.tq && qi < q_len;
-    const int pos = row_valid ? p0 + qi : p0 + q_len - 1;
+    const int pos = i < a.tq && qi < q_len ? p0 + qi : p0 + q_len - 1;  // rows of no query: anything
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t o_col = 256 + x * 128;
 
@@ -600,6 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     }
 
     float m_run = -INFINITY, l_run = 0.f, ref_v = 0.f;
+    bool saw_nan = false;  // a row of K or V that holds one (not every exponential below keeps it)
     bool ok = true;
     for (int j = 0; j < n_x; ++j) {
       if (!wait_warp(&sh->s_full[x][j & 1], (j / 2) & 1, abort)) {
@@ -608,6 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       }
       ts::tc::fence_after_sync();
       const uint32_t s_col = x * 128 + (j & 1) * kKvTile;
+      uint32_t sa[32];
+      ts::tc::tmem_ld32(lane_base + s_col, sa);
       constexpr int kGroups = kKvTile / 32;  // of 32 columns
       const volatile TileInfo* info = &sh->info[j / kTilesPerSpan % kInfos];
       const int word = j % kTilesPerSpan * kGroups;  // of the span's column masks
@@ -628,12 +666,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
                        spoil = seen & info->spoil[word + c];
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
-          const uint32_t z = spoil >> k & 1 ? 0x7fc00000u : r[k];
-          r[k] = keep >> k & 1 ? z : __float_as_uint(-INFINITY);
+          if (!(keep >> k & 1)) r[k] = __float_as_uint(-INFINITY);
+          else if (spoil >> k & 1 || isnan(__uint_as_float(r[k]))) saw_nan = true;
         }
       };
-      uint32_t sa[32];
-      ts::tc::tmem_ld32(lane_base + s_col, sa);
       if (__any_sync(0xffffffffu, m_run == -INFINITY)) {  // a row that has seen nothing yet
         float m = -INFINITY;
 #pragma unroll 1
@@ -648,10 +684,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       const uint64_t slj2 = two(slj, slj);
       float less = m_run == -INFINITY ? 0.f : -m_run;
       uint64_t less2 = two(less, less), sum2 = two(0.f, 0.f);
-#pragma unroll 1
-      for (int c = 0; c < n_some; ++c) {  // P of columns 32 c .. 32 c + 31
+      // P of columns 32 c .. 32 c + 31. Masked columns, and a warp whose maximum moves, run their own
+      // copies of the code: where the paths met again, the registers of a whole row were copied.
+      auto columns = [&](int c, auto masked) {
         ts::tc::wait_ld(sa);
-        if (c >= n_whole) mask(sa, c);
+        if (masked) mask(sa, c);
         uint64_t e[16];  // log2 of P, two columns each
 #pragma unroll
         for (int k = 0; k < 16; ++k) e[k] = fma2(two(sa[2 * k], sa[2 * k + 1]), slj2, less2);
@@ -663,42 +700,56 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           mx[k % 4] = max3f(mx[k % 4], v.x, v.y);
         }
         const float over = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]);
-        if (__any_sync(0xffffffffu, over > kRescaleSlack)) {
-          const float up = over > kRescaleSlack ? over : 0.f, f = ex2(-up);
-          m_run += up;
-          less -= up;
-          less2 = two(less, less);
-          l_run *= f;
-          corr_o *= f;
-          const float2 v = halves(sum2);
-          sum2 = two(v.x * f, v.y * f);
-          const uint64_t up2 = two(-up, -up);
+        if (!__any_sync(0xffffffffu, over > kRescaleSlack)) {
+          uint32_t pw[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) e[k] = add2(e[k], up2);
-#pragma unroll 1
-          for (int b = 0; b < c; ++b) {  // the tile's P so far
-            uint32_t pw[16];
-            ts::tc::wait_st();
-            ts::tc::tmem_ld16(lane_base + s_col + b * 16, pw);
-            ts::tc::wait_ld(pw);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&pw[k]));
-              pw[k] = pack_half2(u.x * f, u.y * f);
-            }
-            ts::tc::tmem_st16(lane_base + s_col + b * 16, pw);
+          for (int k = 0; k < 16; ++k) {
+            float2 v = halves(e[k]);
+            v = k % kFmaEvery == 0 ? exp2_fma(e[k]) : make_float2(ex2(v.x), ex2(v.y));
+            sum2 = add2(sum2, two(v.x, v.y));
+            pw[k] = pack_half2(v.x, v.y);
           }
+          ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
+          return;
+        }
+        const float up = over > kRescaleSlack ? over : 0.f, f = ex2(-up);
+        m_run += up;
+        less -= up;
+        less2 = two(less, less);
+        l_run *= f;
+        corr_o *= f;
+        float2 sum = halves(sum2);
+        sum.x *= f;
+        sum.y *= f;
+#pragma unroll 1
+        for (int b = 0; b < c; ++b) {  // the tile's P so far
+          uint32_t pw[16];
+          ts::tc::wait_st();
+          ts::tc::tmem_ld16(lane_base + s_col + b * 16, pw);
+          ts::tc::wait_ld(pw);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&pw[k]));
+            pw[k] = pack_half2(u.x * f, u.y * f);
+          }
+          ts::tc::tmem_st16(lane_base + s_col + b * 16, pw);
         }
         uint32_t pw[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float2 v = halves(e[k]);
-          const float p = ex2(v.x), q = ex2(v.y);
-          sum2 = add2(sum2, two(p, q));
-          pw[k] = pack_half2(p, q);
+          float2 v = halves(e[k]);
+          v = make_float2(ex2(v.x - up), ex2(v.y - up));
+          sum.x += v.x;
+          sum.y += v.y;
+          pw[k] = pack_half2(v.x, v.y);
         }
+        sum2 = two(sum.x, sum.y);
         ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
-      }
+      };
+#pragma unroll 1
+      for (int c = 0; c < min(n_whole, n_some); ++c) columns(c, std::false_type{});
+#pragma unroll 1
+      for (int c = min(n_whole, n_some); c < n_some; ++c) columns(c, std::true_type{});
 #pragma unroll 1
       for (int c = n_some; c < kGroups; ++c) {
         uint32_t pw[16] = {};
@@ -729,8 +780,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     }
     if (ok && n_x > 0) ok = wait_warp(&sh->o_full[x], 0, abort);
     ts::tc::fence_after_sync();
-    if (ok) {
-      const float inv = l_run > 0.f ? ref_v / (kRefScale * l_run) : l_run;
+    if (ok && x < a.q_tiles) {
+      // A row that saw nothing has a sum of a few 2^-126 at most, and O = 0.
+      float inv = l_run > 0x1p-100f ? ref_v / (kRefScale * l_run) : l_run;
+      if (saw_nan) inv = __uint_as_float(0x7fc00000u);
       // The row goes to the warp's part of its Q tile (no MMA reads it any more), 16 bytes at a
       // time in swizzled places, and from there to memory in whole rows.
       uint8_t* stage = sQ(x) + (warp & 3) * 32 * D * 2;
@@ -777,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   }
   ts::tc::fence_before_sync();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 13) {
     ts::tc::fence_after_sync();
     ts::tc::tmem_dealloc(sh->tmem, kTmemCols);
   }
@@ -793,6 +846,18 @@ bool tc_path(int group, int hkv, int hd, int bs, int dtype, const void* kp, cons
        reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(out)) % 16)
     return false;
   return (q_stride * 2) % 16 == 0;
+}
+
+int sm_count() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (cached[dev] == 0) {
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    cached[dev] = n > 0 ? n : 148;
+  }
+  return cached[dev];
 }
 
 template <typename T, int D>
@@ -866,7 +931,11 @@ extern "C" int ts_paged_prefill_fp8(void* out, const void* query, int64_t query_
   a.scale_log2 = scale * kLog2e;
   const int longest = max_query_len < num_query_tokens ? max_query_len : num_query_tokens;
   const int tiles = (longest + a.tq - 1) / a.tq;
-  const dim3 grid((tiles + kQTiles - 1) / kQTiles, num_kv_heads, num_seqs);
+  // Two query tiles a CTA share each converted K/V tile; one a CTA halves a CTA's time when there
+  // are too few pairs for the SMs (one 512-token chunk over 1,024: see the measurements above).
+  const int64_t pairs = int64_t((tiles + 1) / 2) * num_kv_heads * num_seqs;
+  a.q_tiles = pairs < sm_count() ? 1 : kQTiles;
+  const dim3 grid((tiles + a.q_tiles - 1) / a.q_tiles, num_kv_heads, num_seqs);
   if (dtype == TS_BFLOAT16)
     return head_dim == 128 ? launch<__nv_bfloat16, 128>(a, grid, s)
                            : launch<__nv_bfloat16, 64>(a, grid, s);
