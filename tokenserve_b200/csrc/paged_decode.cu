@@ -28,15 +28,16 @@
 //
 // The 8-bit cache (fp8.cuh: e4m3 codes, one float32 scale per token and KV head) runs the same
 // plan, ring and merge, FP8 = true below. Its block is 2 x (16 D + 64) bytes, about half.
-//   * Codes become f16 operands with integer operations alone: sign | exponent and mantissa << 7
-//     is the f16 number code * 2^-8 (subnormals too), so the products are exact. A byte pair
-//     order falls out of the masks (even bytes, odd bytes); K's is undone in the order of q's
-//     words, V's (read by ldmatrix.trans as pairs of dims) is a permutation of O's rows.
+//   * Codes become f16 operands by the conversion of code pairs (64 a clock and SM; a shift-and-mask
+//     expansion runs at 21). Which codes pair up is free for K, whose dims are taken in the order
+//     of q's words; V's (read by ldmatrix.trans as pairs of dims) pair up by token after a byte
+//     permutation, which permutes O's rows.
 //   * q is scaled per head by a power of two into f16's range (bf16 q stays exact).
 //   * K's scale multiplies the score. V's is added to the exponent of the weight: with t = s +
-//     log2(vs), the running maximum is that of t, w = 2^(t - m) <= 1 goes to the PV product as
-//     f16 (11 bits: 2^-12 of itself, once) and the sum gets 2^(s - m) in 32 bits.
-//   * Slots past the context may hold any codes: they become finite f16 numbers with w = 0.
+//     log2(vs), m is a maximum of t, w = 2^(t - m) goes to the PV product as f16 (11 bits: 2^-12 of
+//     itself, once) and the sum gets 2^(s - m) in 32 bits. m is kept until some t exceeds it by
+//     2^12, so most blocks need no maximum over their tokens and no rescaling of O.
+//   * Slots past the context may hold anything: their scores are masked, their V codes zeroed.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -96,6 +97,11 @@ constexpr int kHeavyParts = TS_DECODE_HEAVY_PARTS;
 static_assert(kPartBlocks >= 2 && kPartBlocks <= 64, "a work item's table fits two registers per lane");
 // Upper bound of the grid's warps (SMs x warps per CTA), used to size the workspace.
 constexpr int kMaxGridWarps = 8192;
+// Least blocks of a partition of the static split over an 8-bit cache.
+#ifndef TS_FP8_MIN_PART
+#define TS_FP8_MIN_PART 4
+#endif
+constexpr int kFp8MinPartBlocks = TS_FP8_MIN_PART;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct DecodeArgs {
@@ -133,6 +139,7 @@ struct DecodeArgs {
   // warps. The main kernel's last CTA re-zeroes [0] and [4], so a later launch can run the
   // same plan (block tables and context lengths unchanged) without the prep kernel.
   int* header;
+  int min_part_blocks;  // the static split gives a group at least this many blocks
   int reuse_plan;  // 1: the workspace holds the prep kernel's plan from an earlier launch
   int grid_warps;  // warps of the main kernel's grid
   // [batch + 1] partitions of one head before sequence b; sequence b's partition k of head h
@@ -241,12 +248,18 @@ __device__ __forceinline__ int ctx_of(const DecodeArgs& a, int b) {
   return ctx < 0 ? 0 : (ctx > cap ? cap : ctx);
 }
 
+// Groups of the static split of WB blocks.
+__device__ __forceinline__ long long static_groups(const DecodeArgs& a, long long WB) {
+  return min((long long)(a.grid_warps / a.num_kv_heads),
+             (WB + a.min_part_blocks - 1) / a.min_part_blocks);
+}
+
 // Static split (small steps): groups of H warps, see kPartBlocks. run0: blocks before this
 // thread's first sequence b0; nblk: its cnt sequences' blocks.
 __device__ void prep_static(DecodeArgs& a, int* warp_sums, long long WB, int run0, int cnt,
                             int b0) {
   const int B = a.batch;
-  const int NG = int(min((long long)(a.grid_warps / a.num_kv_heads), WB));
+  const int NG = int(static_groups(a, WB));
   const GroupSplit gsp(int(WB), NG > 0 ? NG : 1);
   // A group spans at most kPartBlocks blocks (the prep kernel's choice of split), so each
   // group a sequence overlaps holds exactly one of its partitions: the count is the number of
@@ -439,7 +452,7 @@ __global__ void __launch_bounds__(kPrepThreads) decode_prep_kernel(DecodeArgs a,
   const long long WB = total_smem;
   // Static split while every group of the split spans at most min(kStaticMaxBlocksPerWarp,
   // kPartBlocks) blocks (ceil(WB / NG)); dynamic claiming above.
-  const long long NG = min((long long)(a.grid_warps / H), WB);
+  const long long NG = static_groups(a, WB);
   if (NG <= 0 || (WB + NG - 1) / NG > (long long)min(kStaticMaxBlocksPerWarp, kPartBlocks)) {
     prep_dynamic(a, warp_sums, cnt, b0);
   } else {
@@ -498,13 +511,15 @@ __device__ __forceinline__ uint32_t tile_off_fp8(int t, int cg) {
   return t * 64 + ((cg ^ ((t >> 1) & 3)) << 4);
 }
 
-// Codes become f16 numbers times 2^-8 (see the head of the file); K's and V's both.
-constexpr float kCodeScale = 256.f;
-
-// Four codes -> (byte 0, byte 2) and (byte 1, byte 3) as f16x2.
-__device__ __forceinline__ void fp8_expand(uint32_t x, uint32_t& even, uint32_t& odd) {
-  even = ((x << 8) & 0x80008000u) | ((x << 7) & 0x3f803f80u);
-  odd = (x & 0x80008000u) | ((x >> 1) & 0x3f803f80u);
+// Four codes -> (byte 0, byte 1) and (byte 2, byte 3) as f16x2.
+__device__ __forceinline__ void fp8_expand(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  const __half2 a = ts::fp8_half2(x), b = ts::fp8_half2(x >> 16);
+  lo = *reinterpret_cast<const uint32_t*>(&a);
+  hi = *reinterpret_cast<const uint32_t*>(&b);
+}
+// The same for (byte 0, byte 2) and (byte 1, byte 3).
+__device__ __forceinline__ void fp8_expand_even_odd(uint32_t x, uint32_t& even, uint32_t& odd) {
+  fp8_expand(__byte_perm(x, 0, 0x3120), even, odd);
 }
 
 // Byte offset of 16-byte chunk `cg` (dims 8cg..8cg+7) of token `t` inside a K or V tile in
@@ -520,6 +535,15 @@ __device__ __forceinline__ uint32_t tile_off(int t, int cg) {
   }
 }
 
+// m is kept until exceeded by 2^12: weights stay below f16's 2^16.
+constexpr float kFp8MaxSlack = 12.f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct ItemInfo {
   int b, h, blk0, nparts, ctx, nblk, part_global, slot0;
 };
@@ -530,7 +554,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
                         const __grid_constant__ CUtensorMap vmap, const DecodeArgs a) {
   using G = Geometry<D, FP8>;
   using Mma = ts::MmaOp<T>;
-  constexpr float kOutScale = FP8 ? kCodeScale : 1.f;  // what O's accumulators are divided by
   constexpr int S = G::kStages;
   constexpr int KSTEPS = D / 16;
   constexpr int MTILES = D / 16;
@@ -744,7 +767,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       const uint32_t* qrow =
           reinterpret_cast<const uint32_t*>(qb + int64_t(it.h * a.group + head) * D);
       if constexpr (FP8) {
-        // Words (4t, 4t + 2) and (4t + 1, 4t + 3) of each 16 dims, the order fp8_expand gives K.
+        // Dims (4t, 4t + 1) and (4t + 2, 4t + 3) of each 16, the order fp8_expand gives K.
         // The quad holds the head's row: q is multiplied by 2^(14 - exponent of its amax).
         float2 qv[KSTEPS][2];
         uint32_t m = 0;
@@ -759,11 +782,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const int e = max(int(m >> 23), 27);  // biased exponent; tiny rows keep a finite factor
         const float up = __uint_as_float(uint32_t(127 + 14 + 127 - e) << 23);
-        const float down = ldexpf(a.scale_log2 * kCodeScale, e - 127 - 14);
+        const float down = ldexpf(a.scale_log2, e - 127 - 14);
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) {
-          qf[nt][ks][0] = ts::MmaOp<__half>::pack(qv[ks][0].x * up, qv[ks][1].x * up);
-          qf[nt][ks][1] = ts::MmaOp<__half>::pack(qv[ks][0].y * up, qv[ks][1].y * up);
+          qf[nt][ks][0] = ts::MmaOp<__half>::pack(qv[ks][0].x * up, qv[ks][0].y * up);
+          qf[nt][ks][1] = ts::MmaOp<__half>::pack(qv[ks][1].x * up, qv[ks][1].y * up);
         }
         qs[nt][0] = __shfl_sync(0xffffffffu, down, (2 * t) << 2);
         qs[nt][1] = __shfl_sync(0xffffffffu, down, (2 * t + 1) << 2);
@@ -816,8 +839,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       // transposes lane (g, t) has dims (4t, 4t + 2) and (4t + 1, 4t + 3) of head g: 8 bytes.
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float i0 = l_run[nt][0] > 0.f ? kOutScale / l_run[nt][0] : l_run[nt][0];
-        const float i1 = l_run[nt][1] > 0.f ? kOutScale / l_run[nt][1] : l_run[nt][1];
+        const float i0 = l_run[nt][0] > 0.f ? 1.f / l_run[nt][0] : l_run[nt][0];
+        const float i1 = l_run[nt][1] > 0.f ? 1.f / l_run[nt][1] : l_run[nt][1];
         const int head = nt * 8 + g;
         bool vec;
         T* orow = dst_row(0, it.b, it.h * a.group + head, vec);
@@ -972,7 +995,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
 #pragma unroll
       for (int i = 0; i < PER; ++i) acc[i] += w * __ldcg(src + lane + 32 * i);
     }
-    const float inv = lsum > 0.f ? kOutScale / lsum : FP8 ? lsum : 0.f;
+    const float inv = lsum > 0.f ? 1.f / lsum : FP8 ? lsum : 0.f;
     // Lane (hd, kq = lane / NT8) holds dims kq + LPH * i of head hd. Gather each 16-byte chunk
     // (8 consecutive dims) of a head into lane kq = chunk % LPH and store it as one vector.
     constexpr int LPH = 32 / NT8;     // lanes per head
@@ -1046,15 +1069,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       const float s11 = in1 ? sacc[nt][3] * (k1 * qs[nt][1]) : -INFINITY;
       const float t00 = s00 + lv0, t01 = s01 + lv0, t10 = s10 + lv1, t11 = s11 + lv1;
       float bm0 = fmaxf(t00, t10), bm1 = fmaxf(t01, t11);
+      // An item's first block always: its maxima are still -inf.
+      if (__any_sync(0xffffffffu, bm0 > m_run[nt][0] + kFp8MaxSlack ||
+                                      bm1 > m_run[nt][1] + kFp8MaxSlack)) {
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, o));
-        bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, o));
-      }
-      const float mn0 = fmaxf(m_run[nt][0], bm0), mn1 = fmaxf(m_run[nt][1], bm1);
-      const bool moved = mn0 != m_run[nt][0] || mn1 != m_run[nt][1];
-      if (__any_sync(0xffffffffu, moved)) {
-        const float c0 = exp2f(m_run[nt][0] - mn0), c1 = exp2f(m_run[nt][1] - mn1);
+        for (int o = 4; o < 32; o <<= 1) {
+          bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, o));
+          bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, o));
+        }
+        const float mn0 = fmaxf(m_run[nt][0], bm0), mn1 = fmaxf(m_run[nt][1], bm1);
+        const float c0 = ex2(m_run[nt][0] - mn0), c1 = ex2(m_run[nt][1] - mn1);
         l_run[nt][0] *= c0;
         l_run[nt][1] *= c1;
 #pragma unroll
@@ -1067,22 +1091,35 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         m_run[nt][0] = mn0;
         m_run[nt][1] = mn1;
       }
-      l_run[nt][0] += exp2f(s00 - mn0) + exp2f(s10 - mn0);
-      l_run[nt][1] += exp2f(s01 - mn1) + exp2f(s11 - mn1);
-      const uint32_t w0 = MmaH::pack(exp2f(t00 - mn0), exp2f(t01 - mn1));
-      const uint32_t w1 = MmaH::pack(exp2f(t10 - mn0), exp2f(t11 - mn1));
+      const float m0 = m_run[nt][0], m1 = m_run[nt][1];
+      l_run[nt][0] += ex2(s00 - m0) + ex2(s10 - m0);
+      l_run[nt][1] += ex2(s01 - m1) + ex2(s11 - m1);
+      const uint32_t w0 = MmaH::pack(ex2(t00 - m0), ex2(t01 - m1));
+      const uint32_t w1 = MmaH::pack(ex2(t10 - m0), ex2(t11 - m1));
       pb[nt][0] = ts::movmatrix_trans(v0 == 0.f ? 0u : w0);
       pb[nt][1] = ts::movmatrix_trans(v1 == 0.f ? 0u : w1);
     }
+    // Tokens 2t, 2t + 1 and 2t + 8, 2t + 9 of a V word: two bytes each.
+    const bool whole = nvalid >= kBlock;
+    auto token_mask = [&](int tok) {
+      return (tok < nvalid ? 0x0000ffffu : 0u) | (tok + 1 < nvalid ? 0xffff0000u : 0u);
+    };
+    const uint32_t keep0 = token_mask(2 * t), keep1 = token_mask(2 * t + 8);
 #pragma unroll
     for (int mp = 0; mp < MTILES / 2; ++mp) {
       uint32_t r[4];  // dims 2g, 2g + 1 of tokens 2t, 2t + 1 (+ 8), then of the next 16 dims
       ts::ldmatrix_x4_trans(r, vb + tile_off_fp8<D>(row, mp * 2 + (lane >> 4)));
+      if (!whole) {
+        r[0] &= keep0;
+        r[1] &= keep1;
+        r[2] &= keep0;
+        r[3] &= keep1;
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t af[4];
-        fp8_expand(r[2 * u], af[0], af[1]);
-        fp8_expand(r[2 * u + 1], af[2], af[3]);
+        fp8_expand_even_odd(r[2 * u], af[0], af[1]);
+        fp8_expand_even_odd(r[2 * u + 1], af[2], af[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           MmaH::run(oacc[nt][2 * mp + u], af, pb[nt][0], pb[nt][1]);
@@ -1452,6 +1489,7 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
   DecodeArgs a;
   a.k_scales = k_scales;
   a.v_scales = v_scales;
+  a.min_part_blocks = fp8 ? kFp8MinPartBlocks : 1;
   a.out = out;
   a.outs = nullptr;
   a.n_out = 0;
@@ -1647,6 +1685,7 @@ extern "C" int ts_paged_decode_no_alloc(void* out, const void* query, int64_t qu
   uint8_t* ws = static_cast<uint8_t*>(scratch);
   DecodeArgs a;
   a.k_scales = a.v_scales = nullptr;
+  a.min_part_blocks = 1;
   a.out = out;
   a.outs = nullptr;
   a.n_out = 0;
@@ -1771,6 +1810,7 @@ int paged_decode_exchange(bool pull, void* const* dst_outs, int32_t world, int32
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DecodeArgs a;
   a.k_scales = a.v_scales = nullptr;
+  a.min_part_blocks = 1;
   a.out = nullptr;
   // push: this rank's rows go into every rank's buffer; pull: into its own buffer only, and
   // the other ranks fetch them (ts_gather_peers).
