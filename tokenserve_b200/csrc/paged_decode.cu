@@ -102,6 +102,19 @@ constexpr int kMaxGridWarps = 8192;
 #define TS_FP8_MIN_PART 4
 #endif
 constexpr int kFp8MinPartBlocks = TS_FP8_MIN_PART;
+// Warps per CTA over an 8-bit cache: with half the bytes per block the warps' instructions, not HBM,
+// are what a block waits for, and 8 warps left the schedulers idle 60% of the time. Two query tiles
+// (more than 8 query heads per KV head) need the registers of 8.
+#ifndef TS_FP8_WARPS
+#define TS_FP8_WARPS 12
+#endif
+#ifndef TS_FP8_STAGES
+#define TS_FP8_STAGES 48  // stages of a CTA at head_dim 128, over its warps
+#endif
+constexpr int fp8_warps(int nt) { return nt == 1 ? TS_FP8_WARPS : 8; }
+// Partials of a (sequence, head) merged by one warp before the merge of all, over an 8-bit cache.
+constexpr int kMergeGroup = 8;
+constexpr int kMaxWarps = std::max(kWarps, fp8_warps(1));
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct DecodeArgs {
@@ -151,13 +164,14 @@ struct DecodeArgs {
   int4* part_info;
   int* group_first;  // [groups + 1] first partition of each group (static split)
   int* arrive;  // [batch * num_kv_heads]
+  int* group_arrive;  // [slot] of a (sequence, head)'s first slots: its groups of partials (8-bit)
   float* part_o;   // [partition][head_dim][NT * 8]
   float2* part_ml;  // [partition][NT * 8]
 };
 
 // Workspace layout (byte offsets), shared by the size query and the launcher.
 struct WsLayout {
-  size_t chunk_prefix, part_info, group_first, arrive, part_o, part_ml, total;
+  size_t chunk_prefix, part_info, group_first, arrive, group_arrive, part_o, part_ml, total;
 };
 
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -177,7 +191,8 @@ WsLayout ws_layout(int batch, int hkv, int hd, int max_blocks, int nt, int grid_
   w.part_info = w.chunk_prefix + align256(sizeof(int) * (size_t(batch) + 1));
   w.group_first = w.part_info + align256(2 * sizeof(int4) * slots);
   w.arrive = w.group_first + align256(sizeof(int) * (size_t(grid_warps) + 1));
-  w.part_o = w.arrive + align256(sizeof(int) * bh);
+  w.group_arrive = w.arrive + align256(sizeof(int) * bh);
+  w.part_o = w.group_arrive + align256(sizeof(int) * slots);
   w.part_ml = w.part_o + align256(sizeof(float) * slots * hd * nt * 8);
   w.total = w.part_ml + align256(sizeof(float2) * slots * nt * 8);
   return w;
@@ -468,6 +483,11 @@ __global__ void __launch_bounds__(kPrepThreads) decode_prep_kernel(DecodeArgs a,
         for (int e = 0; e < row_elems; ++e) dst[e] = ts::from_float<T>(0.f);
       }
   for (int i = threadIdx.x; i < B * H; i += blockDim.x) a.arrive[i] = 0;
+  if (a.group_arrive != nullptr) {
+    __syncthreads();  // chunk_prefix[B], the step's partitions, is written
+    const int slots = a.chunk_prefix[B] * H;
+    for (int i = threadIdx.x; i < slots; i += blockDim.x) a.group_arrive[i] = 0;
+  }
 }
 
 // Output row (sequence b, query head j) in destination o (< max(n_out, 1)).
@@ -485,12 +505,14 @@ __device__ __forceinline__ uint32_t movmatrix_pack(float lo, float hi) {
   return ts::movmatrix_trans(Mma::pack(lo, hi));
 }
 
-template <int D, bool FP8 = false>
+template <int D, bool FP8 = false, int NT = 1>
 struct Geometry {
+  static constexpr int kWarps = FP8 ? fp8_warps(NT) : ::kWarps;
   static constexpr int kHalves = D / 64;              // 64-column TMA boxes per row (16-bit pool)
   static constexpr int kTileBytes = kBlock * D * (FP8 ? 1 : 2);  // one block's K (or V), one head
   static constexpr int kStageBytes = 2 * kTileBytes;  // K tile then V tile
-  static constexpr int kStages = FP8 ? (D == 128 ? 6 : 10) : (D == 128 ? TS_DECODE_STAGES_D128 : 6);
+  static constexpr int kStages = FP8 ? TS_FP8_STAGES * (D == 128 ? 1 : 2) / kWarps
+                                     : (D == 128 ? TS_DECODE_STAGES_D128 : 6);
   static constexpr bool kOneBox = TS_DECODE_ONE_BOX && D == 128 && !FP8;
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kScaleBytes = FP8 ? 2 * kBlock * 4 : 0;  // a block's K then V scales
@@ -549,11 +571,12 @@ struct ItemInfo {
 };
 
 template <typename T, int D, int NT, bool FP8 = false>
-__global__ void __launch_bounds__(kWarps * 32, 1)
+__global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const DecodeArgs a) {
-  using G = Geometry<D, FP8>;
+  using G = Geometry<D, FP8, NT>;
   using Mma = ts::MmaOp<T>;
+  constexpr int kWarps = G::kWarps;
   constexpr int S = G::kStages;
   constexpr int KSTEPS = D / 16;
   constexpr int MTILES = D / 16;
@@ -562,7 +585,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const uint32_t raw = ts::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // 8-bit: through a shuffle, so that the compiler knows the warp's addresses to be uniform.
+  const int warp = FP8 ? __shfl_sync(0xffffffffu, threadIdx.x / 32, 0) : threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
   const int g = lane >> 2, t = lane & 3;
   // Launched programmatically after the prep kernel (or after the caller's previous kernel when
   // the plan is reused): everything below reads the plan, the tables, the query or the pool, so
@@ -931,41 +956,60 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     }
     __threadfence();
     __syncwarp();
-    int old = 0;
-    if (lane == 0) old = atomicAdd(a.arrive + it.b * a.num_kv_heads + it.h, 1);
-    old = __shfl_sync(0xffffffffu, old, 0);
-    if (old != it.nparts - 1) return;
-    __threadfence();
+    // Of the partials of (b, h) `n` warps arrive at `counter`; whether this one is the last.
+    auto last_of = [&](int* counter, int n) {
+      int old = 0;
+      if (lane == 0) old = atomicAdd(counter, 1);
+      old = __shfl_sync(0xffffffffu, old, 0);
+      if (old != n - 1) return false;
+      __threadfence();
+      return true;
+    };
+    // Many partials of an 8-bit cache (its streams are short beside a merge by one warp: 60 of 75 us
+    // for one 30,000-token sequence) are merged by groups first, each group into its first slot.
+    const bool grouped = FP8 && it.nparts > kMergeGroup;
+    const int in_seq = int(slot - it.slot0);
+    const int groups = (it.nparts + kMergeGroup - 1) / kMergeGroup;
+    int* const group_counter = a.group_arrive + it.slot0 + in_seq / kMergeGroup;
+    if (grouped) {
+      if (!last_of(group_counter, min(kMergeGroup, it.nparts - in_seq / kMergeGroup * kMergeGroup)))
+        return;
+      if (lane == 0) *group_counter = 0;
+    } else if (!last_of(a.arrive + it.b * a.num_kv_heads + it.h, it.nparts)) {
+      return;
+    }
     // Last partition of (b, h) to finish: merge all of them. A long sequence has tens of
     // partitions and its merge can run in the kernel's tail, so the loads of several
     // partitions are kept in flight at once (the sums still run in partition order).
     const int hd = lane % NT8;  // fixed head per lane in the [D][NT8] layout
-    const int64_t slot0 = it.slot0;
-    const int np = it.nparts;
+    int64_t slot0 = it.slot0;
+    int np = it.nparts, stride = 1;
+    constexpr int PER = D * NT8 / 32;
+    float acc[PER];
+    float lsum, mx;
+    auto merge = [&]() {
     // Running max: the lanes of one head split the partitions (32 / NT8 per pass, four passes'
     // loads in flight), then reduce across those lanes.
     constexpr int kLanesPerHead = 32 / NT8;
-    float mx = -INFINITY;
+    mx = -INFINITY;
     for (int p0 = lane / NT8; p0 < np; p0 += 4 * kLanesPerHead) {
       float v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int p = p0 + u * kLanesPerHead;
-        v[u] = p < np ? __ldcg(&a.part_ml[(slot0 + p) * NT8 + hd].x) : -INFINITY;
+        v[u] = p < np ? __ldcg(&a.part_ml[(slot0 + p * stride) * NT8 + hd].x) : -INFINITY;
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) mx = fmaxf(mx, v[u]);
     }
 #pragma unroll
     for (int o = NT8; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    constexpr int PER = D * NT8 / 32;
-    float acc[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-    float lsum = 0.f;
+    lsum = 0.f;
     int p = 0;
     for (; p + 1 < np; p += 2) {  // two partitions' loads in flight
-      const int64_t s0 = slot0 + p, s1 = s0 + 1;
+      const int64_t s0 = slot0 + p * stride, s1 = s0 + stride;
       const float2 ml0 = __ldcg(&a.part_ml[s0 * NT8 + hd]);
       const float2 ml1 = __ldcg(&a.part_ml[s1 * NT8 + hd]);
       const float* src0 = a.part_o + s0 * D * NT8;
@@ -987,7 +1031,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       }
     }
     if (p < np) {
-      const int64_t sl = slot0 + p;
+      const int64_t sl = slot0 + p * stride;
       const float2 ml = __ldcg(&a.part_ml[sl * NT8 + hd]);
       const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mx);
       lsum += w * ml.y;
@@ -995,6 +1039,23 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
 #pragma unroll
       for (int i = 0; i < PER; ++i) acc[i] += w * __ldcg(src + lane + 32 * i);
     }
+    };
+    if (grouped) {
+      slot0 += in_seq / kMergeGroup * kMergeGroup;
+      np = min(kMergeGroup, it.nparts - in_seq / kMergeGroup * kMergeGroup);
+      merge();
+      float* dst = a.part_o + slot0 * D * NT8;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) dst[lane + 32 * i] = acc[i];
+      if (lane < NT8) a.part_ml[slot0 * NT8 + lane] = make_float2(mx, lsum);
+      __threadfence();
+      __syncwarp();
+      if (!last_of(a.arrive + it.b * a.num_kv_heads + it.h, groups)) return;
+      slot0 = it.slot0;
+      np = groups;
+      stride = kMergeGroup;
+    }
+    merge();
     const float inv = lsum > 0.f ? 1.f / lsum : FP8 ? lsum : 0.f;
     // Lane (hd, kq = lane / NT8) holds dims kq + LPH * i of head hd. Gather each 16-byte chunk
     // (8 consecutive dims) of a head into lane kq = chunk % LPH and store it as one vector.
@@ -1353,7 +1414,7 @@ bool make_pool_map_fp8(CUtensorMap* map, const void* pool, int64_t rows, int hd)
 template <typename T, int D, int NT, bool FP8 = false>
 int launch_fast(DecodeArgs a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s,
                 bool plan = true) {
-  using G = Geometry<D, FP8>;
+  using G = Geometry<D, FP8, NT>;
   auto kern = paged_decode_kernel<T, D, NT, FP8>;
   // Once per device: later calls may be captured into a CUDA graph.
   static bool attr_done[64] = {};
@@ -1385,7 +1446,7 @@ int launch_fast(DecodeArgs a, const CUtensorMap& km, const CUtensorMap& vm, cuda
                                                cudaGetErrorString(e));
   }
   cfg.gridDim = dim3(num_sms());
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(G::kWarps * 32);
   cfg.dynamicSmemBytes = G::kSmemBytes;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, km, vm, a);
   if (e != cudaSuccess)
@@ -1427,7 +1488,9 @@ extern "C" size_t ts_paged_decode_workspace_size(int32_t batch, int32_t num_q_he
       (head_dim != 64 && head_dim != 128) || num_q_heads / num_kv_heads > 16)
     return 0;
   const int nt = num_q_heads / num_kv_heads > 8 ? 2 : 1;
-  return ws_layout(batch, num_kv_heads, head_dim, max_blocks_per_seq, nt, num_sms() * kWarps).total;
+  // The larger grid of the two caches' kernels.
+  return ws_layout(batch, num_kv_heads, head_dim, max_blocks_per_seq, nt,
+                   num_sms() * std::max(kWarps, fp8_warps(nt))).total;
 }
 
 namespace {
@@ -1467,11 +1530,12 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
   if (batch > 8192)
     return ts::set_error(TS_ERR_UNSUPPORTED, "paged_decode: batch %d above 8192", batch);
   if (int64_t(batch) * max_blocks_per_seq >= (int64_t(1) << 31) ||
-      max_blocks_per_seq > (1 << 20) || num_sms() * kWarps > kMaxGridWarps)
+      max_blocks_per_seq > (1 << 20) || num_sms() * kMaxWarps > kMaxGridWarps)
     return ts::set_error(TS_ERR_UNSUPPORTED, "paged_decode: batch x max_blocks or grid too large");
   const int group = num_q_heads / num_kv_heads;
   const int nt = group > 8 ? 2 : 1;
-  const WsLayout w = ws_layout(batch, num_kv_heads, head_dim, max_blocks_per_seq, nt, num_sms() * kWarps);
+  const int grid_warps = num_sms() * (fp8 ? fp8_warps(nt) : kWarps);
+  const WsLayout w = ws_layout(batch, num_kv_heads, head_dim, max_blocks_per_seq, nt, grid_warps);
   if (workspace == nullptr || workspace_bytes < w.total)
     return ts::set_error(TS_ERR_WORKSPACE_TOO_SMALL,
                          "paged_decode: workspace of %zu bytes, need %zu", workspace_bytes,
@@ -1511,12 +1575,13 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
   a.group = group;
   a.num_blocks = num_blocks;
   a.scale_log2 = scale * kLog2e;
-  a.grid_warps = num_sms() * kWarps;
+  a.grid_warps = grid_warps;
   a.header = reinterpret_cast<int*>(ws);
   a.chunk_prefix = reinterpret_cast<int*>(ws + w.chunk_prefix);
   a.part_info = reinterpret_cast<int4*>(ws + w.part_info);
   a.group_first = reinterpret_cast<int*>(ws + w.group_first);
   a.arrive = reinterpret_cast<int*>(ws + w.arrive);
+  a.group_arrive = reinterpret_cast<int*>(ws + w.group_arrive);
   a.part_o = reinterpret_cast<float*>(ws + w.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
 #define TS_FAST(T)                                                             \
@@ -1686,6 +1751,7 @@ extern "C" int ts_paged_decode_no_alloc(void* out, const void* query, int64_t qu
   DecodeArgs a;
   a.k_scales = a.v_scales = nullptr;
   a.min_part_blocks = 1;
+  a.group_arrive = nullptr;
   a.out = out;
   a.outs = nullptr;
   a.n_out = 0;
@@ -1811,6 +1877,7 @@ int paged_decode_exchange(bool pull, void* const* dst_outs, int32_t world, int32
   DecodeArgs a;
   a.k_scales = a.v_scales = nullptr;
   a.min_part_blocks = 1;
+  a.group_arrive = nullptr;
   a.out = nullptr;
   // push: this rank's rows go into every rank's buffer; pull: into its own buffer only, and
   // the other ranks fetch them (ts_gather_peers).
