@@ -37,7 +37,8 @@
 //     log2(vs), m is a maximum of t, w = 2^(t - m) goes to the PV product as f16 (11 bits: 2^-12 of
 //     itself, once) and the sum gets 2^(s - m) in 32 bits. m is kept until some t exceeds it by
 //     2^12, so most blocks need no maximum over their tokens and no rescaling of O.
-//   * Slots past the context may hold anything: their scores are masked, their V codes zeroed.
+//   * Slots past the context may hold anything: in a sequence's last block they are made zeros in
+//     shared memory and their scores masked.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -1092,10 +1093,31 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
     if (lane == 0) a.arrive[it.b * a.num_kv_heads + it.h] = 0;
   };
 
-  // One block of an 8-bit cache: scores, online softmax and PV product.
-  auto block_fp8 = [&](uint32_t kb, uint32_t vb, const float* sc, int nvalid) {
-    using MmaH = ts::MmaOp<__half>;
+  // One block of an 8-bit cache: scores, online softmax and PV product. ldmatrix offsets inside a K
+  // or V tile: token row, chunks 2i and 2i + 1 (the swizzle's XOR of an even number).
+  uint32_t chunk_off[D / 32];
+  {
     const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) chunk_off[i] = tile_off_fp8<D>(row, 2 * i + (lane >> 4));
+  }
+  auto block_fp8 = [&](uint8_t* tile, float* sc, int nvalid) {
+    using MmaH = ts::MmaOp<__half>;
+    const bool whole = nvalid >= kBlock;
+    if (!whole) {
+      // Slots past the context may hold anything: zero rows, scales of 1, scores masked below.
+      for (int i = lane; i < (kBlock - nvalid) * (D / 16); i += 32) {
+        uint4* row = reinterpret_cast<uint4*>(tile + nvalid * D) + i;  // whole rows: swizzled or not
+        *row = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(row) + G::kTileBytes) =
+            make_uint4(0, 0, 0, 0);
+      }
+      if (lane >= nvalid && lane < kBlock) sc[lane] = sc[kBlock + lane] = 1.f;
+      __syncwarp();
+    }
+    const uint32_t kb = ts::smem_u32(tile);
+    const float k0 = sc[g], k1 = sc[g + 8];
+    const float lv0 = __log2f(sc[kBlock + g]), lv1 = __log2f(sc[kBlock + g + 8]);
     float sacc[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -1104,7 +1126,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
 #pragma unroll
     for (int kp = 0; kp < KSTEPS / 2; ++kp) {
       uint32_t r[4];  // tokens g and g + 8 of 16 dims, then of the next 16
-      ts::ldmatrix_x4(r, kb + tile_off_fp8<D>(row, kp * 2 + (lane >> 4)));
+      ts::ldmatrix_x4(r, kb + chunk_off[kp]);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t af[4];
@@ -1115,30 +1137,39 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
           MmaH::run(sacc[nt], af, qf[nt][2 * kp + u][0], qf[nt][2 * kp + u][1]);
       }
     }
-    const bool in0 = g < nvalid, in1 = g + 8 < nvalid;
-    const float k0 = sc[g], k1 = sc[g + 8];
-    // In the maximum a scale of 0 counts as 2^-126, so it stays finite; its row weighs nothing.
-    const float v0 = in0 ? sc[kBlock + g] : 1.f, v1 = in1 ? sc[kBlock + g + 8] : 1.f;
-    const float lv0 = __log2f(v0 == 0.f ? 0x1p-126f : v0);
-    const float lv1 = __log2f(v1 == 0.f ? 0x1p-126f : v1);
     uint32_t pb[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float s00 = in0 ? sacc[nt][0] * (k0 * qs[nt][0]) : -INFINITY;
-      const float s01 = in0 ? sacc[nt][1] * (k0 * qs[nt][1]) : -INFINITY;
-      const float s10 = in1 ? sacc[nt][2] * (k1 * qs[nt][0]) : -INFINITY;
-      const float s11 = in1 ? sacc[nt][3] * (k1 * qs[nt][1]) : -INFINITY;
-      const float t00 = s00 + lv0, t01 = s01 + lv0, t10 = s10 + lv1, t11 = s11 + lv1;
-      float bm0 = fmaxf(t00, t10), bm1 = fmaxf(t01, t11);
+      // e: log2 of the sum's terms, e + lv: of the weights, both relative to the maximum kept.
+      float f[4] = {k0 * qs[nt][0], k0 * qs[nt][1], k1 * qs[nt][0], k1 * qs[nt][1]};
+      float e[4], w[4];
+      auto relative = [&]() {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          e[j] = fmaf(sacc[nt][j], f[j], -m_run[nt][j & 1]);
+          if (!whole && (j < 2 ? g : g + 8) >= nvalid) e[j] = -INFINITY;
+          w[j] = e[j] + (j < 2 ? lv0 : lv1);
+        }
+      };
+      relative();
       // An item's first block always: its maxima are still -inf.
-      if (__any_sync(0xffffffffu, bm0 > m_run[nt][0] + kFp8MaxSlack ||
-                                      bm1 > m_run[nt][1] + kFp8MaxSlack)) {
+      if (__any_sync(0xffffffffu, fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > kFp8MaxSlack ||
+                                      m_run[nt][0] == -INFINITY)) {
+        // A scale of 0 counts as 2^-126 here, so that the maximum is finite.
+        float bm[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float s0 = sacc[nt][j] * f[j], s1 = sacc[nt][j + 2] * f[j + 2];
+          const float t0 = whole || g < nvalid ? fmaxf(s0 + lv0, s0 - 126.f) : -INFINITY;
+          const float t1 = whole || g + 8 < nvalid ? fmaxf(s1 + lv1, s1 - 126.f) : -INFINITY;
+          bm[j] = fmaxf(t0, t1);
+        }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
-          bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, o));
-          bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, o));
+          bm[0] = fmaxf(bm[0], __shfl_xor_sync(0xffffffffu, bm[0], o));
+          bm[1] = fmaxf(bm[1], __shfl_xor_sync(0xffffffffu, bm[1], o));
         }
-        const float mn0 = fmaxf(m_run[nt][0], bm0), mn1 = fmaxf(m_run[nt][1], bm1);
+        const float mn0 = fmaxf(m_run[nt][0], bm[0]), mn1 = fmaxf(m_run[nt][1], bm[1]);
         const float c0 = ex2(m_run[nt][0] - mn0), c1 = ex2(m_run[nt][1] - mn1);
         l_run[nt][0] *= c0;
         l_run[nt][1] *= c1;
@@ -1151,31 +1182,17 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
         }
         m_run[nt][0] = mn0;
         m_run[nt][1] = mn1;
+        relative();
       }
-      const float m0 = m_run[nt][0], m1 = m_run[nt][1];
-      l_run[nt][0] += ex2(s00 - m0) + ex2(s10 - m0);
-      l_run[nt][1] += ex2(s01 - m1) + ex2(s11 - m1);
-      const uint32_t w0 = MmaH::pack(ex2(t00 - m0), ex2(t01 - m1));
-      const uint32_t w1 = MmaH::pack(ex2(t10 - m0), ex2(t11 - m1));
-      pb[nt][0] = ts::movmatrix_trans(v0 == 0.f ? 0u : w0);
-      pb[nt][1] = ts::movmatrix_trans(v1 == 0.f ? 0u : w1);
+      l_run[nt][0] += ex2(e[0]) + ex2(e[2]);
+      l_run[nt][1] += ex2(e[1]) + ex2(e[3]);
+      pb[nt][0] = ts::movmatrix_trans(MmaH::pack(ex2(w[0]), ex2(w[1])));
+      pb[nt][1] = ts::movmatrix_trans(MmaH::pack(ex2(w[2]), ex2(w[3])));
     }
-    // Tokens 2t, 2t + 1 and 2t + 8, 2t + 9 of a V word: two bytes each.
-    const bool whole = nvalid >= kBlock;
-    auto token_mask = [&](int tok) {
-      return (tok < nvalid ? 0x0000ffffu : 0u) | (tok + 1 < nvalid ? 0xffff0000u : 0u);
-    };
-    const uint32_t keep0 = token_mask(2 * t), keep1 = token_mask(2 * t + 8);
 #pragma unroll
     for (int mp = 0; mp < MTILES / 2; ++mp) {
       uint32_t r[4];  // dims 2g, 2g + 1 of tokens 2t, 2t + 1 (+ 8), then of the next 16 dims
-      ts::ldmatrix_x4_trans(r, vb + tile_off_fp8<D>(row, mp * 2 + (lane >> 4)));
-      if (!whole) {
-        r[0] &= keep0;
-        r[1] &= keep1;
-        r[2] &= keep0;
-        r[3] &= keep1;
-      }
+      ts::ldmatrix_x4_trans(r, kb + G::kTileBytes + chunk_off[mp]);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t af[4];
@@ -1210,7 +1227,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       const int tok0 = (it.blk0 + md.y) * kBlock;
       const int nvalid = it.ctx - tok0;
       if constexpr (FP8) {
-        block_fp8(kb, vb, scales + s * 2 * kBlock, nvalid);
+        block_fp8(ring + s * G::kStageBytes, scales + s * 2 * kBlock, nvalid);
       } else {
 
       // S^T[token][head] = K Q^T
