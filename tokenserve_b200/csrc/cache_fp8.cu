@@ -8,8 +8,9 @@
 //
 // All three are bound by HBM. A row's D elements are spread over D * size / 16 neighbouring lanes
 // (one 16-byte vector each), so the row's amax is a few shuffles, the row is read once, and the
-// half-layout rotary partner comes from another lane of the row instead of a second load. Rows
-// that do not split that way (odd sizes or alignment) take a warp per row with scalar accesses.
+// half-layout rotary partner comes from another lane of the row instead of a second load. A thread
+// has the vectors of four rows in flight, and no 64-bit division stands before them. Rows that do
+// not split that way (odd sizes or alignment) take a warp per row with scalar accesses.
 #include "fp8.cuh"
 
 namespace {
@@ -36,6 +37,24 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
   for (int o = LPR / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
+
+// Block and offset of a slot; `shift` is log2(block_size), or -1 if that is no power of two.
+struct Place {
+  int64_t block;
+  int off;
+  __device__ __forceinline__ Place(int64_t slot, int block_size, int shift) {
+    block = shift >= 0 ? slot >> shift : slot / block_size;
+    off = int(slot - block * block_size);
+  }
+};
+
+int log2_or_minus_one(int n) {
+  for (int s = 0; s < 31; ++s)
+    if (n == 1 << s) return s;
+  return -1;
+}
+
+constexpr int kInFlight = 4;  // rows of a thread at a time
 
 __device__ __forceinline__ void flag(int32_t* error_flag) {
   if (error_flag != nullptr) atomicExch(error_flag, 1);
@@ -73,7 +92,7 @@ struct AppendArgs {
   float* value_scales;
   const int64_t* slots;
   int64_t num_tokens;
-  int heads, d, block_size;
+  int heads, d, block_size, block_shift;
   int64_t num_slots;
   const int32_t* tags;
   int32_t* tag_pool;
@@ -93,36 +112,48 @@ __device__ __forceinline__ void token_side(const AppendArgs& a, int64_t t) {
   if (s >= 0 && s < a.num_slots && a.tag_pool != nullptr) a.tag_pool[s] = __ldg(a.tags + t);
 }
 
-// Rows (token, K|V, head) in order, LPR lanes each.
+// Rows (token, K|V, head) in order, LPR lanes each, kInFlight rows a thread.
 template <typename T, int LPR>
 __global__ void __launch_bounds__(256) append_fp8_kernel(const AppendArgs a) {
   ts::allow_dependents();
   constexpr int E = Vec<T>::E, D = LPR * E, RPC = 256 / LPR;
   const int c = threadIdx.x % LPR;
-  const int64_t row = int64_t(blockIdx.x) * RPC + threadIdx.x / LPR;
-  const int per_tok = 2 * a.heads;
-  const int64_t t = row / per_tok;
-  const int r = int(row - t * per_tok);
-  const bool is_v = r >= a.heads;
-  const int h = is_v ? r - a.heads : r;
-  const bool in = t < a.num_tokens;
-  const int64_t slot = in ? live_slot(a.slots, t, a.num_slots) : -1;
-  const bool live = slot >= 0;
-  float x[E];
+  const uint32_t per_tok = 2 * a.heads;
+  const uint32_t row0 = blockIdx.x * (RPC * kInFlight) + threadIdx.x / LPR;
+  Vec<T> v[kInFlight];
+  uint32_t tok[kInFlight], r[kInFlight];
+  int64_t slot[kInFlight];
 #pragma unroll
-  for (int e = 0; e < E; ++e) x[e] = 0.f;
-  if (live) {
-    const T* src = static_cast<const T*>(is_v ? a.value : a.key) +
-                   t * (is_v ? a.value_stride : a.key_stride) + int64_t(h) * D + c * E;
-    const Vec<T> v = *reinterpret_cast<const Vec<T>*>(src);
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = ts::to_float(v.v[e]);
+  for (int i = 0; i < kInFlight; ++i) {
+    tok[i] = (row0 + i * RPC) / per_tok;
+    r[i] = row0 + i * RPC - tok[i] * per_tok;
+    slot[i] = tok[i] < a.num_tokens ? live_slot(a.slots, tok[i], a.num_slots) : -1;
   }
-  if (in && r == 0 && c == 0) token_side(a, t);
-  const int64_t blk = live ? slot / a.block_size : 0;
-  const int64_t prow = (blk * a.heads + h) * a.block_size + (live ? slot - blk * a.block_size : 0);
-  store_row_fp8<E, LPR>(x, c, live, (is_v ? a.value_pool : a.key_pool) + prow * D,
-                        (is_v ? a.value_scales : a.key_scales) + prow);
+#pragma unroll
+  for (int i = 0; i < kInFlight; ++i) {
+    const bool is_v = r[i] >= uint32_t(a.heads);
+    const T* src = static_cast<const T*>(is_v ? a.value : a.key) +
+                   int64_t(tok[i]) * (is_v ? a.value_stride : a.key_stride) +
+                   (is_v ? r[i] - a.heads : r[i]) * D + c * E;
+    if (slot[i] >= 0) {
+      v[i] = *reinterpret_cast<const Vec<T>*>(src);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[i].v[e] = ts::from_float<T>(0.f);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kInFlight; ++i) {
+    const bool is_v = r[i] >= uint32_t(a.heads), live = slot[i] >= 0;
+    if (tok[i] < a.num_tokens && r[i] == 0 && c == 0) token_side(a, tok[i]);
+    float x[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = ts::to_float(v[i].v[e]);
+    const Place at(live ? slot[i] : 0, a.block_size, a.block_shift);
+    const int64_t prow = (at.block * a.heads + (is_v ? r[i] - a.heads : r[i])) * a.block_size + at.off;
+    store_row_fp8<E, LPR>(x, c, live, (is_v ? a.value_pool : a.key_pool) + prow * D,
+                          (is_v ? a.value_scales : a.key_scales) + prow);
+  }
 }
 
 // Any head_dim, stride and alignment: one warp per row.
@@ -171,14 +202,12 @@ int launch_append(const AppendArgs& a, cudaStream_t s) {
       (a.value_stride * es) % 16 || !aligned(a.key_pool, cb) || !aligned(a.value_pool, cb))
     lpr = 0;
   const int64_t rows = a.num_tokens * 2 * a.heads;
-  if (lpr == 0) {
+  if (lpr == 0 || rows >= int64_t(4294967295) - 65536) {  // the fast kernel counts rows in 32 bits
     const int64_t g = (rows + 7) / 8;
     append_fp8_any_kernel<T><<<unsigned(g < 65536 ? g : 65536), 256, 0, s>>>(a);
     return ts::launch_status("reshape_and_cache_fp8");
   }
-  const int64_t grid = (rows + 256 / lpr - 1) / (256 / lpr);
-  if (grid > 2147483647)
-    return ts::set_error(TS_ERR_UNSUPPORTED, "reshape_and_cache_fp8: too many tokens");
+  const int64_t per_cta = 256 / lpr * kInFlight, grid = (rows + per_cta - 1) / per_cta;
   switch (lpr) {
     case 4: append_fp8_kernel<T, 4><<<unsigned(grid), 256, 0, s>>>(a); break;
     case 8: append_fp8_kernel<T, 8><<<unsigned(grid), 256, 0, s>>>(a); break;
@@ -201,7 +230,7 @@ struct RotaryArgs {
   const int64_t* slots;
   const int64_t* positions;
   const float* inv_freq;
-  int hq, hkv, d, rd, block_size;
+  int hq, hkv, d, rd, block_size, block_shift;
   float mscale;
   int64_t num_slots;
   int32_t* error_flag;
@@ -217,87 +246,96 @@ __device__ __forceinline__ float2 cos_sin(int64_t pos, float f, float mscale) {
   return make_float2(c * mscale, s * mscale);
 }
 
-// One CTA per token; cos/sin once per token in shared memory, then one 16-byte vector of a head
-// row per thread and pass. Requires rd % (2 E) == 0 (half layout: a lane's partner values sit in
-// one other lane), rows of LPR * 16 bytes, 16-byte aligned.
+// One CTA per token. A thread always has the same dims (c) of its rows: the first kInFlight rows
+// are on their way while the token's cos and sin are computed (in shared memory, once), which it
+// then keeps in registers for all its rows. Requires rd % (2 E) == 0 (half layout: a lane's partner
+// values sit in one other lane), rows of LPR * 16 bytes, 16-byte aligned.
 template <typename T, int LPR, bool INTERLEAVED, bool FP8>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   ts::allow_dependents();
-  constexpr int E = Vec<T>::E, D = LPR * E;
+  constexpr int E = Vec<T>::E, D = LPR * E, RPC = 256 / LPR;
+  constexpr int W = INTERLEAVED ? E / 2 : E;  // angles a lane needs
   const int64_t t = blockIdx.x;
-  const T* in = static_cast<const T*>(a.qkv) + t * a.qkv_stride;
-  const int half = a.rd / 2;
-  __shared__ float2 cs[D / 2];
+  const int c = threadIdx.x % LPR, rows = a.hq + 2 * a.hkv, half = a.rd / 2;
+  const T* in = static_cast<const T*>(a.qkv) + t * a.qkv_stride + c * E;
   const int64_t pos = __ldg(a.positions + t), slot_raw = __ldg(a.slots + t);
+  const int64_t slot = slot_raw < a.num_slots ? slot_raw : -1;
+  Vec<T> v[kInFlight];
+  auto live_row = [&](int r) { return r < rows && (r < a.hq || slot >= 0); };
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+      const int r = r0 + i * RPC;
+      if (r < rows) {
+        v[i] = *reinterpret_cast<const Vec<T>*>(in + r * D);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[i].v[e] = ts::from_float<T>(0.f);
+      }
+    }
+  };
+  load(threadIdx.x / LPR);
+  __shared__ alignas(16) float2 cs[D / 2];
   for (int i = threadIdx.x; i < half; i += blockDim.x)
     cs[i] = cos_sin(pos, __ldg(a.inv_freq + i), a.mscale);
-  const int64_t slot = slot_raw < a.num_slots ? slot_raw : -1;
   if (slot_raw >= a.num_slots && threadIdx.x == 0) flag(a.error_flag);
-  const int64_t blk = slot >= 0 ? slot / a.block_size : 0;
-  const int64_t off = slot >= 0 ? slot - blk * a.block_size : 0;
+  const Place at(slot >= 0 ? slot : 0, a.block_size, a.block_shift);
   __syncthreads();
-  const int c = threadIdx.x % LPR;
-  const int rows = a.hq + 2 * a.hkv;
-  const int rpc = blockDim.x / LPR;
-  for (int r0 = 0; r0 < rows; r0 += rpc) {
-    const int r = r0 + threadIdx.x / LPR;
-    const bool is_q = r < a.hq, is_v = r >= a.hq + a.hkv;
-    const bool live = r < rows && (is_q || slot >= 0);
-    Vec<T> v;
-    if (live) {
-      v = *reinterpret_cast<const Vec<T>*>(in + r * D + c * E);
-    } else {
+  const int i0 = c * E;          // this lane's first dimension
+  const int hl = half / E;       // half layout: lanes with the first halves of the pairs
+  const bool first = c < hl, turned = i0 < a.rd;
+  float2 w[W];
 #pragma unroll
-      for (int e = 0; e < E; ++e) v.v[e] = ts::from_float<T>(0.f);
-    }
-    float x[E];
+  for (int e = 0; e < W; ++e)
+    w[e] = !turned ? make_float2(1.f, 0.f) : cs[(INTERLEAVED ? i0 / 2 : first ? i0 : i0 - half) + e];
+  const int partner = (threadIdx.x % 32) + (first ? hl : (turned ? -hl : 0));
+  const float sign = first ? -1.f : 1.f;  // of the partner's product
+  for (int r0 = threadIdx.x / LPR; r0 - threadIdx.x / LPR < rows; r0 += kInFlight * RPC) {
+    if (r0 >= kInFlight * RPC) load(r0);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = ts::to_float(v.v[e]);
-    const int i0 = c * E;  // this lane's first dimension
-    if (INTERLEAVED) {
-      if (!is_v && i0 < a.rd) {
+    for (int i = 0; i < kInFlight; ++i) {
+      if (r0 - int(threadIdx.x) / LPR + i * RPC >= rows) break;  // for the whole CTA
+      const int r = r0 + i * RPC;
+      const bool is_q = r < a.hq, is_v = r >= a.hq + a.hkv, live = live_row(r);
+      float x[E];
 #pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 w = cs[(i0 + e) / 2];
-          const float p = x[e], q = x[e + 1];
-          x[e] = p * w.x - q * w.y;
-          x[e + 1] = q * w.x + p * w.y;
+      for (int e = 0; e < E; ++e) x[e] = ts::to_float(v[i].v[e]);
+      if (INTERLEAVED) {
+        if (!is_v && turned) {
+#pragma unroll
+          for (int e = 0; e < E; e += 2) {
+            const float p = x[e], q = x[e + 1];
+            x[e] = p * w[e / 2].x - q * w[e / 2].y;
+            x[e + 1] = q * w[e / 2].x + p * w[e / 2].y;
+          }
+        }
+      } else {
+        const uint32_t* raw = reinterpret_cast<const uint32_t*>(&v[i]);
+        Vec<T> o;
+        uint32_t* oraw = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) oraw[k] = __shfl_sync(0xffffffffu, raw[k], partner & 31);
+        if (!is_v && turned) {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            x[e] = x[e] * w[e % W].x + sign * ts::to_float(o.v[e]) * w[e % W].y;
         }
       }
-    } else {
-      // Lanes below half / E hold the first halves of the pairs, the next half / E the second.
-      const int hl = half / E;
-      const bool first = c < hl, turned = c < 2 * hl;
-      const int partner = (threadIdx.x % 32) + (first ? hl : (turned ? -hl : 0));
-      const uint32_t* raw = reinterpret_cast<const uint32_t*>(&v);
-      Vec<T> o;
-      uint32_t* oraw = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) oraw[k] = __shfl_sync(0xffffffffu, raw[k], partner & 31);
-      if (!is_v && turned) {
-        const int j = first ? i0 : i0 - half;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float2 w = cs[j + e];
-          const float y = ts::to_float(o.v[e]);
-          x[e] = first ? x[e] * w.x - y * w.y : x[e] * w.x + y * w.y;
-        }
+      const int h = is_q ? r : (is_v ? r - a.hq - a.hkv : r - a.hq);
+      const int64_t prow = (at.block * a.hkv + h) * a.block_size + at.off;
+      if (FP8) {
+        store_row_fp8<E, LPR>(x, c, live && !is_q,
+                              static_cast<uint8_t*>(is_v ? a.value_pool : a.key_pool) + prow * D,
+                              (is_v ? a.value_scales : a.key_scales) + prow);
       }
-    }
-    const int h = is_q ? r : (is_v ? r - a.hq - a.hkv : r - a.hq);
-    const int64_t prow = (blk * a.hkv + h) * a.block_size + off;
-    if (FP8) {
-      store_row_fp8<E, LPR>(x, c, live && !is_q,
-                            static_cast<uint8_t*>(is_v ? a.value_pool : a.key_pool) + prow * D,
-                            (is_v ? a.value_scales : a.key_scales) + prow);
-    }
-    if (live && (is_q || !FP8)) {
-      T* dst = is_q ? static_cast<T*>(a.q_out) + (t * a.hq + h) * D
-                    : static_cast<T*>(is_v ? a.value_pool : a.key_pool) + prow * D;
-      Vec<T> y;
+      if (live && (is_q || !FP8)) {
+        T* dst = is_q ? static_cast<T*>(a.q_out) + (t * a.hq + h) * D
+                      : static_cast<T*>(is_v ? a.value_pool : a.key_pool) + prow * D;
+        Vec<T> y;
 #pragma unroll
-      for (int e = 0; e < E; ++e) y.v[e] = ts::from_float<T>(x[e]);
-      *reinterpret_cast<Vec<T>*>(dst + c * E) = y;
+        for (int e = 0; e < E; ++e) y.v[e] = ts::from_float<T>(x[e]);
+        *reinterpret_cast<Vec<T>*>(dst + c * E) = y;
+      }
     }
   }
 }
@@ -393,75 +431,96 @@ struct ReadArgs {
   const float* value_scales;
   const int32_t* tables;
   const int32_t* loc;
-  int num_seqs, max_blocks, heads, d, block_size;
+  int num_seqs, max_blocks, heads, d, block_size, block_shift;
   int64_t num_blocks, num_tokens;
   int32_t* error_flag;
 };
 
 constexpr int kReadTokens = 16;  // tokens per CTA
 
-// Pool row (of head 0) of output row t: its sequence by binary search over loc, then the table.
-// -1: t belongs to no sequence (left as it was); -2: its block is not in the pool (zeros).
-__device__ __forceinline__ int64_t source_row(const ReadArgs& a, int64_t t) {
-  if (t >= a.num_tokens || t < __ldg(a.loc) || t >= __ldg(a.loc + a.num_seqs)) return -1;
-  int lo = 0, hi = a.num_seqs;  // loc[lo] <= t < loc[hi]
+// Warp 0 of a CTA finds the pool rows (of head 0) of output rows t0 .. t0 + kReadTokens - 1, one a
+// lane. -1: the row belongs to no sequence (left as it was); -2: its block is not in the pool, or
+// past the table (zeros). The sequence of t0 is narrowed down 32 ways a step; a later row moves on
+// from there.
+__device__ __forceinline__ void find_rows(const ReadArgs& a, int64_t t0, int64_t* src) {
+  const int lane = threadIdx.x;
+  int lo = 0, hi = a.num_seqs;  // loc[lo] <= t0 < loc[hi], or t0 is outside
   while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (__ldg(a.loc + mid) <= t) lo = mid; else hi = mid;
+    const int step = (hi - lo + 31) / 32;
+    const int probe = min(hi, lo + (lane + 1) * step);
+    // Ascending: the probes at or below t0 are the first ones.
+    const int below = __popc(__ballot_sync(0xffffffffu, probe < hi && __ldg(a.loc + probe) <= t0));
+    hi = min(hi, lo + (below + 1) * step);
+    lo += below * step;
   }
-  const int64_t p = t - __ldg(a.loc + lo);
-  const int64_t col = p / a.block_size;
-  if (col >= a.max_blocks) return -2;
-  const int64_t blk = __ldg(a.tables + int64_t(lo) * a.max_blocks + col);
-  if (blk < 0 || blk >= a.num_blocks) return -2;
-  return blk * a.heads * a.block_size + (p - col * a.block_size);
+  const int64_t t = t0 + lane;
+  if (lane >= kReadTokens) return;
+  int64_t s = -1;
+  if (t < a.num_tokens && t >= __ldg(a.loc) && t < __ldg(a.loc + a.num_seqs)) {
+    while (__ldg(a.loc + lo + 1) <= t) ++lo;  // ends: t < loc[num_seqs]
+    const Place at(t - __ldg(a.loc + lo), a.block_size, a.block_shift);
+    s = -2;
+    if (at.block >= 0 && at.block < a.max_blocks) {  // negative: token_start_loc not ascending
+      const int64_t blk = __ldg(a.tables + int64_t(lo) * a.max_blocks + at.block);
+      if (blk >= 0 && blk < a.num_blocks) s = blk * a.heads * a.block_size + at.off;
+    }
+  }
+  if (s == -2) flag(a.error_flag);
+  src[lane] = s;
 }
 
 // CTA = kReadTokens output tokens: their pool rows are looked up once, then every thread turns
-// 8 codes of a (token, K|V, head) row into 8 values. LPR = D / 8 lanes per row.
+// 16 codes of a (token, K|V, head) row into 16 values, kInFlight rows at a time. LPR = D / 16.
 template <typename T, int LPR>
 __global__ void __launch_bounds__(256) read_fp8_kernel(const ReadArgs a) {
-  constexpr int D = LPR * 8;
+  constexpr int D = LPR * 16, RPC = 256 / LPR, E = Vec<T>::E;
   __shared__ int64_t src[kReadTokens];
   const int64_t t0 = int64_t(blockIdx.x) * kReadTokens;
-  if (threadIdx.x < kReadTokens) {
-    const int64_t s = source_row(a, t0 + threadIdx.x);
-    if (s == -2) flag(a.error_flag);
-    src[threadIdx.x] = s;
-  }
+  if (threadIdx.x < 32) find_rows(a, t0, src);
   __syncthreads();
   const int c = threadIdx.x % LPR;
-  const int rows = kReadTokens * 2 * a.heads;
-#pragma unroll 4
-  for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
-    const int tl = r / (2 * a.heads);
-    const int k = r - tl * 2 * a.heads;
-    const bool is_v = k >= a.heads;
-    const int h = is_v ? k - a.heads : k;
-    const int64_t s = src[tl];
-    if (s == -1) continue;
-    uint2 w = make_uint2(0, 0);
-    float sc = 0.f;
-    if (s >= 0) {
-      const int64_t prow = s + int64_t(h) * a.block_size;
-      w = __ldg(reinterpret_cast<const uint2*>((is_v ? a.value_pool : a.key_pool) + prow * D) + c);
-      sc = __ldg((is_v ? a.value_scales : a.key_scales) + prow);
+  const int per_tok = 2 * a.heads, rows = kReadTokens * per_tok;
+  for (int r0 = threadIdx.x / LPR; r0 < rows; r0 += kInFlight * RPC) {
+    uint4 code[kInFlight];
+    float sc[kInFlight];
+    int tok[kInFlight], k[kInFlight];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+      const int r = r0 + i * RPC;
+      tok[i] = r / per_tok;
+      k[i] = r - tok[i] * per_tok;
+      const int64_t s = r < rows ? src[tok[i]] : -1;
+      code[i] = make_uint4(0, 0, 0, 0);
+      sc[i] = 0.f;
+      if (s >= 0) {
+        const bool is_v = k[i] >= a.heads;
+        const int64_t prow = s + int64_t(is_v ? k[i] - a.heads : k[i]) * a.block_size;
+        code[i] = __ldg(reinterpret_cast<const uint4*>((is_v ? a.value_pool : a.key_pool) + prow * D) + c);
+        sc[i] = __ldg((is_v ? a.value_scales : a.key_scales) + prow);
+      }
+      if (s == -1) tok[i] = -1;
     }
-    float f[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 p = __half22float2(ts::fp8_half2((i < 2 ? w.x : w.y) >> (16 * (i & 1))));
-      f[2 * i] = p.x * sc;
-      f[2 * i + 1] = p.y * sc;
-    }
-    T* dst = static_cast<T*>(is_v ? a.value_out : a.key_out) + ((t0 + tl) * a.heads + h) * D + c * 8;
-    constexpr int E = Vec<T>::E;
+    for (int i = 0; i < kInFlight; ++i) {
+      if (tok[i] < 0) continue;
+      const bool is_v = k[i] >= a.heads;
+      T* dst = static_cast<T*>(is_v ? a.value_out : a.key_out) +
+               ((t0 + tok[i]) * a.heads + (is_v ? k[i] - a.heads : k[i])) * D + c * 16;
+      const uint32_t word[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+      float f[16];
 #pragma unroll
-    for (int i = 0; i < 8 / E; ++i) {
-      Vec<T> y;
+      for (int q = 0; q < 8; ++q) {
+        const float2 p = __half22float2(ts::fp8_half2(word[q / 2] >> (16 * (q & 1))));
+        f[2 * q] = p.x * sc[i];
+        f[2 * q + 1] = p.y * sc[i];
+      }
 #pragma unroll
-      for (int e = 0; e < E; ++e) y.v[e] = ts::from_float<T>(f[i * E + e]);
-      *reinterpret_cast<Vec<T>*>(dst + i * E) = y;
+      for (int q = 0; q < 16 / E; ++q) {
+        Vec<T> y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y.v[e] = ts::from_float<T>(f[q * E + e]);
+        *reinterpret_cast<Vec<T>*>(dst + q * E) = y;
+      }
     }
   }
 }
@@ -470,11 +529,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) read_fp8_any_kernel(const ReadArgs a) {
   __shared__ int64_t src[kReadTokens];
   const int64_t t0 = int64_t(blockIdx.x) * kReadTokens;
-  if (threadIdx.x < kReadTokens) {
-    const int64_t s = source_row(a, t0 + threadIdx.x);
-    if (s == -2) flag(a.error_flag);
-    src[threadIdx.x] = s;
-  }
+  if (threadIdx.x < 32) find_rows(a, t0, src);
   __syncthreads();
   const int64_t per_tok = 2 * int64_t(a.heads) * a.d;
   for (int64_t e = threadIdx.x; e < kReadTokens * per_tok; e += 256) {
@@ -499,14 +554,14 @@ __global__ void __launch_bounds__(256) read_fp8_any_kernel(const ReadArgs a) {
 template <typename T>
 int launch_read(const ReadArgs& a, cudaStream_t s) {
   const unsigned g = unsigned((a.num_tokens + kReadTokens - 1) / kReadTokens);
-  const bool vec = aligned(a.key_out, 16) && aligned(a.value_out, 16) && aligned(a.key_pool, 8) &&
-                   aligned(a.value_pool, 8);
+  const bool vec = aligned(a.key_out, 16) && aligned(a.value_out, 16) && aligned(a.key_pool, 16) &&
+                   aligned(a.value_pool, 16);
   if (vec && a.d == 64)
-    read_fp8_kernel<T, 8><<<g, 256, 0, s>>>(a);
+    read_fp8_kernel<T, 4><<<g, 256, 0, s>>>(a);
   else if (vec && a.d == 128)
-    read_fp8_kernel<T, 16><<<g, 256, 0, s>>>(a);
+    read_fp8_kernel<T, 8><<<g, 256, 0, s>>>(a);
   else if (vec && a.d == 256)
-    read_fp8_kernel<T, 32><<<g, 256, 0, s>>>(a);
+    read_fp8_kernel<T, 16><<<g, 256, 0, s>>>(a);
   else
     read_fp8_any_kernel<T><<<g, 256, 0, s>>>(a);
   return ts::launch_status("read_cache_fp8");
@@ -547,7 +602,8 @@ extern "C" int ts_reshape_and_cache_fp8(const void* key, const void* value,
   const AppendArgs a{key, value, key_token_stride, value_token_stride,
                      static_cast<uint8_t*>(key_pool), static_cast<uint8_t*>(value_pool),
                      key_scales, value_scales, slot_mapping, num_tokens, num_kv_heads, head_dim,
-                     block_size, num_blocks * block_size, token_tags, tag_pool, error_flag};
+                     block_size, log2_or_minus_one(block_size), num_blocks * block_size,
+                     token_tags, tag_pool, error_flag};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == TS_FLOAT32) return launch_append<float>(a, s);
   if (dtype == TS_FLOAT16) return launch_append<__half>(a, s);
@@ -592,8 +648,8 @@ extern "C" int ts_rotary_and_cache(const void* qkv, int64_t qkv_token_stride, vo
     return ts::set_error(TS_ERR_MISALIGNED, "rotary_and_cache: pointers not element-aligned");
   const RotaryArgs a{qkv, qkv_token_stride, q_out, key_pool, value_pool, key_scales, value_scales,
                      slot_mapping, positions, inv_freq, num_q_heads, num_kv_heads, head_dim,
-                     rotary_dim, block_size, attention_scaling, num_blocks * block_size,
-                     error_flag};
+                     rotary_dim, block_size, log2_or_minus_one(block_size), attention_scaling,
+                     num_blocks * block_size, error_flag};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == TS_FLOAT32) return launch_rotary<float>(a, num_tokens, interleaved != 0, s);
   if (dtype == TS_FLOAT16) return launch_rotary<__half>(a, num_tokens, interleaved != 0, s);
@@ -629,7 +685,7 @@ extern "C" int ts_read_cache_fp8(void* key_out, void* value_out, const void* key
   const ReadArgs a{key_out, value_out, static_cast<const uint8_t*>(key_pool),
                    static_cast<const uint8_t*>(value_pool), key_scales, value_scales, block_tables,
                    token_start_loc, num_seqs, max_blocks_per_seq, num_kv_heads, head_dim,
-                   block_size, num_blocks, num_tokens, error_flag};
+                   block_size, log2_or_minus_one(block_size), num_blocks, num_tokens, error_flag};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == TS_FLOAT32) return launch_read<float>(a, s);
   if (dtype == TS_FLOAT16) return launch_read<__half>(a, s);
