@@ -56,6 +56,28 @@ int log2_or_minus_one(int n) {
 
 constexpr int kInFlight = 4;  // rows of a thread at a time
 
+// Pairs of floats and the packed fp32 instructions on them.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 __device__ __forceinline__ void flag(int32_t* error_flag) {
   if (error_flag != nullptr) atomicExch(error_flag, 1);
 }
@@ -65,11 +87,11 @@ __device__ __forceinline__ void flag(int32_t* error_flag) {
 template <int E, int LPR>
 __device__ __forceinline__ void store_row_fp8(const float (&x)[E], int c, bool live, uint8_t* row,
                                               float* scale) {
-  uint32_t m = 0;
+  float m = ts::amax3(x[0], x[1], x[2]);
 #pragma unroll
-  for (int e = 0; e < E; ++e) m = max(m, ts::abs_bits(x[e]));
-  const float sc = ts::fp8_row_scale(row_max<LPR>(m));
-  const float inv = 1.f / sc;
+  for (int e = 3; e < E; e += 2) m = ts::amax3(m, x[e], x[e + 1 < E ? e + 1 : e]);
+  float inv;
+  const float sc = ts::fp8_row_scale(row_max<LPR>(__float_as_uint(m)), inv);
   Words<E / 4> w;
 #pragma unroll
   for (int i = 0; i < E / 4; ++i)
@@ -92,7 +114,7 @@ struct AppendArgs {
   float* value_scales;
   const int64_t* slots;
   int64_t num_tokens;
-  int heads, d, block_size, block_shift;
+  int heads, d, block_size, block_shift, tok_shift;  // tok_shift: log2(2 * heads) or -1
   int64_t num_slots;
   const int32_t* tags;
   int32_t* tag_pool;
@@ -125,7 +147,7 @@ __global__ void __launch_bounds__(256) append_fp8_kernel(const AppendArgs a) {
   int64_t slot[kInFlight];
 #pragma unroll
   for (int i = 0; i < kInFlight; ++i) {
-    tok[i] = (row0 + i * RPC) / per_tok;
+    tok[i] = a.tok_shift >= 0 ? (row0 + i * RPC) >> a.tok_shift : (row0 + i * RPC) / per_tok;
     r[i] = row0 + i * RPC - tok[i] * per_tok;
     slot[i] = tok[i] < a.num_tokens ? live_slot(a.slots, tok[i], a.num_slots) : -1;
   }
@@ -150,8 +172,9 @@ __global__ void __launch_bounds__(256) append_fp8_kernel(const AppendArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = ts::to_float(v[i].v[e]);
     const Place at(live ? slot[i] : 0, a.block_size, a.block_shift);
-    const int64_t prow = (at.block * a.heads + (is_v ? r[i] - a.heads : r[i])) * a.block_size + at.off;
-    store_row_fp8<E, LPR>(x, c, live, (is_v ? a.value_pool : a.key_pool) + prow * D,
+    const uint32_t prow =
+        (uint32_t(at.block) * a.heads + (is_v ? r[i] - a.heads : r[i])) * a.block_size + at.off;
+    store_row_fp8<E, LPR>(x, c, live, (is_v ? a.value_pool : a.key_pool) + uint64_t(prow) * D,
                           (is_v ? a.value_scales : a.key_scales) + prow);
   }
 }
@@ -175,7 +198,8 @@ __global__ void __launch_bounds__(256) append_fp8_any_kernel(const AppendArgs a)
                    t * (is_v ? a.value_stride : a.key_stride) + int64_t(h) * a.d;
     uint32_t m = 0;
     for (int i = lane; i < a.d; i += 32) m = max(m, ts::abs_bits(ts::to_float(src[i])));
-    const float sc = ts::fp8_row_scale(row_max<32>(m)), inv = 1.f / sc;
+    float inv;
+    const float sc = ts::fp8_row_scale(row_max<32>(m), inv);
     const int64_t blk = slot / a.block_size;
     const int64_t prow = (blk * a.heads + h) * a.block_size + slot - blk * a.block_size;
     uint8_t* dst = (is_v ? a.value_pool : a.key_pool) + prow * a.d;
@@ -202,7 +226,9 @@ int launch_append(const AppendArgs& a, cudaStream_t s) {
       (a.value_stride * es) % 16 || !aligned(a.key_pool, cb) || !aligned(a.value_pool, cb))
     lpr = 0;
   const int64_t rows = a.num_tokens * 2 * a.heads;
-  if (lpr == 0 || rows >= int64_t(4294967295) - 65536) {  // the fast kernel counts rows in 32 bits
+  // The fast kernel counts the step's and the pool's rows in 32 bits.
+  constexpr int64_t kMost = int64_t(4294967295) - 65536;
+  if (lpr == 0 || rows >= kMost || a.num_slots >= kMost / a.heads) {
     const int64_t g = (rows + 7) / 8;
     append_fp8_any_kernel<T><<<unsigned(g < 65536 ? g : 65536), 256, 0, s>>>(a);
     return ts::launch_status("reshape_and_cache_fp8");
@@ -250,11 +276,14 @@ __device__ __forceinline__ float2 cos_sin(int64_t pos, float f, float mscale) {
 // are on their way while the token's cos and sin are computed (in shared memory, once), which it
 // then keeps in registers for all its rows. Requires rd % (2 E) == 0 (half layout: a lane's partner
 // values sit in one other lane), rows of LPR * 16 bytes, 16-byte aligned.
+#ifndef TS_ROTARY_THREADS
+#define TS_ROTARY_THREADS 128
+#endif
+constexpr int kRotaryThreads = TS_ROTARY_THREADS;
 template <typename T, int LPR, bool INTERLEAVED, bool FP8>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
   ts::allow_dependents();
-  constexpr int E = Vec<T>::E, D = LPR * E, RPC = 256 / LPR;
-  constexpr int W = INTERLEAVED ? E / 2 : E;  // angles a lane needs
+  constexpr int E = Vec<T>::E, D = LPR * E, RPC = kRotaryThreads / LPR;
   const int64_t t = blockIdx.x;
   const int c = threadIdx.x % LPR, rows = a.hq + 2 * a.hkv, half = a.rd / 2;
   const T* in = static_cast<const T*>(a.qkv) + t * a.qkv_stride + c * E;
@@ -284,57 +313,68 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   const int i0 = c * E;          // this lane's first dimension
   const int hl = half / E;       // half layout: lanes with the first halves of the pairs
   const bool first = c < hl, turned = i0 < a.rd;
-  float2 w[W];
+  // cos and sin for each of the lane's dims; with the sign of the partner's product.
+  uint64_t wc[E / 2], ws[E / 2];
 #pragma unroll
-  for (int e = 0; e < W; ++e)
-    w[e] = !turned ? make_float2(1.f, 0.f) : cs[(INTERLEAVED ? i0 / 2 : first ? i0 : i0 - half) + e];
-  const int partner = (threadIdx.x % 32) + (first ? hl : (turned ? -hl : 0));
-  const float sign = first ? -1.f : 1.f;  // of the partner's product
-  for (int r0 = threadIdx.x / LPR; r0 - threadIdx.x / LPR < rows; r0 += kInFlight * RPC) {
+  for (int e = 0; e < E; e += 2) {
+    float2 u = make_float2(1.f, 0.f), v2 = u;
+    if (turned && INTERLEAVED) {
+      u = v2 = cs[(i0 + e) / 2];
+      u.y = -u.y;
+    } else if (turned) {
+      const int j = (first ? i0 : i0 - half) + e;
+      u = cs[j];
+      v2 = cs[j + 1];
+      if (first) u.y = -u.y, v2.y = -v2.y;
+    }
+    wc[e / 2] = two(u.x, v2.x);
+    ws[e / 2] = two(u.y, v2.y);
+  }
+  const int partner = ((threadIdx.x % 32) + (first ? hl : (turned ? -hl : 0))) & 31;
+  // Where the token's rows go: head h at base + h * step.
+  T* const q_row = static_cast<T*>(a.q_out) + t * a.hq * D + c * E;
+  const int64_t first_row = at.block * a.hkv * a.block_size + at.off;
+#pragma unroll 1
+  for (int r0 = threadIdx.x / LPR; r0 - int(threadIdx.x) / LPR < rows; r0 += kInFlight * RPC) {
     if (r0 >= kInFlight * RPC) load(r0);
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
       if (r0 - int(threadIdx.x) / LPR + i * RPC >= rows) break;  // for the whole CTA
       const int r = r0 + i * RPC;
       const bool is_q = r < a.hq, is_v = r >= a.hq + a.hkv, live = live_row(r);
-      float x[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = ts::to_float(v[i].v[e]);
-      if (INTERLEAVED) {
-        if (!is_v && turned) {
-#pragma unroll
-          for (int e = 0; e < E; e += 2) {
-            const float p = x[e], q = x[e + 1];
-            x[e] = p * w[e / 2].x - q * w[e / 2].y;
-            x[e + 1] = q * w[e / 2].x + p * w[e / 2].y;
-          }
-        }
-      } else {
+      Vec<T> o = v[i];
+      if (!INTERLEAVED) {
         const uint32_t* raw = reinterpret_cast<const uint32_t*>(&v[i]);
-        Vec<T> o;
         uint32_t* oraw = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) oraw[k] = __shfl_sync(0xffffffffu, raw[k], partner & 31);
-        if (!is_v && turned) {
+        for (int k = 0; k < 4; ++k) oraw[k] = __shfl_sync(0xffffffffu, raw[k], partner);
+      }
+      float x[E];
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            x[e] = x[e] * w[e % W].x + sign * ts::to_float(o.v[e]) * w[e % W].y;
-        }
+      for (int e = 0; e < E; e += 2) {
+        const float x0 = ts::to_float(v[i].v[e]), x1 = ts::to_float(v[i].v[e + 1]);
+        const float y0 = ts::to_float(o.v[INTERLEAVED ? e + 1 : e]);
+        const float y1 = ts::to_float(o.v[INTERLEAVED ? e : e + 1]);
+        const float2 z = halves(fma2(two(y0, y1), ws[e / 2], mul2(two(x0, x1), wc[e / 2])));
+        x[e] = is_v || !turned ? x0 : z.x;
+        x[e + 1] = is_v || !turned ? x1 : z.y;
       }
       const int h = is_q ? r : (is_v ? r - a.hq - a.hkv : r - a.hq);
-      const int64_t prow = (at.block * a.hkv + h) * a.block_size + at.off;
+      const int64_t prow = first_row + h * a.block_size;
       if (FP8) {
-        store_row_fp8<E, LPR>(x, c, live && !is_q,
-                              static_cast<uint8_t*>(is_v ? a.value_pool : a.key_pool) + prow * D,
-                              (is_v ? a.value_scales : a.key_scales) + prow);
+        // Rows of q only in this warp: nothing to quantise.
+        if (__any_sync(0xffffffffu, !is_q))
+          store_row_fp8<E, LPR>(x, c, live && !is_q,
+                                static_cast<uint8_t*>(is_v ? a.value_pool : a.key_pool) + prow * D,
+                                (is_v ? a.value_scales : a.key_scales) + prow);
       }
       if (live && (is_q || !FP8)) {
-        T* dst = is_q ? static_cast<T*>(a.q_out) + (t * a.hq + h) * D
-                      : static_cast<T*>(is_v ? a.value_pool : a.key_pool) + prow * D;
+        T* dst = is_q ? q_row + r * D
+                      : static_cast<T*>(is_v ? a.value_pool : a.key_pool) + prow * D + c * E;
         Vec<T> y;
 #pragma unroll
         for (int e = 0; e < E; ++e) y.v[e] = ts::from_float<T>(x[e]);
-        *reinterpret_cast<Vec<T>*>(dst + c * E) = y;
+        *reinterpret_cast<Vec<T>*>(dst) = y;
       }
     }
   }
@@ -379,7 +419,8 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryArgs a, int
     }
     uint32_t m = 0;
     for (int i = lane; i < a.d; i += 32) m = max(m, ts::abs_bits(value(i)));
-    const float sc = ts::fp8_row_scale(row_max<32>(m)), inv = 1.f / sc;
+    float inv;
+    const float sc = ts::fp8_row_scale(row_max<32>(m), inv);
     uint8_t* dst = static_cast<uint8_t*>(is_v ? a.value_pool : a.key_pool) + prow * a.d;
     for (int i = lane; i < a.d; i += 32)
       dst[i] = uint8_t(ts::fp8_pack4(value(i), 0.f, 0.f, 0.f, inv));
@@ -392,11 +433,11 @@ void launch_rotary_vec(const RotaryArgs& a, int64_t tokens, bool interleaved, cu
   const unsigned g = unsigned(tokens);
   const bool fp8 = a.key_scales != nullptr;
   if (interleaved)
-    fp8 ? rotary_kernel<T, LPR, true, true><<<g, 256, 0, s>>>(a)
-        : rotary_kernel<T, LPR, true, false><<<g, 256, 0, s>>>(a);
+    fp8 ? rotary_kernel<T, LPR, true, true><<<g, kRotaryThreads, 0, s>>>(a)
+        : rotary_kernel<T, LPR, true, false><<<g, kRotaryThreads, 0, s>>>(a);
   else
-    fp8 ? rotary_kernel<T, LPR, false, true><<<g, 256, 0, s>>>(a)
-        : rotary_kernel<T, LPR, false, false><<<g, 256, 0, s>>>(a);
+    fp8 ? rotary_kernel<T, LPR, false, true><<<g, kRotaryThreads, 0, s>>>(a)
+        : rotary_kernel<T, LPR, false, false><<<g, kRotaryThreads, 0, s>>>(a);
 }
 
 template <typename T>
@@ -602,8 +643,9 @@ extern "C" int ts_reshape_and_cache_fp8(const void* key, const void* value,
   const AppendArgs a{key, value, key_token_stride, value_token_stride,
                      static_cast<uint8_t*>(key_pool), static_cast<uint8_t*>(value_pool),
                      key_scales, value_scales, slot_mapping, num_tokens, num_kv_heads, head_dim,
-                     block_size, log2_or_minus_one(block_size), num_blocks * block_size,
-                     token_tags, tag_pool, error_flag};
+                     block_size, log2_or_minus_one(block_size),
+                     log2_or_minus_one(2 * num_kv_heads), num_blocks * block_size, token_tags,
+                     tag_pool, error_flag};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == TS_FLOAT32) return launch_append<float>(a, s);
   if (dtype == TS_FLOAT16) return launch_append<__half>(a, s);

@@ -19,10 +19,23 @@ constexpr float kE4m3Max = 448.f;
 // Bits of |x|: as unsigned integers they order like the magnitudes, with NaN above infinity.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Scale of a row whose largest |x| has these bits.
-__device__ __forceinline__ float fp8_row_scale(uint32_t amax_bits) {
-  if (amax_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-  return fmaxf(__fdiv_rn(__uint_as_float(amax_bits), kE4m3Max), 0x1p-126f);
+// max(|a|, |b|, |c|), NaN if one is.
+__device__ __forceinline__ float amax3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Scale of a row whose largest |x| has these bits: amax / 448, correctly rounded (a product by the
+// reciprocal and one correction), and 1 / scale to an ulp.
+__device__ __forceinline__ float fp8_row_scale(uint32_t amax_bits, float& inv) {
+  constexpr float kInv = 1.f / kE4m3Max;
+  const float amax = __uint_as_float(amax_bits);
+  float sc = amax * kInv;
+  sc = fmaxf(fmaf(fmaf(-sc, kE4m3Max, amax), kInv, sc), 0x1p-126f);
+  if (amax_bits >= 0x7f800000u) sc = __uint_as_float(0x7fc00000u);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sc));
+  return sc;
 }
 
 // Four codes of x * inv (element 0 in the low byte), saturating; NaN stays NaN.
