@@ -82,9 +82,10 @@ __device__ __forceinline__ void flag(int32_t* error_flag) {
   if (error_flag != nullptr) atomicExch(error_flag, 1);
 }
 
-// One lane's E values of a row -> E codes at row + c * E, the scale from the row's first lane.
-// Every lane of the warp takes part (shuffles); `live` rows are stored.
-template <int E, int LPR>
+// One lane's E values of a row -> E codes at row + c * E, the scale from the row's first lane; with
+// VPL > 1 the lane has E / VPL values of each of VPL parts of the row. Every lane of the warp takes
+// part (shuffles); `live` rows are stored.
+template <int E, int LPR, int VPL = 1>
 __device__ __forceinline__ void store_row_fp8(const float (&x)[E], int c, bool live, uint8_t* row,
                                               float* scale) {
   float m = ts::amax3(x[0], x[1], x[2]);
@@ -92,12 +93,16 @@ __device__ __forceinline__ void store_row_fp8(const float (&x)[E], int c, bool l
   for (int e = 3; e < E; e += 2) m = ts::amax3(m, x[e], x[e + 1 < E ? e + 1 : e]);
   float inv;
   const float sc = ts::fp8_row_scale(row_max<LPR>(__float_as_uint(m)), inv);
-  Words<E / 4> w;
+  constexpr int P = E / VPL;
+  Words<P / 4> w[VPL];
 #pragma unroll
   for (int i = 0; i < E / 4; ++i)
-    w.w[i] = ts::fp8_pack4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], inv);
+    w[i / (P / 4)].w[i % (P / 4)] =
+        ts::fp8_pack4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], inv);
   if (live) {
-    *reinterpret_cast<Words<E / 4>*>(row + c * E) = w;
+#pragma unroll
+    for (int q = 0; q < VPL; ++q)
+      *reinterpret_cast<Words<P / 4>*>(row + (q * LPR + c) * P) = w[q];
     if (c == 0) *scale = sc;
   }
 }
@@ -134,48 +139,53 @@ __device__ __forceinline__ void token_side(const AppendArgs& a, int64_t t) {
   if (s >= 0 && s < a.num_slots && a.tag_pool != nullptr) a.tag_pool[s] = __ldg(a.tags + t);
 }
 
-// Rows (token, K|V, head) in order, LPR lanes each, kInFlight rows a thread.
-template <typename T, int LPR>
+// Rows (token, K|V, head) in order: LPR lanes each with VPL 16-byte vectors, LPR vectors apart (half
+// the lanes with two vectors each take half the shuffles and scale arithmetic), ROWS rows a thread.
+template <typename T, int LPR, int VPL, int ROWS>
 __global__ void __launch_bounds__(256) append_fp8_kernel(const AppendArgs a) {
   ts::allow_dependents();
-  constexpr int E = Vec<T>::E, D = LPR * E, RPC = 256 / LPR;
+  constexpr int E = Vec<T>::E, D = LPR * E * VPL, RPC = 256 / LPR;
   const int c = threadIdx.x % LPR;
   const uint32_t per_tok = 2 * a.heads;
-  const uint32_t row0 = blockIdx.x * (RPC * kInFlight) + threadIdx.x / LPR;
-  Vec<T> v[kInFlight];
-  uint32_t tok[kInFlight], r[kInFlight];
-  int64_t slot[kInFlight];
+  const uint32_t row0 = blockIdx.x * (RPC * ROWS) + threadIdx.x / LPR;
+  Vec<T> v[ROWS][VPL];
+  uint32_t tok[ROWS], r[ROWS];
+  int64_t slot[ROWS];
 #pragma unroll
-  for (int i = 0; i < kInFlight; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     tok[i] = a.tok_shift >= 0 ? (row0 + i * RPC) >> a.tok_shift : (row0 + i * RPC) / per_tok;
     r[i] = row0 + i * RPC - tok[i] * per_tok;
     slot[i] = tok[i] < a.num_tokens ? live_slot(a.slots, tok[i], a.num_slots) : -1;
   }
 #pragma unroll
-  for (int i = 0; i < kInFlight; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     const bool is_v = r[i] >= uint32_t(a.heads);
     const T* src = static_cast<const T*>(is_v ? a.value : a.key) +
                    int64_t(tok[i]) * (is_v ? a.value_stride : a.key_stride) +
                    (is_v ? r[i] - a.heads : r[i]) * D + c * E;
-    if (slot[i] >= 0) {
-      v[i] = *reinterpret_cast<const Vec<T>*>(src);
-    } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[i].v[e] = ts::from_float<T>(0.f);
+    for (int q = 0; q < VPL; ++q) {
+      if (slot[i] >= 0) {
+        v[i][q] = *reinterpret_cast<const Vec<T>*>(src + q * LPR * E);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[i][q].v[e] = ts::from_float<T>(0.f);
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < kInFlight; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     const bool is_v = r[i] >= uint32_t(a.heads), live = slot[i] >= 0;
     if (tok[i] < a.num_tokens && r[i] == 0 && c == 0) token_side(a, tok[i]);
-    float x[E];
+    float x[E * VPL];
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = ts::to_float(v[i].v[e]);
+    for (int e = 0; e < E * VPL; ++e) x[e] = ts::to_float(v[i][e / E].v[e % E]);
     const Place at(live ? slot[i] : 0, a.block_size, a.block_shift);
     const uint32_t prow =
         (uint32_t(at.block) * a.heads + (is_v ? r[i] - a.heads : r[i])) * a.block_size + at.off;
-    store_row_fp8<E, LPR>(x, c, live, (is_v ? a.value_pool : a.key_pool) + uint64_t(prow) * D,
-                          (is_v ? a.value_scales : a.key_scales) + prow);
+    store_row_fp8<E * VPL, LPR, VPL>(x, c, live,
+                                     (is_v ? a.value_pool : a.key_pool) + uint64_t(prow) * D,
+                                     (is_v ? a.value_scales : a.key_scales) + prow);
   }
 }
 
@@ -233,12 +243,14 @@ int launch_append(const AppendArgs& a, cudaStream_t s) {
     append_fp8_any_kernel<T><<<unsigned(g < 65536 ? g : 65536), 256, 0, s>>>(a);
     return ts::launch_status("reshape_and_cache_fp8");
   }
-  const int64_t per_cta = 256 / lpr * kInFlight, grid = (rows + per_cta - 1) / per_cta;
+  constexpr int kRows = 1;  // two as fast for many rows and slower for few, four slower
+  const int lanes = lpr == 4 ? 4 : lpr / 2;
+  const int64_t per_cta = 256 / lanes * kRows, grid = (rows + per_cta - 1) / per_cta;
   switch (lpr) {
-    case 4: append_fp8_kernel<T, 4><<<unsigned(grid), 256, 0, s>>>(a); break;
-    case 8: append_fp8_kernel<T, 8><<<unsigned(grid), 256, 0, s>>>(a); break;
-    case 16: append_fp8_kernel<T, 16><<<unsigned(grid), 256, 0, s>>>(a); break;
-    default: append_fp8_kernel<T, 32><<<unsigned(grid), 256, 0, s>>>(a); break;
+    case 4: append_fp8_kernel<T, 4, 1, kRows><<<unsigned(grid), 256, 0, s>>>(a); break;
+    case 8: append_fp8_kernel<T, 4, 2, kRows><<<unsigned(grid), 256, 0, s>>>(a); break;
+    case 16: append_fp8_kernel<T, 8, 2, kRows><<<unsigned(grid), 256, 0, s>>>(a); break;
+    default: append_fp8_kernel<T, 16, 2, kRows><<<unsigned(grid), 256, 0, s>>>(a); break;
   }
   return ts::launch_status("reshape_and_cache_fp8");
 }
@@ -276,14 +288,16 @@ __device__ __forceinline__ float2 cos_sin(int64_t pos, float f, float mscale) {
 // are on their way while the token's cos and sin are computed (in shared memory, once), which it
 // then keeps in registers for all its rows. Requires rd % (2 E) == 0 (half layout: a lane's partner
 // values sit in one other lane), rows of LPR * 16 bytes, 16-byte aligned.
-#ifndef TS_ROTARY_THREADS
-#define TS_ROTARY_THREADS 128
-#endif
-constexpr int kRotaryThreads = TS_ROTARY_THREADS;
+//
+// 64 threads keep a token's set-up small beside its rows when there are many tokens (16,381 tokens of
+// 32/8 heads: 67 us, 75 with 128, 107 with 256); with few tokens 128 shorten it (256 tokens: 3.6 us,
+// 4.7 with 64).
+constexpr int kRotaryThreads = 128, kRotaryThreadsMany = 64, kRotaryManyTokens = 1024;
 template <typename T, int LPR, bool INTERLEAVED, bool FP8>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
   ts::allow_dependents();
-  constexpr int E = Vec<T>::E, D = LPR * E, RPC = kRotaryThreads / LPR;
+  constexpr int E = Vec<T>::E, D = LPR * E;
+  const int RPC = blockDim.x / LPR;
   const int64_t t = blockIdx.x;
   const int c = threadIdx.x % LPR, rows = a.hq + 2 * a.hkv, half = a.rd / 2;
   const T* in = static_cast<const T*>(a.qkv) + t * a.qkv_stride + c * E;
@@ -431,13 +445,14 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryArgs a, int
 template <typename T, int LPR>
 void launch_rotary_vec(const RotaryArgs& a, int64_t tokens, bool interleaved, cudaStream_t s) {
   const unsigned g = unsigned(tokens);
+  const int threads = tokens < kRotaryManyTokens ? kRotaryThreads : kRotaryThreadsMany;
   const bool fp8 = a.key_scales != nullptr;
   if (interleaved)
-    fp8 ? rotary_kernel<T, LPR, true, true><<<g, kRotaryThreads, 0, s>>>(a)
-        : rotary_kernel<T, LPR, true, false><<<g, kRotaryThreads, 0, s>>>(a);
+    fp8 ? rotary_kernel<T, LPR, true, true><<<g, threads, 0, s>>>(a)
+        : rotary_kernel<T, LPR, true, false><<<g, threads, 0, s>>>(a);
   else
-    fp8 ? rotary_kernel<T, LPR, false, true><<<g, kRotaryThreads, 0, s>>>(a)
-        : rotary_kernel<T, LPR, false, false><<<g, kRotaryThreads, 0, s>>>(a);
+    fp8 ? rotary_kernel<T, LPR, false, true><<<g, threads, 0, s>>>(a)
+        : rotary_kernel<T, LPR, false, false><<<g, threads, 0, s>>>(a);
 }
 
 template <typename T>

@@ -391,41 +391,50 @@ def silu_mul(out: torch.Tensor, gate_up: torch.Tensor) -> None:
 # The operators below run on their tensors' device, on its current stream.
 
 
-def _cuda(what: str, *tensors: torch.Tensor | None) -> torch.device:
-    """The one CUDA device all the (present) tensors live on."""
-    dev = None
+def _cuda(what: str, *tensors: torch.Tensor | None) -> int:
+    """Index of the one CUDA device all the (present) tensors live on."""
+    dev = tensors[0].get_device()  # type: ignore[union-attr]
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda or (dev is not None and t.device != dev):
-            raise KernelError(f"{what}: tensors must be on one CUDA device")
-        dev = t.device
+        if t is not None and t.get_device() != dev:
+            dev = -1
+    if dev < 0:
+        raise KernelError(f"{what}: tensors must be on one CUDA device")
     return dev
 
 
-def _launch(what: str, device: torch.device, fn, *args) -> None:  # type: ignore[no-untyped-def]
-    """Calls ``fn(*args, stream)`` with ``device`` current, on its current stream."""
-    if torch.cuda.current_device() == device.index:
-        _check(fn(*args, _stream()), what)
+# The raw handle of a device's current stream. torch.cuda.current_stream() builds a Stream object
+# for it, 3 us of a small call's 10.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)  # fmt: skip
+
+
+def _launch(what: str, device: int, name: str, *args) -> None:  # type: ignore[no-untyped-def]
+    """Calls the entry point ``name`` with ``device`` current, on its current stream."""
+    fn = getattr(_lib or load_library(), name)
+    if torch.cuda.current_device() == device:
+        code = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            _check(fn(*args, _stream()), what)
+            code = fn(*args, _raw_stream(device))
+    if code:
+        _check(code, what)
 
 
 def _fp8_pool_dims(what: str, key_pool: torch.Tensor, value_pool: torch.Tensor,
-                   key_scales: torch.Tensor, value_scales: torch.Tensor
-                   ) -> tuple[int, int, int, int]:  # fmt: skip
+                   key_scales: torch.Tensor, value_scales: torch.Tensor) -> torch.Size:  # fmt: skip
     shape = key_pool.shape
-    for p in (key_pool, value_pool):
-        if (p.dtype != torch.float8_e4m3fn or len(shape) != 4 or p.shape != shape
-                or not p.is_contiguous()):  # fmt: skip
-            raise KernelError(f"{what}: 8-bit pools must be contiguous float8_e4m3fn "
-                              "[num_blocks, kv_heads, block_size, head_dim]")  # fmt: skip
-    for s in (key_scales, value_scales):
-        if s.dtype != torch.float32 or s.shape != shape[:3] or not s.is_contiguous():
-            raise KernelError(f"{what}: scales must be contiguous float32 "
-                              "[num_blocks, kv_heads, block_size]")  # fmt: skip
-    return shape[0], shape[1], shape[2], shape[3]
+    if (len(shape) != 4 or value_pool.shape != shape or key_pool.dtype != torch.float8_e4m3fn
+            or value_pool.dtype != torch.float8_e4m3fn or not key_pool.is_contiguous()
+            or not value_pool.is_contiguous()):  # fmt: skip
+        raise KernelError(f"{what}: 8-bit pools must be contiguous float8_e4m3fn "
+                          "[num_blocks, kv_heads, block_size, head_dim]")  # fmt: skip
+    rows = shape[:3]
+    if (key_scales.shape != rows or value_scales.shape != rows
+            or key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32
+            or not key_scales.is_contiguous() or not value_scales.is_contiguous()):  # fmt: skip
+        raise KernelError(f"{what}: scales must be contiguous float32 "
+                          "[num_blocks, kv_heads, block_size]")  # fmt: skip
+    return shape
 
 
 def _int_array(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, n: int) -> None:
@@ -488,7 +497,7 @@ def reshape_and_cache_fp8(
     if tag_pool is not None:
         _int_array(what, "tag_pool", tag_pool, torch.int32, nb * bs)
     _error_flag(what, error_flag)
-    _launch(what, dev, load_library().ts_reshape_and_cache_fp8,
+    _launch(what, dev, "ts_reshape_and_cache_fp8",
             _ptr(key), _ptr(value), ks, vs, _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
             _ptr(value_scales), _ptr(slot_mapping), n, h, d, bs, nb, _dtype(key),
             _ptr(token_tags), _ptr(tag_pool), _ptr(error_flag))  # fmt: skip
@@ -543,7 +552,7 @@ def rotary_and_cache(
     half = inv_freq.numel()
     _int_array(what, "inv_freq", inv_freq, torch.float32, half)
     _error_flag(what, error_flag)
-    _launch(what, dev, load_library().ts_rotary_and_cache,
+    _launch(what, dev, "ts_rotary_and_cache",
             _ptr(qkv), qkv.stride(0) if n > 1 else width, _ptr(q_out), _ptr(key_pool),
             _ptr(value_pool), _ptr(key_scales), _ptr(value_scales), _ptr(slot_mapping),
             _ptr(positions), _ptr(inv_freq), n, num_q_heads, hkv, d, 2 * half, int(interleaved),
@@ -575,7 +584,7 @@ def read_cache_fp8(
     width = _tables(what, block_tables, seqs)
     _int_array(what, "token_start_loc", token_start_loc, torch.int32, seqs + 1)
     _error_flag(what, error_flag)
-    _launch(what, dev, load_library().ts_read_cache_fp8,
+    _launch(what, dev, "ts_read_cache_fp8",
             _ptr(key_out), _ptr(value_out), _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
             _ptr(value_scales), _ptr(block_tables), width, _ptr(token_start_loc), seqs, n, h, d,
             bs, nb, _dtype(key_out), _ptr(error_flag))  # fmt: skip
@@ -607,7 +616,7 @@ def paged_decode_fp8(
     if workspace is not None and not workspace.is_contiguous():
         raise KernelError(f"{what}: workspace must be contiguous")
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _launch(what, dev, load_library().ts_paged_decode_fp8,
+    _launch(what, dev, "ts_paged_decode_fp8",
             _ptr(out), _ptr(query), qs, _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
             _ptr(value_scales), _ptr(block_tables), width, _ptr(context_lens), b, hq, hkv, d, bs,
             nb, float(scale), _dtype(query), _ptr(workspace), ws_bytes,
@@ -637,7 +646,7 @@ def paged_prefill_fp8(
     width = _tables(what, block_tables, seqs)
     _int_array(what, "context_lens", context_lens, torch.int32, seqs)
     _int_array(what, "query_start_loc", query_start_loc, torch.int32, seqs + 1)
-    _launch(what, dev, load_library().ts_paged_prefill_fp8,
+    _launch(what, dev, "ts_paged_prefill_fp8",
             _ptr(out), _ptr(query), qs, _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
             _ptr(value_scales), _ptr(block_tables), width, _ptr(query_start_loc),
             _ptr(context_lens), seqs, query.shape[0], int(max_query_len), hq, hkv, d, bs, nb,
