@@ -109,3 +109,13 @@ def test_wrappers_refuse_other_pools_and_host_tensors(lib) -> None:  # type: ign
             match="go together")  # fmt: skip
     refused(ops.rotary_and_cache, qkv, q, kp, vp, slots, slots, torch.ones(32), 4, 2,
             match="qkv's dtype")  # fmt: skip
+
+
+def test_backend_config_refuses_unknown_caches_and_shards() -> None:
+    from tokenserve_b200.backend import CudaPagedBackendConfig
+
+    assert CudaPagedBackendConfig(kv_cache_dtype="fp8_e4m3").kv_cache_dtype == "fp8_e4m3"
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        CudaPagedBackendConfig(kv_cache_dtype="int8")
+    with pytest.raises(ValueError, match="kv_head_shards"):
+        CudaPagedBackendConfig(kv_cache_dtype="fp8_e4m3", kv_head_shards=2)

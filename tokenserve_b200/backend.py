@@ -54,10 +54,18 @@ class CudaPagedBackendConfig:
     #: heads [r * Hkv / N, (r + 1) * Hkv / N) and their query heads in a pool of Hkv / N heads;
     #: each layer's attention output is all-gathered (NCCL) before the O projection.
     kv_head_shards: int = 1
+    #: ``"fp8_e4m3"`` keeps K and V as 8-bit e4m3 codes with one float32 scale per (token, KV head):
+    #: about half the bytes to read in a decode step and twice the blocks in the same memory, for
+    #: a rounding of each K and V value to 4 bits. ``None``: the cache holds the compute dtype.
+    kv_cache_dtype: str | None = None
 
     def __post_init__(self) -> None:
         if self.block_size <= 0 or self.num_blocks <= 0:
             raise ValueError("block_size and num_blocks must be positive")
+        if self.kv_cache_dtype not in (None, "fp8_e4m3"):
+            raise ValueError(f"kv_cache_dtype must be None or 'fp8_e4m3', got {self.kv_cache_dtype!r}")
+        if self.kv_cache_dtype is not None and self.kv_head_shards > 1:
+            raise ValueError("kv_cache_dtype is not available with kv_head_shards")
 
 
 def sample_token(logits: torch.Tensor, item: BatchItem) -> int:
@@ -113,6 +121,7 @@ class CudaPagedBackend(Backend):
                 dtype=config.dtype,
                 shard=shard,
                 group=group,
+                kv_fp8=config.kv_cache_dtype == "fp8_e4m3",
             )
             self._tags = (
                 torch.full((config.num_blocks * config.block_size,), -1, dtype=torch.int32,
@@ -122,16 +131,23 @@ class CudaPagedBackend(Backend):
             self.runner.tag_pool = self._tags
         # Decode steps replay as CUDA graphs on one GPU; a sharded step (its per-layer NCCL
         # all-gather) runs eagerly.
-        self._graphs = (DecodeGraphs(self.runner)
-                        if config.cuda_graphs and not config.verify_kv and shard is None else None)  # fmt: skip
+        self._graphs = DecodeGraphs(self.runner) if self._captures() else None
         r = self.runner
         #: pinned host arena [layers * 2][swap blocks][block plane] (same plane layout as the pool)
         self.swap_space = (
             torch.empty((r.num_layers * 2, config.swap_space_blocks,
                          r.num_kv_heads * r.block_size * r.head_dim), dtype=r.dtype,
                         pin_memory=True)
-            if config.swap_space_blocks > 0 else None
+            if config.swap_space_blocks > 0 and not r.kv_fp8 else None
         )  # fmt: skip
+        #: the arena of an 8-bit cache's scales, same planes
+        self.swap_scales: torch.Tensor | None = None
+        if config.swap_space_blocks > 0 and r.kv_fp8:
+            planes, blocks = r.num_layers * 2, config.swap_space_blocks
+            rows = r.num_kv_heads * r.block_size
+            self.swap_space = torch.empty((planes, blocks, rows * r.head_dim), dtype=torch.uint8,
+                                          pin_memory=True)  # fmt: skip
+            self.swap_scales = torch.empty((planes, blocks, rows), pin_memory=True)
         self._flag = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.num_steps = 0
         self.num_tokens = 0
@@ -142,6 +158,11 @@ class CudaPagedBackend(Backend):
         """The pool as ``[layers * 2, num_blocks, block plane]`` (a view, no copy)."""
         kv = self.runner.kv
         return kv.view(kv.shape[0] * 2, kv.shape[2], -1)
+
+    def _scale_planes(self) -> torch.Tensor | None:
+        """An 8-bit cache's scales in the same planes."""
+        s = self.runner.kv_scales
+        return None if s is None else s.view(s.shape[0] * 2, s.shape[2], -1)
 
     def _pairs(self, pairs: Seq[tuple[int, int]]) -> torch.Tensor:
         host = torch.tensor(list(pairs), dtype=torch.int64).reshape(-1, 2)
@@ -159,7 +180,11 @@ class CudaPagedBackend(Backend):
         if not src_dst:
             return
         with torch.cuda.device(self.device):
-            ops.copy_blocks(self._planes(), self._pairs(src_dst), self._flag)
+            pairs = self._pairs(src_dst)
+            ops.copy_blocks(self._planes(), pairs, self._flag)
+            scales = self._scale_planes()
+            if scales is not None:
+                ops.copy_blocks(scales, pairs, self._flag)
             self._finish("copy_blocks")
 
     def swap_out(self, device_to_host: Seq[tuple[int, int]]) -> None:
@@ -178,10 +203,36 @@ class CudaPagedBackend(Backend):
         if not pairs:
             return
         with torch.cuda.device(self.device):
-            planes = self._planes()
-            dst, src = (self.swap_space, planes) if out else (planes, self.swap_space)
-            ops.swap_blocks(dst, src, self._pairs(pairs), self._flag)
+            moved = self._pairs(pairs)
+            for pool, host in ((self._planes(), self.swap_space),
+                               (self._scale_planes(), self.swap_scales)):  # fmt: skip
+                if pool is not None and host is not None:
+                    dst, src = (host, pool) if out else (pool, host)
+                    ops.swap_blocks(dst, src, moved, self._flag)
             self._finish("swap_out" if out else "swap_in")
+
+    def read_kv(self, block_table: Seq[int], num_tokens: int) -> torch.Tensor:
+        """The first ``num_tokens`` cached rows of a sequence in the compute dtype, ``[layers, 2,
+        num_tokens, kv heads, head_dim]`` (K with its positions applied): a cached prefix handed to
+        another process or kept outside the pool. An 8-bit cache is read back (``code * scale``)."""
+        r, bs = self.runner, self.config.block_size
+        if num_tokens < 0 or num_tokens > len(block_table) * bs:
+            raise ValueError(f"read_kv: {num_tokens} tokens in a table of {len(block_table)} blocks")
+        if any(not 0 <= b < self.config.num_blocks for b in block_table):
+            raise ValueError("read_kv: a block id is outside the pool")
+        shape = (r.num_layers, 2, num_tokens, r.num_kv_heads, r.head_dim)
+        with torch.cuda.device(self.device):
+            out = torch.empty(shape, dtype=r.dtype, device=self.device)
+            if num_tokens == 0:
+                return out
+            table = torch.tensor(list(block_table), dtype=torch.int32, device=self.device)
+            if not r.kv_fp8:
+                rows = r.kv[:, :, table.long()].transpose(3, 4).flatten(2, 3)
+                return out.copy_(rows[:, :, :num_tokens])
+            loc = torch.tensor([0, num_tokens], dtype=torch.int32, device=self.device)
+            for layer in range(r.num_layers):
+                ops.read_cache_fp8(out[layer, 0], out[layer, 1], *r.cache(layer), table[None], loc)
+            return out
 
     def resize_pool(self, num_blocks: int) -> None:
         """Re-creates the KV pool (and the shadow tags) with ``num_blocks`` blocks. Only legal
@@ -195,8 +246,16 @@ class CudaPagedBackend(Backend):
                                         dtype=torch.int32, device=self.device)  # fmt: skip
                 self.runner.tag_pool = self._tags
         self.config = dataclasses.replace(self.config, num_blocks=num_blocks)
-        if self.config.cuda_graphs and not self.config.verify_kv and self.shard is None:
+        if self._captures():
             self._graphs = DecodeGraphs(self.runner)
+
+    def _captures(self) -> bool:
+        """Whether decode steps run as captured graphs. A rotary module that changes its frequencies
+        with the context reads the positions on the host, which a capture does not allow."""
+        c = self.config
+        rope = (getattr(self.runner.model.config, "rope_parameters", None) or {}).get("rope_type")
+        return (c.cuda_graphs and not c.verify_kv and self.shard is None
+                and rope not in ("dynamic", "longrope"))  # fmt: skip
 
     @property
     def max_position_embeddings(self) -> int | None:
@@ -213,7 +272,7 @@ class CudaPagedBackend(Backend):
             self._graphs.mirror.release(seq_id)
 
     async def close(self) -> None:
-        self.runner.kv = torch.empty(0, device=self.device)
+        self.runner.kv, self.runner.kv_scales = torch.empty(0, device=self.device), None
         self._tags = self.runner.tag_pool = None
         torch.cuda.empty_cache()
 

@@ -98,6 +98,7 @@ class PagedLlamaRunner:
         dtype: torch.dtype | None = None,
         shard: HeadShard | None = None,
         group=None,  # type: ignore[no-untyped-def]
+        kv_fp8: bool = False,
     ) -> None:
         self.device = torch.device(device)
         self.model = model.to(self.device).eval()
@@ -116,12 +117,10 @@ class PagedLlamaRunner:
         self.scale = self.head_dim**-0.5
         self.block_size = block_size
         self.num_blocks = num_blocks
+        #: 8-bit cache: e4m3 codes in ``kv`` and one scale per row in ``kv_scales``
+        self.kv_fp8 = kv_fp8
         # [layer][K|V][block][kv head][slot in block][head_dim]
-        self.kv = torch.zeros(
-            (self.num_layers, 2, num_blocks, self.num_kv_heads, block_size, self.head_dim),
-            dtype=self.dtype,
-            device=self.device,
-        )
+        self.kv, self.kv_scales = self._new_pool(num_blocks)
         self.staging = Staging(self.device)
         self._ws = torch.empty(0, dtype=torch.uint8, device=self.device)
         self.base = self.model.model
@@ -135,31 +134,56 @@ class PagedLlamaRunner:
 
     @property
     def block_bytes(self) -> int:
-        """Device bytes one KV block takes over all layers, K and V."""
-        return 2 * self.num_layers * self.num_kv_heads * self.block_size * self.head_dim * (
-            torch.finfo(self.dtype).bits // 8)  # fmt: skip
+        """Device bytes one KV block takes over all layers, K and V (and their scales)."""
+        row = (self.head_dim + 4 if self.kv_fp8
+               else self.head_dim * (torch.finfo(self.dtype).bits // 8))  # fmt: skip
+        return 2 * self.num_layers * self.num_kv_heads * self.block_size * row
+
+    @property
+    def pool_bytes(self) -> int:
+        """Device bytes of the whole KV pool."""
+        return sum(t.numel() * t.element_size() for t in (self.kv, self.kv_scales) if t is not None)
+
+    def _new_pool(self, num_blocks: int) -> tuple[torch.Tensor, torch.Tensor | None]:
+        shape = (self.num_layers, 2, num_blocks, self.num_kv_heads, self.block_size, self.head_dim)
+        if not self.kv_fp8:
+            return torch.zeros(shape, dtype=self.dtype, device=self.device), None
+        codes = torch.zeros(shape, dtype=torch.uint8, device=self.device)
+        return codes.view(torch.float8_e4m3fn), torch.zeros(shape[:5], device=self.device)
 
     def resize_pool(self, num_blocks: int) -> None:
         """Replaces the KV pool by a zeroed one of ``num_blocks`` blocks (the old one is freed
         first, so peak memory is the larger of the two)."""
         if num_blocks <= 0:
             raise ValueError("num_blocks must be positive")
-        shape = (self.num_layers, 2, num_blocks, self.num_kv_heads, self.block_size,
-                 self.head_dim)  # fmt: skip
-        self.kv = torch.empty(0, dtype=self.dtype, device=self.device)
+        self.kv, self.kv_scales = torch.empty(0, dtype=self.dtype, device=self.device), None
         torch.cuda.empty_cache()
-        self.kv = torch.zeros(shape, dtype=self.dtype, device=self.device)
+        self.kv, self.kv_scales = self._new_pool(num_blocks)
         self.num_blocks = num_blocks
+
+    def cache(self, layer: int) -> tuple[torch.Tensor, ...]:
+        """The layer's key and value pools, and their scales if the cache is 8-bit."""
+        kv = (self.kv[layer, 0], self.kv[layer, 1])
+        if self.kv_scales is None:
+            return kv
+        return (*kv, self.kv_scales[layer, 0], self.kv_scales[layer, 1])
 
     def _fuse_weights(self) -> bool:
         """Concatenates Q/K/V and gate/up weights so each is one GEMM; the modules' parameters
         become views of the fused tensors (no extra memory). Returns False (module path) for
-        models this fused path does not cover: biases, non-default RoPE, non-SiLU MLPs."""
+        models this fused path does not cover: biases, non-SiLU MLPs, non-default RoPE. With an
+        8-bit cache RoPE with any fixed frequencies is covered (scaled for long contexts or not);
+        types that change them with the context are not."""
         cfg = self.model.config
         rope_type = (getattr(cfg, "rope_parameters", None) or {}).get("rope_type", "default")
         if (getattr(cfg, "attention_bias", False) or getattr(cfg, "mlp_bias", False)
-                or rope_type != "default" or getattr(cfg, "hidden_act", "silu") != "silu"
-                or getattr(self.rotary, "attention_scaling", 1.0) != 1.0):  # fmt: skip
+                or getattr(cfg, "hidden_act", "silu") != "silu"):  # fmt: skip
+            return False
+        if self.kv_fp8:
+            if (rope_type not in ("default", "linear", "llama3", "yarn")
+                    or 2 * self.rotary.inv_freq.numel() != self.head_dim):  # fmt: skip
+                return False
+        elif rope_type != "default" or getattr(self.rotary, "attention_scaling", 1.0) != 1.0:
             return False
         self._w_qkv, self._w_gu = [], []
         d, sh = self.head_dim, self.shard
@@ -183,6 +207,7 @@ class PagedLlamaRunner:
                 mlp.up_proj.weight.data = g[i:]
                 self._w_gu.append(g)
         self._inv_freq = self.rotary.inv_freq.float().contiguous()
+        self._rope_scaling = float(getattr(self.rotary, "attention_scaling", 1.0))
         self._eps = [(l.input_layernorm.variance_epsilon, l.post_attention_layernorm.variance_epsilon)
                      for l in self.base.layers]  # fmt: skip
         return True
@@ -214,10 +239,10 @@ class PagedLlamaRunner:
 
     def attention(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                   st: DeviceStep) -> torch.Tensor:  # fmt: skip
-        kp, vp = self.kv[layer, 0], self.kv[layer, 1]
         tagged = layer == 0 and self.tag_pool is not None
-        ops.reshape_and_cache(
-            k, v, kp, vp, st.slot_mapping,
+        write = ops.reshape_and_cache_fp8 if self.kv_fp8 else ops.reshape_and_cache
+        write(
+            k, v, *self.cache(layer), st.slot_mapping,
             token_tags=st.tags if tagged else None, tag_pool=self.tag_pool if tagged else None,
         )  # fmt: skip
         return self.attend(layer, q, st)
@@ -227,16 +252,18 @@ class PagedLlamaRunner:
 
         Every layer of a step has the same block tables and context lengths, so layer 0's decode
         call plans the work and the later layers reuse that plan from the workspace."""
-        kp, vp = self.kv[layer, 0], self.kv[layer, 1]
+        cache = self.cache(layer)
+        decode = ops.paged_decode_fp8 if self.kv_fp8 else ops.paged_decode
+        prefill = ops.paged_prefill_fp8 if self.kv_fp8 else ops.paged_prefill
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         nd = st.num_decode
         if nd:
             ws = self.workspace(nd, st.decode_tables.shape[1])
-            ops.paged_decode(out[:nd], q[:nd], kp, vp, st.decode_tables, st.decode_ctx,
-                             self.scale, ws, reuse_plan=layer > 0)  # fmt: skip
+            decode(out[:nd], q[:nd], *cache, st.decode_tables, st.decode_ctx, self.scale, ws,
+                   reuse_plan=layer > 0)  # fmt: skip
         if st.num_prefill:
-            ops.paged_prefill(out[nd:], q[nd:], kp, vp, st.prefill_tables, st.prefill_qsl,
-                              st.prefill_ctx, st.max_query_len, self.scale)  # fmt: skip
+            prefill(out[nd:], q[nd:], *cache, st.prefill_tables, st.prefill_qsl, st.prefill_ctx,
+                    st.max_query_len, self.scale)  # fmt: skip
         return out
 
     def gather_heads(self, o: torch.Tensor) -> torch.Tensor:
@@ -267,8 +294,14 @@ class PagedLlamaRunner:
             at, mlp = layer.self_attn, layer.mlp
             qkv = f.linear(x, self._w_qkv[li])
             q = torch.empty((t, hq, d), dtype=res.dtype, device=res.device)
-            ops.rope_and_cache(qkv, q, self.kv[li, 0], self.kv[li, 1], st.slot_mapping,
-                               st.positions, self._inv_freq, hq, hkv)  # fmt: skip
+            if self.kv_fp8:
+                kp, vp, ks, vs = self.cache(li)
+                ops.rotary_and_cache(qkv, q, kp, vp, st.slot_mapping, st.positions,
+                                     self._inv_freq, hq, hkv, key_scales=ks, value_scales=vs,
+                                     attention_scaling=self._rope_scaling)  # fmt: skip
+            else:
+                ops.rope_and_cache(qkv, q, self.kv[li, 0], self.kv[li, 1], st.slot_mapping,
+                                   st.positions, self._inv_freq, hq, hkv)  # fmt: skip
             o = self.gather_heads(self.attend(li, q, st))
             a = at.o_proj(o.view(t, self.total_q_heads * d))
             x2 = torch.empty_like(res)

@@ -93,7 +93,7 @@ def fit_pool_to_memory(backend: Any, max_num_batched_tokens: int,
                          seed=0)  # fmt: skip
         backend._execute([item])
         torch.cuda.synchronize()
-        temp_pool = runner.kv.numel() * runner.kv.element_size()
+        temp_pool = runner.pool_bytes
         non_pool_peak = torch.cuda.max_memory_allocated() - temp_pool
         free, total = torch.cuda.mem_get_info()
         non_torch = total - free - torch.cuda.memory_reserved()
@@ -110,10 +110,11 @@ def fit_pool_to_memory(backend: Any, max_num_batched_tokens: int,
 def load_cuda(model_name: str, *, dtype: str = "bfloat16", block_size: int = 16,
               num_blocks: int | None = None, max_num_batched_tokens: int = 2048,
               gpu_memory_utilization: float = DEFAULT_GPU_MEMORY_UTILIZATION,
-              device: str = "cuda") -> tuple[Any, Any]:  # fmt: skip
+              device: str = "cuda", kv_cache_dtype: str | None = None) -> tuple[Any, Any]:  # fmt: skip
     """``load_hf`` for the CUDA backend: ``(CudaPagedBackend, HFTokenizer)``.
 
     ``num_blocks=None`` sizes the pool with :func:`fit_pool_to_memory`; a number keeps it.
+    ``kv_cache_dtype="fp8_e4m3"`` keeps the KV cache in 8 bits.
     """
     import torch
     from transformers import AutoModelForCausalLM, AutoTokenizer
@@ -123,7 +124,8 @@ def load_cuda(model_name: str, *, dtype: str = "bfloat16", block_size: int = 16,
     tok = AutoTokenizer.from_pretrained(model_name)
     model = AutoModelForCausalLM.from_pretrained(model_name, dtype=getattr(torch, dtype))
     backend = CudaPagedBackend(model, CudaPagedBackendConfig(
-        block_size=block_size, num_blocks=num_blocks or 1, device=device))  # fmt: skip
+        block_size=block_size, num_blocks=num_blocks or 1, device=device,
+        kv_cache_dtype=kv_cache_dtype))  # fmt: skip
     if num_blocks is None:
         fit_pool_to_memory(backend, max_num_batched_tokens, gpu_memory_utilization)
     try:
@@ -137,7 +139,8 @@ def build_engine(settings: Any) -> Any:
     """tokenserve's ``server.build_engine`` (server.py:42-75) plus ``backend == "cuda"``.
 
     The cuda branch reads ``settings.hf_model`` / ``settings.hf_dtype`` (the model flags the
-    CLI already has) and, when present, ``settings.gpu_memory_utilization``. The engine config's
+    CLI already has) and, when present, ``settings.gpu_memory_utilization`` and
+    ``settings.kv_cache_dtype``. The engine config's
     ``num_blocks`` becomes the sized pool's, and ``max_model_len`` is capped at the model's
     position limit as in the hf branch.
     """
@@ -151,11 +154,14 @@ def build_engine(settings: Any) -> Any:
     if not settings.hf_model:
         raise SystemExit("--hf-model is required with --backend cuda")
     cfg = settings.engine
+    kv_cache_dtype = getattr(settings, "kv_cache_dtype", None)
+    cache = {} if kv_cache_dtype is None else {"kv_cache_dtype": kv_cache_dtype}
     backend, tokenizer = load_cuda(
         settings.hf_model, dtype=settings.hf_dtype, block_size=cfg.block_size,
         max_num_batched_tokens=cfg.scheduler.max_num_batched_tokens,
         gpu_memory_utilization=getattr(settings, "gpu_memory_utilization",
                                        DEFAULT_GPU_MEMORY_UTILIZATION),
+        **cache,
     )  # fmt: skip
     cfg = dataclasses.replace(cfg, num_blocks=backend.config.num_blocks)
     limit = backend.max_position_embeddings
