@@ -110,7 +110,7 @@ constexpr int kFp8MinPartBlocks = TS_FP8_MIN_PART;
 #define TS_FP8_WARPS 12
 #endif
 #ifndef TS_FP8_STAGES
-#define TS_FP8_STAGES 48  // stages of a CTA at head_dim 128, over its warps
+#define TS_FP8_STAGES 24  // stages of a CTA at head_dim 128, over its warps
 #endif
 constexpr int fp8_warps(int nt) { return nt == 1 ? TS_FP8_WARPS : 8; }
 // Partials of a (sequence, head) merged by one warp before the merge of all, over an 8-bit cache.
@@ -511,18 +511,21 @@ struct Geometry {
   static constexpr int kWarps = FP8 ? fp8_warps(NT) : ::kWarps;
   static constexpr int kHalves = D / 64;              // 64-column TMA boxes per row (16-bit pool)
   static constexpr int kTileBytes = kBlock * D * (FP8 ? 1 : 2);  // one block's K (or V), one head
-  static constexpr int kStageBytes = 2 * kTileBytes;  // K tile then V tile
+  // Blocks of a stage: two 8-bit ones share the work that every stage takes.
+  static constexpr int kStageBlocks = FP8 ? 2 : 1;
+  static constexpr int kStageBytes = kStageBlocks * 2 * kTileBytes;  // per block K tile, V tile
   static constexpr int kStages = FP8 ? TS_FP8_STAGES * (D == 128 ? 1 : 2) / kWarps
                                      : (D == 128 ? TS_DECODE_STAGES_D128 : 6);
   static constexpr bool kOneBox = TS_DECODE_ONE_BOX && D == 128 && !FP8;
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kScaleBytes = FP8 ? 2 * kBlock * 4 : 0;  // a block's K then V scales
+  static constexpr int kStageScales = kStageBlocks * kScaleBytes;
   // ring, then one mbarrier (8 B) and one item descriptor (32 B) per stage and the stages'
   // scales, + alignment slack
   static constexpr int kBarBytes = (kWarps * kStages * 8 + 15) / 16 * 16;
   static constexpr int kMetaBytes = kWarps * kStages * 32;
   static constexpr int kSmemBytes = kWarps * kRingBytes + kBarBytes + kMetaBytes +
-                                    kWarps * kStages * kScaleBytes + 1024;
+                                    kWarps * kStages * kStageScales + 1024;
 };
 
 // Byte offset of 16-byte chunk `cg` (dims 16cg..16cg+15) of token `t` inside an 8-bit tile: one
@@ -622,9 +625,9 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
   // slot of the partition}.
   int4* meta =
       reinterpret_cast<int4*>(smem + kWarps * G::kRingBytes + G::kBarBytes) + warp * S * 2;
-  // 8-bit cache: per stage, the block's 16 K scales then its 16 V scales.
+  // 8-bit cache: per stage and block, 16 K scales then 16 V scales.
   float* scales = reinterpret_cast<float*>(smem + kWarps * G::kRingBytes + G::kBarBytes +
-                                           G::kMetaBytes) + warp * S * 2 * kBlock;
+                                           G::kMetaBytes) + warp * S * (G::kStageScales / 4);
 
   if (lane == 0) {
     for (int s = 0; s < S; ++s) ts::mbar_init(&bars[s], 1);
@@ -709,7 +712,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
   };
 
   auto produce = [&](int s) {
-    if (!p_done && p_blk == p_nblk) {
+    if (!p_done && p_blk >= p_nblk) {
       while (f_state >= 0 && f_state < 3) fetch_step();  // first item, or a short one
       if (f_state < 0) {
         p_done = true;
@@ -730,6 +733,46 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       }
       return;
     }
+    if constexpr (FP8) {
+      // The item's next two blocks (the second absent at an odd end). Bits 30 and 29 of the
+      // descriptor's block say that the first, the second is not there.
+      bool valid[2];
+      int row[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int tab = TABW == 1 || p_blk + u < 32 ? p_table[0] : p_table[TABW - 1];
+        const int phys = __shfl_sync(0xffffffffu, tab, (p_blk + u) & 31);
+        const bool present = p_blk + u < p_nblk;
+        valid[u] = present && phys >= 0 && int64_t(phys) < a.num_blocks;
+        if (present && !valid[u] && lane == 0) atomicExch(a.header + 1, 2);  // outside the pool
+        row[u] = (phys * a.num_kv_heads + p_it.h) * kBlock;
+      }
+      if (lane == 0) {
+        meta[2 * s] = make_int4(p_item, p_blk | (valid[0] ? 0 : 1 << 30) | (valid[1] ? 0 : 1 << 29),
+                                p_it.b, p_it.blk0);
+        meta[2 * s + 1] = make_int4(p_it.slot0, p_it.nparts | (p_it.h << 16), p_it.ctx,
+                                    p_it.part_global);  // nparts < 2^16, h < 2^15
+        const int n = int(valid[0]) + int(valid[1]);
+        if (n == 0) {
+          ts::mbar_arrive(&bars[s]);
+        } else {
+          ts::mbar_arrive_expect_tx(&bars[s], n * (2 * G::kTileBytes + G::kScaleBytes));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (!valid[u]) continue;
+            uint8_t* st = ring + s * G::kStageBytes + u * 2 * G::kTileBytes;
+            float* sc = scales + (s * 2 + u) * 2 * kBlock;
+            ts::tma_load_2d(st, &kmap, &bars[s], 0, row[u]);
+            ts::tma_load_2d(st + G::kTileBytes, &vmap, &bars[s], 0, row[u]);
+            ts::bulk_load(sc, a.k_scales + row[u], &bars[s], kBlock * 4);
+            ts::bulk_load(sc + kBlock, a.v_scales + row[u], &bars[s], kBlock * 4);
+          }
+        }
+      }
+      p_blk += 2;
+      if (f_state >= 0 && f_state < 3 && p_nblk - p_blk <= 2 * kPrefetchBlocks) fetch_step();
+      return;
+    }
     const int tab = TABW == 1 || p_blk < 32 ? p_table[0] : p_table[TABW - 1];
     const int phys = __shfl_sync(0xffffffffu, tab, p_blk & 31);
     const bool valid = phys >= 0 && int64_t(phys) < a.num_blocks;
@@ -738,15 +781,10 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       meta[2 * s + 1] = make_int4(p_it.slot0, p_it.nparts | (p_it.h << 16), p_it.ctx,
                                   p_it.part_global);  // nparts < 2^16, h < 2^15
       if (valid) {
-        ts::mbar_arrive_expect_tx(&bars[s], G::kStageBytes + G::kScaleBytes);
+        ts::mbar_arrive_expect_tx(&bars[s], G::kStageBytes);
         const int row = (phys * a.num_kv_heads + p_it.h) * kBlock;
         uint8_t* st = ring + s * G::kStageBytes;
-        if constexpr (FP8) {
-          ts::tma_load_2d(st, &kmap, &bars[s], 0, row);
-          ts::tma_load_2d(st + G::kTileBytes, &vmap, &bars[s], 0, row);
-          ts::bulk_load(scales + s * 2 * kBlock, a.k_scales + row, &bars[s], kBlock * 4);
-          ts::bulk_load(scales + s * 2 * kBlock + kBlock, a.v_scales + row, &bars[s], kBlock * 4);
-        } else if constexpr (G::kOneBox) {
+        if constexpr (G::kOneBox) {
           ts::tma_load_2d(st, &kmap, &bars[s], 0, 2 * row);
           ts::tma_load_2d(st + G::kTileBytes, &vmap, &bars[s], 0, 2 * row);
         } else {
@@ -1093,7 +1131,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
     if (lane == 0) a.arrive[it.b * a.num_kv_heads + it.h] = 0;
   };
 
-  // One block of an 8-bit cache: scores, online softmax and PV product. ldmatrix offsets inside a K
+  // The blocks of a stage of an 8-bit cache: scores, online softmax and PV product. ldmatrix offsets inside a K
   // or V tile: token row, chunks 2i and 2i + 1 (the swizzle's XOR of an even number).
   uint32_t chunk_off[D / 32];
   {
@@ -1101,68 +1139,85 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) chunk_off[i] = tile_off_fp8<D>(row, 2 * i + (lane >> 4));
   }
-  auto block_fp8 = [&](uint8_t* tile, float* sc, int nvalid) {
+  // Two blocks in a stage, n0 and n1 tokens of which are the sequence's (at most 0: none; 16 and
+  // more: all).
+  auto blocks_fp8 = [&](uint8_t* tile, float* sc, int n0, int n1) {
     using MmaH = ts::MmaOp<__half>;
-    const bool whole = nvalid >= kBlock;
+    constexpr int B = 2, kBlockBytes = 2 * G::kTileBytes;
+    const bool whole = n0 >= kBlock && n1 >= kBlock;
     if (!whole) {
       // Slots past the context may hold anything: zero rows, scales of 1, scores masked below.
-      for (int i = lane; i < (kBlock - nvalid) * (D / 16); i += 32) {
-        uint4* row = reinterpret_cast<uint4*>(tile + nvalid * D) + i;  // whole rows: swizzled or not
-        *row = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(row) + G::kTileBytes) =
-            make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const int n = max(0, u ? n1 : n0);
+        if (n >= kBlock) continue;
+        uint8_t* base = tile + u * kBlockBytes + n * D;  // whole rows: swizzled or not
+        for (int i = lane; i < (kBlock - n) * (D / 16); i += 32) {
+          reinterpret_cast<uint4*>(base)[i] = make_uint4(0, 0, 0, 0);
+          reinterpret_cast<uint4*>(base + G::kTileBytes)[i] = make_uint4(0, 0, 0, 0);
+        }
+        if (lane >= n && lane < kBlock)
+          sc[u * 2 * kBlock + lane] = sc[u * 2 * kBlock + kBlock + lane] = 1.f;
       }
-      if (lane >= nvalid && lane < kBlock) sc[lane] = sc[kBlock + lane] = 1.f;
       __syncwarp();
     }
     const uint32_t kb = ts::smem_u32(tile);
-    const float k0 = sc[g], k1 = sc[g + 8];
-    const float lv0 = __log2f(sc[kBlock + g]), lv1 = __log2f(sc[kBlock + g + 8]);
-    float sacc[NT][4];
+    float sacc[NT][4 * B];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sacc[nt][j] = 0.f;
+      for (int j = 0; j < 4 * B; ++j) sacc[nt][j] = 0.f;
 #pragma unroll
-    for (int kp = 0; kp < KSTEPS / 2; ++kp) {
-      uint32_t r[4];  // tokens g and g + 8 of 16 dims, then of the next 16
-      ts::ldmatrix_x4(r, kb + chunk_off[kp]);
+    for (int u = 0; u < B; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t af[4];
-        fp8_expand(r[2 * u], af[0], af[2]);
-        fp8_expand(r[2 * u + 1], af[1], af[3]);
+      for (int kp = 0; kp < KSTEPS / 2; ++kp) {
+        uint32_t r[4];  // tokens g and g + 8 of 16 dims, then of the next 16
+        ts::ldmatrix_x4(r, kb + u * kBlockBytes + chunk_off[kp]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          MmaH::run(sacc[nt], af, qf[nt][2 * kp + u][0], qf[nt][2 * kp + u][1]);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t af[4];
+          fp8_expand(r[2 * h], af[0], af[2]);
+          fp8_expand(r[2 * h + 1], af[1], af[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            MmaH::run(*reinterpret_cast<float(*)[4]>(&sacc[nt][4 * u]), af, qf[nt][2 * kp + h][0],
+                      qf[nt][2 * kp + h][1]);
+        }
       }
+    // Token of value j of a head pair: 16 (j / 4) + g + 8 (j / 2 % 2); its scales.
+    float ks[2 * B], lv[2 * B];
+#pragma unroll
+    for (int i = 0; i < 2 * B; ++i) {
+      ks[i] = sc[i / 2 * 2 * kBlock + g + 8 * (i % 2)];
+      lv[i] = __log2f(sc[i / 2 * 2 * kBlock + kBlock + g + 8 * (i % 2)]);
     }
-    uint32_t pb[NT][2];
+    auto in_context = [&](int i) { return g + 8 * (i % 2) < (i / 2 ? n1 : n0); };
+    uint32_t pb[NT][2 * B];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       // e: log2 of the sum's terms, e + lv: of the weights, both relative to the maximum kept.
-      float f[4] = {k0 * qs[nt][0], k0 * qs[nt][1], k1 * qs[nt][0], k1 * qs[nt][1]};
-      float e[4], w[4];
+      float e[4 * B], w[4 * B];
       auto relative = [&]() {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          e[j] = fmaf(sacc[nt][j], f[j], -m_run[nt][j & 1]);
-          if (!whole && (j < 2 ? g : g + 8) >= nvalid) e[j] = -INFINITY;
-          w[j] = e[j] + (j < 2 ? lv0 : lv1);
+        for (int j = 0; j < 4 * B; ++j) {
+          e[j] = fmaf(sacc[nt][j], ks[j / 2] * qs[nt][j & 1], -m_run[nt][j & 1]);
+          if (!whole && !in_context(j / 2)) e[j] = -INFINITY;
+          w[j] = e[j] + lv[j / 2];
         }
       };
       relative();
-      // An item's first block always: its maxima are still -inf.
-      if (__any_sync(0xffffffffu, fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > kFp8MaxSlack ||
-                                      m_run[nt][0] == -INFINITY)) {
-        // A scale of 0 counts as 2^-126 here, so that the maximum is finite.
-        float bm[2];
+      float top = w[0];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float s0 = sacc[nt][j] * f[j], s1 = sacc[nt][j + 2] * f[j + 2];
-          const float t0 = whole || g < nvalid ? fmaxf(s0 + lv0, s0 - 126.f) : -INFINITY;
-          const float t1 = whole || g + 8 < nvalid ? fmaxf(s1 + lv1, s1 - 126.f) : -INFINITY;
-          bm[j] = fmaxf(t0, t1);
+      for (int j = 1; j < 4 * B; ++j) top = fmaxf(top, w[j]);
+      // An item's first blocks always: its maxima are still -inf.
+      if (__any_sync(0xffffffffu, top > kFp8MaxSlack || m_run[nt][0] == -INFINITY)) {
+        // A scale of 0 counts as 2^-126 here, so that the maximum is finite.
+        float bm[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 4 * B; ++j) {
+          const float s = sacc[nt][j] * (ks[j / 2] * qs[nt][j & 1]);
+          if (whole || in_context(j / 2))
+            bm[j & 1] = fmaxf(bm[j & 1], fmaxf(s + lv[j / 2], s - 126.f));
         }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
@@ -1184,25 +1239,29 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
         m_run[nt][1] = mn1;
         relative();
       }
-      l_run[nt][0] += ex2(e[0]) + ex2(e[2]);
-      l_run[nt][1] += ex2(e[1]) + ex2(e[3]);
-      pb[nt][0] = ts::movmatrix_trans(MmaH::pack(ex2(w[0]), ex2(w[1])));
-      pb[nt][1] = ts::movmatrix_trans(MmaH::pack(ex2(w[2]), ex2(w[3])));
-    }
 #pragma unroll
-    for (int mp = 0; mp < MTILES / 2; ++mp) {
-      uint32_t r[4];  // dims 2g, 2g + 1 of tokens 2t, 2t + 1 (+ 8), then of the next 16 dims
-      ts::ldmatrix_x4_trans(r, kb + G::kTileBytes + chunk_off[mp]);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t af[4];
-        fp8_expand_even_odd(r[2 * u], af[0], af[1]);
-        fp8_expand_even_odd(r[2 * u + 1], af[2], af[3]);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          MmaH::run(oacc[nt][2 * mp + u], af, pb[nt][0], pb[nt][1]);
+      for (int i = 0; i < 2 * B; ++i) {
+        l_run[nt][0] += ex2(e[2 * i]);
+        l_run[nt][1] += ex2(e[2 * i + 1]);
+        pb[nt][i] = ts::movmatrix_trans(MmaH::pack(ex2(w[2 * i]), ex2(w[2 * i + 1])));
       }
     }
+#pragma unroll
+    for (int u = 0; u < B; ++u)
+#pragma unroll
+      for (int mp = 0; mp < MTILES / 2; ++mp) {
+        uint32_t r[4];  // dims 2g, 2g + 1 of tokens 2t, 2t + 1 (+ 8), then of the next 16 dims
+        ts::ldmatrix_x4_trans(r, kb + u * kBlockBytes + G::kTileBytes + chunk_off[mp]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t af[4];
+          fp8_expand_even_odd(r[2 * h], af[0], af[1]);
+          fp8_expand_even_odd(r[2 * h + 1], af[2], af[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            MmaH::run(oacc[nt][2 * mp + h], af, pb[nt][2 * u], pb[nt][2 * u + 1]);
+        }
+      }
   };
 
   uint32_t k = 0;
@@ -1221,15 +1280,16 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       if (cur_item >= 0) finish_item();
       start_item(md, meta[2 * s + 1]);
     }
-    if ((md.y & 0x40000000) == 0) {
+    if constexpr (FP8) {
+      const int left = it.ctx - (it.blk0 + (md.y & 0xffff)) * kBlock;  // of the context, from here
+      const int n0 = md.y >> 30 & 1 ? 0 : left, n1 = md.y >> 29 & 1 ? 0 : left - kBlock;
+      if (n0 > 0 || n1 > 0)
+        blocks_fp8(ring + s * G::kStageBytes, scales + s * (G::kStageScales / 4), n0, n1);
+    } else if ((md.y & 0x40000000) == 0) {
       const uint32_t kb = ts::smem_u32(ring + s * G::kStageBytes);
       const uint32_t vb = kb + G::kTileBytes;
       const int tok0 = (it.blk0 + md.y) * kBlock;
       const int nvalid = it.ctx - tok0;
-      if constexpr (FP8) {
-        block_fp8(ring + s * G::kStageBytes, scales + s * 2 * kBlock, nvalid);
-      } else {
-
       // S^T[token][head] = K Q^T
       float sacc[NT][4];
 #pragma unroll
@@ -1297,7 +1357,6 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
             Mma::run(oacc[nt][mt], af, pb[nt][2], pb[nt][3]);
           }
         }
-      }
       }
     }
     __syncwarp();
