@@ -95,7 +95,7 @@ struct Args {
 // A span as the scout leaves it: references of K and V, the columns to mask (page outside the
 // pool) or to spoil (V row NaN), if any; the blocks (negative: none); each row's factor for K and
 // for V, fp16 high and low part, or kDropped.
-struct TileInfo {
+struct alignas(16) TileInfo {
   float ref_k, ref_v;
   uint32_t any, dropped;  // dropped: bit 0, 1: K, V has rows of factor kDropped
   uint32_t skip[4], spoil[4];
@@ -111,6 +111,15 @@ struct Shared {
   uint32_t tmem;
   int abort;
 };
+
+// ref_k, ref_v, any and dropped of a description in one load.
+__device__ __forceinline__ float4 load_refs(const volatile TileInfo* info) {
+  float4 v;
+  asm volatile("ld.volatile.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(ts::smem_u32(const_cast<const TileInfo*>(info))));
+  return v;
+}
 
 template <int D>
 struct Geo {
@@ -634,6 +643,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       ts::mbar_arrive(&sh->q_full);
     }
 
+    const int pos_max = __reduce_max_sync(0xffffffffu, pos);
+    const int pos_min = __reduce_min_sync(0xffffffffu, pos);
     float m_run = -INFINITY, l_run = 0.f, ref_v = 0.f;
     bool saw_nan = false;  // a row of K or V that holds one (not every exponential below keeps it)
     bool ok = true;
@@ -649,16 +660,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       constexpr int kGroups = kKvTile / 32;  // of 32 columns
       const volatile TileInfo* info = &sh->info[j / kTilesPerSpan % kInfos];
       const int word = j % kTilesPerSpan * kGroups;  // of the span's column masks
-      const float slj = fmaxf(sl * info->ref_k, 0x1p-126f);  // > 0, so that -inf stays -inf
+      const float4 refs = load_refs(info);
+      const float slj = fmaxf(sl * refs.x, 0x1p-126f);  // > 0, so that -inf stays -inf
       // O is in units of V's reference: it shrinks when that grows.
       const float ref_old = ref_v;
-      ref_v = info->ref_v;
-      const bool odd_columns = info->any != 0;
+      ref_v = refs.y;
+      const bool odd_columns = __float_as_uint(refs.z) != 0;
       float corr_o = ref_v != ref_old && j > 0 ? ref_old / ref_v : 1.f;
       const int limit = pos - j * kKvTile;  // columns c <= limit are visible
       // Column groups of 32 that some row of the warp sees, and those every row sees whole.
-      const int n_some = min(kGroups, max(0, __reduce_max_sync(0xffffffffu, limit) + 32) / 32);
-      const int n_whole = odd_columns ? 0 : max(0, __reduce_min_sync(0xffffffffu, limit) + 1) / 32;
+      const int n_some = min(kGroups, max(0, pos_max - j * kKvTile + 32) / 32);
+      const int n_whole = odd_columns ? 0 : max(0, pos_min - j * kKvTile + 1) / 32;
       auto mask = [&](uint32_t (&r)[32], int c) {
         const int lim = limit - 32 * c;
         const uint32_t seen = lim >= 31 ? ~0u : lim < 0 ? 0u : (2u << lim) - 1;
