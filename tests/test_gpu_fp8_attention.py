@@ -141,6 +141,36 @@ def test_decode_plan_reuse_strided_queries_and_shared_workspace(cuda_device) -> 
         check_decode(decode(q, cache, tab, ctx, ws=ws, reuse=reuse), q, cache, tab, lens)
 
 
+def test_decode_refuses_a_small_or_misaligned_workspace(cuda_device) -> None:  # type: ignore[no-untyped-def]
+    gen = torch.Generator(device=cuda_device).manual_seed(15)
+    nb, tab = tables_for([40], 16, gen)
+    cache = make_cache(gen, nb, 2, 16, 128)
+    q = torch.randn(1, 8, 128, generator=gen, device=cuda_device).to(BF)
+    ctx = torch.tensor([40], dtype=torch.int32, device=cuda_device)
+    n = ops.decode_workspace_size(1, 8, 2, 128, tab.shape[1], 16, BF)
+    ws = torch.empty(n + 512, dtype=torch.uint8, device=cuda_device)
+    out = torch.full_like(q, 7.0)
+    for bad, text in ((ws[:256], "workspace of 256 bytes"), (ws[1 : n + 1], "256-byte aligned")):
+        with pytest.raises(ops.KernelError, match=text):
+            decode(q, cache, tab, ctx, ws=bad, out=out)
+    with pytest.raises(ops.KernelError, match="workspace"):
+        ops.paged_decode_fp8(out, q, *cache, tab, ctx, 0.1, None)
+    assert (out == 7).all()
+
+
+def test_a_plan_for_another_batch_is_refused_on_the_device(cuda_device) -> None:  # type: ignore[no-untyped-def]
+    gen = torch.Generator(device=cuda_device).manual_seed(16)
+    nb, tab = tables_for([40, 60], 16, gen)
+    cache = make_cache(gen, nb, 2, 16, 128)
+    q = torch.randn(2, 8, 128, generator=gen, device=cuda_device).to(BF)
+    ctx = torch.tensor([40, 60], dtype=torch.int32, device=cuda_device)
+    n = ops.decode_workspace_size(2, 8, 2, 128, tab.shape[1], 16, BF)
+    ws = torch.zeros(n, dtype=torch.uint8, device=cuda_device)
+    check_decode(decode(q, cache, tab, ctx, ws=ws), q, cache, tab, [40, 60])
+    out = decode(q[:1], cache, tab[:1], ctx[:1], ws=ws, reuse=True)
+    assert (out == 7).all() and int(ws[4:8].view(torch.int32)) == 4
+
+
 def test_a_nan_row_spoils_its_own_sequence_alone(cuda_device) -> None:  # type: ignore[no-untyped-def]
     gen = torch.Generator(device=cuda_device).manual_seed(6)
     lens = [50, 60, 70, 80]
@@ -258,6 +288,61 @@ def test_prefill_of_uneven_magnitudes(cuda_device, kind) -> None:  # type: ignor
     ctx = torch.tensor(ctxs, dtype=torch.int32, device=cuda_device)
     out = prefill(q, cache, tab, qsl, ctx, 150, scale)
     check_prefill(out, q, cache, tab, chunks, ctxs, scale)
+
+
+@pytest.mark.parametrize(("dtype", "hq", "d"), [(BF, 8, 128), (FH, 8, 64), (F32, 4, 64)])
+@pytest.mark.parametrize("which", ["key", "value"])
+def test_a_nan_row_reaches_only_the_queries_that_see_it(cuda_device, dtype, hq, d, which) -> None:  # type: ignore[no-untyped-def]
+    """One position of a chunk holds a NaN, for each place of it in the column groups."""
+    gen = torch.Generator(device=cuda_device).manual_seed(13)
+    chunk, ctx = 100, 230
+    qsl = torch.tensor([0, chunk], dtype=torch.int32, device=cuda_device)
+    cl = torch.tensor([ctx], dtype=torch.int32, device=cuda_device)
+    nb, tab = tables_for([ctx], 16, gen)
+    q = torch.randn(chunk, hq, d, generator=gen, device=cuda_device).to(dtype)
+    for at in (130, 131, 134, 159, 160, 191, 192, 200, 229):
+        kp, vp, ks, vs = make_cache(gen, nb, 2, 16, d)
+        row = torch.randn(1, 2, d, generator=gen, device=cuda_device).to(dtype)
+        bad = row.clone()
+        bad[0, :, 5] = float("nan")
+        slot = tab[0, at // 16].long()[None] * 16 + at % 16
+        ops.reshape_and_cache_fp8(*((bad, row) if which == "key" else (row, bad)), kp, vp, ks, vs,
+                                  slot)  # fmt: skip
+        out = prefill(q, (kp, vp, ks, vs), tab, qsl, cl, chunk)
+        first = at - (ctx - chunk)  # the first query that sees it
+        assert torch.isnan(out[first:]).all()
+        if first:
+            check_prefill(out[:first], q[:first], (kp, vp, ks, vs), tab, [first], [at])
+
+
+@pytest.mark.parametrize(("dtype", "hq", "d"), [(BF, 8, 128), (FH, 4, 64), (F32, 4, 64)])
+@pytest.mark.parametrize("bad", [-1, -(2**31), 2**31 - 1, 40])
+def test_pages_outside_the_pool_are_skipped(cuda_device, dtype, hq, d, bad) -> None:  # type: ignore[no-untyped-def]
+    """Attention over the other blocks alone: their tokens' positions stay where they were, which only
+    the causal mask uses (the chunk lies in a block after the skipped ones)."""
+    gen = torch.Generator(device=cuda_device).manual_seed(14)
+    ctx = 150
+    nb, tab = tables_for([ctx, ctx], 16, gen, spare=40 - 20)
+    kp, vp, ks, vs = make_cache(gen, nb, 2, 16, d)
+    cache = (kp, vp, ks, vs)
+    assert nb == 40
+    broken, kept = tab.clone(), {0: [0, 1, 2, 4, 5, 7, 8, 9], 1: [5, 6, 8, 9]}
+    for i, blocks in kept.items():
+        for j in range(10):
+            if j not in blocks:
+                broken[i, j] = bad
+    lens = [len(b) * 16 - 10 for b in kept.values()]  # the last block holds 6 tokens
+    whole = torch.zeros_like(tab)
+    for i, blocks in kept.items():
+        whole[i, : len(blocks)] = tab[i, blocks]
+    cl = torch.tensor([ctx, ctx], dtype=torch.int32, device=cuda_device)
+    q = torch.randn(2, hq, d, generator=gen, device=cuda_device).to(dtype)
+    check_decode(decode(q, cache, broken, cl), q, cache, whole, lens)
+    chunks = [4, 6]
+    qsl = torch.tensor([0, 4, 10], dtype=torch.int32, device=cuda_device)
+    q = torch.randn(10, hq, d, generator=gen, device=cuda_device).to(dtype)
+    out = prefill(q, cache, broken, qsl, cl, 6)
+    check_prefill(out, q, cache, whole, chunks, lens)
 
 
 # ------------------------------------------------------------------------------ together

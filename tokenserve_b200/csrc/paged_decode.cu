@@ -180,7 +180,9 @@ inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 int num_sms();
 
 // grid_warps: warps of the decode grid on the device the call runs on (its SMs x kWarps).
-WsLayout ws_layout(int batch, int hkv, int hd, int max_blocks, int nt, int grid_warps) {
+// fp8: with the counters of the grouped merge.
+WsLayout ws_layout(int batch, int hkv, int hd, int max_blocks, int nt, int grid_warps,
+                   bool fp8 = false) {
   WsLayout w;
   // A sequence is cut at most once per kPartBlocks blocks and once per group boundary; each cut
   // gives one partition per head (groups x heads <= grid warps).
@@ -193,7 +195,7 @@ WsLayout ws_layout(int batch, int hkv, int hd, int max_blocks, int nt, int grid_
   w.group_first = w.part_info + align256(2 * sizeof(int4) * slots);
   w.arrive = w.group_first + align256(sizeof(int) * (size_t(grid_warps) + 1));
   w.group_arrive = w.arrive + align256(sizeof(int) * bh);
-  w.part_o = w.group_arrive + align256(sizeof(int) * slots);
+  w.part_o = w.group_arrive + (fp8 ? align256(sizeof(int) * slots) : 0);
   w.part_ml = w.part_o + align256(sizeof(float) * slots * hd * nt * 8);
   w.total = w.part_ml + align256(sizeof(float2) * slots * nt * 8);
   return w;
@@ -1566,7 +1568,7 @@ extern "C" size_t ts_paged_decode_workspace_size(int32_t batch, int32_t num_q_he
   const int nt = num_q_heads / num_kv_heads > 8 ? 2 : 1;
   // The larger grid of the two caches' kernels.
   return ws_layout(batch, num_kv_heads, head_dim, max_blocks_per_seq, nt,
-                   num_sms() * std::max(kWarps, fp8_warps(nt))).total;
+                   num_sms() * std::max(kWarps, fp8_warps(nt)), true).total;
 }
 
 namespace {
@@ -1611,7 +1613,7 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
   const int group = num_q_heads / num_kv_heads;
   const int nt = group > 8 ? 2 : 1;
   const int grid_warps = num_sms() * (fp8 ? fp8_warps(nt) : kWarps);
-  const WsLayout w = ws_layout(batch, num_kv_heads, head_dim, max_blocks_per_seq, nt, grid_warps);
+  const WsLayout w = ws_layout(batch, num_kv_heads, head_dim, max_blocks_per_seq, nt, grid_warps, fp8);
   if (workspace == nullptr || workspace_bytes < w.total)
     return ts::set_error(TS_ERR_WORKSPACE_TOO_SMALL,
                          "paged_decode: workspace of %zu bytes, need %zu", workspace_bytes,
@@ -1657,7 +1659,7 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
   a.part_info = reinterpret_cast<int4*>(ws + w.part_info);
   a.group_first = reinterpret_cast<int*>(ws + w.group_first);
   a.arrive = reinterpret_cast<int*>(ws + w.arrive);
-  a.group_arrive = reinterpret_cast<int*>(ws + w.group_arrive);
+  a.group_arrive = fp8 ? reinterpret_cast<int*>(ws + w.group_arrive) : nullptr;
   a.part_o = reinterpret_cast<float*>(ws + w.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
 #define TS_FAST(T)                                                             \

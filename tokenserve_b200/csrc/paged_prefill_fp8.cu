@@ -86,6 +86,7 @@ struct Args {
   const int32_t* qsl;
   const int32_t* context_lens;
   int max_blocks, num_q_heads, num_kv_heads, group;
+  int num_tokens;  // query rows: none past them is read or written
   int tq;       // query tokens per tile
   int q_tiles;  // query tiles per CTA, 1 or 2
   int64_t num_blocks;
@@ -399,7 +400,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   using Mma = ts::MmaOp<T>;
   const int pair = blockIdx.x, h = blockIdx.y, seq = blockIdx.z;
   const int q0 = __shfl_sync(0xffffffffu, a.qsl[seq], 0);
-  const int q_len = __shfl_sync(0xffffffffu, a.qsl[seq + 1], 0) - q0;
+  const int q_end = __shfl_sync(0xffffffffu, a.qsl[seq + 1], 0);
+  if (q0 < 0 || q_end > a.num_tokens) return;  // not a chunk of this call's rows
+  const int q_len = q_end - q0;
   const int tile0 = pair * a.q_tiles;
   if (tile0 * a.tq >= q_len) return;
   const int ctx = min(__shfl_sync(0xffffffffu, a.context_lens[seq], 0), a.max_blocks * kBlock);
@@ -938,6 +941,7 @@ extern "C" int ts_paged_prefill_fp8(void* out, const void* query, int64_t query_
   a.num_q_heads = num_q_heads;
   a.num_kv_heads = num_kv_heads;
   a.group = group;
+  a.num_tokens = num_query_tokens;
   a.tq = kRows / group;
   a.num_blocks = num_blocks;
   a.scale_log2 = scale * kLog2e;

@@ -463,7 +463,8 @@ def _attention_rows(what: str, out: torch.Tensor, query: torch.Tensor, kv_heads:
     stride = _rows(query, query.shape[1], head_dim, f"{what}: query")
     if out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
         raise KernelError(f"{what}: out must be contiguous, of the query's shape and dtype")
-    return query.shape[1], max(stride, query.shape[1] * head_dim) if query.shape[0] < 2 else stride
+    # A single row's stride says nothing.
+    return query.shape[1], stride if query.shape[0] > 1 else query.shape[1] * head_dim
 
 
 def reshape_and_cache_fp8(
@@ -490,7 +491,7 @@ def reshape_and_cache_fp8(
     n = key.shape[0]
     ks, vs = _rows(key, h, d, f"{what}: key"), _rows(value, h, d, f"{what}: value")
     if n == 1:  # a single row's stride says nothing
-        ks, vs = max(ks, h * d), max(vs, h * d)
+        ks = vs = h * d
     _int_array(what, "slot_mapping", slot_mapping, torch.int64, n)
     if token_tags is not None:
         _int_array(what, "token_tags", token_tags, torch.int32, n)
