@@ -66,8 +66,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // true maximum, at least 1, well inside its normal range.
 constexpr float kRescaleSlack = 14.f;
 // One of so many column pairs takes its 2^x from the FMA pipe (64 sequences of 512 new tokens: none
-// 928 us, one of 8 912, of 4 899, of 3 919, of 2 937).
-constexpr int kFmaEvery = 4;
+// 894 us, one of 16 885, of 8 876, of 4 886, of 3 896).
+constexpr int kFmaEvery = 8;
 // S_A [0,128) and S_B [128,256), two buffers each, O_A [256,384), O_B [384,512).
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRefScale = 128.f;    // fp16 values are code * scale / ref * 128 <= 57344
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   Scout scout(a, seq, h, n_kv, lane);
   if (warp == 12) scout.load(scout.look_up(0));
   if (warp == 14 && lane == 0) {
-    ts::mbar_init(&sh->q_full, 128 * kQTiles);
+    ts::mbar_init(&sh->q_full, 4 * kQTiles);  // one arrival a warp, here and below
     for (int i = 0; i < kStages; ++i) {
       ts::mbar_init(&sh->k_full[i], kUnits / 2);
       ts::mbar_init(&sh->k_empty[i], 1);
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     for (int x = 0; x < kQTiles; ++x) {
       for (int b = 0; b < 2; ++b) {
         ts::mbar_init(&sh->s_full[x][b], 1);
-        ts::mbar_init(&sh->p_full[x][b], 128);
+        ts::mbar_init(&sh->p_full[x][b], 4);
       }
       ts::mbar_init(&sh->pv_done[x], 1);
       ts::mbar_init(&sh->o_full[x], 1);
@@ -643,7 +643,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         }
       }
       ts::fence_proxy_async_smem();
-      ts::mbar_arrive(&sh->q_full);
+      __syncwarp();
+      if (lane == 0) ts::mbar_arrive(&sh->q_full);
     }
 
     const int pos_max = __reduce_max_sync(0xffffffffu, pos);
@@ -791,7 +792,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       }
       ts::tc::wait_st();
       ts::tc::fence_before_sync();
-      ts::mbar_arrive(&sh->p_full[x][j & 1]);
+      __syncwarp();
+      if (lane == 0) ts::mbar_arrive(&sh->p_full[x][j & 1]);
     }
     if (ok && n_x > 0) ok = wait_warp(&sh->o_full[x], 0, abort);
     ts::tc::fence_after_sync();
