@@ -555,8 +555,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           const int n_x = x ? n_t[1] : n_t[0];
           const uint32_t s_tmem = tmem + x * 128 + b * kKvTile;
           if (j >= 0 && j < n_x) {
-            ok = wait_warp(&sh->p_full[x][b], (j / 2) & 1, abort) &&
-                 wait_warp(&sh->v_full[sv], (j / kStages) & 1, abort);
+            // The first query tile has waited for this V already (and below for this K): a wait
+            // costs a hundred clocks even then.
+            ok = ((x == 1 && j < n_t[0]) || wait_warp(&sh->v_full[sv], (j / kStages) & 1, abort)) &&
+                 wait_warp(&sh->p_full[x][b], (j / 2) & 1, abort);
             if (!ok) break;
             ts::tc::fence_after_sync();
             const uint32_t dv = v_lo + sv * (G::kKvBytes >> 4);
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
             if (x == last_user(j) && j + kStages < n_max) ts::tc::commit_elect(&sh->v_empty[sv]);
           }
           if (i < n_x) {
-            ok = wait_warp(&sh->k_full[sk], (i / kStages) & 1, abort);
+            ok = (x == 1 && i < n_t[0]) || wait_warp(&sh->k_full[sk], (i / kStages) & 1, abort);
             if (!ok) break;
             ts::tc::fence_after_sync();
             const uint32_t dq = q_lo + x * (G::kQBytes >> 4);
