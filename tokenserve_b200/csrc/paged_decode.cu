@@ -37,6 +37,9 @@
 //     log2(vs), m is a maximum of t, w = 2^(t - m) goes to the PV product as f16 (11 bits: 2^-12 of
 //     itself, once) and the sum gets 2^(s - m) in 32 bits. m is kept until some t exceeds it by
 //     2^12, so most blocks need no maximum over their tokens and no rescaling of O.
+//   * Two blocks a stage and 12 warps a CTA: with half the bytes a block, instructions bind first (374 a
+//     block of one head). 256 sequences, median 1,024 tokens, 32/8 heads of 128: 168 us, 5.5 TB/s
+//     (0.84 of the copy rate; 512 sequences 0.92), 280 us over the 16-bit cache.
 //   * Slots past the context may hold anything: in a sequence's last block they are made zeros in
 //     shared memory and their scores masked.
 #include <cuda.h>
