@@ -106,6 +106,13 @@ constexpr int kMaxGridWarps = 8192;
 #define TS_FP8_MIN_PART 4
 #endif
 constexpr int kFp8MinPartBlocks = TS_FP8_MIN_PART;
+// Largest partition of its static split, and so the most blocks of a group: an even split to larger
+// steps than over a 16-bit cache.
+#ifndef TS_FP8_STATIC_MAX
+#define TS_FP8_STATIC_MAX 128
+#endif
+constexpr int kFp8StaticMax = TS_FP8_STATIC_MAX;
+static_assert(kFp8StaticMax >= kPartBlocks && kFp8StaticMax % 32 == 0, "table registers per lane");
 // Warps per CTA over an 8-bit cache: with half the bytes per block the warps' instructions, not HBM,
 // are what a block waits for, and 8 warps left the schedulers idle 60% of the time. Two query tiles
 // (more than 8 query heads per KV head) need the registers of 8.
@@ -157,6 +164,7 @@ struct DecodeArgs {
   // same plan (block tables and context lengths unchanged) without the prep kernel.
   int* header;
   int min_part_blocks;  // the static split gives a group at least this many blocks
+  int static_max;       // and is taken while a group has at most this many
   int reuse_plan;  // 1: the workspace holds the prep kernel's plan from an earlier launch
   int grid_warps;  // warps of the main kernel's grid
   // [batch + 1] partitions of one head before sequence b; sequence b's partition k of head h
@@ -248,15 +256,15 @@ struct GroupSplit {
 };
 
 // Calls f(group, group start, first block, end block) for every partition of blocks [u0, u1):
-// its pieces inside one group's range, each cut into kPartBlocks-block partitions, in order.
+// its pieces inside one group's range, each cut into partitions of `most` blocks, in order.
 template <typename F>
-__device__ __forceinline__ void for_each_chunk(int u0, int u1, const GroupSplit& gsp, F&& f) {
+__device__ __forceinline__ void for_each_chunk(int u0, int u1, const GroupSplit& gsp, int most, F&& f) {
   const int g0 = gsp.group_of(u0), g1 = gsp.group_of(u1 - 1);
   int gs = gsp.start(g0);
   for (int g = g0; g <= g1; ++g) {
     const int gn = gsp.start(g + 1);
     const int lo = max(u0, gs), hi = min(u1, gn);
-    for (int c = lo; c < hi; c += kPartBlocks) f(g, gs, c, min(hi, c + kPartBlocks));
+    for (int c = lo; c < hi; c += most) f(g, gs, c, min(hi, c + most));
     gs = gn;
   }
 }
@@ -282,7 +290,7 @@ __device__ void prep_static(DecodeArgs& a, int* warp_sums, long long WB, int run
   const int B = a.batch;
   const int NG = int(static_groups(a, WB));
   const GroupSplit gsp(int(WB), NG > 0 ? NG : 1);
-  // A group spans at most kPartBlocks blocks (the prep kernel's choice of split), so each
+  // A group spans at most static_max blocks (the prep kernel's choice of split), so each
   // group a sequence overlaps holds exactly one of its partitions: the count is the number of
   // groups its blocks [u, u + n) touch.
   int c = 0;
@@ -330,7 +338,7 @@ __device__ void prep_static(DecodeArgs& a, int* warp_sums, long long WB, int run
       const int ctx = ctx_of(a, b), n = blocks_of(ctx);
       int k = 0;
       if (n > 0)
-        for_each_chunk(u, u + n, gsp, [&](int g, int gs, int lo, int hi) {
+        for_each_chunk(u, u + n, gsp, a.static_max, [&](int g, int gs, int lo, int hi) {
           a.part_info[2 * (runc + k)] = make_int4(b, lo - u, hi - lo, k);
           if (lo == gs) a.group_first[g] = runc + k;  // the partition that opens group g
           ++k;
@@ -471,10 +479,10 @@ __global__ void __launch_bounds__(kPrepThreads) decode_prep_kernel(DecodeArgs a,
   if (threadIdx.x % 32 == 0 && wsum) atomicAdd(&total_smem, wsum);
   __syncthreads();
   const long long WB = total_smem;
-  // Static split while every group of the split spans at most min(kStaticMaxBlocksPerWarp,
-  // kPartBlocks) blocks (ceil(WB / NG)); dynamic claiming above.
+  // Static split while every group of the split spans at most static_max blocks (ceil(WB / NG));
+  // dynamic claiming above.
   const long long NG = static_groups(a, WB);
-  if (NG <= 0 || (WB + NG - 1) / NG > (long long)min(kStaticMaxBlocksPerWarp, kPartBlocks)) {
+  if (NG <= 0 || (WB + NG - 1) / NG > (long long)a.static_max) {
     prep_dynamic(a, warp_sums, cnt, b0);
   } else {
     int total_blocks = 0;
@@ -655,7 +663,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
   }
 
   // ---- producer state (warp-uniform except the tables, one table entry per lane)
-  constexpr int TABW = (kPartBlocks + 31) / 32;  // table entries per lane
+  constexpr int TABW = ((FP8 ? kFp8StaticMax : kPartBlocks) + 31) / 32;  // table entries per lane
   int p_item = -1, p_blk = 0, p_nblk = 0;
   ItemInfo p_it{};
   int p_table[TABW];
@@ -745,7 +753,10 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       int row[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int tab = TABW == 1 || p_blk + u < 32 ? p_table[0] : p_table[TABW - 1];
+        int tab = p_table[0];
+#pragma unroll
+        for (int w = 1; w < TABW; ++w)
+          if (p_blk + u >= 32 * w) tab = p_table[w];
         const int phys = __shfl_sync(0xffffffffu, tab, (p_blk + u) & 31);
         const bool present = p_blk + u < p_nblk;
         valid[u] = present && phys >= 0 && int64_t(phys) < a.num_blocks;
@@ -1635,6 +1646,7 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
   a.k_scales = k_scales;
   a.v_scales = v_scales;
   a.min_part_blocks = fp8 ? kFp8MinPartBlocks : 1;
+  a.static_max = fp8 ? kFp8StaticMax : std::min(kStaticMaxBlocksPerWarp, kPartBlocks);
   a.out = out;
   a.outs = nullptr;
   a.n_out = 0;
@@ -1832,6 +1844,7 @@ extern "C" int ts_paged_decode_no_alloc(void* out, const void* query, int64_t qu
   DecodeArgs a;
   a.k_scales = a.v_scales = nullptr;
   a.min_part_blocks = 1;
+  a.static_max = std::min(kStaticMaxBlocksPerWarp, kPartBlocks);
   a.group_arrive = nullptr;
   a.out = out;
   a.outs = nullptr;
@@ -1958,6 +1971,7 @@ int paged_decode_exchange(bool pull, void* const* dst_outs, int32_t world, int32
   DecodeArgs a;
   a.k_scales = a.v_scales = nullptr;
   a.min_part_blocks = 1;
+  a.static_max = std::min(kStaticMaxBlocksPerWarp, kPartBlocks);
   a.group_arrive = nullptr;
   a.out = nullptr;
   // push: this rank's rows go into every rank's buffer; pull: into its own buffer only, and
