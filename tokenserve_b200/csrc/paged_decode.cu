@@ -38,8 +38,8 @@
 //     itself, once) and the sum gets 2^(s - m) in 32 bits. m is kept until some t exceeds it by
 //     2^12, so most blocks need no maximum over their tokens and no rescaling of O.
 //   * Two blocks a stage and 12 warps a CTA: with half the bytes a block, instructions bind first (374 a
-//     block of one head). 256 sequences, median 1,024 tokens, 32/8 heads of 128: 168 us, 5.5 TB/s
-//     (0.84 of the copy rate; 512 sequences 0.92), 280 us over the 16-bit cache.
+//     block of one head). 256 sequences, median 1,024 tokens, 32/8 heads of 128: 171 us, 5.4 TB/s
+//     (0.83 of the copy rate; 512 sequences 0.92), 280 us over the 16-bit cache.
 //   * Slots past the context may hold anything: in a sequence's last block they are made zeros in
 //     shared memory and their scores masked.
 #include <cuda.h>
@@ -107,7 +107,9 @@ constexpr int kMaxGridWarps = 8192;
 #endif
 constexpr int kFp8MinPartBlocks = TS_FP8_MIN_PART;
 // Largest partition of its static split, and so the most blocks of a group: an even split to larger
-// steps than over a 16-bit cache.
+// steps than over a 16-bit cache. 64 / 96 / 128 / 192 / 256 blocks: 64 sequences of 64/8 heads, median
+// 4,096 tokens, take 170 / 171 / 146 / 149 / 149 us, 32 of 8,000 tokens 133 / 114 / 115 / 126 / 121, 256
+// of median 1,024 170 / 170 / 172 / 175 / 178.
 #ifndef TS_FP8_STATIC_MAX
 #define TS_FP8_STATIC_MAX 128
 #endif
