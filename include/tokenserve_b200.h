@@ -424,7 +424,7 @@ int ts_read_cache_fp8(void* key_out, void* value_out, const void* key_pool, cons
 /*
  * ts_paged_decode over an 8-bit cache: out and query of `dtype`, the workspace (and its size, from
  * ts_paged_decode_workspace_size) and the plan as there; reuse_plan = 1 is
- * ts_paged_decode_planned. Shapes as ts_paged_decode: bf16/fp16 queries with block size 16,
+ * ts_paged_decode_planned (a plan that ts_paged_decode made counts as another grid's). Shapes as ts_paged_decode: bf16/fp16 queries with block size 16,
  * head_dim 64 or 128 and at most 16 query heads per KV head on tensor cores, else head_dim 32, 64,
  * 128 or 256 on CUDA cores (no workspace).
  *

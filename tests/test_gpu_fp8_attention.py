@@ -171,6 +171,28 @@ def test_a_plan_for_another_batch_is_refused_on_the_device(cuda_device) -> None:
     assert (out == 7).all() and int(ws[4:8].view(torch.int32)) == 4
 
 
+@pytest.mark.parametrize("hq", [4, 16])  # 12 and 8 warps a CTA, the latter as over a 16-bit cache
+def test_a_plan_for_a_16_bit_cache_is_refused_on_the_device(cuda_device, hq) -> None:  # type: ignore[no-untyped-def]
+    gen = torch.Generator(device=cuda_device).manual_seed(17)
+    lens = [400, 60]
+    nb, tab = tables_for(lens, 16, gen)
+    cache = make_cache(gen, nb, 1, 16, 128)
+    plain = torch.zeros(2, nb, 1, 16, 128, dtype=BF, device=cuda_device)
+    q = torch.randn(2, hq, 128, generator=gen, device=cuda_device).to(BF)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    n = ops.decode_workspace_size(2, hq, 1, 128, tab.shape[1], 16, BF)
+    ws = torch.zeros(n, dtype=torch.uint8, device=cuda_device)
+    out = torch.full_like(q, 7)
+    ops.paged_decode(out, q, plain[0], plain[1], tab, ctx, 0.1, ws)
+    assert (out == 0).all()
+    out = decode(q, cache, tab, ctx, ws=ws, reuse=True)
+    assert (out == 7).all() and int(ws[4:8].view(torch.int32)) == 4
+    check_decode(decode(q, cache, tab, ctx, ws=ws), q, cache, tab, lens)
+    out = torch.full_like(q, 7)
+    ops.paged_decode(out, q, plain[0], plain[1], tab, ctx, 0.1, ws, reuse_plan=True)
+    assert (out == 7).all() and int(ws[4:8].view(torch.int32)) == 4
+
+
 def test_a_nan_row_spoils_its_own_sequence_alone(cuda_device) -> None:  # type: ignore[no-untyped-def]
     gen = torch.Generator(device=cuda_device).manual_seed(6)
     lens = [50, 60, 70, 80]

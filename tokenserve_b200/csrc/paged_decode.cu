@@ -475,6 +475,7 @@ __global__ void __launch_bounds__(kPrepThreads) decode_prep_kernel(DecodeArgs a,
     a.header[7] = a.num_kv_heads;
     a.header[8] = a.max_blocks;
     a.header[9] = a.grid_warps;
+    a.header[10] = a.static_max;
   }
   __syncthreads();
   const int wsum = __reduce_add_sync(0xffffffffu, unsigned(sum));
@@ -619,7 +620,8 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
   if (a.reuse_plan) {
     // The plan must have been made for this batch, head count, table width and grid.
     if (__ldg(a.header + 6) != a.batch || __ldg(a.header + 7) != a.num_kv_heads ||
-        __ldg(a.header + 8) != a.max_blocks || __ldg(a.header + 9) != a.grid_warps) {
+        __ldg(a.header + 8) != a.max_blocks || __ldg(a.header + 9) != a.grid_warps ||
+        __ldg(a.header + 10) != a.static_max) {  // the last: a plan for the other cache
       if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.header + 1, 4);
       return;
     }

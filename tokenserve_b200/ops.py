@@ -457,7 +457,7 @@ def _tables(what: str, t: torch.Tensor, rows: int) -> int:
 def _attention_rows(what: str, out: torch.Tensor, query: torch.Tensor, kv_heads: int,
                     head_dim: int) -> tuple[int, int]:  # fmt: skip
     """Query heads and token stride of ``query [T, Hq, D]``, checked against ``out``."""
-    if query.dim() != 3 or query.shape[1] == 0 or query.shape[1] % kv_heads:
+    if query.dim() != 3 or query.shape[1] == 0 or query.shape[1] % max(kv_heads, 1):
         raise KernelError(f"{what}: query must be [tokens, heads, {head_dim}] with a multiple of "
                           f"{kv_heads} heads, got {tuple(query.shape)}")  # fmt: skip
     stride = _rows(query, query.shape[1], head_dim, f"{what}: query")
@@ -488,8 +488,8 @@ def reshape_and_cache_fp8(
                 token_tags, tag_pool, error_flag)  # fmt: skip
     if key.dtype != value.dtype or key.shape != value.shape:
         raise KernelError(f"{what}: key and value must have one shape and dtype")
-    n = key.shape[0]
     ks, vs = _rows(key, h, d, f"{what}: key"), _rows(value, h, d, f"{what}: value")
+    n = key.shape[0]
     if n == 1:  # a single row's stride says nothing
         ks = vs = h * d
     _int_array(what, "slot_mapping", slot_mapping, torch.int64, n)
@@ -581,7 +581,7 @@ def read_cache_fp8(
     for t in (key_out, value_out):
         if t.shape != (n, h, d) or t.dtype != key_out.dtype or not t.is_contiguous():
             raise KernelError(f"{what}: outputs must be contiguous [tokens, {h}, {d}] of one dtype")
-    seqs = block_tables.shape[0]
+    seqs = block_tables.shape[0] if block_tables.dim() else -1
     width = _tables(what, block_tables, seqs)
     _int_array(what, "token_start_loc", token_start_loc, torch.int32, seqs + 1)
     _error_flag(what, error_flag)
