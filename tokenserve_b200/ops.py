@@ -162,11 +162,13 @@ def _dtype(t: torch.Tensor) -> int:
 
 def _rows(t: torch.Tensor, heads: int, head_dim: int, what: str) -> int:
     """Token stride (elements) of a [tokens, heads, head_dim] view with contiguous rows."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
-        raise KernelError(f"{what}: expected [tokens, {heads}, {head_dim}], got {tuple(t.shape)}")
-    if t.stride(2) != 1 or t.stride(1) != head_dim:
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        raise KernelError(f"{what}: expected [tokens, {heads}, {head_dim}], got {tuple(shape)}")
+    stride = t.stride()
+    if stride[2] != 1 or stride[1] != head_dim:
         raise KernelError(f"{what}: heads and head_dim must be contiguous")
-    return t.stride(0)
+    return stride[0]
 
 
 def _pool_dims(pool: torch.Tensor) -> tuple[int, int, int, int]:
@@ -420,17 +422,20 @@ def _launch(what: str, device: int, name: str, *args) -> None:  # type: ignore[n
         _check(code, what)
 
 
+_E4M3, _F32, _I32, _I64 = torch.float8_e4m3fn, torch.float32, torch.int32, torch.int64
+
+
 def _fp8_pool_dims(what: str, key_pool: torch.Tensor, value_pool: torch.Tensor,
                    key_scales: torch.Tensor, value_scales: torch.Tensor) -> torch.Size:  # fmt: skip
     shape = key_pool.shape
-    if (len(shape) != 4 or value_pool.shape != shape or key_pool.dtype != torch.float8_e4m3fn
-            or value_pool.dtype != torch.float8_e4m3fn or not key_pool.is_contiguous()
+    if (len(shape) != 4 or value_pool.shape != shape or key_pool.dtype != _E4M3
+            or value_pool.dtype != _E4M3 or not key_pool.is_contiguous()
             or not value_pool.is_contiguous()):  # fmt: skip
         raise KernelError(f"{what}: 8-bit pools must be contiguous float8_e4m3fn "
                           "[num_blocks, kv_heads, block_size, head_dim]")  # fmt: skip
-    rows = shape[:3]
-    if (key_scales.shape != rows or value_scales.shape != rows
-            or key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32
+    rows = key_scales.shape
+    if (rows != shape[:3] or value_scales.shape != rows
+            or key_scales.dtype != _F32 or value_scales.dtype != _F32
             or not key_scales.is_contiguous() or not value_scales.is_contiguous()):  # fmt: skip
         raise KernelError(f"{what}: scales must be contiguous float32 "
                           "[num_blocks, kv_heads, block_size]")  # fmt: skip
@@ -444,27 +449,29 @@ def _int_array(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, n: int
 
 
 def _error_flag(what: str, t: torch.Tensor | None) -> None:
-    if t is not None and (t.dtype != torch.int32 or t.numel() < 1):
+    if t is not None and (t.dtype != _I32 or t.numel() < 1):
         raise KernelError(f"{what}: error_flag must be an int32 tensor")
 
 
 def _tables(what: str, t: torch.Tensor, rows: int) -> int:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != rows or not t.is_contiguous():
+    shape = t.shape
+    if t.dtype != _I32 or len(shape) != 2 or shape[0] != rows or not t.is_contiguous():
         raise KernelError(f"{what}: block_tables must be contiguous int32 [{rows}, max_blocks]")
-    return t.shape[1]
+    return shape[1]
 
 
 def _attention_rows(what: str, out: torch.Tensor, query: torch.Tensor, kv_heads: int,
                     head_dim: int) -> tuple[int, int]:  # fmt: skip
     """Query heads and token stride of ``query [T, Hq, D]``, checked against ``out``."""
-    if query.dim() != 3 or query.shape[1] == 0 or query.shape[1] % max(kv_heads, 1):
+    shape = query.shape
+    if len(shape) != 3 or shape[1] == 0 or shape[1] % max(kv_heads, 1):
         raise KernelError(f"{what}: query must be [tokens, heads, {head_dim}] with a multiple of "
-                          f"{kv_heads} heads, got {tuple(query.shape)}")  # fmt: skip
-    stride = _rows(query, query.shape[1], head_dim, f"{what}: query")
-    if out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+                          f"{kv_heads} heads, got {tuple(shape)}")  # fmt: skip
+    stride = _rows(query, shape[1], head_dim, f"{what}: query")
+    if out.shape != shape or out.dtype != query.dtype or not out.is_contiguous():
         raise KernelError(f"{what}: out must be contiguous, of the query's shape and dtype")
     # A single row's stride says nothing.
-    return query.shape[1], stride if query.shape[0] > 1 else query.shape[1] * head_dim
+    return shape[1], stride if shape[0] > 1 else shape[1] * head_dim
 
 
 def reshape_and_cache_fp8(
@@ -492,16 +499,16 @@ def reshape_and_cache_fp8(
     n = key.shape[0]
     if n == 1:  # a single row's stride says nothing
         ks = vs = h * d
-    _int_array(what, "slot_mapping", slot_mapping, torch.int64, n)
+    _int_array(what, "slot_mapping", slot_mapping, _I64, n)
     if token_tags is not None:
-        _int_array(what, "token_tags", token_tags, torch.int32, n)
+        _int_array(what, "token_tags", token_tags, _I32, n)
     if tag_pool is not None:
-        _int_array(what, "tag_pool", tag_pool, torch.int32, nb * bs)
+        _int_array(what, "tag_pool", tag_pool, _I32, nb * bs)
     _error_flag(what, error_flag)
     _launch(what, dev, "ts_reshape_and_cache_fp8",
-            _ptr(key), _ptr(value), ks, vs, _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
-            _ptr(value_scales), _ptr(slot_mapping), n, h, d, bs, nb, _dtype(key),
-            _ptr(token_tags), _ptr(tag_pool), _ptr(error_flag))  # fmt: skip
+            key.data_ptr(), value.data_ptr(), ks, vs, key_pool.data_ptr(), value_pool.data_ptr(),
+            key_scales.data_ptr(), value_scales.data_ptr(), slot_mapping.data_ptr(), n, h, d, bs,
+            nb, _dtype(key), _ptr(token_tags), _ptr(tag_pool), _ptr(error_flag))  # fmt: skip
 
 
 def rotary_and_cache(
@@ -541,23 +548,25 @@ def rotary_and_cache(
     dev = _cuda(what, qkv, q_out, key_pool, value_pool, key_scales, value_scales, slot_mapping,
                 positions, inv_freq, error_flag)  # fmt: skip
     n, width = qkv.shape if qkv.dim() == 2 else (-1, -1)
+    stride = qkv.stride()
     if hkv != num_kv_heads or num_q_heads <= 0 or width != (num_q_heads + 2 * hkv) * d or (
-            qkv.stride(1) != 1):  # fmt: skip
+            stride[1] != 1):  # fmt: skip
         raise KernelError(f"{what}: qkv must be [tokens, (q heads + 2 kv heads) * head_dim] with "
                           "contiguous rows and the pool's kv heads")  # fmt: skip
     if q_out.shape != (n, num_q_heads, d) or q_out.dtype != qkv.dtype or not q_out.is_contiguous():
         raise KernelError(f"{what}: q_out must be a contiguous [tokens, q heads, head_dim] of "
                           "qkv's dtype")  # fmt: skip
-    _int_array(what, "slot_mapping", slot_mapping, torch.int64, n)
-    _int_array(what, "positions", positions, torch.int64, n)
+    _int_array(what, "slot_mapping", slot_mapping, _I64, n)
+    _int_array(what, "positions", positions, _I64, n)
     half = inv_freq.numel()
-    _int_array(what, "inv_freq", inv_freq, torch.float32, half)
+    _int_array(what, "inv_freq", inv_freq, _F32, half)
     _error_flag(what, error_flag)
     _launch(what, dev, "ts_rotary_and_cache",
-            _ptr(qkv), qkv.stride(0) if n > 1 else width, _ptr(q_out), _ptr(key_pool),
-            _ptr(value_pool), _ptr(key_scales), _ptr(value_scales), _ptr(slot_mapping),
-            _ptr(positions), _ptr(inv_freq), n, num_q_heads, hkv, d, 2 * half, int(interleaved),
-            float(attention_scaling), bs, nb, _dtype(qkv), _ptr(error_flag))  # fmt: skip
+            qkv.data_ptr(), stride[0] if n > 1 else width, q_out.data_ptr(),
+            key_pool.data_ptr(), value_pool.data_ptr(), _ptr(key_scales), _ptr(value_scales),
+            slot_mapping.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), n, num_q_heads, hkv,
+            d, 2 * half, int(interleaved), float(attention_scaling), bs, nb, _dtype(qkv),
+            _ptr(error_flag))  # fmt: skip
 
 
 def read_cache_fp8(
@@ -583,12 +592,13 @@ def read_cache_fp8(
             raise KernelError(f"{what}: outputs must be contiguous [tokens, {h}, {d}] of one dtype")
     seqs = block_tables.shape[0] if block_tables.dim() else -1
     width = _tables(what, block_tables, seqs)
-    _int_array(what, "token_start_loc", token_start_loc, torch.int32, seqs + 1)
+    _int_array(what, "token_start_loc", token_start_loc, _I32, seqs + 1)
     _error_flag(what, error_flag)
     _launch(what, dev, "ts_read_cache_fp8",
-            _ptr(key_out), _ptr(value_out), _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
-            _ptr(value_scales), _ptr(block_tables), width, _ptr(token_start_loc), seqs, n, h, d,
-            bs, nb, _dtype(key_out), _ptr(error_flag))  # fmt: skip
+            key_out.data_ptr(), value_out.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(),
+            key_scales.data_ptr(), value_scales.data_ptr(), block_tables.data_ptr(), width,
+            token_start_loc.data_ptr(), seqs, n, h, d, bs, nb, _dtype(key_out),
+            _ptr(error_flag))  # fmt: skip
 
 
 def paged_decode_fp8(
@@ -613,15 +623,15 @@ def paged_decode_fp8(
     hq, qs = _attention_rows(what, out, query, hkv, d)
     b = query.shape[0]
     width = _tables(what, block_tables, b)
-    _int_array(what, "context_lens", context_lens, torch.int32, b)
+    _int_array(what, "context_lens", context_lens, _I32, b)
     if workspace is not None and not workspace.is_contiguous():
         raise KernelError(f"{what}: workspace must be contiguous")
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     _launch(what, dev, "ts_paged_decode_fp8",
-            _ptr(out), _ptr(query), qs, _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
-            _ptr(value_scales), _ptr(block_tables), width, _ptr(context_lens), b, hq, hkv, d, bs,
-            nb, float(scale), _dtype(query), _ptr(workspace), ws_bytes,
-            int(reuse_plan))  # fmt: skip
+            out.data_ptr(), query.data_ptr(), qs, key_pool.data_ptr(), value_pool.data_ptr(),
+            key_scales.data_ptr(), value_scales.data_ptr(), block_tables.data_ptr(), width,
+            context_lens.data_ptr(), b, hq, hkv, d, bs, nb, float(scale), _dtype(query),
+            _ptr(workspace), ws_bytes, int(reuse_plan))  # fmt: skip
 
 
 def paged_prefill_fp8(
@@ -645,10 +655,10 @@ def paged_prefill_fp8(
     hq, qs = _attention_rows(what, out, query, hkv, d)
     seqs = context_lens.numel()
     width = _tables(what, block_tables, seqs)
-    _int_array(what, "context_lens", context_lens, torch.int32, seqs)
-    _int_array(what, "query_start_loc", query_start_loc, torch.int32, seqs + 1)
+    _int_array(what, "context_lens", context_lens, _I32, seqs)
+    _int_array(what, "query_start_loc", query_start_loc, _I32, seqs + 1)
     _launch(what, dev, "ts_paged_prefill_fp8",
-            _ptr(out), _ptr(query), qs, _ptr(key_pool), _ptr(value_pool), _ptr(key_scales),
-            _ptr(value_scales), _ptr(block_tables), width, _ptr(query_start_loc),
-            _ptr(context_lens), seqs, query.shape[0], int(max_query_len), hq, hkv, d, bs, nb,
-            float(scale), _dtype(query))  # fmt: skip
+            out.data_ptr(), query.data_ptr(), qs, key_pool.data_ptr(), value_pool.data_ptr(),
+            key_scales.data_ptr(), value_scales.data_ptr(), block_tables.data_ptr(), width,
+            query_start_loc.data_ptr(), context_lens.data_ptr(), seqs, query.shape[0],
+            int(max_query_len), hq, hkv, d, bs, nb, float(scale), _dtype(query))  # fmt: skip
