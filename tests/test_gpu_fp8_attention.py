@@ -9,7 +9,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.fp8_reference import E4M3, attention, make_cache, rows_of, tables_for
+from tests.fp8_reference import E4M3, HALF_STEP, attention, make_cache, rows_of, tables_for
 from tokenserve_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -416,6 +416,45 @@ def test_a_model_step_over_the_cache(cuda_device) -> None:  # type: ignore[no-un
         _, off = attention(q[i : i + 1], *rows_of(kp, ks, tab[i], n), *rows_of(vp, vs, tab[i], n),
                            d**-0.5, None)  # fmt: skip
         assert ((out[i].double() - want).abs() <= off[0] + 2.0**-23 * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])  # tensor cores, CUDA cores
+def test_blocks_whose_offsets_pass_32_bits(cuda_device, dtype) -> None:  # type: ignore[no-untyped-def]
+    """Every operator on the last blocks of pools of 4.6 GB each, and on block 0."""
+    gen = torch.Generator(device=cuda_device).manual_seed(13)
+    nb, hq, hkv, bs, d, n = 140_000, 32, 16, 16, 128, 150
+    assert (nb - 20) * hkv * bs * d > 2**32
+    kp = torch.empty(nb, hkv, bs, d, dtype=torch.uint8, device=cuda_device).view(E4M3)
+    vp = torch.empty_like(kp)
+    ks = torch.empty(nb, hkv, bs, device=cuda_device)
+    vs = torch.empty_like(ks)
+    cache = (kp, vp, ks, vs)
+    last = nb - 1 - torch.arange(9, device=cuda_device)
+    tab = torch.cat([last, torch.zeros(1, device=cuda_device)]).to(torch.int32)[None]
+    pos = torch.arange(n, device=cuda_device)
+    slots = tab[0, pos // bs].long() * bs + pos % bs
+    k = torch.randn(n, hkv, d, generator=gen, device=cuda_device).to(dtype)
+    v = torch.randn(n, hkv, d, generator=gen, device=cuda_device).to(dtype)
+    half = n // 2
+    ops.reshape_and_cache_fp8(k[:half], v[:half], kp, vp, ks, vs, slots[:half])
+    q = torch.randn(n, hq, d, generator=gen, device=cuda_device).to(dtype)
+    qkv = torch.cat([q[half:].flatten(1), k[half:].flatten(1), v[half:].flatten(1)], 1)
+    still = torch.zeros(d // 2, device=cuda_device)  # nothing turns
+    ops.rotary_and_cache(qkv, torch.empty_like(q[half:]), kp, vp, slots[half:], pos[half:], still, hq,
+                         hkv, key_scales=ks, value_scales=vs)  # fmt: skip
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    loc = torch.tensor([0, n], dtype=torch.int32, device=cuda_device)
+    ops.read_cache_fp8(ko, vo, *cache, tab, loc)
+    for x, o in ((k, ko), (v, vo)):
+        # Half a step: 2^-4 of the value, or of the smallest normal (2^-6 of a code, 448 the row's
+        # largest); fp32 steps of the scale and the quotient; the output's own rounding.
+        x, o = x.double(), o.double()
+        least = x.abs().amax(-1, keepdim=True) / 448 * 2.0**-6
+        lim = torch.maximum(x.abs(), least) * 2.0**-4 * (1 + 2.0**-18) + o.abs() * HALF_STEP[dtype]
+        assert ((o - x).abs() <= lim).all()
+    ctx = torch.tensor([n], dtype=torch.int32, device=cuda_device)
+    check_decode(decode(q[-1:], cache, tab, ctx), q[-1:], cache, tab, [n])
+    check_prefill(prefill(q, cache, tab, loc, ctx, n), q, cache, tab, [n], [n])
 
 
 def test_captured_step_replays_on_new_inputs_on_another_stream(cuda_device) -> None:  # type: ignore[no-untyped-def]
