@@ -1103,6 +1103,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       slot0 += in_seq / kMergeGroup * kMergeGroup;
       np = min(kMergeGroup, it.nparts - in_seq / kMergeGroup * kMergeGroup);
       merge();
+      __syncwarp();  // every lane has read the first slot's maximum and sum, replaced below
       float* dst = a.part_o + slot0 * D * NT8;
 #pragma unroll
       for (int i = 0; i < PER; ++i) dst[lane + 32 * i] = acc[i];
