@@ -772,6 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       for (int c = 0; c < min(n_whole, n_some); ++c) columns(c, std::false_type{});
 #pragma unroll 1
       for (int c = min(n_whole, n_some); c < n_some; ++c) columns(c, std::true_type{});
+      if (n_some == 0) ts::tc::wait_ld(sa);  // nothing above has waited for the load
 #pragma unroll 1
       for (int c = n_some; c < kGroups; ++c) {
         uint32_t pw[16] = {};
