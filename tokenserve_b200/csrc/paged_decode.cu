@@ -34,9 +34,11 @@
 //     permutation, which permutes O's rows.
 //   * q is scaled per head by a power of two into f16's range (bf16 q stays exact).
 //   * K's scale multiplies the score. V's is added to the exponent of the weight: with t = s +
-//     log2(vs), m is a maximum of t, w = 2^(t - m) goes to the PV product as f16 (11 bits: 2^-12 of
-//     itself, once) and the sum gets 2^(s - m) in 32 bits. m is kept until some t exceeds it by
-//     2^12, so most blocks need no maximum over their tokens and no rescaling of O.
+//     log2(vs), w = 2^(t - mt) goes to the PV product as f16 and the sum gets 2^(s - m) in 32 bits,
+//     m a maximum of s and mt one of t: V rows of any magnitude, zero rows among them, leave the sum
+//     in range. Both are kept until some s or t exceeds its one by 2^12, so most blocks need no maximum
+//     over their tokens and no rescaling of O; the output is O 2^(mt - m) / sum. A weight's rounding
+//     to 11 bits is at most 2^-11 of it down to 2^-14 of the largest w, 2^-25 of that below.
 //   * Two blocks a stage and 12 warps a CTA: with half the bytes a block, instructions bind first (374 a
 //     block of one head). 256 sequences, median 1,024 tokens, 32/8 heads of 128: 171 us, 5.4 TB/s
 //     (0.83 of the copy rate; 512 sequences 0.92), 280 us over the 16-bit cache.
@@ -181,11 +183,12 @@ struct DecodeArgs {
   int* group_arrive;  // [slot] of a (sequence, head)'s first slots: its groups of partials (8-bit)
   float* part_o;   // [partition][head_dim][NT * 8]
   float2* part_ml;  // [partition][NT * 8]
+  float* part_t;  // [partition][NT * 8] maximum that O's weights are relative to (8-bit)
 };
 
 // Workspace layout (byte offsets), shared by the size query and the launcher.
 struct WsLayout {
-  size_t chunk_prefix, part_info, group_first, arrive, group_arrive, part_o, part_ml, total;
+  size_t chunk_prefix, part_info, group_first, arrive, group_arrive, part_o, part_ml, part_t, total;
 };
 
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -193,7 +196,7 @@ inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 int num_sms();
 
 // grid_warps: warps of the decode grid on the device the call runs on (its SMs x kWarps).
-// fp8: with the counters of the grouped merge.
+// fp8: with the counters of the grouped merge and the weights' maxima.
 WsLayout ws_layout(int batch, int hkv, int hd, int max_blocks, int nt, int grid_warps,
                    bool fp8 = false) {
   WsLayout w;
@@ -210,7 +213,8 @@ WsLayout ws_layout(int batch, int hkv, int hd, int max_blocks, int nt, int grid_
   w.group_arrive = w.arrive + align256(sizeof(int) * bh);
   w.part_o = w.group_arrive + (fp8 ? align256(sizeof(int) * slots) : 0);
   w.part_ml = w.part_o + align256(sizeof(float) * slots * hd * nt * 8);
-  w.total = w.part_ml + align256(sizeof(float2) * slots * nt * 8);
+  w.part_t = w.part_ml + align256(sizeof(float2) * slots * nt * 8);
+  w.total = w.part_t + (fp8 ? align256(sizeof(float) * slots * nt * 8) : 0);
   return w;
 }
 
@@ -577,7 +581,7 @@ __device__ __forceinline__ uint32_t tile_off(int t, int cg) {
   }
 }
 
-// m is kept until exceeded by 2^12: weights stay below f16's 2^16.
+// The maxima are kept until exceeded by 2^12: weights stay below f16's 2^16.
 constexpr float kFp8MaxSlack = 12.f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -832,6 +836,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
   uint32_t qf[NT][KSTEPS][2];
   float oacc[NT][MTILES][4];
   float m_run[NT][2], l_run[NT][2];
+  float t_run[NT][2];  // 8-bit cache: maximum that the weights, and O, are relative to
   float qs[NT][2];  // 8-bit cache: score factor of heads 2t, 2t + 1 (softmax scale, q's scale)
 
   auto start_item = [&](const int4& m0, const int4& m1) {
@@ -884,7 +889,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       for (int mt = 0; mt < MTILES; ++mt)
 #pragma unroll
         for (int j = 0; j < 4; ++j) oacc[nt][mt][j] = 0.f;
-      m_run[nt][0] = m_run[nt][1] = -INFINITY;
+      m_run[nt][0] = m_run[nt][1] = t_run[nt][0] = t_run[nt][1] = -INFINITY;
       l_run[nt][0] = l_run[nt][1] = 0.f;
     }
   };
@@ -923,8 +928,12 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       // transposes lane (g, t) has dims (4t, 4t + 2) and (4t + 1, 4t + 3) of head g: 8 bytes.
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float i0 = l_run[nt][0] > 0.f ? 1.f / l_run[nt][0] : l_run[nt][0];
-        const float i1 = l_run[nt][1] > 0.f ? 1.f / l_run[nt][1] : l_run[nt][1];
+        float inv[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)  // nothing seen: 0; a NaN stays one
+          inv[j] = l_run[nt][j] > 0.f ? ex2(t_run[nt][j] - m_run[nt][j]) * (1.f / l_run[nt][j])
+                                      : l_run[nt][j];
+        const float i0 = inv[0], i1 = inv[1];
         const int head = nt * 8 + g;
         bool vec;
         T* orow = dst_row(0, it.b, it.h * a.group + head, vec);
@@ -1011,6 +1020,9 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       for (int nt = 0; nt < NT; ++nt) {
         a.part_ml[slot * NT8 + nt * 8 + 2 * t] = make_float2(m_run[nt][0], l_run[nt][0]);
         a.part_ml[slot * NT8 + nt * 8 + 2 * t + 1] = make_float2(m_run[nt][1], l_run[nt][1]);
+        if constexpr (FP8)
+          *reinterpret_cast<float2*>(a.part_t + slot * NT8 + nt * 8 + 2 * t) =
+              make_float2(t_run[nt][0], t_run[nt][1]);
       }
     }
     __threadfence();
@@ -1045,24 +1057,36 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
     int np = it.nparts, stride = 1;
     constexpr int PER = D * NT8 / 32;
     float acc[PER];
-    float lsum, mx;
+    float lsum, mx, tx;  // tx: the largest of the weights' maxima (8-bit)
     auto merge = [&]() {
     // Running max: the lanes of one head split the partitions (32 / NT8 per pass, four passes'
     // loads in flight), then reduce across those lanes.
     constexpr int kLanesPerHead = 32 / NT8;
-    mx = -INFINITY;
+    mx = tx = -INFINITY;
     for (int p0 = lane / NT8; p0 < np; p0 += 4 * kLanesPerHead) {
-      float v[4];
+      float v[4], vt[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int p = p0 + u * kLanesPerHead;
         v[u] = p < np ? __ldcg(&a.part_ml[(slot0 + p * stride) * NT8 + hd].x) : -INFINITY;
+        vt[u] = FP8 && p < np ? __ldcg(&a.part_t[(slot0 + p * stride) * NT8 + hd]) : -INFINITY;
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) mx = fmaxf(mx, v[u]);
+      for (int u = 0; u < 4; ++u) {
+        mx = fmaxf(mx, v[u]);
+        if (FP8) tx = fmaxf(tx, vt[u]);
+      }
     }
 #pragma unroll
-    for (int o = NT8; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    for (int o = NT8; o < 32; o <<= 1) {
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (FP8) tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, o));
+    }
+    // Factor of a partial's O, whose sum has the factor w.
+    auto o_factor = [&](int64_t s, float m, float w) {
+      if constexpr (FP8) return m == -INFINITY ? 0.f : exp2f(__ldcg(&a.part_t[s * NT8 + hd]) - tx);
+      return w;
+    };
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
     lsum = 0.f;
@@ -1083,10 +1107,11 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       const float w1 = ml1.x == -INFINITY ? 0.f : exp2f(ml1.x - mx);
       lsum += w0 * ml0.y;
       lsum += w1 * ml1.y;
+      const float f0 = o_factor(s0, ml0.x, w0), f1 = o_factor(s1, ml1.x, w1);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        acc[i] += w0 * x0[i];
-        acc[i] += w1 * x1[i];
+        acc[i] += f0 * x0[i];
+        acc[i] += f1 * x1[i];
       }
     }
     if (p < np) {
@@ -1094,20 +1119,24 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       const float2 ml = __ldcg(&a.part_ml[sl * NT8 + hd]);
       const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mx);
       lsum += w * ml.y;
+      const float f = o_factor(sl, ml.x, w);
       const float* src = a.part_o + sl * D * NT8;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] += w * __ldcg(src + lane + 32 * i);
+      for (int i = 0; i < PER; ++i) acc[i] += f * __ldcg(src + lane + 32 * i);
     }
     };
     if (grouped) {
       slot0 += in_seq / kMergeGroup * kMergeGroup;
       np = min(kMergeGroup, it.nparts - in_seq / kMergeGroup * kMergeGroup);
       merge();
-      __syncwarp();  // every lane has read the first slot's maximum and sum, replaced below
+      __syncwarp();  // every lane has read the first slot's maxima and sum, replaced below
       float* dst = a.part_o + slot0 * D * NT8;
 #pragma unroll
       for (int i = 0; i < PER; ++i) dst[lane + 32 * i] = acc[i];
-      if (lane < NT8) a.part_ml[slot0 * NT8 + lane] = make_float2(mx, lsum);
+      if (lane < NT8) {
+        a.part_ml[slot0 * NT8 + lane] = make_float2(mx, lsum);
+        a.part_t[slot0 * NT8 + lane] = tx;
+      }
       __threadfence();
       __syncwarp();
       if (!last_of(a.arrive + it.b * a.num_kv_heads + it.h, groups)) return;
@@ -1116,7 +1145,8 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       stride = kMergeGroup;
     }
     merge();
-    const float inv = lsum > 0.f ? 1.f / lsum : FP8 ? lsum : 0.f;
+    float inv = lsum > 0.f ? 1.f / lsum : FP8 ? lsum : 0.f;
+    if (FP8 && lsum > 0.f) inv *= ex2(tx - mx);
     // Lane (hd, kq = lane / NT8) holds dims kq + LPH * i of head hd. Gather each 16-byte chunk
     // (8 consecutive dims) of a head into lane kq = chunk % LPH and store it as one vector.
     constexpr int LPH = 32 / NT8;     // lanes per head
@@ -1216,39 +1246,51 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
     uint32_t pb[NT][2 * B];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      // e: log2 of the sum's terms, e + lv: of the weights, both relative to the maximum kept.
+      // e: log2 of the sum's terms, w: of the weights, each relative to the maximum kept.
       float e[4 * B], w[4 * B];
       auto relative = [&]() {
+        const float shift[2] = {m_run[nt][0] - t_run[nt][0], m_run[nt][1] - t_run[nt][1]};
 #pragma unroll
         for (int j = 0; j < 4 * B; ++j) {
           e[j] = fmaf(sacc[nt][j], ks[j / 2] * qs[nt][j & 1], -m_run[nt][j & 1]);
           if (!whole && !in_context(j / 2)) e[j] = -INFINITY;
-          w[j] = e[j] + lv[j / 2];
+          w[j] = e[j] + (lv[j / 2] + shift[j & 1]);
         }
       };
       relative();
-      float top = w[0];
+      float top = fmaxf(e[0], w[0]);
 #pragma unroll
-      for (int j = 1; j < 4 * B; ++j) top = fmaxf(top, w[j]);
+      for (int j = 1; j < 4 * B; ++j) top = ts::max3f(top, e[j], w[j]);
       // An item's first blocks always: its maxima are still -inf.
       if (__any_sync(0xffffffffu, top > kFp8MaxSlack || m_run[nt][0] == -INFINITY)) {
-        // A scale of 0 counts as 2^-126 here, so that the maximum is finite.
-        float bm[2] = {-INFINITY, -INFINITY};
+        // A scale of 0 counts as 2^-126 here, so that the weights' maximum is finite too.
+        float bm[2] = {-INFINITY, -INFINITY}, bt[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int j = 0; j < 4 * B; ++j) {
           const float s = sacc[nt][j] * (ks[j / 2] * qs[nt][j & 1]);
-          if (whole || in_context(j / 2))
-            bm[j & 1] = fmaxf(bm[j & 1], fmaxf(s + lv[j / 2], s - 126.f));
+          if (whole || in_context(j / 2)) {
+            bm[j & 1] = fmaxf(bm[j & 1], s);
+            bt[j & 1] = ts::max3f(bt[j & 1], s + lv[j / 2], s - 126.f);
+          }
         }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
-          bm[0] = fmaxf(bm[0], __shfl_xor_sync(0xffffffffu, bm[0], o));
-          bm[1] = fmaxf(bm[1], __shfl_xor_sync(0xffffffffu, bm[1], o));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            bm[j] = fmaxf(bm[j], __shfl_xor_sync(0xffffffffu, bm[j], o));
+            bt[j] = fmaxf(bt[j], __shfl_xor_sync(0xffffffffu, bt[j], o));
+          }
         }
-        const float mn0 = fmaxf(m_run[nt][0], bm[0]), mn1 = fmaxf(m_run[nt][1], bm[1]);
-        const float c0 = ex2(m_run[nt][0] - mn0), c1 = ex2(m_run[nt][1] - mn1);
-        l_run[nt][0] *= c0;
-        l_run[nt][1] *= c1;
+        float c[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float mn = fmaxf(m_run[nt][j], bm[j]), tn = fmaxf(t_run[nt][j], bt[j]);
+          l_run[nt][j] *= ex2(m_run[nt][j] - mn);
+          c[j] = ex2(t_run[nt][j] - tn);
+          m_run[nt][j] = mn;
+          t_run[nt][j] = tn;
+        }
+        const float c0 = c[0], c1 = c[1];
 #pragma unroll
         for (int mt = 0; mt < MTILES; ++mt) {
           oacc[nt][mt][0] *= c0;
@@ -1256,8 +1298,6 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
           oacc[nt][mt][2] *= c0;
           oacc[nt][mt][3] *= c1;
         }
-        m_run[nt][0] = mn0;
-        m_run[nt][1] = mn1;
         relative();
       }
 #pragma unroll
@@ -1682,6 +1722,7 @@ int paged_decode_call(void* out, const void* query, int64_t query_token_stride,
   a.group_arrive = fp8 ? reinterpret_cast<int*>(ws + w.group_arrive) : nullptr;
   a.part_o = reinterpret_cast<float*>(ws + w.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+  a.part_t = fp8 ? reinterpret_cast<float*>(ws + w.part_t) : nullptr;
 #define TS_FAST(T)                                                             \
   if (fp8 && head_dim == 128)                                                  \
     return nt == 1 ? launch_fast<T, 128, 1, true>(a, km, vm, s, plan)          \
@@ -1851,6 +1892,7 @@ extern "C" int ts_paged_decode_no_alloc(void* out, const void* query, int64_t qu
   a.min_part_blocks = 1;
   a.static_max = std::min(kStaticMaxBlocksPerWarp, kPartBlocks);
   a.group_arrive = nullptr;
+  a.part_t = nullptr;
   a.out = out;
   a.outs = nullptr;
   a.n_out = 0;
@@ -1978,6 +2020,7 @@ int paged_decode_exchange(bool pull, void* const* dst_outs, int32_t world, int32
   a.min_part_blocks = 1;
   a.static_max = std::min(kStaticMaxBlocksPerWarp, kPartBlocks);
   a.group_arrive = nullptr;
+  a.part_t = nullptr;
   a.out = nullptr;
   // push: this rank's rows go into every rank's buffer; pull: into its own buffer only, and
   // the other ranks fetch them (ts_gather_peers).
