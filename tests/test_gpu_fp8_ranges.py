@@ -9,7 +9,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.fp8_reference import make_cache, tables_for
+from tests.fp8_reference import attention, make_cache, rows_of, tables_for
 from tests.test_gpu_fp8_attention import check_decode, check_prefill, decode, prefill
 from tokenserve_b200 import ops
 
@@ -117,3 +117,84 @@ def test_decode_of_value_rows_over_many_binades(cuda_device, span) -> None:  # t
     q = torch.randn(len(lens), 8, 128, generator=gen, device=cuda_device).to(BF)
     ctx = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
     check_decode(decode(q, (kp, vp, ks, vs), tab, ctx), q, (kp, vp, ks, vs), tab, lens)
+
+
+def value_slack(q, cache, tab, chunks, ctxs):  # type: ignore[no-untyped-def]
+    """What the tensor-core prefill may add to ``attention``'s bound where V's magnitudes differ.
+
+    V's tile holds code * scale / 2^n * 64 in fp16, 2^n <= the largest scale of a group of 32
+    tokens, its factor as a sum of two fp16 numbers: off by 2^-25 (448 + 2) / 64 < 2^-22 times 2^n
+    beside 2^-11 of itself. A weight is p 2^n over the largest such product (of those kept, which
+    is not above the row's), rounded to fp16: off by 2^-25 of that product below fp16's range."""
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    kp, vp, ks, vs = cache
+    d, at = q.shape[-1], 0
+    for i, (n, c) in enumerate(zip(chunks, ctxs, strict=True)):
+        kc, ksc = rows_of(kp, ks, tab[i], c)
+        vc, vsc = rows_of(vp, vs, tab[i], c)
+        hkv = kc.shape[0]
+        pad = torch.nn.functional.pad(vsc, (0, -c % 32)).unflatten(1, (-1, 32)).amax(-1)
+        top = pad.repeat_interleave(32, 1)[:, :c].clamp_min(2.0**-120)
+        top = torch.maximum(top, top.cummax(1).values * 2.0**-60)
+        see = (torch.arange(c, device=q.device)[None, :]
+               <= c - n + torch.arange(n, device=q.device)[:, None])  # fmt: skip
+        s = torch.einsum("nhgd,hkd->nhgk", q[at : at + n].double().unflatten(1, (hkv, -1)),
+                         kc * ksc[..., None]) * d**-0.5  # fmt: skip
+        p = torch.softmax(s.masked_fill(~see[:, None, None], -float("inf")), -1)
+        held = torch.einsum("nhgk,hk->nhg", p, top) * 2.0**-22
+        units = (vc * (vsc / top)[..., None]).abs().cumsum(1)[:, c - n :]  # of the keys a row sees
+        tail = (p * top[None, :, None]).amax(-1)[..., None] * units.transpose(0, 1)[:, :, None] * 2.0**-23
+        out[at : at + n] = (held[..., None] + tail).flatten(1, 2)
+        at += n
+    return out
+
+
+def check_prefill_wide(out, q, cache, tab, chunks, ctxs):  # type: ignore[no-untyped-def]
+    slack, at = value_slack(q, cache, tab, chunks, ctxs), 0
+    for i, (n, c) in enumerate(zip(chunks, ctxs, strict=True)):
+        rows = slice(at, at + n)
+        at += n
+        want, off = attention(q[rows], *rows_of(cache[0], cache[2], tab[i], c),
+                              *rows_of(cache[1], cache[3], tab[i], c), q.shape[-1] ** -0.5, c - n,
+                              k_half=2.0**-11)  # fmt: skip
+        off, got, most = off + slack[rows], out[rows].double(), torch.finfo(q.dtype).max
+        # An output past the type's largest number is that type's infinity (fp16: past 65504).
+        past = (want.abs() + off > most) & torch.isinf(got) & (got * want > 0)
+        bad = ((got - want).abs() - off).masked_fill(past, 0.0)
+        assert (bad <= 0).all(), (i, n, c, float(bad.max()))
+
+
+WIDE_CHUNKS, WIDE_CTX = [40, 150, 64, 1], [900, 150, 64, 700]
+
+
+@pytest.mark.parametrize(("dtype", "hq", "hkv", "d"), [(BF, 8, 2, 128), (FH, 8, 2, 128), (FH, 4, 4, 64)])
+@pytest.mark.parametrize("kind", ["blocks", "rows", "outlier", "growing", "zeros"])
+def test_prefill_of_value_rows_over_many_binades(cuda_device, dtype, hq, hkv, d, kind) -> None:  # type: ignore[no-untyped-def]
+    """Blocks of 32 tokens and single rows of magnitudes 2^+-20, a row 2^24 times larger than all
+    others whose softmax weight is nothing, magnitudes that grow along the context, runs of zeros."""
+    gen = torch.Generator(device=cuda_device).manual_seed(31)
+    nb, tab = tables_for(WIDE_CTX, 16, gen)
+    cache = make_cache(gen, nb, hkv, 16, d)
+    kp, vp, ks, vs = cache
+    q = torch.randn(sum(WIDE_CHUNKS), hq, d, generator=gen, device=cuda_device).abs().to(dtype)
+    wide = lambda *s: torch.exp2(torch.randint(-20, 21, s, generator=gen,  # noqa: E731
+                                               device=cuda_device).float())  # fmt: skip
+    for i, c in enumerate(WIDE_CTX):
+        blocks = tab[i, : -(-c // 16)].long()
+        if kind == "blocks":
+            vs[blocks] *= wide(len(blocks) // 2 + 1, 1, 1).repeat_interleave(2, 0)[: len(blocks)]
+        elif kind == "rows":
+            vs[blocks] *= wide(*vs[blocks].shape)
+        elif kind == "growing":
+            vs[blocks] *= torch.exp2(torch.arange(len(blocks), device=cuda_device) - 20.0)[:, None, None]
+        elif kind == "zeros":
+            zero_rows(cache, tab, i, [range(0), range(96), range(20, 40), range(650)][i], keys=i == 1)
+        else:  # codes of K all negative, q positive: a score of about -100
+            blk = blocks[len(blocks) // 3]
+            kp.view(torch.uint8)[blk, :, 5] = 0xF0
+            ks[blk, :, 5] = 0.03
+            vs[blk, :, 5] *= 2.0**24
+    qsl = torch.tensor([0, *WIDE_CHUNKS], device=cuda_device).cumsum(0).to(torch.int32)
+    ctx = torch.tensor(WIDE_CTX, dtype=torch.int32, device=cuda_device)
+    out = prefill(q, cache, tab, qsl, ctx, max(WIDE_CHUNKS))
+    check_prefill_wide(out, q, cache, tab, WIDE_CHUNKS, WIDE_CTX)

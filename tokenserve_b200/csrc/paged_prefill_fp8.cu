@@ -11,29 +11,35 @@
 //     each row's factor and the span's references, left in shared memory.
 //   * warps 8-11, 14, 15 (converters) take the blocks of 64-token tiles (4 of K, 4 of V) in turn: codes from
 //     global memory two blocks ahead into registers, times the row's factor, as fp16 into the
-//     swizzled layout the MMAs read. Values are relative to the span's largest scale (K) or the
-//     largest so far (V) times 2^-7, so they fill fp16's range whatever their magnitude; a factor
-//     is two fp16 parts, so a value is rounded once, to 2^-11 of itself. K's reference is a factor
-//     on the tile's scores; when V's grows, O is rescaled.
+//     swizzled layout the MMAs read. K's values are relative to the span's largest scale, V's to the
+//     largest of their 32 tokens (as a power of two), so the largest fill fp16's range; a factor is
+//     two fp16 parts, so a value is off by 2^-11 of itself, or by 2^-31 of the largest value in the
+//     span (K) or the 32 tokens (V, whose reference is 2^-60 of the largest so far at least): rows
+//     whose scale is less than 2^-20 of the reference lose bits. K's reference is a factor on the
+//     tile's scores, V's is added to the exponent of the 32 tokens' weights.
 //   * warps 0-3 / 4-7 (softmax, one warpgroup per query tile, thread = row): q's row is scaled by a
 //     power of two into fp16's range and written to shared memory; then per tile, 32 columns at a
-//     time: 2^(s - m), P in fp16 (11 bits) back to TMEM over S, sums in fp32. m is the maximum of
-//     the row's first tile and is kept while no score exceeds it by 2^14, so the exponentials wait
+//     time: 2^(t - mt) with t = s + log2(V's reference), P in fp16 (11 bits) back to TMEM over S. The
+//     sum of 2^(s - m) is theirs times one factor per 32 columns, in fp32. mt is the maximum of
+//     the row's first tile and is kept while no t exceeds it by 2^14, so the exponentials wait
 //     for no maximum; a warp with a row past that takes the columns, and all before them, to the
-//     new maximum. Columns no row of a warp sees are skipped. Everything is in loops over few columns: unrolled over a
-//     whole row, the roles' code outgrew the instruction caches (a quarter of the stalls).
+//     new maximum. The output is O 2^(mt - m) / sum. Columns no row of a warp sees are skipped.
+//     Everything is in loops over few columns: unrolled over a whole row, the roles' code outgrew
+//     the instruction caches (a quarter of the stalls).
 //   * warp 13: tcgen05.mma, S_x = Q_x K^T and O_x += P_x V, in the order PV_A(j), QK_A(j+2),
 //     PV_B(j), QK_B(j+2): each query tile has two S buffers of 64 columns, so its softmax finds the
 //     next tile's scores ready and waits for no MMA (with one buffer of 128 columns a tile's
 //     softmax, PV and QK took turns: 5,000 clocks per 128 tokens).
-// 64 sequences of 257-512 new tokens over 900-1,600 cached ones, 32/8 heads of 128: 861 us, 666 TFLOP/s
-// (0.41 of cuBLAS bf16); tensor pipe 44%, issue slots 57% busy: what binds is the way of a tile's
+// 64 sequences of 257-512 new tokens over 900-1,600 cached ones, 32/8 heads of 128: 846 us, 678 TFLOP/s
+// (0.42 of cuBLAS bf16); tensor pipe 44%, issue slots 57% busy: what binds is the way of a tile's
 // scores through softmax and MMAs and back. Without the exponentials 832 us, without the
 // conversion 807 us, without both 653 us (of 888 us then).
 // A page outside the pool is skipped (its columns are masked). A V row with a NaN scale is stored
 // as zeros and its column's weight set to NaN for the rows that see it, so rows before it in the
 // chunk stay clean. Tokens past the last visible key are stored as zeros: their slots may hold
 // anything. Other shapes and fp32 queries run on CUDA cores (attention_portable.cu).
+#include <cstddef>
+
 #include "fp8.cuh"
 #include "tcgen05.cuh"
 
@@ -66,7 +72,7 @@ constexpr int kThreads = 512;
 constexpr int kMaxTries = 1 << 22, kMaxNaps = 1 << 22;  // of a bounded wait
 constexpr uint32_t kDropped = 0x80008000u;  // factor of a row whose codes are not used
 constexpr float kLog2e = 1.4426950408889634f;
-// A stale row max is kept unless exceeded by 2^14: P stays below fp16's 2^16, and weights near the
+// A stale maximum is kept unless exceeded by 2^14: P stays below fp16's 2^16, and weights near the
 // true maximum, at least 1, well inside its normal range.
 constexpr float kRescaleSlack = 14.f;
 // One of so many column pairs takes its 2^x from the FMA pipe (64 sequences of 512 new tokens: none
@@ -74,9 +80,11 @@ constexpr float kRescaleSlack = 14.f;
 constexpr int kFmaEvery = 8;
 // S_A [0,128) and S_B [128,256), two buffers each, O_A [256,384), O_B [384,512).
 constexpr uint32_t kTmemCols = 512;
-constexpr float kRefScale = 128.f;    // fp16 values are code * scale / ref * 128 <= 57344
-// V's reference starts, and grows, to this times the scales seen, so that it seldom grows.
-constexpr float kRefRoom = 8.f;
+constexpr float kRefScale = 128.f;    // K's fp16 values are code * scale / ref * 128 <= 57344
+constexpr int kRefLog = 6;  // V's are code * scale * 2^(6 - n) < 57344, 2^n <= the largest scale
+// V's n stays within this of the context's largest so far: a weight's exponent t - mt is then above
+// fp32's -126 wherever 2^(s - m) is above 2^-52, so the weights' sums give the softmax's sum.
+constexpr int kRefSpread = 60;
 
 struct Args {
   void* out;
@@ -97,16 +105,20 @@ struct Args {
   float scale_log2;
 };
 
-// A span as the scout leaves it: references of K and V, the columns to mask (page outside the
-// pool) or to spoil (V row NaN), if any; the blocks (negative: none); each row's factor for K and
-// for V, fp16 high and low part, or kDropped.
+// A span as the scout leaves it: references of K and, as n, of each 32 rows of V; the columns to
+// mask (page outside the pool) or to spoil (V row NaN), if any; the blocks (negative: none); each
+// row's factor for K and for V, fp16 high and low part, or kDropped.
 struct alignas(16) TileInfo {
-  float ref_k, ref_v;
+  float ref_k;
   uint32_t any, dropped;  // dropped: bit 0, 1: K, V has rows of factor kDropped
+  float log_v[4];
   uint32_t skip[4], spoil[4];
   int block[kSpan / kBlock];
-  uint32_t factor[2][kSpan];
+  alignas(16) uint32_t factor[2][kSpan];  // written 16 bytes at a time
 };
+static_assert(offsetof(TileInfo, factor) % 16 == 0 && sizeof(TileInfo) % 16 == 0 &&
+                  offsetof(TileInfo, any) == 4,
+              "vector accesses of a description");
 
 struct Shared {
   uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
@@ -117,11 +129,11 @@ struct Shared {
   int abort;
 };
 
-// ref_k, ref_v, any and dropped of a description in one load.
-__device__ __forceinline__ float4 load_refs(const volatile TileInfo* info) {
-  float4 v;
-  asm volatile("ld.volatile.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+// ref_k and any of a description in one load.
+__device__ __forceinline__ float2 load_refs(const volatile TileInfo* info) {
+  float2 v;
+  asm volatile("ld.volatile.shared.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
                : "r"(ts::smem_u32(const_cast<const TileInfo*>(info))));
   return v;
 }
@@ -255,12 +267,11 @@ __device__ __forceinline__ uint32_t split_factor(float f) {
   return uint32_t(__half_as_ushort(hi)) | (uint32_t(__half_as_ushort(lo)) << 16);
 }
 
-// Largest finite value of the warp's 128 scales.
-__device__ __forceinline__ float top(const float (&sc)[4]) {
+// Bits of the largest finite value of four scales; scales are not negative and order like their bits.
+__device__ __forceinline__ uint32_t top_bits(const float (&sc)[4]) {
   auto fin = [](float v) { return isfinite(v) ? v : 0.f; };
   const float m = fmaxf(fmaxf(fin(sc[0]), fin(sc[1])), fmaxf(fin(sc[2]), fin(sc[3])));
-  // Not negative, so they order like their bits.
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(m, 0.f))));
+  return __float_as_uint(fmaxf(m, 0.f));
 }
 
 // The scout warp: describes the spans of a KV head's keys, n_kv of them visible. Lane l looks after
@@ -294,7 +305,7 @@ struct Scout {
 
   __device__ __forceinline__ void run(Shared* sh, volatile int* abort) {
     const int spans = (n_kv + kSpan - 1) / kSpan;
-    float run_v = 0x1p-126f;  // V's reference: never below the scales seen
+    int run_n = -127;  // exponent of the largest V scale so far
 #pragma unroll 1
     for (int t = 0; t < spans; ++t) {
       const int next = look_up(t + 1);
@@ -311,19 +322,26 @@ struct Scout {
       if (t >= kAhead && !wait_ahead(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1, abort))
         return;
       TileInfo* info = &sh->info[t % kInfos];
-      const float ref_k = fmaxf(top(k), 0x1p-126f), top_v = top(v);
-      if (top_v > run_v) run_v = fminf(top_v * kRefRoom, 0x1p127f);
-      const float inv_k = 1.f / ref_k, inv_v = 1.f / run_v;
+      const float ref_k = fmaxf(
+          __uint_as_float(__reduce_max_sync(0xffffffffu, top_bits(k))), 0x1p-126f);
+      // n of the lane's 32 tokens (8 lanes).
+      int n = int(top_bits(v) >> 23) - 127;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) n = max(n, __shfl_xor_sync(0xffffffffu, n, o));
+      run_n = max(run_n, __reduce_max_sync(0xffffffffu, n));
+      n = max(n, max(run_n - kRefSpread, -120));  // 2^(6 - n) stays finite
+      const float inv_k = 1.f / ref_k, up_v = __uint_as_float(uint32_t(127 + kRefLog - n) << 23);
       // A NaN K row makes NaN scores; a NaN V row is stored as zeros (see the head of the file).
       uint32_t fk[4], fv[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         fk[i] = i < reach ? split_factor(k[i] * inv_k * kRefScale) : kDropped;
-        fv[i] = i < reach && !(spoil >> i & 1) ? split_factor(v[i] * inv_v * kRefScale) : kDropped;
+        fv[i] = i < reach && !(spoil >> i & 1) ? split_factor(v[i] * up_v) : kDropped;
       }
       *reinterpret_cast<uint4*>(&info->factor[0][4 * lane]) = make_uint4(fk[0], fk[1], fk[2], fk[3]);
       *reinterpret_cast<uint4*>(&info->factor[1][4 * lane]) = make_uint4(fv[0], fv[1], fv[2], fv[3]);
       if (lane % 4 == 0) info->block[lane / 4] = phys;
+      if (lane % 8 == 0) info->log_v[lane / 8] = float(n);
       const bool any = __any_sync(0xffffffffu, spoil != 0 || k_odd || phys == -2);
       const bool past = __any_sync(0xffffffffu, reach < 4);
       if (any) {
@@ -343,7 +361,6 @@ struct Scout {
       }
       if (lane == 0) {
         info->ref_k = ref_k;
-        info->ref_v = run_v;
         info->any = any;
         info->dropped = uint32_t(past) | uint32_t(past || any) << 1;
       }
@@ -655,7 +672,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
 
     const int pos_max = __reduce_max_sync(0xffffffffu, pos);
     const int pos_min = __reduce_min_sync(0xffffffffu, pos);
-    float m_run = -INFINITY, l_run = 0.f, ref_v = 0.f;
+    // Maximum that the weights and O are relative to, the one of the sum, the sum.
+    float t_run = -INFINITY, m_run = -INFINITY, l_run = 0.f;
     bool saw_nan = false;  // a row of K or V that holds one (not every exponential below keeps it)
     bool ok = true;
     for (int j = 0; j < n_x; ++j) {
@@ -670,13 +688,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       constexpr int kGroups = kKvTile / 32;  // of 32 columns
       const volatile TileInfo* info = &sh->info[j / kTilesPerSpan % kInfos];
       const int word = j % kTilesPerSpan * kGroups;  // of the span's column masks
-      const float4 refs = load_refs(info);
+      const float2 refs = load_refs(info);
       const float slj = fmaxf(sl * refs.x, 0x1p-126f);  // > 0, so that -inf stays -inf
-      // O is in units of V's reference: it shrinks when that grows.
-      const float ref_old = ref_v;
-      ref_v = refs.y;
-      const bool odd_columns = __float_as_uint(refs.z) != 0;
-      float corr_o = ref_v != ref_old && j > 0 ? ref_old / ref_v : 1.f;
+      const bool odd_columns = __float_as_uint(refs.y) != 0;
+      float corr_o = 1.f;  // of O, when the weights' maximum moves
       const int limit = pos - j * kKvTile;  // columns c <= limit are visible
       // Column groups of 32 that some row of the warp sees, and those every row sees whole.
       const int n_some = min(kGroups, max(0, pos_max - j * kKvTile + 32) / 32);
@@ -692,26 +707,29 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           else if (spoil >> k & 1 || isnan(__uint_as_float(r[k]))) saw_nan = true;
         }
       };
-      if (__any_sync(0xffffffffu, m_run == -INFINITY)) {  // a row that has seen nothing yet
-        float m = -INFINITY;
+      if (__any_sync(0xffffffffu, t_run == -INFINITY)) {  // a row that has seen nothing yet
+        float m = -INFINITY, mt = -INFINITY;
 #pragma unroll 1
         for (int c = 0; c < n_some; ++c) {
           ts::tc::wait_ld(sa);
           if (c >= n_whole) mask(sa, c);
-          m = fmaxf(m, max32(sa));
+          const float s = max32(sa) * slj;
+          m = fmaxf(m, s);
+          mt = fmaxf(mt, s + info->log_v[word + c]);
           ts::tc::tmem_ld32(lane_base + s_col + (c + 1 < n_some ? c + 1 : 0) * 32, sa);
         }
-        if (m_run == -INFINITY) m_run = m * slj;
+        if (t_run == -INFINITY) m_run = m, t_run = mt;
       }
       const uint64_t slj2 = two(slj, slj);
-      float less = m_run == -INFINITY ? 0.f : -m_run;
-      uint64_t less2 = two(less, less), sum2 = two(0.f, 0.f);
       // P of columns 32 c .. 32 c + 31. Masked columns, and a warp whose maximum moves, run their own
       // copies of the code: where the paths met again, the registers of a whole row were copied.
       auto columns = [&](int c, auto masked) {
+        const float log_v = info->log_v[word + c];
+        const float less = t_run == -INFINITY ? 0.f : log_v - t_run;
+        const uint64_t less2 = two(less, less);
         ts::tc::wait_ld(sa);
         if (masked) mask(sa, c);
-        uint64_t e[16];  // log2 of P, two columns each
+        uint64_t e[16], sum2 = two(0.f, 0.f);  // log2 of P, two columns each; their sum
 #pragma unroll
         for (int k = 0; k < 16; ++k) e[k] = fma2(two(sa[2 * k], sa[2 * k + 1]), slj2, less2);
         if (c + 1 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 1) * 32, sa);
@@ -732,17 +750,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
             pw[k] = pack_half2(v.x, v.y);
           }
           ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
+          // From the weights' maximum and reference to the sum's; nothing seen: 0.
+          const float2 sum = halves(sum2);
+          l_run += (sum.x + sum.y) * (t_run == -INFINITY ? 0.f : ex2(-less - m_run));
           return;
         }
         const float up = over > kRescaleSlack ? over : 0.f, f = ex2(-up);
-        m_run += up;
-        less -= up;
-        less2 = two(less, less);
-        l_run *= f;
+        t_run += up;
         corr_o *= f;
-        float2 sum = halves(sum2);
-        sum.x *= f;
-        sum.y *= f;
+        if (up > 0.f && t_run - log_v > m_run) {
+          l_run *= ex2(m_run - (t_run - log_v));
+          m_run = t_run - log_v;
+        }
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll 1
         for (int b = 0; b < c; ++b) {  // the tile's P so far
           uint32_t pw[16];
@@ -765,8 +785,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           sum.y += v.y;
           pw[k] = pack_half2(v.x, v.y);
         }
-        sum2 = two(sum.x, sum.y);
         ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
+        l_run += (sum.x + sum.y) * (t_run == -INFINITY ? 0.f : ex2(up - less - m_run));
       };
 #pragma unroll 1
       for (int c = 0; c < min(n_whole, n_some); ++c) columns(c, std::false_type{});
@@ -778,8 +798,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         uint32_t pw[16] = {};
         ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
       }
-      const float2 sums = halves(sum2);
-      l_run += sums.x + sums.y;
       if (j > 0 && __any_sync(0xffffffffu, corr_o != 1.f)) {
         // O holds the tiles up to j - 1 (up to j - 2 it does since S of tile j was ready).
         if (!wait_warp(&sh->pv_done[x], (j - 1) & 1, abort)) {
@@ -805,9 +823,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     if (ok && n_x > 0) ok = wait_warp(&sh->o_full[x], 0, abort);
     ts::tc::fence_after_sync();
     if (ok && x < a.q_tiles) {
-      // A row that saw nothing has a sum of a few 2^-126 at most, and O = 0.
-      float inv = l_run > 0x1p-100f ? ref_v / (kRefScale * l_run) : l_run;
-      if (saw_nan) inv = __uint_as_float(0x7fc00000u);
+      // A row that saw nothing has a sum of 0, and O = 0. An infinite score makes NaNs.
+      float inv = l_run > 0.f ? ex2(t_run - m_run) * (1.f / float(1 << kRefLog)) / l_run : l_run;
+      if (saw_nan || m_run == INFINITY) inv = __uint_as_float(0x7fc00000u);
       // The row goes to the warp's part of its Q tile (no MMA reads it any more), 16 bytes at a
       // time in swizzled places, and from there to memory in whole rows.
       uint8_t* stage = sQ(x) + (warp & 3) * 32 * D * 2;
