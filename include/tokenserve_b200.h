@@ -441,7 +441,9 @@ int ts_paged_decode_fp8(void* out, const void* query, int64_t query_token_stride
 /*
  * ts_paged_prefill over an 8-bit cache (the chunk's rows already written). Arguments as there.
  * A query row whose position is negative (context shorter than the chunk) sees nothing and gets
- * zeros; rows of no sequence are left as they were.
+ * zeros; rows of no sequence are left as they were. Waits inside the kernel are bounded (about a
+ * second); rows of a tile that gave up are NaN. A block outside the pool is skipped, as in
+ * ts_paged_prefill.
  *
  * Replaces: the same eager attention as ts_paged_prefill (src/tokenserve/backends/hf.py:62-71).
  */

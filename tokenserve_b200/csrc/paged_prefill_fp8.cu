@@ -30,7 +30,7 @@
 //     PV_B(j), QK_B(j+2): each query tile has two S buffers of 64 columns, so its softmax finds the
 //     next tile's scores ready and waits for no MMA (with one buffer of 128 columns a tile's
 //     softmax, PV and QK took turns: 5,000 clocks per 128 tokens).
-// 64 sequences of 257-512 new tokens over 900-1,600 cached ones, 32/8 heads of 128: 846 us, 678 TFLOP/s
+// 64 sequences of 257-512 new tokens over 900-1,600 cached ones, 32/8 heads of 128: 841 us, 682 TFLOP/s
 // (0.42 of cuBLAS bf16); tensor pipe 44%, issue slots 57% busy: what binds is the way of a tile's
 // scores through softmax and MMAs and back. Without the exponentials 832 us, without the
 // conversion 807 us, without both 653 us (of 888 us then).
@@ -126,7 +126,6 @@ struct Shared {
   uint64_t info_full[kInfos], converted[kAhead];
   TileInfo info[kInfos];
   uint32_t tmem;
-  int abort;
 };
 
 // ref_k and any of a description in one load.
@@ -145,9 +144,10 @@ struct Geo {
   static constexpr int kSmemBytes = kTiles + int(sizeof(Shared)) + 1024;
 };
 
-// Bounded wait (a try sleeps for some time, so the tries last about a second); sets *abort when it
-// gives up. A loop of few instructions: there are many waits, and all roles share the caches.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, volatile int* abort) {
+// Bounded wait (a try sleeps for some time, so the tries last about a second), false when it gives up:
+// the waits of the roles that depend on this one give up in turn, and the rows become NaN. A loop of
+// few instructions: there are many waits, and all roles share the caches.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase) {
   uint32_t ok;
   // Four tries a turn of the loop: two instructions a try instead of six.
   asm volatile(
@@ -169,23 +169,21 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, volatile
       : "=r"(ok)
       : "r"(ts::smem_u32(bar)), "r"(phase), "n"(kMaxTries / 4)
       : "memory");
-  if (!ok) *abort = 1;
   return ok != 0;
 }
 // For the warps that run ahead: naps between tries leave the issue slots to the others.
-__device__ __forceinline__ bool wait_ahead(uint64_t* bar, uint32_t phase, volatile int* abort) {
+__device__ __forceinline__ bool wait_ahead(uint64_t* bar, uint32_t phase) {
   bool ok = ts::mbar_try_wait(bar, phase);
 #pragma unroll 1
   for (int i = 0; !ok && i < kMaxNaps; ++i) {
     __nanosleep(100);
     ok = ts::mbar_try_wait(bar, phase);
   }
-  if (!ok) *abort = 1;
   return __all_sync(0xffffffffu, ok);
 }
 // The same for a whole warp, with one answer.
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase, volatile int* abort) {
-  return __all_sync(0xffffffffu, wait_bar(bar, phase, abort));
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase) {
+  return __all_sync(0xffffffffu, wait_bar(bar, phase));
 }
 
 __device__ __forceinline__ float max3f(float a, float b, float c) {
@@ -303,7 +301,7 @@ struct Scout {
     }
   }
 
-  __device__ __forceinline__ void run(Shared* sh, volatile int* abort) {
+  __device__ __forceinline__ void run(Shared* sh) {
     const int spans = (n_kv + kSpan - 1) / kSpan;
     int run_n = -127;  // exponent of the largest V scale so far
 #pragma unroll 1
@@ -319,7 +317,7 @@ struct Scout {
         k_odd |= !isfinite(k[i]);
         if (!isfinite(v[i])) spoil |= 1u << i;
       }
-      if (t >= kAhead && !wait_ahead(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1, abort))
+      if (t >= kAhead && !wait_ahead(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1))
         return;
       TileInfo* info = &sh->info[t % kInfos];
       const float ref_k = fmaxf(
@@ -446,7 +444,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
   auto sK = [&](int st) { return smem + kQTiles * G::kQBytes + st * G::kKvBytes; };
   auto sV = [&](int st) { return sK(kStages + st); };
   Shared* sh = reinterpret_cast<Shared*>(smem + G::kTiles);
-  volatile int* abort = &sh->abort;
 
   // Through a shuffle, so that the compiler knows a role's control flow to be uniform.
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -498,7 +495,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       ts::mbar_init(&sh->o_full[x], 1);
     }
     ts::mbar_init(&sh->drain, 1);
-    sh->abort = 0;
     ts::fence_mbar_init();
   }
   if (warp == 13) {
@@ -512,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
 
   if (warp >= 8) {
     if (warp == 12) {
-      scout.run(sh, abort);
+      scout.run(sh);
     } else if (warp != 13) {
       // ---------------------------------------------------------- converters
       const int total = n_max * kUnits;
@@ -521,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       auto fetch = [&](Codes<D>& c, int u) -> bool {
         if (u >= total) return true;
         const int j = u / kUnits, k = u % kUnits, t = j / kTilesPerSpan;
-        if (!wait_ahead(&sh->info_full[t % kInfos], (t / kInfos) & 1, abort)) return false;
+        if (!wait_ahead(&sh->info_full[t % kInfos], (t / kInfos) & 1)) return false;
         const int phys =
             sh->info[t % kInfos].block[j % kTilesPerSpan * (kUnits / 2) + k % (kUnits / 2)];
         const uint8_t* pool = (k < kUnits / 2 ? a.key_pool : a.value_pool) + h * kBlock * D;
@@ -532,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         const int j = u / kUnits, k = u % kUnits, st = j % kStages, t = j / kTilesPerSpan;
         const bool is_v = k >= kUnits / 2;
         if (j >= kStages && !wait_ahead(is_v ? &sh->v_empty[st] : &sh->k_empty[st],
-                                       ((j - kStages) / kStages) & 1, abort))
+                                       ((j - kStages) / kStages) & 1))
           return false;
         const TileInfo& info = sh->info[t % kInfos];
         const int row0 = k % (kUnits / 2) * kBlock;
@@ -566,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       const uint32_t v_lo = ts::smem_u32(sV(0)) >> 4 | uint32_t(kKvHalf >> 4) << 16;
       // The last query tile to use KV tile j releases its K (after QK) and V (after PV).
       auto last_user = [&](int j) { return j < n_t[1] ? 1 : 0; };
-      bool ok = wait_warp(&sh->q_full, 0, abort);
+      bool ok = wait_warp(&sh->q_full, 0);
       // Step i: PV(i - 2) then QK(i), of each query tile in turn.
 #pragma unroll 1
       for (int i = 0; ok && i < n_max + 2; ++i) {
@@ -578,8 +574,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           if (j >= 0 && j < n_x) {
             // The first query tile has waited for this V already (and below for this K): a wait
             // costs a hundred clocks even then.
-            ok = ((x == 1 && j < n_t[0]) || wait_warp(&sh->v_full[sv], (j / kStages) & 1, abort)) &&
-                 wait_warp(&sh->p_full[x][b], (j / 2) & 1, abort);
+            ok = ((x == 1 && j < n_t[0]) || wait_warp(&sh->v_full[sv], (j / kStages) & 1)) &&
+                 wait_warp(&sh->p_full[x][b], (j / 2) & 1);
             if (!ok) break;
             ts::tc::fence_after_sync();
             const uint32_t dv = v_lo + sv * (G::kKvBytes >> 4);
@@ -591,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
             if (x == last_user(j) && j + kStages < n_max) ts::tc::commit_elect(&sh->v_empty[sv]);
           }
           if (i < n_x) {
-            ok = (x == 1 && i < n_t[0]) || wait_warp(&sh->k_full[sk], (i / kStages) & 1, abort);
+            ok = (x == 1 && i < n_t[0]) || wait_warp(&sh->k_full[sk], (i / kStages) & 1);
             if (!ok) break;
             ts::tc::fence_after_sync();
             const uint32_t dq = q_lo + x * (G::kQBytes >> 4);
@@ -677,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     bool saw_nan = false;  // a row of K or V that holds one (not every exponential below keeps it)
     bool ok = true;
     for (int j = 0; j < n_x; ++j) {
-      if (!wait_warp(&sh->s_full[x][j & 1], (j / 2) & 1, abort)) {
+      if (!wait_warp(&sh->s_full[x][j & 1], (j / 2) & 1)) {
         ok = false;
         break;
       }
@@ -800,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       }
       if (j > 0 && __any_sync(0xffffffffu, corr_o != 1.f)) {
         // O holds the tiles up to j - 1 (up to j - 2 it does since S of tile j was ready).
-        if (!wait_warp(&sh->pv_done[x], (j - 1) & 1, abort)) {
+        if (!wait_warp(&sh->pv_done[x], (j - 1) & 1)) {
           ok = false;
           break;
         }
@@ -820,9 +816,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       __syncwarp();
       if (lane == 0) ts::mbar_arrive(&sh->p_full[x][j & 1]);
     }
-    if (ok && n_x > 0) ok = wait_warp(&sh->o_full[x], 0, abort);
+    if (ok && n_x > 0) ok = wait_warp(&sh->o_full[x], 0);
+    if (!ok) m_run = INFINITY;  // a wait gave up: the rows become NaN below, whatever O holds
     ts::tc::fence_after_sync();
-    if (ok && x < a.q_tiles) {
+    if (x < a.q_tiles) {
       // A row that saw nothing has a sum of 0, and O = 0. An infinite score makes NaNs.
       float inv = l_run > 0.f ? ex2(t_run - m_run) * (1.f / float(1 << kRefLog)) / l_run : l_run;
       if (saw_nan || m_run == INFINITY) inv = __uint_as_float(0x7fc00000u);
