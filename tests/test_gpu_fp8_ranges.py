@@ -198,3 +198,30 @@ def test_prefill_of_value_rows_over_many_binades(cuda_device, dtype, hq, hkv, d,
     ctx = torch.tensor(WIDE_CTX, dtype=torch.int32, device=cuda_device)
     out = prefill(q, cache, tab, qsl, ctx, max(WIDE_CHUNKS))
     check_prefill_wide(out, q, cache, tab, WIDE_CHUNKS, WIDE_CTX)
+
+
+@pytest.mark.parametrize("which", ["key", "value"])
+@pytest.mark.parametrize(("hq", "hkv", "d"), [(8, 1, 128), (16, 1, 64)])
+def test_decode_of_a_nan_row_wherever_it_stands(cuda_device, which, hq, hkv, d) -> None:  # type: ignore[no-untyped-def]
+    """The only token, the only one of a last block or of a last partition, all tokens of a context,
+    one in the middle of many partitions: the sequence's rows become NaN, the others stay clean."""
+    gen = torch.Generator(device=cuda_device).manual_seed(41)
+    lens = [1, 17, 65, 129, 400, 2049, 9000, 50]
+    bad = [range(1), range(16, 17), range(64, 65), range(129), range(399, 400), range(2048, 2049),
+           range(4444, 4445), range(0)]  # fmt: skip
+    nb, tab = tables_for(lens, 16, gen)
+    cache = make_cache(gen, nb, hkv, 16, d)
+    for i, rows in enumerate(bad):
+        for p in rows:
+            for pool, sc in (((cache[0], cache[2]) if which == "key" else (cache[1], cache[3])),):
+                pool.view(torch.uint8)[int(tab[i, p // 16]), :, p % 16] = 0x7F
+                sc[int(tab[i, p // 16]), :, p % 16] = float("nan")
+    q = torch.randn(len(lens), hq, d, generator=gen, device=cuda_device).to(BF)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    out = decode(q, cache, tab, ctx)
+    assert torch.isnan(out[:-1]).all()
+    check_decode(out[-1:], q[-1:], cache, tab[-1:], lens[-1:])
+    qsl = torch.arange(len(lens) + 1, dtype=torch.int32, device=cuda_device)
+    out = prefill(q, cache, tab, qsl, ctx, 1)
+    assert torch.isnan(out[:-1]).all()
+    check_prefill(out[-1:], q[-1:], cache, tab[-1:], [1], lens[-1:])

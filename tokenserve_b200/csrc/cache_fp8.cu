@@ -11,8 +11,8 @@
 // half-layout rotary partner comes from another lane of the row instead of a second load. A thread
 // has the vectors of four rows in flight, and no 64-bit division stands before them. Rows that do
 // not split that way (odd sizes or alignment) take a warp per row with scalar accesses. Measured with
-// heads of 128: append of 32,768 tokens x 8 bf16 heads 41 us (0.76 of the copy rate), rotary + append
-// of 16,381 tokens of 32/8 heads 69 us (0.82), reading 64 ragged contexts back 87 us (0.84).
+// heads of 128: append of 32,768 tokens x 8 bf16 heads 38 us (0.83 of the copy rate), rotary + append
+// of 16,381 tokens of 32/8 heads 72 us (0.78), reading 64 ragged contexts back 87 us (0.84).
 #include "fp8.cuh"
 
 namespace {
@@ -58,49 +58,34 @@ int log2_or_minus_one(int n) {
 
 constexpr int kInFlight = 4;  // rows of a thread at a time
 
-// Pairs of floats and the packed fp32 instructions on them.
-__device__ __forceinline__ uint64_t two(float a, float b) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  return v;
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 __device__ __forceinline__ void flag(int32_t* error_flag) {
   if (error_flag != nullptr) atomicExch(error_flag, 1);
 }
 
 // One lane's E values of a row -> E codes at row + c * E, the scale from the row's first lane; with
 // VPL > 1 the lane has E / VPL values of each of VPL parts of the row. Every lane of the warp takes
-// part (shuffles); `live` rows are stored.
-template <int E, int LPR, int VPL = 1>
+// part (shuffles); `live` rows are stored. BRANCH: rows of a small scale have code of their own
+// (append 37.7 us, 42.8 without; rotary + append 72.3 without, 73.5 with).
+template <int E, int LPR, int VPL, bool BRANCH>
 __device__ __forceinline__ void store_row_fp8(const float (&x)[E], int c, bool live, uint8_t* row,
                                               float* scale) {
   float m = ts::amax3(x[0], x[1], x[2]);
 #pragma unroll
   for (int e = 3; e < E; e += 2) m = ts::amax3(m, x[e], x[e + 1 < E ? e + 1 : e]);
-  float inv;
-  const float sc = ts::fp8_row_scale(row_max<LPR>(__float_as_uint(m)), inv);
+  const float sc = ts::fp8_row_scale(row_max<LPR>(__float_as_uint(m)));
+  const ts::Fp8Divide by(sc);
   constexpr int P = E / VPL;
   Words<P / 4> w[VPL];
+  if (BRANCH && !by.small()) {
 #pragma unroll
-  for (int i = 0; i < E / 4; ++i)
-    w[i / (P / 4)].w[i % (P / 4)] =
-        ts::fp8_pack4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], inv);
+    for (int i = 0; i < E / 4; ++i)
+      w[i / (P / 4)].w[i % (P / 4)] = by.pack4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i)
+      w[i / (P / 4)].w[i % (P / 4)] = by.pack4(x[4 * i] * by.up, x[4 * i + 1] * by.up,
+                                               x[4 * i + 2] * by.up, x[4 * i + 3] * by.up);
+  }
   if (live) {
 #pragma unroll
     for (int q = 0; q < VPL; ++q)
@@ -185,7 +170,7 @@ __global__ void __launch_bounds__(256) append_fp8_kernel(const AppendArgs a) {
     const Place at(live ? slot[i] : 0, a.block_size, a.block_shift);
     const uint32_t prow =
         (uint32_t(at.block) * a.heads + (is_v ? r[i] - a.heads : r[i])) * a.block_size + at.off;
-    store_row_fp8<E * VPL, LPR, VPL>(x, c, live,
+    store_row_fp8<E * VPL, LPR, VPL, true>(x, c, live,
                                      (is_v ? a.value_pool : a.key_pool) + uint64_t(prow) * D,
                                      (is_v ? a.value_scales : a.key_scales) + prow);
   }
@@ -210,13 +195,12 @@ __global__ void __launch_bounds__(256) append_fp8_any_kernel(const AppendArgs a)
                    t * (is_v ? a.value_stride : a.key_stride) + int64_t(h) * a.d;
     uint32_t m = 0;
     for (int i = lane; i < a.d; i += 32) m = max(m, ts::abs_bits(ts::to_float(src[i])));
-    float inv;
-    const float sc = ts::fp8_row_scale(row_max<32>(m), inv);
+    const float sc = ts::fp8_row_scale(row_max<32>(m));
+    const ts::Fp8Divide by(sc);
     const int64_t blk = slot / a.block_size;
     const int64_t prow = (blk * a.heads + h) * a.block_size + slot - blk * a.block_size;
     uint8_t* dst = (is_v ? a.value_pool : a.key_pool) + prow * a.d;
-    for (int i = lane; i < a.d; i += 32)
-      dst[i] = uint8_t(ts::fp8_pack4(ts::to_float(src[i]), 0.f, 0.f, 0.f, inv));
+    for (int i = lane; i < a.d; i += 32) dst[i] = by.one(ts::to_float(src[i]));
     if (lane == 0) (is_v ? a.value_scales : a.key_scales)[prow] = sc;
   }
 }
@@ -343,8 +327,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
       v2 = cs[j + 1];
       if (first) u.y = -u.y, v2.y = -v2.y;
     }
-    wc[e / 2] = two(u.x, v2.x);
-    ws[e / 2] = two(u.y, v2.y);
+    wc[e / 2] = ts::two(u.x, v2.x);
+    ws[e / 2] = ts::two(u.y, v2.y);
   }
   const int partner = ((threadIdx.x % 32) + (first ? hl : (turned ? -hl : 0))) & 31;
   // Where the token's rows go: head h at base + h * step.
@@ -371,7 +355,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
         const float x0 = ts::to_float(v[i].v[e]), x1 = ts::to_float(v[i].v[e + 1]);
         const float y0 = ts::to_float(o.v[INTERLEAVED ? e + 1 : e]);
         const float y1 = ts::to_float(o.v[INTERLEAVED ? e : e + 1]);
-        const float2 z = halves(fma2(two(y0, y1), ws[e / 2], mul2(two(x0, x1), wc[e / 2])));
+        const float2 z = ts::halves(
+            ts::fma2(ts::two(y0, y1), ws[e / 2], ts::mul2(ts::two(x0, x1), wc[e / 2])));
         x[e] = is_v || !turned ? x0 : z.x;
         x[e + 1] = is_v || !turned ? x1 : z.y;
       }
@@ -380,7 +365,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
       if (FP8) {
         // Rows of q only in this warp: nothing to quantise.
         if (__any_sync(0xffffffffu, !is_q))
-          store_row_fp8<E, LPR>(x, c, live && !is_q,
+          store_row_fp8<E, LPR, 1, false>(x, c, live && !is_q,
                                 static_cast<uint8_t*>(is_v ? a.value_pool : a.key_pool) + prow * D,
                                 (is_v ? a.value_scales : a.key_scales) + prow);
       }
@@ -435,11 +420,10 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryArgs a, int
     }
     uint32_t m = 0;
     for (int i = lane; i < a.d; i += 32) m = max(m, ts::abs_bits(value(i)));
-    float inv;
-    const float sc = ts::fp8_row_scale(row_max<32>(m), inv);
+    const float sc = ts::fp8_row_scale(row_max<32>(m));
+    const ts::Fp8Divide by(sc);
     uint8_t* dst = static_cast<uint8_t*>(is_v ? a.value_pool : a.key_pool) + prow * a.d;
-    for (int i = lane; i < a.d; i += 32)
-      dst[i] = uint8_t(ts::fp8_pack4(value(i), 0.f, 0.f, 0.f, inv));
+    for (int i = lane; i < a.d; i += 32) dst[i] = by.one(value(i));
     if (lane == 0) (is_v ? a.value_scales : a.key_scales)[prow] = sc;
   }
 }

@@ -27,23 +27,42 @@ __device__ __forceinline__ float amax3(float a, float b, float c) {
 }
 
 // Scale of a row whose largest |x| has these bits: amax / 448, correctly rounded (a product by the
-// reciprocal and one correction), and 1 / scale to an ulp.
-__device__ __forceinline__ float fp8_row_scale(uint32_t amax_bits, float& inv) {
+// reciprocal and one correction).
+__device__ __forceinline__ float fp8_row_scale(uint32_t amax_bits) {
   constexpr float kInv = 1.f / kE4m3Max;
   const float amax = __uint_as_float(amax_bits);
   float sc = amax * kInv;
   sc = fmaxf(fmaf(fmaf(-sc, kE4m3Max, amax), kInv, sc), 0x1p-126f);
   if (amax_bits >= 0x7f800000u) sc = __uint_as_float(0x7fc00000u);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sc));
   return sc;
 }
 
-// Four codes of x * inv (element 0 in the low byte), saturating; NaN stays NaN.
-__device__ __forceinline__ uint32_t fp8_pack4(float x0, float x1, float x2, float x3, float inv) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x0 * inv, x1 * inv), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x2 * inv, x3 * inv), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
+// Divides a row by its scale. With y = 1 / scale correctly rounded and q = x y, q + (x - q scale) y is
+// x / scale correctly rounded (P. Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990), where the residual is exact: codes come from quotients above
+// 2^-11, so scales above 2^-90 leave it 2^-124 and more. A smaller scale is taken times 2^60 with its
+// row. y itself is the hardware's approximation with one such correction.
+struct Fp8Divide {
+  float less, inv, up;
+  __device__ __forceinline__ explicit Fp8Divide(float scale) {
+    up = scale < 0x1p-90f ? 0x1p60f : 1.f;
+    less = -scale * up;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale * up));
+    inv = fmaf(fmaf(less, inv, 1.f), inv, inv);
+  }
+  __device__ __forceinline__ bool small() const { return up != 1.f; }
+
+  // Codes of a pair (low byte: a); saturating, NaN stays NaN. `a` and `b` are already times `up`.
+  __device__ __forceinline__ uint32_t pair(float a, float b) const {
+    const uint64_t x = two(a, b), y = two(inv, inv), q = mul2(x, y);
+    const float2 f = halves(fma2(fma2(q, two(less, less), x), y, q));
+    return __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+  }
+  __device__ __forceinline__ uint32_t pack4(float x0, float x1, float x2, float x3) const {
+    return pair(x0, x1) | pair(x2, x3) << 16;
+  }
+  __device__ __forceinline__ uint8_t one(float x) const { return uint8_t(pair(x * up, 0.f)); }
+};
 
 // Two codes (low half of `w`) as f16x2; exact, e4m3's values are f16 numbers.
 __device__ __forceinline__ __half2 fp8_half2(uint32_t w) {
