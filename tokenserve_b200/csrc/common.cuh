@@ -136,10 +136,21 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
   return d;
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Pairs of floats and the packed fp32 instructions on them.
 __device__ __forceinline__ uint64_t two(float a, float b) {
   uint64_t v;
   asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t two(uint32_t a, uint32_t b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
   return v;
 }
 __device__ __forceinline__ float2 halves(uint64_t v) {
@@ -150,6 +161,11 @@ __device__ __forceinline__ float2 halves(uint64_t v) {
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {

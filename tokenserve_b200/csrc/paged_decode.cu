@@ -584,12 +584,6 @@ __device__ __forceinline__ uint32_t tile_off(int t, int cg) {
 // The maxima are kept until exceeded by 2^12: weights stay below f16's 2^16.
 constexpr float kFp8MaxSlack = 12.f;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 struct ItemInfo {
   int b, h, blk0, nparts, ctx, nblk, part_global, slot0;
 };
@@ -931,7 +925,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
         float inv[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)  // nothing seen: 0; a NaN stays one
-          inv[j] = l_run[nt][j] > 0.f ? ex2(t_run[nt][j] - m_run[nt][j]) * (1.f / l_run[nt][j])
+          inv[j] = l_run[nt][j] > 0.f ? ts::ex2(t_run[nt][j] - m_run[nt][j]) * (1.f / l_run[nt][j])
                                       : l_run[nt][j];
         const float i0 = inv[0], i1 = inv[1];
         const int head = nt * 8 + g;
@@ -1146,7 +1140,7 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
     }
     merge();
     float inv = lsum > 0.f ? 1.f / lsum : FP8 ? lsum : 0.f;
-    if (FP8 && lsum > 0.f) inv *= ex2(tx - mx);
+    if (FP8 && lsum > 0.f) inv *= ts::ex2(tx - mx);
     // Lane (hd, kq = lane / NT8) holds dims kq + LPH * i of head hd. Gather each 16-byte chunk
     // (8 consecutive dims) of a head into lane kq = chunk % LPH and store it as one vector.
     constexpr int LPH = 32 / NT8;     // lanes per head
@@ -1285,8 +1279,8 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float mn = fmaxf(m_run[nt][j], bm[j]), tn = fmaxf(t_run[nt][j], bt[j]);
-          l_run[nt][j] *= ex2(m_run[nt][j] - mn);
-          c[j] = ex2(t_run[nt][j] - tn);
+          l_run[nt][j] *= ts::ex2(m_run[nt][j] - mn);
+          c[j] = ts::ex2(t_run[nt][j] - tn);
           m_run[nt][j] = mn;
           t_run[nt][j] = tn;
         }
@@ -1302,9 +1296,9 @@ __global__ void __launch_bounds__((FP8 ? fp8_warps(NT) : kWarps) * 32, 1)
       }
 #pragma unroll
       for (int i = 0; i < 2 * B; ++i) {
-        l_run[nt][0] += ex2(e[2 * i]);
-        l_run[nt][1] += ex2(e[2 * i + 1]);
-        pb[nt][i] = ts::movmatrix_trans(MmaH::pack(ex2(w[2 * i]), ex2(w[2 * i + 1])));
+        l_run[nt][0] += ts::ex2(e[2 * i]);
+        l_run[nt][1] += ts::ex2(e[2 * i + 1]);
+        pb[nt][i] = ts::movmatrix_trans(MmaH::pack(ts::ex2(w[2 * i]), ts::ex2(w[2 * i + 1])));
       }
     }
 #pragma unroll

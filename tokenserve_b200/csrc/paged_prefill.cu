@@ -90,18 +90,6 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t phase, volatile
   return false;
 }
 
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <bool BF16>
 __global__ void __maxnreg__(kMaxRegs)
     paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap qmap,
@@ -358,9 +346,9 @@ __global__ void __maxnreg__(kMaxRegs)
           const float x1 = fmaf(__uint_as_float(sr[c + 1]), sl, -m_run);
           const float x2 = fmaf(__uint_as_float(sr[c + 2]), sl, -m_run);
           const float x3 = fmaf(__uint_as_float(sr[c + 3]), sl, -m_run);
-          xa = max3f(xa, x0, x1);
-          xb = max3f(xb, x2, x3);
-          const float p0 = ex2(x0), p1 = ex2(x1), p2 = ex2(x2), p3 = ex2(x3);
+          xa = ts::max3f(xa, x0, x1);
+          xb = ts::max3f(xb, x2, x3);
+          const float p0 = ts::ex2(x0), p1 = ts::ex2(x1), p2 = ts::ex2(x2), p3 = ts::ex2(x3);
           sum0 += p0 + p2;
           sum1 += p1 + p3;
           const uint32_t h01 = Mma::pack(p0, p1), h23 = Mma::pack(p2, p3);
@@ -379,7 +367,7 @@ __global__ void __maxnreg__(kMaxRegs)
         float mx = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 128; c += 2)
-          mx = max3f(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+          mx = ts::max3f(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
         m_run = mx * sl;
       }
       exp_pass();
@@ -388,7 +376,7 @@ __global__ void __maxnreg__(kMaxRegs)
       if (j > 0 && __any_sync(0xffffffffu, xm > kRescaleSlack)) {
         load_s();
         if (xm > kRescaleSlack) {
-          corr = ex2(-xm);
+          corr = ts::ex2(-xm);
           m_run += xm;
         }
         exp_pass();

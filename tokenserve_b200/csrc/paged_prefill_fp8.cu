@@ -186,52 +186,13 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase) {
   return __all_sync(0xffffffffu, wait_bar(bar, phase));
 }
 
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Maximum of 32 floats given as bits.
 __device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
   float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int k = 0; k < 32; k += 2)
-    m[k / 2 % 4] = max3f(m[k / 2 % 4], __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
-  return fmaxf(max3f(m[0], m[1], m[2]), m[3]);
-}
-
-// Pairs of floats, for the packed fp32 instructions.
-__device__ __forceinline__ uint64_t two(float a, float b) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  return v;
-}
-__device__ __forceinline__ uint64_t two(uint32_t a, uint32_t b) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
-  return v;
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
+    m[k / 2 % 4] = ts::max3f(m[k / 2 % 4], __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
+  return fmaxf(ts::max3f(m[0], m[1], m[2]), m[3]);
 }
 
 // 2^x of two x <= 15 on the FMA pipe, for some of the columns: the exponential unit (16 a clock) is
@@ -239,17 +200,18 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // 4 fitted to least relative error on [-1/2, 1/2] (2.9e-6, under fp16's 4.9e-4), n added to the
 // exponent. x below -126 gives 2^-126, which is 0 in fp16 and nothing beside a sum's 1. A NaN is lost.
 __device__ __forceinline__ float2 exp2_fma(uint64_t x2) {
-  float2 x = halves(x2);
-  x2 = two(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const uint64_t t2 = add2(x2, two(12582912.f, 12582912.f));  // 1.5 * 2^23: n in the low bits
-  const uint64_t n2 = add2(t2, two(-12582912.f, -12582912.f));
-  const uint64_t f2 = fma2(n2, two(-1.f, -1.f), x2);
-  uint64_t p2 = fma2(f2, two(0.009582851082086563f, 0.009582851082086563f),
-                     two(0.055906426161527634f, 0.055906426161527634f));
-  p2 = fma2(p2, f2, two(0.24024099111557007f, 0.24024099111557007f));
-  p2 = fma2(p2, f2, two(0.6931241750717163f, 0.6931241750717163f));
-  p2 = fma2(p2, f2, two(1.f, 1.f));
-  const float2 t = halves(t2), p = halves(p2);
+  float2 x = ts::halves(x2);
+  x2 = ts::two(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  // 1.5 * 2^23: n in the low bits.
+  const uint64_t t2 = ts::add2(x2, ts::two(12582912.f, 12582912.f));
+  const uint64_t n2 = ts::add2(t2, ts::two(-12582912.f, -12582912.f));
+  const uint64_t f2 = ts::fma2(n2, ts::two(-1.f, -1.f), x2);
+  uint64_t p2 = ts::fma2(f2, ts::two(0.009582851082086563f, 0.009582851082086563f),
+                     ts::two(0.055906426161527634f, 0.055906426161527634f));
+  p2 = ts::fma2(p2, f2, ts::two(0.24024099111557007f, 0.24024099111557007f));
+  p2 = ts::fma2(p2, f2, ts::two(0.6931241750717163f, 0.6931241750717163f));
+  p2 = ts::fma2(p2, f2, ts::two(1.f, 1.f));
+  const float2 t = ts::halves(t2), p = ts::halves(p2);
   return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(p.x)),
                      __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(p.y)));
 }
@@ -716,46 +678,46 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         }
         if (t_run == -INFINITY) m_run = m, t_run = mt;
       }
-      const uint64_t slj2 = two(slj, slj);
+      const uint64_t slj2 = ts::two(slj, slj);
       // P of columns 32 c .. 32 c + 31. Masked columns, and a warp whose maximum moves, run their own
       // copies of the code: where the paths met again, the registers of a whole row were copied.
       auto columns = [&](int c, auto masked) {
         const float log_v = info->log_v[word + c];
         const float less = t_run == -INFINITY ? 0.f : log_v - t_run;
-        const uint64_t less2 = two(less, less);
+        const uint64_t less2 = ts::two(less, less);
         ts::tc::wait_ld(sa);
         if (masked) mask(sa, c);
-        uint64_t e[16], sum2 = two(0.f, 0.f);  // log2 of P, two columns each; their sum
+        uint64_t e[16], sum2 = ts::two(0.f, 0.f);  // log2 of P, two columns each; their sum
 #pragma unroll
-        for (int k = 0; k < 16; ++k) e[k] = fma2(two(sa[2 * k], sa[2 * k + 1]), slj2, less2);
+        for (int k = 0; k < 16; ++k) e[k] = ts::fma2(ts::two(sa[2 * k], sa[2 * k + 1]), slj2, less2);
         if (c + 1 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 1) * 32, sa);
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float2 v = halves(e[k]);
-          mx[k % 4] = max3f(mx[k % 4], v.x, v.y);
+          const float2 v = ts::halves(e[k]);
+          mx[k % 4] = ts::max3f(mx[k % 4], v.x, v.y);
         }
-        const float over = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]);
+        const float over = fmaxf(ts::max3f(mx[0], mx[1], mx[2]), mx[3]);
         if (!__any_sync(0xffffffffu, over > kRescaleSlack)) {
           uint32_t pw[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            float2 v = halves(e[k]);
-            v = k % kFmaEvery == 0 ? exp2_fma(e[k]) : make_float2(ex2(v.x), ex2(v.y));
-            sum2 = add2(sum2, two(v.x, v.y));
+            float2 v = ts::halves(e[k]);
+            v = k % kFmaEvery == 0 ? exp2_fma(e[k]) : make_float2(ts::ex2(v.x), ts::ex2(v.y));
+            sum2 = ts::add2(sum2, ts::two(v.x, v.y));
             pw[k] = pack_half2(v.x, v.y);
           }
           ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
           // From the weights' maximum and reference to the sum's; nothing seen: 0.
-          const float2 sum = halves(sum2);
-          l_run += (sum.x + sum.y) * (t_run == -INFINITY ? 0.f : ex2(-less - m_run));
+          const float2 sum = ts::halves(sum2);
+          l_run += (sum.x + sum.y) * (t_run == -INFINITY ? 0.f : ts::ex2(-less - m_run));
           return;
         }
-        const float up = over > kRescaleSlack ? over : 0.f, f = ex2(-up);
+        const float up = over > kRescaleSlack ? over : 0.f, f = ts::ex2(-up);
         t_run += up;
         corr_o *= f;
         if (up > 0.f && t_run - log_v > m_run) {
-          l_run *= ex2(m_run - (t_run - log_v));
+          l_run *= ts::ex2(m_run - (t_run - log_v));
           m_run = t_run - log_v;
         }
         float2 sum = make_float2(0.f, 0.f);
@@ -775,14 +737,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
         uint32_t pw[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          float2 v = halves(e[k]);
-          v = make_float2(ex2(v.x - up), ex2(v.y - up));
+          float2 v = ts::halves(e[k]);
+          v = make_float2(ts::ex2(v.x - up), ts::ex2(v.y - up));
           sum.x += v.x;
           sum.y += v.y;
           pw[k] = pack_half2(v.x, v.y);
         }
         ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
-        l_run += (sum.x + sum.y) * (t_run == -INFINITY ? 0.f : ex2(up - less - m_run));
+        l_run += (sum.x + sum.y) * (t_run == -INFINITY ? 0.f : ts::ex2(up - less - m_run));
       };
 #pragma unroll 1
       for (int c = 0; c < min(n_whole, n_some); ++c) columns(c, std::false_type{});
@@ -821,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     ts::tc::fence_after_sync();
     if (x < a.q_tiles) {
       // A row that saw nothing has a sum of 0, and O = 0. An infinite score makes NaNs.
-      float inv = l_run > 0.f ? ex2(t_run - m_run) * (1.f / float(1 << kRefLog)) / l_run : l_run;
+      float inv = l_run > 0.f ? ts::ex2(t_run - m_run) * (1.f / float(1 << kRefLog)) / l_run : l_run;
       if (saw_nan || m_run == INFINITY) inv = __uint_as_float(0x7fc00000u);
       // The row goes to the warp's part of its Q tile (no MMA reads it any more), 16 bytes at a
       // time in swizzled places, and from there to memory in whole rows.
