@@ -135,7 +135,10 @@ def value_slack(q, cache, tab, chunks, ctxs):  # type: ignore[no-untyped-def]
         hkv = kc.shape[0]
         pad = torch.nn.functional.pad(vsc, (0, -c % 32)).unflatten(1, (-1, 32)).amax(-1)
         top = pad.repeat_interleave(32, 1)[:, :c].clamp_min(2.0**-120)
-        top = torch.maximum(top, top.cummax(1).values * 2.0**-60)
+        # ... and 2^-60 of the largest scale up to the end of the token's 128 at least.
+        run = torch.nn.functional.pad(vsc, (0, -c % 128)).unflatten(1, (-1, 128)).amax(-1)
+        run = run.cummax(1).values.repeat_interleave(128, 1)[:, :c]
+        top = torch.maximum(top, run * 2.0**-60)
         see = (torch.arange(c, device=q.device)[None, :]
                <= c - n + torch.arange(n, device=q.device)[:, None])  # fmt: skip
         s = torch.einsum("nhgd,hkd->nhgk", q[at : at + n].double().unflatten(1, (hkv, -1)),
