@@ -119,48 +119,14 @@ def test_decode_of_value_rows_over_many_binades(cuda_device, span) -> None:  # t
     check_decode(decode(q, (kp, vp, ks, vs), tab, ctx), q, (kp, vp, ks, vs), tab, lens)
 
 
-def value_slack(q, cache, tab, chunks, ctxs):  # type: ignore[no-untyped-def]
-    """What the tensor-core prefill may add to ``attention``'s bound where V's magnitudes differ.
-
-    V's tile holds code * scale / 2^n * 64 in fp16, 2^n <= the largest scale of a group of 32
-    tokens, its factor as a sum of two fp16 numbers: off by 2^-25 (448 + 2) / 64 < 2^-22 times 2^n
-    beside 2^-11 of itself. A weight is p 2^n over the largest such product (of those kept, which
-    is not above the row's), rounded to fp16: off by 2^-25 of that product below fp16's range."""
-    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
-    kp, vp, ks, vs = cache
-    d, at = q.shape[-1], 0
-    for i, (n, c) in enumerate(zip(chunks, ctxs, strict=True)):
-        kc, ksc = rows_of(kp, ks, tab[i], c)
-        vc, vsc = rows_of(vp, vs, tab[i], c)
-        hkv = kc.shape[0]
-        pad = torch.nn.functional.pad(vsc, (0, -c % 32)).unflatten(1, (-1, 32)).amax(-1)
-        top = pad.repeat_interleave(32, 1)[:, :c].clamp_min(2.0**-120)
-        # ... and 2^-60 of the largest scale up to the end of the token's 128 at least.
-        run = torch.nn.functional.pad(vsc, (0, -c % 128)).unflatten(1, (-1, 128)).amax(-1)
-        run = run.cummax(1).values.repeat_interleave(128, 1)[:, :c]
-        top = torch.maximum(top, run * 2.0**-60)
-        see = (torch.arange(c, device=q.device)[None, :]
-               <= c - n + torch.arange(n, device=q.device)[:, None])  # fmt: skip
-        s = torch.einsum("nhgd,hkd->nhgk", q[at : at + n].double().unflatten(1, (hkv, -1)),
-                         kc * ksc[..., None]) * d**-0.5  # fmt: skip
-        p = torch.softmax(s.masked_fill(~see[:, None, None], -float("inf")), -1)
-        held = torch.einsum("nhgk,hk->nhg", p, top) * 2.0**-22
-        units = (vc * (vsc / top)[..., None]).abs().cumsum(1)[:, c - n :]  # of the keys a row sees
-        tail = (p * top[None, :, None]).amax(-1)[..., None] * units.transpose(0, 1)[:, :, None] * 2.0**-23
-        out[at : at + n] = (held[..., None] + tail).flatten(1, 2)
-        at += n
-    return out
-
-
 def check_prefill_wide(out, q, cache, tab, chunks, ctxs):  # type: ignore[no-untyped-def]
-    slack, at = value_slack(q, cache, tab, chunks, ctxs), 0
+    at = 0
     for i, (n, c) in enumerate(zip(chunks, ctxs, strict=True)):
         rows = slice(at, at + n)
         at += n
         want, off = attention(q[rows], *rows_of(cache[0], cache[2], tab[i], c),
-                              *rows_of(cache[1], cache[3], tab[i], c), q.shape[-1] ** -0.5, c - n,
-                              k_half=2.0**-11)  # fmt: skip
-        off, got, most = off + slack[rows], out[rows].double(), torch.finfo(q.dtype).max
+                              *rows_of(cache[1], cache[3], tab[i], c), q.shape[-1] ** -0.5, c - n)
+        got, most = out[rows].double(), torch.finfo(q.dtype).max
         # An output past the type's largest number is that type's infinity (fp16: past 65504).
         past = (want.abs() + off > most) & torch.isinf(got) & (got * want > 0)
         bad = ((got - want).abs() - off).masked_fill(past, 0.0)
@@ -173,7 +139,7 @@ WIDE_CHUNKS, WIDE_CTX = [40, 150, 64, 1], [900, 150, 64, 700]
 @pytest.mark.parametrize(("dtype", "hq", "hkv", "d"), [(BF, 8, 2, 128), (FH, 8, 2, 128), (FH, 4, 4, 64)])
 @pytest.mark.parametrize("kind", ["blocks", "rows", "outlier", "growing", "zeros"])
 def test_prefill_of_value_rows_over_many_binades(cuda_device, dtype, hq, hkv, d, kind) -> None:  # type: ignore[no-untyped-def]
-    """Blocks of 32 tokens and single rows of magnitudes 2^+-20, a row 2^24 times larger than all
+    """Within the bound for exact K and V codes: blocks of 32 tokens and single rows of magnitudes 2^+-20, a row 2^24 times larger than all
     others whose softmax weight is nothing, magnitudes that grow along the context, runs of zeros."""
     gen = torch.Generator(device=cuda_device).manual_seed(31)
     nb, tab = tables_for(WIDE_CTX, 16, gen)
@@ -228,3 +194,57 @@ def test_decode_of_a_nan_row_wherever_it_stands(cuda_device, which, hq, hkv, d) 
     out = prefill(q, cache, tab, qsl, ctx, 1)
     assert torch.isnan(out[:-1]).all()
     check_prefill(out[-1:], q[-1:], cache, tab[-1:], [1], lens[-1:])
+
+
+def exact(q, cache, tab, chunks, ctxs):  # type: ignore[no-untyped-def]
+    """The attention in 64 bits, ``[T, Hq, D]``."""
+    out, at = [], 0
+    for i, (n, c) in enumerate(zip(chunks, ctxs, strict=True)):
+        out.append(attention(q[at : at + n], *rows_of(cache[0], cache[2], tab[i], c),
+                             *rows_of(cache[1], cache[3], tab[i], c), q.shape[-1] ** -0.5, c - n)[0])  # fmt: skip
+        at += n
+    return torch.cat(out)
+
+
+@pytest.mark.parametrize(("hq", "hkv", "d"), [(8, 2, 128), (4, 4, 64), (16, 1, 128)])
+def test_fp16_outputs_lose_little_beside_their_own_rounding(cuda_device, hq, hkv, d) -> None:  # type: ignore[no-untyped-def]
+    """Codes are exact in the tiles, so what is left beside the output's rounding is one rounding of
+    the weights, to 11 bits as well: two independent errors of one size in the 2-norm, sqrt(2) times
+    the output's rounding together (a row's weights average theirs, so less than that of each row)."""
+    gen = torch.Generator(device=cuda_device).manual_seed(51)
+    chunks, ctxs = [200, 64, 1, 300], [700, 64, 900, 300]
+    nb, tab = tables_for(ctxs, 16, gen)
+    cache = make_cache(gen, nb, hkv, 16, d)
+    q = torch.randn(sum(chunks), hq, d, generator=gen, device=cuda_device).to(FH)
+    qsl = torch.tensor([0, *chunks], device=cuda_device).cumsum(0).to(torch.int32)
+    ctx = torch.tensor(ctxs, dtype=torch.int32, device=cuda_device)
+    want = exact(q, cache, tab, chunks, ctxs)
+    own = (want.to(FH).double() - want).norm()
+    got = prefill(q, cache, tab, qsl, ctx, max(chunks)).double()
+    assert (got - want).norm() <= 1.5 * own, float((got - want).norm() / own)
+    check_prefill(got.to(FH), q, cache, tab, chunks, ctxs, k_half=0.0)
+
+
+@pytest.mark.parametrize(("dtype", "d"), [(BF, 128), (FH, 64)])
+def test_zero_rows_that_take_nearly_all_weight(cuda_device, dtype, d) -> None:  # type: ignore[no-untyped-def]
+    """Positions 20..39 hold zero V rows with scores about 2^70 times the others' weights, so the
+    outputs (bf16: 2^-70 of V) come from the small weights of the other rows alone."""
+    gen = torch.Generator(device=cuda_device).manual_seed(61)
+    chunks, ctxs = [60, 5], [90, 200]
+    nb, tab = tables_for(ctxs, 16, gen)
+    cache = make_cache(gen, nb, 2, 16, d)
+    kp, vp, ks, vs = cache
+    if dtype == FH:  # outputs of fp16's normal range
+        vs.mul_(2.0**60)
+    q = torch.randn(sum(chunks), 8, d, generator=gen, device=cuda_device).abs().to(dtype)
+    want = 48.0 / (0.8 * d**0.5)  # K's value that gives q's mean row a score of 48 (2^70)
+    for i in range(2):
+        zero_rows(cache, tab, i, range(20, 40), keys=False)
+        for p in range(20, 40):
+            kp.view(torch.uint8)[int(tab[i, p // 16]), :, p % 16] = 0x70  # 128
+            ks[int(tab[i, p // 16]), :, p % 16] = want / 128
+    qsl = torch.tensor([0, *chunks], device=cuda_device).cumsum(0).to(torch.int32)
+    ctx = torch.tensor(ctxs, dtype=torch.int32, device=cuda_device)
+    out = prefill(q, cache, tab, qsl, ctx, max(chunks))
+    check_prefill_wide(out, q, cache, tab, chunks, ctxs)
+    check_decode(decode(q[59:61], cache, tab, ctx), q[59:61], cache, tab, ctxs)

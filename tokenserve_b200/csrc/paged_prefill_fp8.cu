@@ -7,37 +7,34 @@
 // and by the exponentials (one per score), so the cache's 8 bits must cost neither of them:
 //   * CTA = (sequence, KV head, pair of query tiles); a tile's 128 rows are 128/G tokens x the G
 //     query heads of the KV head, so a converted K/V tile serves 256 rows.
-//   * warp 12 (scout) runs up to four spans of 128 tokens ahead: block table, the span's scales,
-//     each row's factor and the span's references, left in shared memory.
-//   * warps 8-11, 14, 15 (converters) take the blocks of 64-token tiles (4 of K, 4 of V) in turn: codes from
-//     global memory two blocks ahead into registers, times the row's factor, as fp16 into the
-//     swizzled layout the MMAs read. K's values are relative to the span's largest scale, V's to the
-//     largest of their 32 tokens (as a power of two), so the largest fill fp16's range; a factor is
-//     two fp16 parts, so a value is off by 2^-11 of itself, or by 2^-31 of the largest value in the
-//     span (K) or the 32 tokens (V, whose reference is 2^-60 of the largest so far at least): rows
-//     whose scale is less than 2^-20 of the reference lose bits. K's reference is a factor on the
-//     tile's scores, V's is added to the exponent of the 32 tokens' weights.
+//   * warp 12 (scout) runs up to four spans of 128 tokens ahead: block table, the span's scales and
+//     references, left in shared memory.
+//   * warps 8-11, 14, 15 (converters) take the blocks of 64-token tiles (4 of K, 4 of V) in turn:
+//     codes from global memory two blocks ahead into registers, as fp16 (exact) into the swizzled
+//     layout the MMAs read.
 //   * warps 0-3 / 4-7 (softmax, one warpgroup per query tile, thread = row): q's row is scaled by a
 //     power of two into fp16's range and written to shared memory; then per tile, 32 columns at a
-//     time: 2^(t - mt) with t = s + log2(V's reference), P in fp16 (11 bits) back to TMEM over S. The
-//     sum of 2^(s - m) is theirs times one factor per 32 columns, in fp32. mt is the maximum of
-//     the row's first tile and is kept while no t exceeds it by 2^14, so the exponentials wait
-//     for no maximum; a warp with a row past that takes the columns, and all before them, to the
-//     new maximum. The output is O 2^(mt - m) / sum. Columns no row of a warp sees are skipped.
+//     time: s = S times K's scale, u = 2^(s + n - mt), P = u times V's scale over 2^n, rounded to
+//     fp16 (11 bits), back to TMEM over S. 2^n is the largest V scale of the 32 tokens, mt the maximum
+//     of s + log2(V's scale) over the row's first tile, kept while no P exceeds 2^14, so the
+//     exponentials wait for no maximum; a warp with a row past that takes the columns, and all
+//     before them, to the new maximum. The softmax's sum, of 2^(s - m) with a maximum m of s, is that
+//     of u times one factor per 32 columns, in fp32. The output is O 2^(mt - m) / sum. So a key of any
+//     magnitude takes no bits from the others unless its weight does: P is off by 2^-11 of itself,
+//     or by 2^-25 of the largest P below 2^-14 of that. Columns no row of a warp sees are skipped.
 //     Everything is in loops over few columns: unrolled over a whole row, the roles' code outgrew
 //     the instruction caches (a quarter of the stalls).
 //   * warp 13: tcgen05.mma, S_x = Q_x K^T and O_x += P_x V, in the order PV_A(j), QK_A(j+2),
 //     PV_B(j), QK_B(j+2): each query tile has two S buffers of 64 columns, so its softmax finds the
 //     next tile's scores ready and waits for no MMA (with one buffer of 128 columns a tile's
 //     softmax, PV and QK took turns: 5,000 clocks per 128 tokens).
-// 64 sequences of 257-512 new tokens over 900-1,600 cached ones, 32/8 heads of 128: 841 us, 682 TFLOP/s
-// (0.42 of cuBLAS bf16); tensor pipe 44%, issue slots 57% busy: what binds is the way of a tile's
-// scores through softmax and MMAs and back. Without the exponentials 832 us, without the
-// conversion 807 us, without both 653 us (of 888 us then).
+// 64 sequences of 257-512 new tokens over 900-1,600 cached ones, 32/8 heads of 128: 844 us, 680 TFLOP/s
+// (0.42 of cuBLAS bf16), fp16 841 us: what binds is the way of a tile's scores through softmax and
+// MMAs and back. Codes times scales in fp16 tiles (one rounding of K and V each) took 841 us and left
+// fp16 outputs 4.6e-4 off 64 bits instead of 2.9e-4 (2.1e-4 is their own rounding).
 // A page outside the pool is skipped (its columns are masked). A V row with a NaN scale is stored
-// as zeros and its column's weight set to NaN for the rows that see it, so rows before it in the
-// chunk stay clean. Tokens past the last visible key are stored as zeros: their slots may hold
-// anything. Other shapes and fp32 queries run on CUDA cores (attention_portable.cu).
+// as zeros and rows that see it become NaN, so rows before it in the chunk stay clean. V's rows past
+// the last visible key are stored as zeros: their slots may hold anything. Other shapes and fp32 queries run on CUDA cores (attention_portable.cu).
 #include <cstddef>
 
 #include "fp8.cuh"
@@ -70,21 +67,19 @@ constexpr int kConverters = 6;  // converter warps
 constexpr int kUnits = 2 * kKvTile / kBlock;  // blocks of a tile, K then V
 constexpr int kThreads = 512;
 constexpr int kMaxTries = 1 << 22, kMaxNaps = 1 << 22;  // of a bounded wait
-constexpr uint32_t kDropped = 0x80008000u;  // factor of a row whose codes are not used
 constexpr float kLog2e = 1.4426950408889634f;
-// A stale maximum is kept unless exceeded by 2^14: P stays below fp16's 2^16, and weights near the
-// true maximum, at least 1, well inside its normal range.
-constexpr float kRescaleSlack = 14.f;
-// One of so many column pairs takes its 2^x from the FMA pipe (64 sequences of 512 new tokens: none
-// 894 us, one of 16 885, of 8 876, of 4 886, of 3 896).
-constexpr int kFmaEvery = 8;
+// A stale maximum is kept while 32 columns' u add up to 2^14 at most: P, below 2 u, stays below fp16's
+// 2^16, and weights near the true maximum, at least 1, are well inside its normal range.
+constexpr float kMostSumU = 0x1p14f;
 // S_A [0,128) and S_B [128,256), two buffers each, O_A [256,384), O_B [384,512).
 constexpr uint32_t kTmemCols = 512;
-constexpr float kRefScale = 128.f;    // K's fp16 values are code * scale / ref * 128 <= 57344
-constexpr int kRefLog = 6;  // V's are code * scale * 2^(6 - n) < 57344, 2^n <= the largest scale
-// V's n stays within this of the context's largest so far: a weight's exponent t - mt is then above
-// fp32's -126 wherever 2^(s - m) is above 2^-52, so the weights' sums give the softmax's sum.
+// A group's n stays within this of the context's largest so far: u is then above fp32's 2^-126
+// wherever 2^(s - m) is above 2^-64. (V rows below 2^-60 of the largest scale so far may lose bits.)
 constexpr int kRefSpread = 60;
+// log2(V's scale / 2^n) counts as this at least in mt, so that rows of zeros leave u, up to 2^100 then,
+// and its sums finite.
+constexpr float kLeastLog = -100.f;
+constexpr float kMostSum = 0x1p60f;  // of a group's 2^(s - m), before m has to move
 
 struct Args {
   void* out;
@@ -105,19 +100,17 @@ struct Args {
   float scale_log2;
 };
 
-// A span as the scout leaves it: references of K and, as n, of each 32 rows of V; the columns to
-// mask (page outside the pool) or to spoil (V row NaN), if any; the blocks (negative: none); each
-// row's factor for K and for V, fp16 high and low part, or kDropped.
+// A span as the scout leaves it: log2 of V's reference, n, for each 32 rows; the columns to mask (page
+// outside the pool) or to spoil (V row NaN), if any; the blocks (negative: none); K's scale of each
+// row and V's over 2^n, 0 for rows whose codes are not used (past the last key, or NaN).
 struct alignas(16) TileInfo {
-  float ref_k;
-  uint32_t any, dropped;  // dropped: bit 0, 1: K, V has rows of factor kDropped
   float log_v[4];
   uint32_t skip[4], spoil[4];
   int block[kSpan / kBlock];
-  alignas(16) uint32_t factor[2][kSpan];  // written 16 bytes at a time
+  float scale[2][kSpan];
+  uint32_t any, dropped;  // dropped: V has rows that are not used
 };
-static_assert(offsetof(TileInfo, factor) % 16 == 0 && sizeof(TileInfo) % 16 == 0 &&
-                  offsetof(TileInfo, any) == 4,
+static_assert(offsetof(TileInfo, scale) % 16 == 0 && sizeof(TileInfo) % 16 == 0,
               "vector accesses of a description");
 
 struct Shared {
@@ -127,15 +120,6 @@ struct Shared {
   TileInfo info[kInfos];
   uint32_t tmem;
 };
-
-// ref_k and any of a description in one load.
-__device__ __forceinline__ float2 load_refs(const volatile TileInfo* info) {
-  float2 v;
-  asm volatile("ld.volatile.shared.v2.f32 {%0, %1}, [%2];"
-               : "=f"(v.x), "=f"(v.y)
-               : "r"(ts::smem_u32(const_cast<const TileInfo*>(info))));
-  return v;
-}
 
 template <int D>
 struct Geo {
@@ -186,45 +170,9 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase) {
   return __all_sync(0xffffffffu, wait_bar(bar, phase));
 }
 
-// Maximum of 32 floats given as bits.
-__device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
-  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int k = 0; k < 32; k += 2)
-    m[k / 2 % 4] = ts::max3f(m[k / 2 % 4], __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
-  return fmaxf(ts::max3f(m[0], m[1], m[2]), m[3]);
-}
-
-// 2^x of two x <= 15 on the FMA pipe, for some of the columns: the exponential unit (16 a clock) is
-// what a tile's softmax waits for. x = n + f with n the nearest integer, 2^f by a polynomial of degree
-// 4 fitted to least relative error on [-1/2, 1/2] (2.9e-6, under fp16's 4.9e-4), n added to the
-// exponent. x below -126 gives 2^-126, which is 0 in fp16 and nothing beside a sum's 1. A NaN is lost.
-__device__ __forceinline__ float2 exp2_fma(uint64_t x2) {
-  float2 x = ts::halves(x2);
-  x2 = ts::two(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  // 1.5 * 2^23: n in the low bits.
-  const uint64_t t2 = ts::add2(x2, ts::two(12582912.f, 12582912.f));
-  const uint64_t n2 = ts::add2(t2, ts::two(-12582912.f, -12582912.f));
-  const uint64_t f2 = ts::fma2(n2, ts::two(-1.f, -1.f), x2);
-  uint64_t p2 = ts::fma2(f2, ts::two(0.009582851082086563f, 0.009582851082086563f),
-                     ts::two(0.055906426161527634f, 0.055906426161527634f));
-  p2 = ts::fma2(p2, f2, ts::two(0.24024099111557007f, 0.24024099111557007f));
-  p2 = ts::fma2(p2, f2, ts::two(0.6931241750717163f, 0.6931241750717163f));
-  p2 = ts::fma2(p2, f2, ts::two(1.f, 1.f));
-  const float2 t = ts::halves(t2), p = ts::halves(p2);
-  return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(p.x)),
-                     __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(p.y)));
-}
-
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// Two fp16 parts of a row's factor, hi + lo = f to 2^-22 of it.
-__device__ __forceinline__ uint32_t split_factor(float f) {
-  const __half hi = __float2half_rn(f), lo = __float2half_rn(f - __half2float(hi));
-  return uint32_t(__half_as_ushort(hi)) | (uint32_t(__half_as_ushort(lo)) << 16);
 }
 
 // Bits of the largest finite value of four scales; scales are not negative and order like their bits.
@@ -272,37 +220,29 @@ struct Scout {
       const int reach = n_kv - t * kSpan - 4 * lane;  // of its tokens, those below n_kv
       float k[4] = {ks.x, ks.y, ks.z, ks.w}, v[4] = {vs.x, vs.y, vs.z, vs.w};
       uint32_t spoil = 0;
-      bool k_odd = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i >= reach) k[i] = v[i] = 0.f;
-        k_odd |= !isfinite(k[i]);
         if (!isfinite(v[i])) spoil |= 1u << i;
       }
       if (t >= kAhead && !wait_ahead(&sh->converted[t % kAhead], ((t - kAhead) / kAhead) & 1))
         return;
       TileInfo* info = &sh->info[t % kInfos];
-      const float ref_k = fmaxf(
-          __uint_as_float(__reduce_max_sync(0xffffffffu, top_bits(k))), 0x1p-126f);
       // n of the lane's 32 tokens (8 lanes).
       int n = int(top_bits(v) >> 23) - 127;
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) n = max(n, __shfl_xor_sync(0xffffffffu, n, o));
       run_n = max(run_n, __reduce_max_sync(0xffffffffu, n));
-      n = max(n, max(run_n - kRefSpread, -120));  // 2^(6 - n) stays finite
-      const float inv_k = 1.f / ref_k, up_v = __uint_as_float(uint32_t(127 + kRefLog - n) << 23);
-      // A NaN K row makes NaN scores; a NaN V row is stored as zeros (see the head of the file).
-      uint32_t fk[4], fv[4];
+      n = min(max(n, max(run_n - kRefSpread, -126)), 126);
+      const float inv_v = __uint_as_float(uint32_t(127 - n) << 23);
+      // A NaN V row is stored as zeros (see the head of the file).
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fk[i] = i < reach ? split_factor(k[i] * inv_k * kRefScale) : kDropped;
-        fv[i] = i < reach && !(spoil >> i & 1) ? split_factor(v[i] * up_v) : kDropped;
-      }
-      *reinterpret_cast<uint4*>(&info->factor[0][4 * lane]) = make_uint4(fk[0], fk[1], fk[2], fk[3]);
-      *reinterpret_cast<uint4*>(&info->factor[1][4 * lane]) = make_uint4(fv[0], fv[1], fv[2], fv[3]);
+      for (int i = 0; i < 4; ++i) v[i] = spoil >> i & 1 ? 0.f : v[i] * inv_v;
+      *reinterpret_cast<float4*>(&info->scale[0][4 * lane]) = make_float4(k[0], k[1], k[2], k[3]);
+      *reinterpret_cast<float4*>(&info->scale[1][4 * lane]) = make_float4(v[0], v[1], v[2], v[3]);
       if (lane % 4 == 0) info->block[lane / 4] = phys;
       if (lane % 8 == 0) info->log_v[lane / 8] = float(n);
-      const bool any = __any_sync(0xffffffffu, spoil != 0 || k_odd || phys == -2);
+      const bool any = __any_sync(0xffffffffu, spoil != 0 || phys == -2);
       const bool past = __any_sync(0xffffffffu, reach < 4);
       if (any) {
         uint32_t skip = (phys == -2 ? 0xfu : 0u) << lane % 8 * 4;
@@ -320,9 +260,8 @@ struct Scout {
         info->skip[lane] = info->spoil[lane] = 0;
       }
       if (lane == 0) {
-        info->ref_k = ref_k;
         info->any = any;
-        info->dropped = uint32_t(past) | uint32_t(past || any) << 1;
+        info->dropped = past || any;
       }
       __syncwarp();
       if (lane == 0) ts::mbar_arrive(&sh->info_full[t % kInfos]);
@@ -347,27 +286,22 @@ struct Codes {
       for (int hf = 0; hf < kHalves; ++hf)
         raw[i][hf] = block != nullptr ? __ldg(src + i * (D / 2) + hf * 8) : make_uint2(0, 0);
   }
-  // Rows row0 .. row0 + 15 of the fp16 tile at `dst` (128-byte swizzled halves of 64 columns);
-  // `factor`: of those rows.
-  __device__ __forceinline__ void store(uint8_t* dst, const uint32_t* factor, int row0, bool dropped,
-                                        int lane) {
+  // Rows row0 .. row0 + 15 of the fp16 tile at `dst` (128-byte swizzled halves of 64 columns), with
+  // `scale` (of those rows) only where it is not 0.
+  __device__ __forceinline__ void store(uint8_t* dst, const float* scale, int row0, int lane) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = row0 + i * 4 + lane / 8;
-      const uint32_t f = factor[i * 4 + lane / 8];
-      const __half2 f2 = *reinterpret_cast<const __half2*>(&f);
-      const __half2 h2 = __low2half2(f2), l2 = __high2half2(f2);
+      const bool used = scale == nullptr || scale[i * 4 + lane / 8] != 0.f;
       uint8_t* base = dst + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
 #pragma unroll
       for (int hf = 0; hf < kHalves; ++hf) {
-        uint2 w = raw[i][hf];
-        if (dropped && f == kDropped) w = make_uint2(0, 0);
+        const uint2 w = used ? raw[i][hf] : make_uint2(0, 0);
         uint32_t v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const __half2 x = ts::fp8_half2((k < 2 ? w.x : w.y) >> (16 * (k & 1)));
-          const __half2 y = __hfma2(x, h2, __hmul2(x, l2));
-          v[k] = *reinterpret_cast<const uint32_t*>(&y);
+          v[k] = *reinterpret_cast<const uint32_t*>(&x);
         }
         *reinterpret_cast<uint4*>(base + hf * kKvHalf) = make_uint4(v[0], v[1], v[2], v[3]);
       }
@@ -494,8 +428,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           return false;
         const TileInfo& info = sh->info[t % kInfos];
         const int row0 = k % (kUnits / 2) * kBlock;
-        c.store(is_v ? sV(st) : sK(st), info.factor[is_v] + j % kTilesPerSpan * kKvTile + row0, row0,
-                info.dropped >> int(is_v) & 1, lane);
+        // K's rows past the last key make scores that are masked; V's are zeros.
+        c.store(is_v ? sV(st) : sK(st),
+                is_v && info.dropped ? info.scale[1] + j % kTilesPerSpan * kKvTile + row0 : nullptr,
+                row0, lane);
         ts::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -585,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     float sl = 0.f;
     {
       asm volatile("cp.async.wait_all;" ::: "memory");
-      const float base = fabsf(a.scale_log2) / kRefScale;
+      const float base = fabsf(a.scale_log2);
       constexpr int kBatch = 4;  // rows of a lane at a time
 #pragma unroll 1
       for (int w0 = lane / kQLanes; w0 < 32; w0 += kBatch * kQRows) {
@@ -628,11 +564,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       if (lane == 0) ts::mbar_arrive(&sh->q_full);
     }
 
+    const uint64_t sl2 = ts::two(sl, sl);
     const int pos_max = __reduce_max_sync(0xffffffffu, pos);
     const int pos_min = __reduce_min_sync(0xffffffffu, pos);
     // Maximum that the weights and O are relative to, the one of the sum, the sum.
     float t_run = -INFINITY, m_run = -INFINITY, l_run = 0.f;
-    bool saw_nan = false;  // a row of K or V that holds one (not every exponential below keeps it)
+    bool saw_nan = false;  // a V row that holds one; one of K is in the scores
     bool ok = true;
     for (int j = 0; j < n_x; ++j) {
       if (!wait_warp(&sh->s_full[x][j & 1], (j / 2) & 1)) {
@@ -646,81 +583,118 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
       constexpr int kGroups = kKvTile / 32;  // of 32 columns
       const volatile TileInfo* info = &sh->info[j / kTilesPerSpan % kInfos];
       const int word = j % kTilesPerSpan * kGroups;  // of the span's column masks
-      const float2 refs = load_refs(info);
-      const float slj = fmaxf(sl * refs.x, 0x1p-126f);  // > 0, so that -inf stays -inf
-      const bool odd_columns = __float_as_uint(refs.y) != 0;
+      const bool odd_columns = info->any != 0;
       float corr_o = 1.f;  // of O, when the weights' maximum moves
       const int limit = pos - j * kKvTile;  // columns c <= limit are visible
       // Column groups of 32 that some row of the warp sees, and those every row sees whole.
       const int n_some = min(kGroups, max(0, pos_max - j * kKvTile + 32) / 32);
       const int n_whole = odd_columns ? 0 : max(0, pos_min - j * kKvTile + 1) / 32;
-      auto mask = [&](uint32_t (&r)[32], int c) {
+      // K's (w = 0) scales, or V's over 2^n (1), of columns 32 c + 4 k .. 32 c + 4 k + 3.
+      const uint32_t scale_at = ts::smem_u32(&sh->info[j / kTilesPerSpan % kInfos].scale[0][word * 32]);
+      auto scales = [&](int w, int c, int k) {
+        ulonglong2 v;
+        asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];"
+                     : "=l"(v.x), "=l"(v.y)
+                     : "r"(scale_at + w * (kSpan * 4) + c * 128 + k * 16));
+        return v;
+      };
+      // Scores of columns 32 c .. 32 c + 31, which `sa` holds raw, plus `plus`.
+      auto scores = [&](int c, float plus, uint64_t (&e)[16]) {
+        const uint64_t plus2 = ts::two(plus, plus);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const ulonglong2 ks = scales(0, c, k);
+          e[2 * k] = ts::fma2(ts::two(sa[4 * k], sa[4 * k + 1]), ts::mul2(ks.x, sl2), plus2);
+          e[2 * k + 1] = ts::fma2(ts::two(sa[4 * k + 2], sa[4 * k + 3]), ts::mul2(ks.y, sl2), plus2);
+        }
+      };
+      // Maximum of scores, and of scores plus log2(V's scale / 2^n).
+      auto maxima = [&](int c, const uint64_t (&e)[16], float& m, float& mt) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float2 v = ts::halves(e[k]);
+          const ulonglong2 vs2 = scales(1, c, k / 2);
+          const float2 vs = ts::halves(k % 2 ? vs2.y : vs2.x);
+          m = ts::max3f(m, v.x, v.y);
+          mt = ts::max3f(mt, v.x + fmaxf(__log2f(vs.x), kLeastLog),
+                         v.y + fmaxf(__log2f(vs.y), kLeastLog));
+        }
+      };
+      auto mask = [&](uint64_t (&e)[16], int c) {
         const int lim = limit - 32 * c;
         const uint32_t seen = lim >= 31 ? ~0u : lim < 0 ? 0u : (2u << lim) - 1;
         const uint32_t keep = seen & ~info->skip[word + c],
                        spoil = seen & info->spoil[word + c];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          if (!(keep >> k & 1)) r[k] = __float_as_uint(-INFINITY);
-          else if (spoil >> k & 1 || isnan(__uint_as_float(r[k]))) saw_nan = true;
+        for (int k = 0; k < 16; ++k) {
+          float2 v = ts::halves(e[k]);
+          e[k] = ts::two(keep >> 2 * k & 1 ? v.x : -INFINITY, keep >> (2 * k + 1) & 1 ? v.y : -INFINITY);
         }
+        saw_nan |= spoil != 0;
       };
       if (__any_sync(0xffffffffu, t_run == -INFINITY)) {  // a row that has seen nothing yet
         float m = -INFINITY, mt = -INFINITY;
 #pragma unroll 1
         for (int c = 0; c < n_some; ++c) {
           ts::tc::wait_ld(sa);
-          if (c >= n_whole) mask(sa, c);
-          const float s = max32(sa) * slj;
-          m = fmaxf(m, s);
-          mt = fmaxf(mt, s + info->log_v[word + c]);
+          uint64_t e[16];
+          scores(c, 0.f, e);
+          if (c >= n_whole) mask(e, c);
+          float mg = -INFINITY;
+          maxima(c, e, m, mg);
+          mt = fmaxf(mt, mg + info->log_v[word + c]);
           ts::tc::tmem_ld32(lane_base + s_col + (c + 1 < n_some ? c + 1 : 0) * 32, sa);
         }
         if (t_run == -INFINITY) m_run = m, t_run = mt;
       }
-      const uint64_t slj2 = ts::two(slj, slj);
       // P of columns 32 c .. 32 c + 31. Masked columns, and a warp whose maximum moves, run their own
       // copies of the code: where the paths met again, the registers of a whole row were copied.
       auto columns = [&](int c, auto masked) {
         const float log_v = info->log_v[word + c];
         const float less = t_run == -INFINITY ? 0.f : log_v - t_run;
-        const uint64_t less2 = ts::two(less, less);
         ts::tc::wait_ld(sa);
-        if (masked) mask(sa, c);
         uint64_t e[16], sum2 = ts::two(0.f, 0.f);  // log2 of P, two columns each; their sum
-#pragma unroll
-        for (int k = 0; k < 16; ++k) e[k] = ts::fma2(ts::two(sa[2 * k], sa[2 * k + 1]), slj2, less2);
+        scores(c, less, e);
+        if (masked) mask(e, c);
         if (c + 1 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 1) * 32, sa);
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // From the weights' maximum and reference to the sum's; nothing seen: 0.
+        const float to_sum = t_run == -INFINITY ? 0.f : ts::ex2(-less - m_run);
+        uint32_t pw[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float2 v = ts::halves(e[k]);
-          mx[k % 4] = ts::max3f(mx[k % 4], v.x, v.y);
-        }
-        const float over = fmaxf(ts::max3f(mx[0], mx[1], mx[2]), mx[3]);
-        if (!__any_sync(0xffffffffu, over > kRescaleSlack)) {
-          uint32_t pw[16];
+        for (int k = 0; k < 8; ++k) {
+          const ulonglong2 vs = scales(1, c, k);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float2 v = ts::halves(e[k]);
-            v = k % kFmaEvery == 0 ? exp2_fma(e[k]) : make_float2(ts::ex2(v.x), ts::ex2(v.y));
-            sum2 = ts::add2(sum2, ts::two(v.x, v.y));
-            pw[k] = pack_half2(v.x, v.y);
+          for (int i = 0; i < 2; ++i) {
+            float2 u = ts::halves(e[2 * k + i]);
+            u = make_float2(ts::ex2(u.x), ts::ex2(u.y));
+            sum2 = ts::add2(sum2, ts::two(u.x, u.y));
+            u = ts::halves(ts::mul2(ts::two(u.x, u.y), i ? vs.y : vs.x));
+            pw[2 * k + i] = pack_half2(u.x, u.y);
           }
+        }
+        const float2 s2 = ts::halves(sum2);
+        const float sum_u = s2.x + s2.y, part = sum_u * to_sum;
+        if (__all_sync(0xffffffffu, sum_u <= kMostSumU && part <= kMostSum)) {
           ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
-          // From the weights' maximum and reference to the sum's; nothing seen: 0.
-          const float2 sum = ts::halves(sum2);
-          l_run += (sum.x + sum.y) * (t_run == -INFINITY ? 0.f : ts::ex2(-less - m_run));
+          l_run += part;
           return;
         }
-        const float up = over > kRescaleSlack ? over : 0.f, f = ts::ex2(-up);
+        // Once more, with the maxima that the columns need; the next columns' load is repeated.
+        if (c + 1 < n_some) ts::tc::wait_ld(sa);
+        ts::tc::tmem_ld32(lane_base + s_col + c * 32, sa);
+        ts::tc::wait_ld(sa);
+        scores(c, less, e);
+        if (masked) mask(e, c);
+        float m = -INFINITY, mt = -INFINITY;
+        maxima(c, e, m, mt);
+        m += -less;  // s
+        const float up = fmaxf(mt, 0.f), f = ts::ex2(-up);
+        if (m > m_run) {
+          l_run *= ts::ex2(m_run - m);
+          m_run = m;
+        }
         t_run += up;
         corr_o *= f;
-        if (up > 0.f && t_run - log_v > m_run) {
-          l_run *= ts::ex2(m_run - (t_run - log_v));
-          m_run = t_run - log_v;
-        }
-        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll 1
         for (int b = 0; b < c; ++b) {  // the tile's P so far
           uint32_t pw[16];
@@ -734,17 +708,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
           }
           ts::tc::tmem_st16(lane_base + s_col + b * 16, pw);
         }
-        uint32_t pw[16];
+        float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          float2 v = ts::halves(e[k]);
-          v = make_float2(ts::ex2(v.x - up), ts::ex2(v.y - up));
-          sum.x += v.x;
-          sum.y += v.y;
-          pw[k] = pack_half2(v.x, v.y);
+        for (int k = 0; k < 8; ++k) {
+          const ulonglong2 vs = scales(1, c, k);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float2 u = ts::halves(e[2 * k + i]);
+            u = make_float2(ts::ex2(u.x - up), ts::ex2(u.y - up));
+            sum += u.x + u.y;
+            u = ts::halves(ts::mul2(ts::two(u.x, u.y), i ? vs.y : vs.x));
+            pw[2 * k + i] = pack_half2(u.x, u.y);
+          }
         }
         ts::tc::tmem_st16(lane_base + s_col + c * 16, pw);
-        l_run += (sum.x + sum.y) * (t_run == -INFINITY ? 0.f : ts::ex2(up - less - m_run));
+        l_run += sum * (t_run == -INFINITY ? 0.f : ts::ex2(up - less - m_run));
+        if (c + 1 < n_some) ts::tc::tmem_ld32(lane_base + s_col + (c + 1) * 32, sa);
       };
 #pragma unroll 1
       for (int c = 0; c < min(n_whole, n_some); ++c) columns(c, std::false_type{});
@@ -783,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_fp8_kernel(const Ar
     ts::tc::fence_after_sync();
     if (x < a.q_tiles) {
       // A row that saw nothing has a sum of 0, and O = 0. An infinite score makes NaNs.
-      float inv = l_run > 0.f ? ts::ex2(t_run - m_run) * (1.f / float(1 << kRefLog)) / l_run : l_run;
+      float inv = l_run > 0.f ? ts::ex2(t_run - m_run) / l_run : l_run;
       if (saw_nan || m_run == INFINITY) inv = __uint_as_float(0x7fc00000u);
       // The row goes to the warp's part of its Q tile (no MMA reads it any more), 16 bytes at a
       // time in swizzled places, and from there to memory in whole rows.
