@@ -16,9 +16,9 @@
 //     power of two into fp16's range and written to shared memory; then per tile, 32 columns at a
 //     time: s = S times K's scale, u = 2^(s + n - mt), P = u times V's scale over 2^n, rounded to
 //     fp16 (11 bits), back to TMEM over S. 2^n is the largest V scale of the 32 tokens, mt the maximum
-//     of s + log2(V's scale) over the row's first tile, kept while no P exceeds 2^14, so the
-//     exponentials wait for no maximum; a warp with a row past that takes the columns, and all
-//     before them, to the new maximum. The softmax's sum, of 2^(s - m) with a maximum m of s, is that
+//     of s + log2(V's scale) over the row's first tile, kept while 32 columns' u add up to 2^14 at
+//     most, so the exponentials wait for no maximum; a warp with a row past that takes the columns,
+//     and all before them, to the new maximum. The softmax's sum, of 2^(s - m) with a maximum m of s, is that
 //     of u times one factor per 32 columns, in fp32. The output is O 2^(mt - m) / sum. So a key of any
 //     magnitude takes no bits from the others unless its weight does: P is off by 2^-11 of itself,
 //     or by 2^-25 of the largest P below 2^-14 of that. Columns no row of a warp sees are skipped.
@@ -34,7 +34,8 @@
 // fp16 outputs 4.6e-4 off 64 bits instead of 2.9e-4 (2.1e-4 is their own rounding).
 // A page outside the pool is skipped (its columns are masked). A V row with a NaN scale is stored
 // as zeros and rows that see it become NaN, so rows before it in the chunk stay clean. V's rows past
-// the last visible key are stored as zeros: their slots may hold anything. Other shapes and fp32 queries run on CUDA cores (attention_portable.cu).
+// the last visible key are stored as zeros: their slots may hold anything. Other shapes and fp32
+// queries run on CUDA cores (attention_portable.cu).
 #include <cstddef>
 
 #include "fp8.cuh"
@@ -913,7 +914,7 @@ extern "C" int ts_paged_prefill_fp8(void* out, const void* query, int64_t query_
   const int longest = max_query_len < num_query_tokens ? max_query_len : num_query_tokens;
   const int tiles = (longest + a.tq - 1) / a.tq;
   // Two query tiles a CTA share each converted K/V tile; one a CTA shortens a CTA's time when there
-  // are too few pairs for the SMs (one 512-token chunk over 1,024 tokens: 35 us instead of 45).
+  // are too few pairs for the SMs (one 512-token chunk over 1,024 tokens: 32 us instead of 38).
   const int64_t pairs = int64_t((tiles + 1) / 2) * num_kv_heads * num_seqs;
   a.q_tiles = pairs < sm_count() ? 1 : kQTiles;
   const dim3 grid((tiles + a.q_tiles - 1) / a.q_tiles, num_kv_heads, num_seqs);
