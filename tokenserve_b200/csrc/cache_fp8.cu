@@ -12,7 +12,7 @@
 // has the vectors of four rows in flight, and no 64-bit division stands before them. Rows that do
 // not split that way (odd sizes or alignment) take a warp per row with scalar accesses. Measured with
 // heads of 128: append of 32,768 tokens x 8 bf16 heads 38 us (0.83 of the copy rate), rotary + append
-// of 16,381 tokens of 32/8 heads 72 us (0.78), reading 64 ragged contexts back 87 us (0.84).
+// of 16,381 tokens of 32/8 heads 71 us (0.79), reading 64 ragged contexts back 87 us (0.84).
 #include "fp8.cuh"
 
 namespace {
@@ -65,7 +65,7 @@ __device__ __forceinline__ void flag(int32_t* error_flag) {
 // One lane's E values of a row -> E codes at row + c * E, the scale from the row's first lane; with
 // VPL > 1 the lane has E / VPL values of each of VPL parts of the row. Every lane of the warp takes
 // part (shuffles); `live` rows are stored. BRANCH: rows of a small scale have code of their own
-// (append 37.7 us, 42.8 without; rotary + append 72.3 without, 73.5 with).
+// (append 37.7 us, 42.8 without; rotary + append 71.3 without, 72.1 with).
 template <int E, int LPR, int VPL, bool BRANCH>
 __device__ __forceinline__ void store_row_fp8(const float (&x)[E], int c, bool live, uint8_t* row,
                                               float* scale) {
@@ -275,9 +275,10 @@ __device__ __forceinline__ float2 cos_sin(int64_t pos, float f, float mscale) {
 // then keeps in registers for all its rows. Requires rd % (2 E) == 0 (half layout: a lane's partner
 // values sit in one other lane), rows of LPR * 16 bytes, 16-byte aligned.
 //
-// 64 threads keep a token's set-up small beside its rows when there are many tokens (16,381 tokens of
-// 32/8 heads: 67 us, 75 with 128, 107 with 256); with few tokens 128 shorten it (256 tokens: 3.6 us,
-// 4.7 with 64).
+// 64 threads keep a token's set-up small beside its rows when there are many tokens (8,192 tokens of
+// 32/8 heads: 39 us, 44 with 128); with few tokens 128 shorten it (256 tokens: 4.0 us, 5.2 with 64). The
+// two cross between 1,024 and 1,536 tokens with 32/8, 64/8 and 16/16 heads, near 300 with 8/1, where
+// the difference up to 1,024 tokens is 0.7 us.
 constexpr int kRotaryThreads = 128, kRotaryThreadsMany = 64, kRotaryManyTokens = 1024;
 template <typename T, int LPR, bool INTERLEAVED, bool FP8>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
@@ -363,8 +364,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
       const int h = is_q ? r : (is_v ? r - a.hq - a.hkv : r - a.hq);
       const int64_t prow = first_row + h * a.block_size;
       if (FP8) {
-        // Rows of q only in this warp: nothing to quantise.
-        if (__any_sync(0xffffffffu, !is_q))
+        // Rows of q only in the CTA's step: nothing to quantise.
+        if (r0 - int(threadIdx.x) / LPR + (i + 1) * RPC > a.hq)
           store_row_fp8<E, LPR, 1, false>(x, c, live && !is_q,
                                 static_cast<uint8_t*>(is_v ? a.value_pool : a.key_pool) + prow * D,
                                 (is_v ? a.value_scales : a.key_scales) + prow);
