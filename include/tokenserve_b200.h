@@ -359,7 +359,8 @@ int ts_rope_and_cache(const void* qkv, int64_t qkv_token_stride, void* q_out, vo
  * occur in no other row. Scales are not negative. All pools contiguous. A (token, head) takes
  * head_dim + 4 bytes instead of 2 head_dim, so attention reads, and a pool holds, about half.
  * Blocks are copied and swapped like those of a 16-bit pool, with one more call for the scales
- * (planes of num_kv_heads * block_size * 4 bytes per block).
+ * (planes of num_kv_heads * block_size * 4 bytes per block). No output of the calls below overlaps
+ * one of their inputs.
  */
 
 /*
@@ -424,9 +425,10 @@ int ts_read_cache_fp8(void* key_out, void* value_out, const void* key_pool, cons
 /*
  * ts_paged_decode over an 8-bit cache: out and query of `dtype`, the workspace (and its size, from
  * ts_paged_decode_workspace_size) and the plan as there; reuse_plan = 1 is
- * ts_paged_decode_planned (a plan that ts_paged_decode made counts as another grid's). Shapes as ts_paged_decode: bf16/fp16 queries with block size 16,
- * head_dim 64 or 128 and at most 16 query heads per KV head on tensor cores, else head_dim 32, 64,
- * 128 or 256 on CUDA cores (no workspace).
+ * ts_paged_decode_planned (a plan that ts_paged_decode made counts as another grid's). Shapes as
+ * ts_paged_decode: bf16/fp16 queries with block size 16, head_dim 64 or 128 and at most 16 query
+ * heads per KV head on tensor cores, else head_dim 32, 64, 128 or 256 on CUDA cores (no workspace).
+ * A weight times V's scale is rounded to fp16, relative to the row's largest.
  *
  * Replaces: the same eager attention as ts_paged_decode (src/tokenserve/backends/hf.py:71).
  */

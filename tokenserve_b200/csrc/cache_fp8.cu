@@ -11,7 +11,7 @@
 // half-layout rotary partner comes from another lane of the row instead of a second load. A thread
 // has the vectors of four rows in flight, and no 64-bit division stands before them. Rows that do
 // not split that way (odd sizes or alignment) take a warp per row with scalar accesses. Measured with
-// heads of 128: append of 32,768 tokens x 8 bf16 heads 38 us (0.83 of the copy rate), rotary + append
+// heads of 128: append of 32,768 tokens x 8 bf16 heads 38 us (0.82 of the copy rate), rotary + append
 // of 16,381 tokens of 32/8 heads 71 us (0.79), reading 64 ragged contexts back 87 us (0.84).
 #include "fp8.cuh"
 
