@@ -248,3 +248,39 @@ def test_zero_rows_that_take_nearly_all_weight(cuda_device, dtype, d) -> None:  
     out = prefill(q, cache, tab, qsl, ctx, max(chunks))
     check_prefill_wide(out, q, cache, tab, chunks, ctxs)
     check_decode(decode(q[59:61], cache, tab, ctx), q[59:61], cache, tab, ctxs)
+
+
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 3.0])
+@pytest.mark.parametrize(("dtype", "hq", "hkv", "d"), [(BF, 8, 2, 128), (FH, 12, 1, 64), (torch.float32, 4, 2, 64)])
+def test_softmax_scales_of_any_sign(cuda_device, scale, dtype, hq, hkv, d) -> None:  # type: ignore[no-untyped-def]
+    gen = torch.Generator(device=cuda_device).manual_seed(71)
+    chunks, ctxs = [70, 5], [200, 333]
+    nb, tab = tables_for(ctxs, 16, gen)
+    cache = make_cache(gen, nb, hkv, 16, d)
+    q = torch.randn(sum(chunks), hq, d, generator=gen, device=cuda_device).to(dtype)
+    qsl = torch.tensor([0, *chunks], device=cuda_device).cumsum(0).to(torch.int32)
+    ctx = torch.tensor(ctxs, dtype=torch.int32, device=cuda_device)
+    n = ops.decode_workspace_size(2, hq, hkv, d, tab.shape[1], 16, dtype)
+    ws = torch.empty(max(n, 256), dtype=torch.uint8, device=cuda_device)
+    pre, dec, at = torch.full_like(q, 7.0), torch.full_like(q[:2], 7.0), 0
+    ops.paged_prefill_fp8(pre, q, *cache, tab, qsl, ctx, max(chunks), scale)
+    ops.paged_decode_fp8(dec, q[:2], *cache, tab, ctx, scale, ws)
+    for i, (n, c) in enumerate(zip(chunks, ctxs, strict=True)):
+        rows = (*rows_of(cache[0], cache[2], tab[i], c), *rows_of(cache[1], cache[3], tab[i], c))
+        for got, x, pos in ((pre[at : at + n], q[at : at + n], c - n), (dec[i : i + 1], q[i : i + 1], None)):
+            want, off = attention(x, *rows, scale, pos)
+            assert ((got.double() - want).abs() <= off).all()
+        at += n
+
+
+@pytest.mark.parametrize(("hq", "hkv", "d"), [(32, 1, 128), (100, 1, 64), (128, 1, 128), (66, 2, 128)])
+def test_prefill_of_many_query_heads_per_kv_head(cuda_device, hq, hkv, d) -> None:  # type: ignore[no-untyped-def]
+    """Up to 128 rows of a tile are one token's heads; some of a tile's rows belong to no query."""
+    gen = torch.Generator(device=cuda_device).manual_seed(hq)
+    chunks, ctxs = [9, 1, 30], [100, 1, 30]
+    nb, tab = tables_for(ctxs, 16, gen)
+    cache = make_cache(gen, nb, hkv, 16, d)
+    q = torch.randn(sum(chunks), hq, d, generator=gen, device=cuda_device).to(BF)
+    qsl = torch.tensor([0, *chunks], device=cuda_device).cumsum(0).to(torch.int32)
+    ctx = torch.tensor(ctxs, dtype=torch.int32, device=cuda_device)
+    check_prefill(prefill(q, cache, tab, qsl, ctx, max(chunks)), q, cache, tab, chunks, ctxs, k_half=0.0)
